@@ -23,7 +23,9 @@ BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libferret_hip.so")
 NATIVE = os.path.join(PKG, "_native.so")
 SOURCES = ["skinny.hip", "bf16_tiled.hip", "fp8_mid.hip", "int4_moe.hip", "fp8_tiled.hip", "fp8_square.hip",
-           "routing.hip", "moe_tail.hip", "ue8m0.hip", "dispatch.hip"]
+           "routing.hip", "moe_tail.hip", "ue8m0.hip", "norm.hip", "latent_cache.hip", "latent_attention.hip",
+           "expanded_attention.hip",
+           "dispatch.hip"]
 ARCH = "gfx950"
 
 HIPCC_FLAGS = [

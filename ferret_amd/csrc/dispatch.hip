@@ -38,6 +38,7 @@ extern "C" const char* ferret_error_string(int code) {
     case FERRET_ERR_NULL: return "a required pointer is NULL";
     case FERRET_ERR_SHAPE: return "sizes out of range or not supported";
     case FERRET_ERR_WORKSPACE: return "workspace missing or too small";
+    case FERRET_ERR_ALIGN: return "a pointer or stride is off its bound";
     default: break;
   }
   return code > 0 ? hipGetErrorString((hipError_t)code) : "unknown ferret error";

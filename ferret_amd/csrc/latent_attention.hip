@@ -1,0 +1,715 @@
+// Latent attention in its absorbed form, over the paged cache (latent.hpp): every
+// head of a token attends the same rows, of which the 512 latents are key and
+// value at once:
+//   s_ij = scale * (ql_i . c_j + qr_i . k_j)      c_j latents, k_j rotary key
+//   o_i  = sum_j softmax_j(s_ij) c_j              512 latents, expanded by the caller
+// Token i of a sequence of `len` keys and n new tokens sees keys j <= len - n + i
+// (causal) or all of them.  A row that sees none gives zeros and lse -inf.
+//
+// Work.  The n * H query rows of a sequence are cut into tiles of MR, the keys into
+// tiles of 64 ("steps").  All (sequence, row tile, step) triples form one line that
+// is dealt to the work-groups in equal pieces, so a ragged batch loads the card
+// evenly whatever its lengths; a row tile that is cut leaves fp32 partials (O, m, l)
+// in the workspace, which a second kernel joins in order (deterministic).  A
+// work-group finds its piece by itself from lens and cu_q: no host read, so the
+// call can be captured into a graph and replayed with other lengths.
+//
+// One step: the 64 cached rows come into LDS by asynchronous loads, once for key and
+// value.  S^T = K Q^T is dealt to the four waves by queries (WQ) and keys (WK), with
+// the keys as MFMA rows, so that a lane holds the scores of one query; its softmax
+// terms go through LDS as bf16, and for O^T = V^T P^T every wave takes all queries
+// and a quarter of the 512 columns.  So no product is done twice and a row is read
+// from LDS WQ times as key and once as value; the output tile stays in registers.
+// V^T is read with the transposing LDS loads (ds_read_b64_tr): 16 columns by key.
+// e4m3 rows stay e4m3 in LDS.  Keys are widened and scaled in one instruction (exact);
+// values are widened unscaled, and each probability is multiplied by its key's power
+// of two instead, before it is rounded to bf16 (exact, so nothing is lost): one copy
+// of P per block of 128 columns, that is per wave.
+//
+// Numerics: S, m, l and O are fp32; P is rounded to bf16 for the MFMA (half an ulp,
+// 2^-9 relative, random over the keys), l sums the unrounded P.  The running
+// maximum moves only when a score passes it by more than 2^8: P stays <= 256 and the
+// rescaling of O, 256 registers, is skipped for nearly all steps.
+#include "attention.hpp"
+#include "latent.hpp"
+
+#include <initializer_list>
+
+namespace ferret {
+namespace {
+
+constexpr int kKeys = kLatentKeys, kUnits = kLatentUnits;
+constexpr int kAhead = 4;      // LDS fragments read ahead
+constexpr int kFence = 4;      // fragments between scheduling fences
+
+struct Args {
+  const uint16_t *ql, *qr;
+  int ql_t, ql_h, qr_t, qr_h;  // strides of tokens and heads, in elements
+  const uint8_t* data;
+  const uint32_t* scales;
+  Pages pages;
+  const int32_t *lens, *cu_q;
+  int B, T, H;
+  float scale_log2;  // scale * log2(e)
+  int causal;
+  int min_steps;
+  uint16_t* out;  // [T, H, 512]
+  float* lse;     // [T, H] or null
+  // The workspace: rows [T * H] (int4), then ml [2 * kUnits][MR] (m and l), then the
+  // partial outputs [2 * kUnits][MR][512].  A row's record is {first work-group,
+  // pieces, first slot odd, row in tile}.
+  uint8_t* ws;
+  __host__ __device__ int4* rows() const { return reinterpret_cast<int4*>(ws); }
+  __host__ __device__ float2* ml() const {
+    return reinterpret_cast<float2*>(ws + (((size_t)T * H * sizeof(int4) + 255) & ~(size_t)255));
+  }
+  __host__ __device__ float* part(int mr) const { return reinterpret_cast<float*>(ml() + 2 * kUnits * mr); }
+};
+
+template <int MR>
+__device__ __forceinline__ LatentSeq sequence(const Args& a, int b) {
+  return latent_seq(a.cu_q[b], a.cu_q[b + 1], a.lens[b], a.T, a.H, MR, a.pages.max_pages * a.pages.page_size);
+}
+
+template <bool F8>
+struct Tile {
+  static constexpr int kRowB = F8 ? kRowE4m3 : kRowBf16;
+  static constexpr int kChunks = kRowB / 16;
+  static constexpr int kFrags = kRowB / 64;        // 16-byte chunks per lane of a key fragment row
+  static constexpr int kLoads = 8 * kChunks / 64;  // per group of 8 rows
+  static constexpr int kData = kKeys * kRowB;
+  static constexpr int kBytes = kData + (F8 ? kKeys * 4 : 0);  // then the scale words
+  static constexpr int kBufs = F8 ? 3 : 2;
+  static constexpr int kVmem = 2 * kLoads + (F8 ? 1 : 0);  // loads of a wave per step
+};
+
+// What only the ends of a piece need, kept in LDS: scalar registers are short.
+struct Side {
+  uint16_t* out;
+  float* lse;
+  float2* ml;
+  float* part;
+  int4* rows;
+  const uint16_t *ql, *qr;
+  int ql_t, ql_h, qr_t, qr_h;
+  int chunk, seq_at, b;  // the deal, the sequence at hand and its place on the line
+  int first_row;         // the tile's first row among all [T * H]
+  int slot;              // of the partial result, -1 for a whole tile
+  int end;               // of this work-group's share of the line
+};
+
+// LDS after the tile buffers.
+template <int MR, bool F8>
+struct Lds {
+  static constexpr int kCopies = F8 ? 4 : 1;
+  static constexpr int kP = Tile<F8>::kBufs * Tile<F8>::kBytes;  // P [copy][query][64 keys] bf16
+  static constexpr int kTop = kP + kCopies * MR * 128;           // maxima [4][MR], then factors [MR]
+  static constexpr int kValid = kTop + 5 * MR * 4;               // validity of the 16-row blocks, per buffer
+  static constexpr int kMove = kValid + 16;                      // which waves saw the maximum move
+  static constexpr int kSide = kMove + 16;
+  static constexpr int kBytes = kSide + sizeof(Side);
+};
+static_assert(Lds<64, true>::kBytes <= 160 * 1024 && Lds<64, false>::kBytes <= 160 * 1024, "LDS of a CU");
+
+// Chunk c (16 bytes) of row r stands at chunk c ^ swz(r): the 16 rows of a key
+// fragment, and the rows of two transposed blocks (4 rows of two chunks each, or 8 of
+// one), fall on distinct banks (a row is 32 banks past a multiple of 64).
+__device__ __forceinline__ int swz(int r) { return ((r >> 1) & 4) | (r & 2) | ((r >> 2) & 1); }
+
+// QF 16-query fragments per wave of the first product, WQ x WK waves over queries x keys.
+template <int QF, int WQ, bool F8>
+__global__ __launch_bounds__(256, 1) void latent_attention_kernel(Args a) {
+  using L = Tile<F8>;
+  constexpr int MR = 16 * QF * WQ, MF = QF * WQ;
+  using M = Lds<MR, F8>;
+  constexpr int WK = 4 / WQ;
+  constexpr int KT = kKeys / 16 / WK;     // 16-key blocks of a wave's scores
+  constexpr int CT = kLatent / 16 / 4;    // 16-column blocks of a wave's output
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int r16 = lane & 15, g = lane >> 4;
+  const int wq = wave / WK, wk = wave % WK;
+  float* const tops = reinterpret_cast<float*>(lds + M::kTop);
+  Side* const side = reinterpret_cast<Side*>(lds + M::kSide);
+
+  // ---- this work-group's piece [start, end) of the line
+  int cur;
+  {
+    int* tot = reinterpret_cast<int*>(lds);  // wave totals, then the sequence found and its place
+    const int per = (a.B + 255) / 256;
+    const int b0 = threadIdx.x * per;
+    int mine = 0;
+    for (int i = 0; i < per && b0 + i < a.B; ++i) mine += sequence<MR>(a, b0 + i).work();
+    int incl = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int o = __shfl_up(incl, off, 64);
+      if (lane >= off) incl += o;
+    }
+    if (lane == 63) tot[wave] = incl;
+    __syncthreads();
+    int before = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) before += tot[w];
+      total += tot[w];
+    }
+    const int chunk = latent_chunk(total, a.min_steps);
+    const int start = (int)min((long long)blockIdx.x * chunk, (long long)total);
+    const int excl = before + incl - mine;
+    if (start >= total) return;
+    if (excl <= start && start < excl + mine) {
+      int at = excl;
+      for (int i = 0; i < per; ++i) {
+        const int w = sequence<MR>(a, b0 + i).work();
+        if (start < at + w) {
+          side->b = b0 + i;
+          side->seq_at = at;
+          side->chunk = chunk;
+          side->end = min(start + chunk, total);
+          side->out = a.out;
+          side->lse = a.lse;
+          side->rows = a.rows();
+          side->ml = a.ml();
+          side->part = a.part(MR);
+          side->ql = a.ql;
+          side->qr = a.qr;
+          side->ql_t = a.ql_t;
+          side->ql_h = a.ql_h;
+          side->qr_t = a.qr_t;
+          side->qr_h = a.qr_h;
+          break;
+        }
+        at += w;
+      }
+    }
+    cur = uniform(start);
+    __syncthreads();
+  }
+
+  // ---- lane constants
+  int load_off[L::kLoads];  // source bytes within a group of 8 rows, even group
+#pragma unroll
+  for (int j = 0; j < L::kLoads; ++j) {
+    const int slot = j * 64 + lane, row = slot / L::kChunks, pos = slot % L::kChunks;
+    load_off[j] = row * L::kRowB + ((pos ^ swz(row)) << 4);
+  }
+
+  while (cur < uniform(side->end)) {
+    int b = uniform(side->b), seq_at = uniform(side->seq_at);
+    LatentSeq s = sequence<MR>(a, b);
+    while (cur >= seq_at + s.work() && b + 1 < a.B) {  // the next sequence with rows
+      seq_at += s.work();
+      s = sequence<MR>(a, ++b);
+    }
+    b = uniform(b);
+    const int len = uniform(s.len), steps = uniform(s.steps), q0 = uniform(s.q0);
+    const int tile = uniform((cur - seq_at) / steps), s0 = uniform(cur - seq_at - tile * steps);
+    const int s1 = uniform(min(steps, s0 + (side->end - cur)));
+    const int row0 = tile * MR, row_last = uniform(min(row0 + MR, s.rows) - 1);
+    // keys seen by the first and by the last token of the tile
+    const int past = len - uniform(s.n) + 1;
+    const int see_all = uniform(max(a.causal ? past + row0 / a.H : len, 0));
+    const int see_any = uniform(max(a.causal ? past + row_last / a.H : len, 0));
+    const int last = min(s1, (see_any + kKeys - 1) / kKeys);
+    const int chunk = side->chunk, first_row = q0 * a.H + row0;
+    __syncthreads();  // the piece before is done with its record and buffers
+    if (threadIdx.x == 0) {
+      side->b = b;
+      side->seq_at = seq_at;
+      side->first_row = first_row;
+      side->slot = s0 == 0 && s1 == steps ? -1 : latent_slot(blockIdx.x, cur, chunk);
+    }
+    if (s0 == 0 && (int)threadIdx.x <= row_last - row0) {  // where the pieces of this tile's rows stand
+      const LatentRecord r = latent_record(blockIdx.x, cur, steps, chunk);
+      side->rows[first_row + threadIdx.x] = make_int4(r.block, r.pieces, r.odd, threadIdx.x);
+    }
+
+    f32x4 o[CT][MF];
+    float m[QF], l[QF];
+#pragma unroll
+    for (int f = 0; f < QF; ++f) {
+      m[f] = -INFINITY;
+      l[f] = 0.f;
+    }
+#pragma unroll
+    for (int f = 0; f < MF; ++f)
+#pragma unroll
+      for (int c = 0; c < CT; ++c) o[c][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    // Step t's rows into its buffer: this wave's 16 of the 64.  The page table is read
+    // by scalar loads, which the count of vector loads in flight does not see.
+    const auto* table = (const __attribute__((address_space(4))) int32_t*)(a.pages.table +
+                                                                          (long long)b * a.pages.max_pages);
+    auto issue = [&](int t) {
+      uint8_t* buf = lds + (t % L::kBufs) * L::kBytes;
+      const int pos = t * kKeys + wave * 16;
+      const int page = uniform(pos / a.pages.page_size);
+      int id = -1;
+      if (page < a.pages.max_pages) id = table[page];
+      const long long at = page_row(id, a.pages.pages, a.pages.page_size, pos - page * a.pages.page_size);
+      const bool ok = at >= 0;
+      const long long row = ok ? at : 0;  // some row: masked
+      if (lane == 0) lds[M::kValid + (t % L::kBufs) * 4 + wave] = ok ? 1 : 0;
+      const uint8_t* src = a.data + row * L::kRowB;
+      const uint32_t dst = uniform(lds_address(buf) + wave * 16 * L::kRowB);
+#pragma unroll
+      for (int j = 0; j < L::kLoads; ++j) dma_16(src, load_off[j], dst + j * 1024);
+#pragma unroll
+      for (int j = 0; j < L::kLoads; ++j)  // the odd group: one bit of the swizzle differs
+        dma_16(src + 8 * L::kRowB, load_off[j] ^ 64, dst + 8 * L::kRowB + j * 1024);
+      if constexpr (F8)
+        if (lane < 16) dma_4(a.scales + row, lane * 4, uniform(lds_address(buf) + L::kData + wave * 64));
+    };
+
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < L::kBufs - 1; ++i)
+      if (s0 + i < last) issue(s0 + i);
+    __builtin_amdgcn_sched_barrier(0);
+
+    // ---- queries: B fragments (rows past the tile's repeat its last one)
+    u32x4 qf[QF][18];
+    int sees[QF];
+#pragma unroll
+    for (int f = 0; f < QF; ++f) {
+      const int r = row0 + (wq * QF + f) * 16 + r16;
+      const int rc = min(r, row_last), tok = rc / a.H, head = rc - tok * a.H;
+      sees[f] = r <= row_last ? max(a.causal ? past + tok : len, 0) : 0;
+      const uint16_t* ql = side->ql + (long long)(q0 + tok) * side->ql_t + (long long)head * side->ql_h;
+      const uint16_t* qr = side->qr + (long long)(q0 + tok) * side->qr_t + (long long)head * side->qr_h;
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        qf[f][k] = ld_u32x4(ql + (F8 ? 64 * (k >> 1) + 16 * g + 8 * (k & 1) : 32 * k + 8 * g));
+#pragma unroll
+      for (int k = 0; k < 2; ++k) qf[f][16 + k] = ld_u32x4(qr + 32 * k + 8 * g);
+    }
+    wait_vmcnt<0>();  // the queries, so that no wait for them stands in the loop; the first steps come with them
+    __builtin_amdgcn_sched_barrier(0);
+
+    for (int t = s0; t < last; ++t) {
+      // Step t has landed for every wave, and the buffer refilled below has been read.
+      if (L::kBufs == 3 && t + 1 < last) wait_vmcnt<L::kVmem>();
+      else wait_vmcnt<0>();
+      lds_barrier();
+      if (t + L::kBufs - 1 < last) issue(t + L::kBufs - 1);
+      __builtin_amdgcn_sched_barrier(0);
+      uint8_t* buf = lds + (t % L::kBufs) * L::kBytes;
+      const uint32_t* words = reinterpret_cast<const uint32_t*>(buf + L::kData);
+
+      // ---- S^T: 16 keys x 16 queries per block.  Key fragments are read kAhead
+      // fragments before their use; the scheduling fences keep the compiler from
+      // hoisting more of them than the registers hold.
+      f32x4 sc[KT][QF];
+#pragma unroll
+      for (int k = 0; k < KT; ++k)
+#pragma unroll
+        for (int f = 0; f < QF; ++f) sc[k][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+      {
+        // chunk 4j + g: the swizzle touches 8 chunks at most, j >> 1 is an offset
+        const uint8_t* row = buf + (wk * KT * 16 + r16) * L::kRowB;
+        const uint8_t* const at[2] = {row + ((g ^ swz(r16)) << 4), row + (((4 + g) ^ swz(r16)) << 4)};
+        uint32_t word[KT];
+        if constexpr (F8)
+#pragma unroll
+          for (int k = 0; k < KT; ++k) word[k] = words[(wk * KT + k) * 16 + r16];
+        const auto frag = [&](int i) {
+          const int k = i / L::kFrags, j = i % L::kFrags;
+          return ld_u32x4(at[j & 1] + k * 16 * L::kRowB + (j >> 1) * 128);
+        };
+        u32x4 ring[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) ring[i] = frag(i);
+        static_for<0, KT * L::kFrags>([&](auto ic) {
+          constexpr int i = decltype(ic)::value, k = i / L::kFrags, j = i % L::kFrags;
+          const u32x4 c = ring[i % kAhead];
+          if constexpr (i + kAhead < KT * L::kFrags) ring[i % kAhead] = frag(i + kAhead);
+          if constexpr (F8 && j < 8) {
+            const float e = __uint_as_float(((word[k] >> (8 * (j >> 1))) & 255u) << 23);
+            const bf16x8 lo = e4m3x8_to_bf16x8_scaled(c[0], c[1], e), hi = e4m3x8_to_bf16x8_scaled(c[2], c[3], e);
+#pragma unroll
+            for (int f = 0; f < QF; ++f) sc[k][f] = mfma_bf16(lo, __builtin_bit_cast(bf16x8, qf[f][2 * j]), sc[k][f]);
+#pragma unroll
+            for (int f = 0; f < QF; ++f)
+              sc[k][f] = mfma_bf16(hi, __builtin_bit_cast(bf16x8, qf[f][2 * j + 1]), sc[k][f]);
+          } else {
+#pragma unroll
+            for (int f = 0; f < QF; ++f)
+              sc[k][f] = mfma_bf16_16x16x32(c, qf[f][F8 ? j + 8 : j], sc[k][f]);
+          }
+          if constexpr (i % kFence == kFence - 1) __builtin_amdgcn_sched_barrier(0);
+        });
+      }
+      __builtin_amdgcn_sched_barrier(0);
+
+      // ---- masks: only where the step passes what some row sees, or misses a page
+      const uint32_t ok = uniform(*reinterpret_cast<const uint32_t*>(lds + M::kValid + (t % L::kBufs) * 4));
+      if ((t + 1) * kKeys > see_all || ok != 0x01010101u) {
+#pragma unroll
+        for (int f = 0; f < QF; ++f) {
+          const int left = sees[f] - (t * kKeys + wk * KT * 16 + 4 * g);
+#pragma unroll
+          for (int k = 0; k < KT; ++k) {
+            const int upto = (ok >> (8 * (wk * KT + k))) & 1 ? left - k * 16 : 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[k][f][i] = i < upto ? sc[k][f][i] : -INFINITY;
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        // A value that a row does not see must not reach it as 0 * NaN: rows that
+        // no query sees become zeros, and Inf and NaN of rows that some do not see
+        // are cleared.  A query that sees such a row has NaN in its l: its key is
+        // the same row.
+        lds_barrier();  // the keys have been read
+        constexpr int VC = F8 ? kLatent / 16 : kLatent / 8;  // chunks of a row's values
+#pragma unroll 1
+        for (int i = threadIdx.x; i < kKeys * VC; i += 256) {
+          const int r = i / VC, key = t * kKeys + r;
+          const bool none = key >= see_any || !((ok >> (8 * (r >> 4))) & 1);
+          if (!none && key < see_all) continue;
+          u32x4* p = reinterpret_cast<u32x4*>(buf + r * L::kRowB + (((i % VC) ^ swz(r)) << 4));
+          u32x4 v = {0u, 0u, 0u, 0u};
+          if (!none) {
+            v = *p;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              if constexpr (F8) {
+                const uint32_t nan = (((v[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+                v[w] &= ~(nan * 255u);
+              } else {
+                if ((v[w] & 0x7f80u) == 0x7f80u) v[w] &= 0xffff0000u;
+                if ((v[w] & 0x7f800000u) == 0x7f800000u) v[w] &= 0x0000ffffu;
+              }
+            }
+          }
+          *p = v;
+        }
+        if constexpr (F8) {
+          if (threadIdx.x < kKeys) {
+            const int r = threadIdx.x;
+            if (t * kKeys + r >= see_any || !((ok >> (8 * (r >> 4))) & 1))
+              reinterpret_cast<uint32_t*>(buf + L::kData)[r] = 0x7f7f7f7fu;
+          }
+          lds_barrier();  // the scale words are read next
+        }
+      }
+
+      // ---- softmax terms of the lane's queries (column r16 of each fragment), with
+      // the maximum of the steps before
+      bool move = false;
+#pragma unroll
+      for (int f = 0; f < QF; ++f) {
+        float v = sc[0][f][0];
+#pragma unroll
+        for (int k = 0; k < KT; ++k)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v = fmaxf(v, sc[k][f][i]);
+        v = fmaxf(v, __shfl_xor(v, 16, 64));
+        v = fmaxf(v, __shfl_xor(v, 32, 64)) * a.scale_log2;
+        move = move || v > m[f] + kLazy;  // from -inf: any finite score
+        if (g == 0) tops[wk * MR + (wq * QF + f) * 16 + r16] = v;
+      }
+      const bool mine = __any(move);
+      if (lane == 0) lds[M::kMove + wave] = mine ? 1 : 0;
+      float pend[QF];  // this step's part of l
+      const auto put_p = [&]() {
+#pragma unroll
+        for (int f = 0; f < QF; ++f) {
+          const float base = m[f] == -INFINITY ? 0.f : m[f];
+          const int q = (wq * QF + f) * 16 + r16;
+          pend[f] = 0.f;
+#pragma unroll
+          for (int k = 0; k < KT; ++k) {
+            f32x4 p;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              p[i] = __builtin_amdgcn_exp2f(fmaf(sc[k][f][i], a.scale_log2, -base));
+              pend[f] += p[i];
+            }
+            const int kb = wk * KT + k;  // 16-key block of the step: 2 chunks
+            uint8_t* to = lds + M::kP + q * 128 + (((2 * kb + (g >> 1)) ^ (r16 >> 1)) << 4) + (g & 1) * 8;
+            if constexpr (F8) {
+              const u32x4 w4 = *reinterpret_cast<const u32x4*>(words + kb * 16 + 4 * g);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                float e[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) e[i] = p[i] * __uint_as_float(((w4[i] >> (8 * c)) & 255u) << 23);
+                *reinterpret_cast<u32x2*>(to + c * MR * 128) = u32x2{pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3])};
+              }
+            } else {
+              *reinterpret_cast<u32x2*>(to) = u32x2{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3])};
+            }
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      put_p();
+      lds_barrier();
+      if (uniform(*reinterpret_cast<const uint32_t*>(lds + M::kMove)) != 0) {
+        // The maximum of some query moves: again with the new one, O follows.
+#pragma unroll
+        for (int f = 0; f < QF; ++f) {
+          const int q = (wq * QF + f) * 16 + r16;
+          float to = m[f];
+#pragma unroll
+          for (int w = 0; w < WK; ++w) to = fmaxf(to, tops[w * MR + q]);
+          const float by = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[f] - to);
+          m[f] = to;
+          l[f] *= by;
+          if (wk == 0 && g == 0) tops[4 * MR + q] = by;
+        }
+        put_p();
+        lds_barrier();
+#pragma unroll
+        for (int f = 0; f < MF; ++f) {
+          const float by = tops[4 * MR + f * 16 + r16];
+#pragma unroll
+          for (int c = 0; c < CT; ++c) o[c][f] *= by;
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+#pragma unroll
+      for (int f = 0; f < QF; ++f) l[f] += pend[f];
+
+      // ---- O^T += V^T P^T, 32 keys at a time: lane (column r16, key octet g)
+      __builtin_amdgcn_sched_barrier(0);
+      {
+        const uint8_t* pbuf = lds + M::kP + (F8 ? wave * MR * 128 : 0) + r16 * 128;
+        const uint8_t* const pat[2] = {pbuf + ((g ^ (r16 >> 1)) << 4), pbuf + (((4 + g) ^ (r16 >> 1)) << 4)};
+        // The wave's columns start on a multiple of 8 chunks, so the swizzled block
+        // is an exclusive-or into the address, whose low bits are the swizzle's.
+        const int row = 8 * g + (F8 ? r16 >> 1 : r16 >> 2);
+        const uint32_t at = (uint32_t)(t % L::kBufs) * L::kBytes + row * L::kRowB + wave * (F8 ? 128 : 256) +
+                            ((swz(row) ^ (F8 ? 0 : (lane >> 1) & 1)) << 4) + 8 * (lane & 1);
+        const auto frag = [&](int i) {  // i = (half, block)
+          const int h = i / CT, c = i % CT;
+          if constexpr (F8) {
+            const u32x2 v = lds_tr8(lds + (at ^ (c << 4)) + h * 32 * L::kRowB);
+            return u32x4{v[0], v[1], 0u, 0u};
+          } else {  // rows 4 further: the lowest bit of the swizzle flips
+            const uint8_t* p = lds + (at ^ ((c & 3) << 5)) + (c >> 2) * 128 + h * 32 * L::kRowB;
+            const uint8_t* p4 = lds + (at ^ ((c & 3) << 5) ^ 16) + (c >> 2) * 128 + (h * 32 + 4) * L::kRowB;
+            const u32x2 v0 = lds_tr16(p), v1 = lds_tr16(p4);
+            return u32x4{v0[0], v0[1], v1[0], v1[1]};
+          }
+        };
+        u32x4 ring[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) ring[i] = frag(i);
+        static_for<0, kKeys / 32>([&](auto hc) {
+          constexpr int h = decltype(hc)::value;
+          u32x4 p[MF];
+#pragma unroll
+          for (int f = 0; f < MF; ++f) {
+            p[f] = ld_u32x4(pat[h] + f * 16 * 128);
+          }
+          static_for<0, CT>([&](auto cc) {
+            constexpr int c = decltype(cc)::value, i = h * CT + c;
+            const u32x4 v = ring[i % kAhead];
+            if constexpr (i + kAhead < kKeys / 32 * CT) ring[i % kAhead] = frag(i + kAhead);
+            const bf16x8 vb = F8 ? e4m3x8_to_bf16x8(v[0], v[1]) : __builtin_bit_cast(bf16x8, v);
+#pragma unroll
+            for (int f = 0; f < MF; ++f) o[c][f] = mfma_bf16(vb, __builtin_bit_cast(bf16x8, p[f]), o[c][f]);
+            if constexpr (i % kFence == kFence - 1) __builtin_amdgcn_sched_barrier(0);
+          });
+        });
+      }
+    }
+
+    // ---- the piece's result: l of all waves, then a quarter of the columns per wave
+    __syncthreads();  // the last step's maxima and factors have been read
+#pragma unroll
+    for (int f = 0; f < QF; ++f) {
+      float sum = l[f];
+      sum += __shfl_xor(sum, 16, 64);
+      sum += __shfl_xor(sum, 32, 64);
+      const int q = (wq * QF + f) * 16 + r16;
+      if (g == 0) tops[wk * MR + q] = sum;
+      if (wk == 0 && g == 0) tops[4 * MR + q] = m[f];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int f = 0; f < MF; ++f) {
+      const int r = f * 16 + r16;
+      float sum = tops[r];
+#pragma unroll
+      for (int w = 1; w < WK; ++w) sum += tops[w * MR + r];
+      const float top = tops[4 * MR + r];
+      const int col = wave * CT * 16 + 4 * g;
+      if (row0 + r <= row_last) {
+        const int slot = uniform(side->slot);
+        if (slot < 0) {
+          const long long at = side->first_row + r;
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          uint16_t* to = side->out + at * kLatent + col;
+#pragma unroll
+          for (int c = 0; c < CT; ++c)
+            *reinterpret_cast<u32x2*>(to + c * 16) =
+                u32x2{pack_bf16x2(o[c][f][0] * inv, o[c][f][1] * inv), pack_bf16x2(o[c][f][2] * inv, o[c][f][3] * inv)};
+          if (wave == 0 && g == 0 && side->lse != nullptr)
+            side->lse[at] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+        } else {
+          const long long at = (long long)slot * MR + r;
+          if (wave == 0 && g == 0) side->ml[at] = make_float2(top, sum);
+          if (last > s0) {
+            float* to = side->part + at * kLatent + col;
+#pragma unroll
+            for (int c = 0; c < CT; ++c) *reinterpret_cast<f32x4*>(to + c * 16) = o[c][f];
+          }
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    cur += s1 - s0;
+  }
+}
+
+// Joins the pieces of the query rows that were cut.  COLS columns of a row per
+// 256 threads: COLS / 4 lanes across, the pieces dealt to 1024 / COLS groups.
+template <int COLS>
+__global__ __launch_bounds__(256) void latent_join_kernel(Args a, int mr) {
+  constexpr int LANES = COLS / 4, GROUPS = 256 / LANES;
+  __shared__ f32x4 red[256];
+  __shared__ float stat[8];
+  const long long row = blockIdx.x;
+  // rows behind the last sequence have no record
+  if (row < (long long)max(a.cu_q[0], 0) * a.H || row >= (long long)min(a.cu_q[a.B], a.T) * a.H) return;
+  const int4 rec = a.rows()[row];
+  const float2* ml = a.ml();
+  const float* part = a.part(mr);
+  const LatentRecord where{rec.x, rec.y, rec.z};
+  const int pieces = rec.y;
+  if (!latent_record_joins(where) || (unsigned)rec.w >= (unsigned)mr) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const auto slot_row = [&](int j) { return (long long)latent_record_slot(where, j) * mr + rec.w; };
+  float top = -INFINITY;
+  for (int j = threadIdx.x; j < pieces; j += 256) top = fmaxf(top, ml[slot_row(j)].x);
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  if (lane == 0) stat[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(stat[0], stat[1]), fmaxf(stat[2], stat[3]));
+  float sum = 0.f;
+  const float base = top == -INFINITY ? 0.f : top;
+  for (int j = threadIdx.x; j < pieces; j += 256) {
+    const float2 v = ml[slot_row(j)];
+    if (v.y != 0.f) sum += v.y * __builtin_amdgcn_exp2f(v.x - base);  // NaN too: its maximum may be -inf
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+  if (lane == 0) stat[4 + wave] = sum;
+  __syncthreads();
+  sum = (stat[4] + stat[5]) + (stat[6] + stat[7]);
+  const int across = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  const int col = blockIdx.y * COLS + across * 4;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  if (top > -INFINITY) {
+#pragma unroll 4
+    for (int j = group; j < pieces; j += GROUPS) {
+      const long long at = slot_row(j);
+      const float mj = ml[at].x;
+      if (mj > -INFINITY) acc += *reinterpret_cast<const f32x4*>(part + at * kLatent + col) *
+                                 __builtin_amdgcn_exp2f(mj - top);
+    }
+  }
+  red[threadIdx.x] = acc;
+  __syncthreads();
+  if (group != 0) return;
+  for (int i = 1; i < GROUPS; ++i) acc += red[i * LANES + across];
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  *reinterpret_cast<u32x2*>(a.out + row * kLatent + col) =
+      u32x2{pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv)};
+  if (a.lse != nullptr && col == 0)
+    a.lse[row] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+template <int QF, int WQ, bool F8>
+int launch(const Args& a, hipStream_t st) {
+  constexpr int mr = 16 * QF * WQ, lds = Lds<mr, F8>::kBytes;
+  FERRET_HIP_CHECK((set_lds_limit_once<latent_attention_kernel<QF, WQ, F8>>(lds)));
+  hipLaunchKernelGGL((latent_attention_kernel<QF, WQ, F8>), dim3(kUnits), dim3(256), lds, st, a);
+  FERRET_HIP_CHECK(hipGetLastError());
+  const unsigned rows = (unsigned)((long long)a.T * a.H);
+  if (rows <= 1024)
+    hipLaunchKernelGGL((latent_join_kernel<128>), dim3(rows, 4), dim3(256), 0, st, a, mr);
+  else
+    hipLaunchKernelGGL((latent_join_kernel<512>), dim3(rows, 1), dim3(256), 0, st, a, mr);
+  return (int)hipGetLastError();
+}
+
+template <bool F8>
+int launch_rows(int mr, const Args& a, hipStream_t st) {
+  switch (mr) {
+    case 16: return launch<1, 1, F8>(a, st);
+    case 32: return launch<2, 1, F8>(a, st);
+    default: return launch<2, 2, F8>(a, st);
+  }
+}
+
+// Query rows per tile by the rows that a sequence has on average.
+int tile_rows(int T, int B, int H) {
+  const long long rows = (long long)T * H / B;
+  return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+}
+
+}  // namespace
+}  // namespace ferret
+
+using namespace ferret;
+
+int ferret_check_pages(const int32_t* page_table, int B, int max_pages, int pages, int page_size);
+
+extern "C" size_t ferret_latent_attention_workspace(int B, int T, int H) {
+  if (B < 1 || T < 1 || H < 1 || (long long)T * H >= (1LL << 31)) return 0;
+  const size_t mr = tile_rows(T, B, H), rows = ((size_t)T * H * sizeof(int4) + 255) & ~(size_t)255;
+  return rows + 2 * kUnits * mr * (sizeof(float2) + kLatent * sizeof(float));
+}
+
+extern "C" int ferret_latent_attention(const void* q_latent, long long ql_token, long long ql_head,
+                                       const void* q_rotary, long long qr_token, long long qr_head, const void* data,
+                                       const void* scales, int pages, int page_size, const int32_t* page_table,
+                                       const int32_t* lens, const int32_t* cu_q, int B, int max_pages, int T, int H,
+                                       float scale, int causal, void* out, float* lse, void* ws, size_t ws_bytes,
+                                       void* stream) {
+  FERRET_REQUIRE(q_latent && q_rotary && data && lens && cu_q && out, FERRET_ERR_NULL);
+  const int rc = ferret_check_pages(page_table, B, max_pages, pages, page_size);
+  if (rc != FERRET_OK) return rc;
+  FERRET_REQUIRE(T >= 1 && H >= 1 && H <= 1024 && (long long)T * H < (1LL << 31), FERRET_ERR_SHAPE);
+  FERRET_REQUIRE(scale > 0.f && scale < 1e30f, FERRET_ERR_SHAPE);
+  for (const long long stride : {ql_token, ql_head, qr_token, qr_head})
+    FERRET_REQUIRE(stride >= 0 && stride < (1LL << 31), FERRET_ERR_SHAPE);
+  const auto bits = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
+  FERRET_REQUIRE(((bits(q_latent) | bits(q_rotary) | bits(data) | bits(out)) & 15) == 0 &&
+                     ((bits(scales) | bits(lse)) & 3) == 0 && ((ql_token | ql_head | qr_token | qr_head) & 7) == 0,
+                 FERRET_ERR_ALIGN);
+  const int mr = tile_rows(T, B, H);
+  // steps of the whole batch are counted in 32 bits
+  const long long tiles = (long long)T * H / mr + B, most = ((long long)max_pages * page_size + kKeys - 1) / kKeys;
+  FERRET_REQUIRE(tiles * most < (1LL << 31), FERRET_ERR_SHAPE);
+  FERRET_REQUIRE(ws != nullptr && ws_bytes >= ferret_latent_attention_workspace(B, T, H) && (bits(ws) & 15) == 0,
+                 FERRET_ERR_WORKSPACE);
+  Args a;
+  a.ql = static_cast<const uint16_t*>(q_latent);
+  a.qr = static_cast<const uint16_t*>(q_rotary);
+  a.ql_t = (int)ql_token;
+  a.ql_h = (int)ql_head;
+  a.qr_t = (int)qr_token;
+  a.qr_h = (int)qr_head;
+  a.data = static_cast<const uint8_t*>(data);
+  a.scales = static_cast<const uint32_t*>(scales);
+  a.pages = Pages{page_table, max_pages, pages, page_size};
+  a.lens = lens;
+  a.cu_q = cu_q;
+  a.B = B;
+  a.T = T;
+  a.H = H;
+  a.scale_log2 = scale * kLog2e;
+  a.causal = causal != 0;
+  a.min_steps = 2;
+  a.out = static_cast<uint16_t*>(out);
+  a.lse = lse;
+  a.ws = static_cast<uint8_t*>(ws);
+  return scales != nullptr ? launch_rows<true>(mr, a, (hipStream_t)stream)
+                           : launch_rows<false>(mr, a, (hipStream_t)stream);
+}

@@ -16,6 +16,7 @@
 #include <Python.h>
 #include <ATen/ATen.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -72,6 +73,30 @@ class Call {
     return &t;
   }
   const at::Tensor* in(PyObject* o, int ndim, at::ScalarType type) { return in(o, ndim, type, type); }
+
+  // A required tensor of `ndim` dimensions whose last is packed; the others have any strides.
+  const at::Tensor* rows(PyObject* o, int ndim, at::ScalarType type) {
+    if (!ok_ || !THPVariable_CheckExact(o)) {
+      ok_ = false;
+      return nullptr;
+    }
+    const at::Tensor& t = THPVariable_Unpack(o);
+    if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || t.key_set().has_any(kWrapped) ||
+        t.dim() != ndim || t.scalar_type() != type || t.stride(ndim - 1) != 1) {
+      ok_ = false;
+      return nullptr;
+    }
+    for (const int64_t s : t.sizes()) require(s <= INT_MAX);
+    if (!has_device_) {
+      device_ = t.device();
+      has_device_ = true;
+    }
+    require(t.device() == device_);
+    return &t;
+  }
+
+  // The tensors are on the current device (the one whose stream is taken).
+  void require_current() { require(has_device_ && device_.index() == c10::hip::current_device()); }
 
   // A caller's output of exactly this shape, or a new one.
   at::Tensor out(PyObject* o, at::IntArrayRef shape, at::ScalarType type, at::ScalarType or_type) {
@@ -403,11 +428,214 @@ NATIVE(moe_combine, 3) {
   return wrap(y);
 }
 
+bool as_float(PyObject* o, float* v) {
+  const double x = PyFloat_CheckExact(o) ? PyFloat_AS_DOUBLE(o) : -1.0;
+  *v = (float)x;
+  return x >= 0.0;
+}
+
+// The stride of dimension d, 0 where it has one element.
+int64_t step(const at::Tensor* t, int d) { return t->size(d) == 1 ? 0 : t->stride(d); }
+
+// x, w, residual, eps, residual_out of a norm.
+struct Norm {
+  const at::Tensor *x, *w, *r = nullptr;
+  at::Tensor ro;
+  float eps;
+  int M, K;
+  int64_t xs, rs;
+  bool read(Call& c, PyObject* const* a, PyObject* out) {
+    x = c.rows(a[0], 2, kBf16);
+    w = c.in(a[1], 1, kBf16);
+    if (!c.ok() || !as_float(a[3], &eps)) return false;
+    M = x->size(0), K = x->size(1);
+    c.require(w->size(0) == K);
+    if (a[2] == Py_None) {
+      c.require(out == Py_None);
+    } else {
+      r = c.rows(a[2], 2, kBf16);
+      if (!c.ok() || r->size(0) != M || r->size(1) != K) return false;
+    }
+    c.require_current();
+    if (r != nullptr) ro = c.out(out, {M, K}, kBf16);
+    xs = step(x, 0) != 0 ? step(x, 0) : K;
+    rs = r != nullptr && step(r, 0) != 0 ? step(r, 0) : K;
+    return c.ok();
+  }
+  PyObject* residual() const {
+    if (r != nullptr) return wrap(ro);
+    Py_RETURN_NONE;
+  }
+};
+
+// x, w, residual, eps, out, residual_out -> (y, residual_out or None)
+NATIVE(rms_norm, 6) {
+  Call c;
+  Norm n;
+  if (!n.read(c, a, a[5])) Py_RETURN_NONE;
+  const at::Tensor y = c.out(a[4], {n.M, n.K}, kBf16);
+  if (!c.ok()) Py_RETURN_NONE;
+  void* st = stream();
+  if (!run("ferret_rms_norm", [&] {
+        return ferret_rms_norm(ptr(n.x), n.xs, n.r ? ptr(n.r) : nullptr, n.rs, ptr(n.w), n.eps, n.M, n.K, ptr(y),
+                               ptr(n.ro), st);
+      }))
+    return declined();
+  return Py_BuildValue("(NN)", wrap(y), n.residual());
+}
+
+// x, w, residual, eps, q, scale, residual_out -> (q, scale, residual_out or None)
+NATIVE(rms_norm_e4m3, 7) {
+  Call c;
+  Norm n;
+  if (!n.read(c, a, a[6])) Py_RETURN_NONE;
+  const at::Tensor q = c.out(a[4], {n.M, n.K}, kFp8, at::kByte);
+  const at::Tensor s = c.out(a[5], {n.M, n.K / 128}, kF32);
+  if (!c.ok()) Py_RETURN_NONE;
+  void* st = stream();
+  if (!run("ferret_rms_norm_e4m3", [&] {
+        return ferret_rms_norm_e4m3(ptr(n.x), n.xs, n.r ? ptr(n.r) : nullptr, n.rs, ptr(n.w), n.eps, n.M, n.K, ptr(q),
+                                    ptr_as<float>(s), ptr(n.ro), st);
+      }))
+    return declined();
+  return Py_BuildValue("(NNN)", wrap(q), wrap(s), n.residual());
+}
+
+// A latent cache and a batch's index tensors: data, scales (or None); page_table, starts, lens (or null).
+struct Cache {
+  const at::Tensor *data, *scales = nullptr, *table, *starts, *lens = nullptr;
+  int pages, page_size, B, max_pages;
+  bool read(Call& c, PyObject* d, PyObject* s, PyObject* t, PyObject* at, PyObject* ln) {
+    const bool f8 = s != Py_None;
+    data = c.in(d, 3, f8 ? at::kByte : kBf16);
+    if (f8) scales = c.in(s, 3, at::kByte);
+    table = c.in(t, 2, kI32);
+    starts = c.in(at, 1, kI32);
+    if (ln != nullptr) lens = c.in(ln, 1, kI32);
+    if (!c.ok()) return false;
+    pages = data->size(0), page_size = data->size(1), max_pages = table->size(1);
+    const int64_t b = starts->size(0) - 1;
+    B = (int)b;
+    c.require(data->size(2) == (f8 ? 640 : 576) && b >= 1 && table->size(0) == b &&
+              (lens == nullptr || lens->size(0) == b));
+    if (f8) c.require(scales->size(0) == pages && scales->size(1) == page_size && scales->size(2) == 4);
+    c.require_current();
+    return c.ok();
+  }
+  void* scale_ptr() const { return scales != nullptr ? ptr(scales) : nullptr; }
+};
+
+// data, scales, latent, rotary, page_table, lens, cu_q -> True
+NATIVE(latent_cache_write, 7) {
+  Call c;
+  Cache k;
+  if (!k.read(c, a[0], a[1], a[4], a[6], a[5])) Py_RETURN_NONE;
+  const auto* lat = c.rows(a[2], 2, kBf16);
+  const auto* rot = c.rows(a[3], 2, kBf16);
+  if (!c.ok()) Py_RETURN_NONE;
+  const int T = lat->size(0);
+  if (lat->size(1) != 512 || rot->size(0) != T || rot->size(1) != 64) Py_RETURN_NONE;
+  void* st = stream();
+  if (!run("ferret_latent_cache_write", [&] {
+        return ferret_latent_cache_write(ptr(lat), T > 1 ? step(lat, 0) : 512, ptr(rot), T > 1 ? step(rot, 0) : 64,
+                                         ptr_as<int32_t>(k.table), ptr_as<int32_t>(k.lens),
+                                         ptr_as<int32_t>(k.starts), k.B, k.max_pages, T, ptr(k.data), k.scale_ptr(),
+                                         k.pages, k.page_size, st);
+      }))
+    return declined();
+  Py_RETURN_TRUE;
+}
+
+// data, scales, page_table, cu_k, total, latent, rotary -> (latent, rotary)
+NATIVE(latent_cache_read, 7) {
+  Call c;
+  Cache k;
+  int total;
+  if (!k.read(c, a[0], a[1], a[2], a[3], nullptr) || !as_int(a[4], &total) || total < 1) Py_RETURN_NONE;
+  const at::Tensor lat = c.out(a[5], {total, 512}, kBf16);
+  const at::Tensor rot = c.out(a[6], {total, 64}, kBf16);
+  if (!c.ok()) Py_RETURN_NONE;
+  void* st = stream();
+  if (!run("ferret_latent_cache_read", [&] {
+        return ferret_latent_cache_read(ptr(k.data), k.scale_ptr(), k.pages, k.page_size, ptr_as<int32_t>(k.table),
+                                        ptr_as<int32_t>(k.starts), k.B, k.max_pages, total, ptr(lat), ptr(rot), st);
+      }))
+    return declined();
+  return Py_BuildValue("(NN)", wrap(lat), wrap(rot));
+}
+
+// q_latent, q_rotary, data, scales, page_table, lens, cu_q, scale, causal, return_lse, out, workspace
+// -> out, or (out, lse)
+NATIVE(latent_attention, 12) {
+  Call c;
+  Cache k;
+  float scale;
+  if (!k.read(c, a[2], a[3], a[4], a[6], a[5])) Py_RETURN_NONE;
+  const auto* ql = c.rows(a[0], 3, kBf16);
+  const auto* qr = c.rows(a[1], 3, kBf16);
+  if (!c.ok() || !as_float(a[7], &scale)) Py_RETURN_NONE;
+  const int T = ql->size(0), H = ql->size(1);
+  c.require(ql->size(2) == 512 && qr->size(0) == T && qr->size(1) == H && qr->size(2) == 64);
+  const bool causal = a[8] == Py_True, with_lse = a[9] == Py_True;
+  const at::Tensor o = c.out(a[10], {T, H, 512}, kBf16);
+  const size_t need = ferret_latent_attention_workspace(k.B, T, H);
+  if (!c.ok() || need == 0) Py_RETURN_NONE;
+  const at::Tensor ws = c.workspace(a[11], need);
+  if (!c.ok()) Py_RETURN_NONE;
+  const at::Tensor lse = with_lse ? c.fresh({T, H}, kF32) : at::Tensor();
+  void* st = stream();
+  if (!run("ferret_latent_attention", [&] {
+        return ferret_latent_attention(ptr(ql), step(ql, 0), step(ql, 1), ptr(qr), step(qr, 0), step(qr, 1),
+                                       ptr(k.data), k.scale_ptr(), k.pages, k.page_size, ptr_as<int32_t>(k.table),
+                                       ptr_as<int32_t>(k.lens), ptr_as<int32_t>(k.starts), k.B, k.max_pages, T, H,
+                                       scale, causal, ptr(o), ptr_as<float>(lse), ptr(ws), need, st);
+      }))
+    return declined();
+  if (!with_lse) return wrap(o);
+  return Py_BuildValue("(NN)", wrap(o), wrap(lse));
+}
+
+// q_nope, q_rotary, k_nope, k_rotary, v, cu_q, cu_k, scale, causal, return_lse, out -> out, or (out, lse)
+NATIVE(latent_attention_expanded, 11) {
+  Call c;
+  float scale;
+  const auto* qn = c.rows(a[0], 3, kBf16);
+  const auto* qr = c.rows(a[1], 3, kBf16);
+  const auto* kn = c.rows(a[2], 3, kBf16);
+  const auto* kr = c.rows(a[3], 2, kBf16);
+  const auto* v = c.rows(a[4], 3, kBf16);
+  const auto* cu_q = c.in(a[5], 1, kI32);
+  const auto* cu_k = c.in(a[6], 1, kI32);
+  if (!c.ok() || !as_float(a[7], &scale)) Py_RETURN_NONE;
+  const int T = qn->size(0), H = qn->size(1), S = kn->size(0), B = (int)cu_q->size(0) - 1;
+  c.require(qn->size(2) == 128 && qr->size(0) == T && qr->size(1) == H && qr->size(2) == 64 && kn->size(1) == H &&
+            kn->size(2) == 128 && kr->size(0) == S && kr->size(1) == 64 && v->size(0) == S && v->size(1) == H &&
+            v->size(2) == 128 && B >= 1 && cu_k->size(0) == B + 1);
+  c.require_current();
+  const bool causal = a[8] == Py_True, with_lse = a[9] == Py_True;
+  const at::Tensor o = c.out(a[10], {T, H, 128}, kBf16);
+  if (!c.ok()) Py_RETURN_NONE;
+  const at::Tensor lse = with_lse ? c.fresh({T, H}, kF32) : at::Tensor();
+  void* st = stream();
+  if (!run("ferret_latent_attention_expanded", [&] {
+        return ferret_latent_attention_expanded(
+            ptr(qn), step(qn, 0), step(qn, 1), ptr(qr), step(qr, 0), step(qr, 1), ptr(kn), step(kn, 0), step(kn, 1),
+            ptr(kr), step(kr, 0), ptr(v), step(v, 0), step(v, 1), ptr_as<int32_t>(cu_q), ptr_as<int32_t>(cu_k), B, T,
+            S, H, scale, causal, ptr(o), ptr_as<float>(lse), st);
+      }))
+    return declined();
+  if (!with_lse) return wrap(o);
+  return Py_BuildValue("(NN)", wrap(o), wrap(lse));
+}
+
 #define METHOD(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {METHOD(linear_bf16),   METHOD(fp8_gemm_blockscale), METHOD(fp8_gemm_ue8m0),
                           METHOD(moe_route_topk), METHOD(moe_permute),         METHOD(moe_w13_fp8),
                           METHOD(moe_w2_fp8),     METHOD(moe_w13_w4a16),       METHOD(quant_act_e4m3),
-                          METHOD(moe_combine),    {nullptr, nullptr, 0, nullptr}};
+                          METHOD(moe_combine),    METHOD(rms_norm),            METHOD(rms_norm_e4m3),
+                          METHOD(latent_cache_write), METHOD(latent_cache_read), METHOD(latent_attention),
+                          METHOD(latent_attention_expanded),
+                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", "Native call path of ferret_amd.ops.", -1, kMethods,
                        nullptr, nullptr, nullptr, nullptr};
 

@@ -14,6 +14,7 @@ import warnings
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libferret_hip.so")
 
 _c_int, _c_void_p, _c_size_t, _c_char_p = ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_char_p
+_c_i64, _c_float = ctypes.c_longlong, ctypes.c_float
 _vp = _c_void_p
 
 # name -> (restype, argtypes); must list every function of include/ferret_hip.h
@@ -49,6 +50,18 @@ SIGNATURES = {
     "ferret_moe_w2_fp8_ex": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int,
                                       _c_int, _vp, _c_int, _vp]),
     "ferret_workspace_bytes": (_c_size_t, [_c_int, _c_int, _c_int, _c_int, _c_int]),
+    "ferret_rms_norm": (_c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_float, _c_int, _c_int, _vp, _vp, _vp]),
+    "ferret_rms_norm_e4m3": (_c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_float, _c_int, _c_int, _vp, _vp, _vp, _vp]),
+    "ferret_latent_cache_write": (_c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _vp,
+                                           _c_int, _c_int, _vp]),
+    "ferret_latent_cache_read": (_c_int, [_vp, _vp, _c_int, _c_int, _vp, _vp, _c_int, _c_int, _c_int, _vp, _vp, _vp]),
+    "ferret_latent_attention_workspace": (_c_size_t, [_c_int, _c_int, _c_int]),
+    "ferret_latent_attention_expanded": (_c_int, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp,
+                                                  _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _c_int, _c_int, _c_int,
+                                                  _c_int, _c_float, _c_int, _vp, _vp, _vp]),
+    "ferret_latent_attention": (_c_int, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _c_int, _c_int, _vp, _vp,
+                                         _vp, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _vp, _vp, _vp,
+                                         _c_size_t, _vp]),
 }
 
 

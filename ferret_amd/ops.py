@@ -458,3 +458,310 @@ def moe_combine(o: torch.Tensor, weights: torch.Tensor, out: torch.Tensor | None
                                         T, topk, N, _dev(out, "out", torch.bfloat16, 2), _stream())
     _lib.check("ferret_moe_combine", rc)
     return out
+
+
+# ---- the attention block around the projections -------------------------------------------------------------------
+
+def _rows(t: torch.Tensor, name: str, shape: tuple, dtype=torch.bfloat16) -> tuple:
+    """A tensor of packed last dimension and any other strides (a slice of a wider
+    projection, a transposed product): pointer, then the strides of the other
+    dimensions in elements, all on the kernels' bounds of 16 bytes."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.device.type != "cuda":
+        raise ValueError(f"{name} must be a GPU tensor (got {t.device}); ferret_amd has no CPU path")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must have dtype {dtype}, got {t.dtype}")
+    if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+        want = ", ".join("*" if n is None else str(n) for n in shape)
+        raise ValueError(f"{name} must be [{want}], got shape {tuple(t.shape)}")
+    if t.stride(-1) != 1 and t.shape[-1] != 1:
+        raise ValueError(f"{name}'s last dimension must be packed, got strides {t.stride()}")
+    unit = 16 // t.element_size()
+    strides = [t.stride(d) if t.shape[d] != 1 else 0 for d in range(t.dim() - 1)]
+    if t.data_ptr() % 16 or any(s < 0 or s % unit for s in strides):
+        raise ValueError(f"{name} must start on a 16-byte bound with strides of multiples of {unit} elements, "
+                         f"got strides {t.stride()} at offset {t.data_ptr() % 16}")
+    return (t.data_ptr(), *strides)
+
+
+class _on:
+    """The device of `t` as the current one (a no-op where it is already)."""
+
+    def __init__(self, t: torch.Tensor):
+        self._guard = None if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+    def __enter__(self):
+        if self._guard is not None:
+            self._guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
+
+
+def _norm_args(x, w, residual, residual_out):
+    if not isinstance(x, torch.Tensor) or x.dim() != 2:
+        raise ValueError("x must be a 2-D tensor [M, K]")
+    M, K = x.shape
+    xp, xs = _rows(x, "x", (None, None))
+    wp = _dev(w, "w", torch.bfloat16, 1)
+    if w.shape[0] != K:
+        raise ValueError(f"w must be [{K}], got {tuple(w.shape)}")
+    rp, rs, ro = 0, 0, None
+    if residual is not None:
+        rp, rs = _rows(residual, "residual", (M, K))
+        ro = torch.empty((M, K), dtype=torch.bfloat16, device=x.device) if residual_out is None else residual_out
+        _out(ro, "residual_out", (M, K), torch.bfloat16, x.device)
+    elif residual_out is not None:
+        raise ValueError("residual_out needs a residual")
+    _same_device(x, w, residual)
+    return M, K, xp, xs or K, wp, rp, rs or K, ro
+
+
+def rms_norm(x: torch.Tensor, w: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6,
+             out: torch.Tensor | None = None, residual_out: torch.Tensor | None = None):
+    """(y, residual_out) bf16 [M, K]: y = s * rsqrt(mean(s^2) + eps) * w for s = x (+ residual).
+
+    The sum and the norm are fp32 (the norm is of the sum, not of its bf16
+    copy); residual_out is bf16(s), None without a residual.  x and residual
+    may be row slices of wider tensors; `out` may be x and `residual_out` the
+    residual itself (in place).  K % 8 == 0, K <= 32768.
+    """
+    r = _lib.native().rms_norm(x, w, residual, float(eps), out, residual_out)
+    if r is not None:
+        return r
+    M, K, xp, xs, wp, rp, rs, ro = _norm_args(x, w, residual, residual_out)
+    if out is None:
+        out = torch.empty((M, K), dtype=torch.bfloat16, device=x.device)
+    yp = _out(out, "out", (M, K), torch.bfloat16, x.device)
+    with _on(x):
+        rc = _lib.load().ferret_rms_norm(xp, xs, rp, rs, wp, eps, M, K, yp, ro.data_ptr() if ro is not None else 0,
+                                         _stream())
+    _lib.check("ferret_rms_norm", rc)
+    return out, ro
+
+
+def rms_norm_e4m3(x: torch.Tensor, w: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6,
+                  q: torch.Tensor | None = None, scale: torch.Tensor | None = None,
+                  residual_out: torch.Tensor | None = None):
+    """(q, scale, residual_out): rms_norm with its result as e4m3 codes [M, K] and fp32 scales
+    [M, K/128] by the 1x128 absmax/448 rule of quant_act_e4m3, taken of the fp32 result.  K % 128 == 0."""
+    r = _lib.native().rms_norm_e4m3(x, w, residual, float(eps), q, scale, residual_out)
+    if r is not None:
+        return r
+    M, K, xp, xs, wp, rp, rs, ro = _norm_args(x, w, residual, residual_out)
+    if q is None:
+        q = torch.empty((M, K), dtype=FP8, device=x.device)
+    if scale is None:
+        scale = torch.empty((M, K // 128), dtype=torch.float32, device=x.device)
+    qp = _out(q, "q", (M, K), (FP8, torch.uint8), x.device)
+    sp = _out(scale, "scale", (M, K // 128), torch.float32, x.device)
+    with _on(x):
+        rc = _lib.load().ferret_rms_norm_e4m3(xp, xs, rp, rs, wp, eps, M, K, qp, sp,
+                                              ro.data_ptr() if ro is not None else 0, _stream())
+    _lib.check("ferret_rms_norm_e4m3", rc)
+    return q, scale, ro
+
+
+LATENT, ROTARY = 512, 64          # a cached row: normed key-value latents and rotary key values
+_ROW = {torch.bfloat16: LATENT + ROTARY, torch.uint8: LATENT + 2 * ROTARY}
+
+
+@dataclass
+class LatentCache:
+    """A paged cache of latent rows (one per token: 512 latents, 64 rotary key values).
+
+    bf16: data [pages, page_size, 576], scales None.  e4m3: data uint8 [pages,
+    page_size, 640] (512 codes, then the rotary values as bf16) and scales uint8
+    [pages, page_size, 4], one exponent byte per 128 latents (byte b: 2^(b-127)).
+    """
+    data: torch.Tensor
+    scales: torch.Tensor | None = None
+
+    @classmethod
+    def empty(cls, num_pages: int, page_size: int, dtype=torch.bfloat16, device="cuda") -> "LatentCache":
+        """A cache of zeros; dtype torch.bfloat16 or torch.float8_e4m3fn."""
+        if dtype == torch.bfloat16:
+            return cls(torch.zeros((num_pages, page_size, LATENT + ROTARY), dtype=dtype, device=device))
+        if dtype == FP8:
+            return cls(torch.zeros((num_pages, page_size, LATENT + 2 * ROTARY), dtype=torch.uint8, device=device),
+                       torch.full((num_pages, page_size, LATENT // 128), 16, dtype=torch.uint8, device=device))
+        raise ValueError(f"a latent cache is bf16 or e4m3, got {dtype}")
+
+    @property
+    def num_pages(self) -> int:
+        return self.data.shape[0]
+
+    @property
+    def page_size(self) -> int:
+        return self.data.shape[1]
+
+
+def _latent_cache(cache) -> None:
+    if not isinstance(cache, LatentCache):
+        raise TypeError(f"cache must be a LatentCache, got {type(cache).__name__}")
+
+
+def _cache(cache: LatentCache, page_table: torch.Tensor, starts: torch.Tensor, name: str, lens=None):
+    """Checks of the cache and of a batch's index tensors: data, scales, pages, page_size, table, B, max_pages."""
+    data, scales = cache.data, cache.scales
+    dp = _dev(data, "cache.data", torch.bfloat16 if scales is None else torch.uint8, 3)
+    if data.shape[2] != _ROW[data.dtype]:
+        raise ValueError(f"cache.data must be [pages, page_size, {_ROW[data.dtype]}] for {data.dtype}, "
+                         f"got {tuple(data.shape)}")
+    if data.shape[1] < 16 or data.shape[1] % 16:
+        raise ValueError(f"page_size must be a multiple of 16, got {data.shape[1]}")
+    sp = 0
+    if scales is not None:
+        sp = _out(scales, "cache.scales", (*data.shape[:2], LATENT // 128), torch.uint8, data.device)
+    tp = _dev(page_table, "page_table", torch.int32, 2)
+    _dev(starts, name, torch.int32, 1)
+    B = starts.shape[0] - 1
+    if B < 1 or page_table.shape[0] != B:
+        raise ValueError(f"page_table must be [B, max_pages] and {name} [B + 1], got {tuple(page_table.shape)}, "
+                         f"{tuple(starts.shape)}")
+    if lens is not None:
+        _out(lens, "lens", (B,), torch.int32, data.device)
+    _same_device(data, scales, page_table, starts, lens)
+    return dp, sp, data.shape[0], data.shape[1], tp, B, page_table.shape[1]
+
+
+def latent_cache_write(cache: LatentCache, latent: torch.Tensor, rotary: torch.Tensor, page_table: torch.Tensor,
+                       lens: torch.Tensor, cu_q: torch.Tensor) -> None:
+    """Writes new tokens' rows into the cache: latent bf16 [T, 512] and rotary bf16 [T, 64]
+    (row slices of wider tensors allowed), packed by cu_q int32 [B+1], token i of
+    sequence b to position lens[b] - n + i of the pages that page_table [B,
+    max_pages] names.  Rows behind the last sequence, negative positions and
+    entries that are no page are dropped.  Pages that are written must belong to
+    one sequence.  e4m3 caches are quantised on the way (one power-of-two scale
+    per 128 latents, so that reading back is exact)."""
+    _latent_cache(cache)
+    if _lib.native().latent_cache_write(cache.data, cache.scales, latent, rotary, page_table, lens, cu_q):
+        return
+    dp, sp, pages, page_size, tp, B, max_pages = _cache(cache, page_table, cu_q, "cu_q", lens)
+    lp, ls = _rows(latent, "latent", (None, LATENT))
+    T = latent.shape[0]
+    rp, rs = _rows(rotary, "rotary", (T, ROTARY))
+    _same_device(cache.data, latent, rotary)
+    with _on(latent):
+        rc = _lib.load().ferret_latent_cache_write(lp, ls or LATENT, rp, rs or ROTARY, tp, lens.data_ptr(),
+                                                   cu_q.data_ptr(), B, max_pages, T, dp, sp, pages, page_size,
+                                                   _stream())
+    _lib.check("ferret_latent_cache_write", rc)
+
+
+def latent_cache_read(cache: LatentCache, page_table: torch.Tensor, cu_k: torch.Tensor, total: int,
+                      latent: torch.Tensor | None = None, rotary: torch.Tensor | None = None):
+    """(latent bf16 [total, 512], rotary bf16 [total, 64]): the first cu_k[b+1] - cu_k[b] rows of every
+    sequence, packed, exactly.  Rows behind cu_k[B] are left as they were (unset where
+    the outputs are new); rows of entries that are no page are zeros."""
+    _latent_cache(cache)
+    r = _lib.native().latent_cache_read(cache.data, cache.scales, page_table, cu_k, total, latent, rotary)
+    if r is not None:
+        return r
+    dp, sp, pages, page_size, tp, B, max_pages = _cache(cache, page_table, cu_k, "cu_k")
+    dev = cache.data.device
+    if latent is None:
+        latent = torch.empty((total, LATENT), dtype=torch.bfloat16, device=dev)
+    if rotary is None:
+        rotary = torch.empty((total, ROTARY), dtype=torch.bfloat16, device=dev)
+    lp = _out(latent, "latent", (total, LATENT), torch.bfloat16, dev)
+    rp = _out(rotary, "rotary", (total, ROTARY), torch.bfloat16, dev)
+    with _on(cache.data):
+        rc = _lib.load().ferret_latent_cache_read(dp, sp, pages, page_size, tp, cu_k.data_ptr(), B, max_pages, total,
+                                                  lp, rp, _stream())
+    _lib.check("ferret_latent_cache_read", rc)
+    return latent, rotary
+
+
+def latent_attention_workspace_bytes(num_sequences: int, num_tokens: int, num_heads: int) -> int:
+    """Bytes of the partial results that latent_attention joins."""
+    return int(_lib.load().ferret_latent_attention_workspace(num_sequences, num_tokens, num_heads))
+
+
+def latent_attention(q_latent: torch.Tensor, q_rotary: torch.Tensor, cache: LatentCache, page_table: torch.Tensor,
+                     lens: torch.Tensor, cu_q: torch.Tensor, scale: float, causal: bool = True,
+                     return_lse: bool = False, out: torch.Tensor | None = None,
+                     workspace: torch.Tensor | None = None):
+    """out bf16 [T, H, 512] (or (out, lse fp32 [T, H])): latent attention in its absorbed form over the paged cache.
+
+    q_latent bf16 [T, H, 512] (queries times the key projection) and q_rotary
+    bf16 [T, H, 64], any token and head strides; new tokens packed by cu_q, the
+    last of the lens[b] keys of their sequence, each seeing the keys up to its
+    own (causal) or all.  One token, several or a chunk of a prompt per
+    sequence.  Tokens that see no key get zeros (lse -inf); rows behind the last
+    sequence are left as they were (unset where `out` is new).  Work is dealt by
+    the lengths on the device: nothing is read back, a captured call replays
+    with other lengths.  `workspace` of latent_attention_workspace_bytes is
+    taken from torch's caching allocator unless one is passed; calls that
+    overlap in time (streams, graphs) need one each.
+    """
+    _latent_cache(cache)
+    r = _lib.native().latent_attention(q_latent, q_rotary, cache.data, cache.scales, page_table, lens, cu_q,
+                                       float(scale), bool(causal), bool(return_lse), out, workspace)
+    if r is not None:
+        return r
+    dp, sp, pages, page_size, tp, B, max_pages = _cache(cache, page_table, cu_q, "cu_q", lens)
+    lp, lt, lh = _rows(q_latent, "q_latent", (None, None, LATENT))
+    T, H = q_latent.shape[:2]
+    rp, rt, rh = _rows(q_rotary, "q_rotary", (T, H, ROTARY))
+    _same_device(cache.data, q_latent, q_rotary, out, workspace)
+    dev = q_latent.device
+    if out is None:
+        out = torch.empty((T, H, LATENT), dtype=torch.bfloat16, device=dev)
+    op = _out(out, "out", (T, H, LATENT), torch.bfloat16, dev)
+    lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
+    need = latent_attention_workspace_bytes(B, T, H)
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    with _on(q_latent):
+        rc = _lib.load().ferret_latent_attention(lp, lt, lh, rp, rt, rh, dp, sp, pages, page_size, tp, lens.data_ptr(),
+                                                 cu_q.data_ptr(), B, max_pages, T, H, scale, int(causal), op,
+                                                 lse.data_ptr() if lse is not None else 0,
+                                                 _dev(workspace, "workspace"), need, _stream())
+    _lib.check("ferret_latent_attention", rc)
+    return (out, lse) if return_lse else out
+
+
+def latent_attention_expanded(q_nope: torch.Tensor, q_rotary: torch.Tensor, k_nope: torch.Tensor,
+                              k_rotary: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
+                              scale: float, causal: bool = True, return_lse: bool = False,
+                              out: torch.Tensor | None = None):
+    """out bf16 [T, H, 128] (or (out, lse fp32 [T, H])): latent attention in its expanded form over ragged prompts.
+
+    q_nope bf16 [T, H, 128], q_rotary [T, H, 64], k_nope and v [S, H, 128] (the two
+    halves of a key-value projection of latent_cache_read's rows), k_rotary [S, 64]
+    shared by the heads; any strides but the last.  New tokens packed by cu_q
+    int32 [B+1], keys by cu_k; the n new tokens of a sequence are the last of its
+    keys, each seeing the keys up to its own (causal) or all.  Tokens that see
+    no key get zeros (lse -inf); rows behind the last sequence are left as they
+    were (unset where `out` is new).
+    """
+    r = _lib.native().latent_attention_expanded(q_nope, q_rotary, k_nope, k_rotary, v, cu_q, cu_k, float(scale),
+                                                bool(causal), bool(return_lse), out)
+    if r is not None:
+        return r
+    qp, qt, qh = _rows(q_nope, "q_nope", (None, None, 128))
+    T, H = q_nope.shape[:2]
+    rp, rt, rh = _rows(q_rotary, "q_rotary", (T, H, ROTARY))
+    kp, ks, kh = _rows(k_nope, "k_nope", (None, H, 128))
+    S = k_nope.shape[0]
+    krp, krs = _rows(k_rotary, "k_rotary", (S, ROTARY))
+    vp, vs, vh = _rows(v, "v", (S, H, 128))
+    cqp, ckp = _dev(cu_q, "cu_q", torch.int32, 1), _dev(cu_k, "cu_k", torch.int32, 1)
+    B = cu_q.shape[0] - 1
+    if B < 1 or cu_k.shape[0] != B + 1:
+        raise ValueError(f"cu_q and cu_k must both be [B + 1], got {tuple(cu_q.shape)}, {tuple(cu_k.shape)}")
+    _same_device(q_nope, q_rotary, k_nope, k_rotary, v, cu_q, cu_k, out)
+    dev = q_nope.device
+    if out is None:
+        out = torch.empty((T, H, 128), dtype=torch.bfloat16, device=dev)
+    op = _out(out, "out", (T, H, 128), torch.bfloat16, dev)
+    lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
+    with _on(q_nope):
+        rc = _lib.load().ferret_latent_attention_expanded(
+            qp, qt, qh, rp, rt, rh, kp, ks, kh, krp, krs, vp, vs, vh, cqp, ckp, B, T, S, H, scale, int(causal), op,
+            lse.data_ptr() if lse is not None else 0, _stream())
+    _lib.check("ferret_latent_attention_expanded", rc)
+    return (out, lse) if return_lse else out

@@ -201,5 +201,114 @@ def _(o, weights):
     return o.new_empty((weights.shape[0], o.shape[1]), dtype=torch.bfloat16)
 
 
+# ---- the attention block around the projections ------------------------------------------------------
+
+@torch.library.custom_op(f"{_NS}::rms_norm", mutates_args=())
+def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
+    """Root-mean-square norm of bf16 rows, bf16 out."""
+    return _ops.rms_norm(x, w, eps=eps)[0]
+
+
+@rms_norm.register_fake
+def _(x, w, eps=1e-6):
+    return x.new_empty(x.shape, dtype=torch.bfloat16)
+
+
+@torch.library.custom_op(f"{_NS}::add_rms_norm", mutates_args=())
+def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, w: torch.Tensor,
+                 eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
+    """(norm of x + residual, bf16(x + residual))."""
+    return _ops.rms_norm(x, w, residual, eps=eps)
+
+
+@add_rms_norm.register_fake
+def _(x, residual, w, eps=1e-6):
+    return x.new_empty(x.shape, dtype=torch.bfloat16), x.new_empty(x.shape, dtype=torch.bfloat16)
+
+
+@torch.library.custom_op(f"{_NS}::rms_norm_e4m3", mutates_args=())
+def rms_norm_e4m3(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
+    """rms_norm as e4m3 codes [M, K] and fp32 1x128 scales [M, K/128]."""
+    return _ops.rms_norm_e4m3(x, w, eps=eps)[:2]
+
+
+@rms_norm_e4m3.register_fake
+def _(x, w, eps=1e-6):
+    M, K = x.shape
+    return x.new_empty((M, K), dtype=FP8), x.new_empty((M, K // 128), dtype=torch.float32)
+
+
+@torch.library.custom_op(f"{_NS}::add_rms_norm_e4m3", mutates_args=())
+def add_rms_norm_e4m3(x: torch.Tensor, residual: torch.Tensor, w: torch.Tensor,
+                      eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """add_rms_norm with its norm as e4m3 codes and fp32 1x128 scales."""
+    return _ops.rms_norm_e4m3(x, w, residual, eps=eps)
+
+
+@add_rms_norm_e4m3.register_fake
+def _(x, residual, w, eps=1e-6):
+    M, K = x.shape
+    return (x.new_empty((M, K), dtype=FP8), x.new_empty((M, K // 128), dtype=torch.float32),
+            x.new_empty((M, K), dtype=torch.bfloat16))
+
+
+@torch.library.custom_op(f"{_NS}::latent_cache_write", mutates_args=("data", "scales"))
+def latent_cache_write(data: torch.Tensor, scales: torch.Tensor | None, latent: torch.Tensor, rotary: torch.Tensor,
+                       page_table: torch.Tensor, lens: torch.Tensor, cu_q: torch.Tensor) -> None:
+    """New tokens' rows into the paged latent cache (data, scales of an ops.LatentCache), in place."""
+    _ops.latent_cache_write(_ops.LatentCache(data, scales), latent, rotary, page_table, lens, cu_q)
+
+
+@latent_cache_write.register_fake
+def _(data, scales, latent, rotary, page_table, lens, cu_q):
+    return None
+
+
+@torch.library.custom_op(f"{_NS}::latent_cache_read", mutates_args=())
+def latent_cache_read(data: torch.Tensor, scales: torch.Tensor | None, page_table: torch.Tensor, cu_k: torch.Tensor,
+                      total: int) -> tuple[torch.Tensor, torch.Tensor]:
+    """(latent bf16 [total, 512], rotary bf16 [total, 64]) of a batch's cached rows, packed by cu_k."""
+    return _ops.latent_cache_read(_ops.LatentCache(data, scales), page_table, cu_k, total)
+
+
+@latent_cache_read.register_fake
+def _(data, scales, page_table, cu_k, total):
+    return (data.new_empty((total, _ops.LATENT), dtype=torch.bfloat16),
+            data.new_empty((total, _ops.ROTARY), dtype=torch.bfloat16))
+
+
+@torch.library.custom_op(f"{_NS}::latent_attention", mutates_args=())
+def latent_attention(q_latent: torch.Tensor, q_rotary: torch.Tensor, data: torch.Tensor, scales: torch.Tensor | None,
+                     page_table: torch.Tensor, lens: torch.Tensor, cu_q: torch.Tensor, scale: float,
+                     causal: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
+    """(out bf16 [T, H, 512], lse fp32 [T, H]): absorbed latent attention over the paged cache."""
+    return _ops.latent_attention(q_latent, q_rotary, _ops.LatentCache(data, scales), page_table, lens, cu_q, scale,
+                                 causal=causal, return_lse=True)
+
+
+@latent_attention.register_fake
+def _(q_latent, q_rotary, data, scales, page_table, lens, cu_q, scale, causal=True):
+    T, H, _ = q_latent.shape
+    return (q_latent.new_empty((T, H, _ops.LATENT), dtype=torch.bfloat16),
+            q_latent.new_empty((T, H), dtype=torch.float32))
+
+
+@torch.library.custom_op(f"{_NS}::latent_attention_expanded", mutates_args=())
+def latent_attention_expanded(q_nope: torch.Tensor, q_rotary: torch.Tensor, k_nope: torch.Tensor,
+                              k_rotary: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
+                              scale: float, causal: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
+    """(out bf16 [T, H, 128], lse fp32 [T, H]): expanded latent attention over ragged prompts."""
+    return _ops.latent_attention_expanded(q_nope, q_rotary, k_nope, k_rotary, v, cu_q, cu_k, scale, causal=causal,
+                                          return_lse=True)
+
+
+@latent_attention_expanded.register_fake
+def _(q_nope, q_rotary, k_nope, k_rotary, v, cu_q, cu_k, scale, causal=True):
+    T, H, _ = q_nope.shape
+    return q_nope.new_empty((T, H, 128), dtype=torch.bfloat16), q_nope.new_empty((T, H), dtype=torch.float32)
+
+
 OPS = ("linear_bf16", "fp8_gemm_blockscale", "fp8_gemm_ue8m0", "quant_act_e4m3", "moe_route_topk", "moe_permute",
-       "moe_w13_fp8", "moe_w13_w4a16", "int4_tile_weights", "moe_w2_fp8", "moe_combine")
+       "moe_w13_fp8", "moe_w13_w4a16", "int4_tile_weights", "moe_w2_fp8", "moe_combine", "rms_norm",
+       "add_rms_norm", "rms_norm_e4m3", "add_rms_norm_e4m3", "latent_cache_write", "latent_cache_read",
+       "latent_attention", "latent_attention_expanded")

@@ -30,6 +30,7 @@ extern "C" {
 #define FERRET_ERR_NULL (-1)      /* a required pointer is NULL */
 #define FERRET_ERR_SHAPE (-2)     /* sizes out of range / not supported */
 #define FERRET_ERR_WORKSPACE (-3) /* workspace missing or too small */
+#define FERRET_ERR_ALIGN (-4)     /* a pointer or stride off its bound */
 
 /* Library version string, e.g. "ferret-hip 0.1.0 gfx950". */
 const char* ferret_version(void);
@@ -265,6 +266,110 @@ int ferret_moe_w2_fp8(const void* h, const float* sh, const void* w, const float
  * this is the library's own contract.  Requirements: N % 8 == 0, 1 <= topk <= 64.
  */
 int ferret_moe_combine(const void* o, const float* w, int T, int topk, int N, void* y, void* stream);
+
+/*
+ * Root-mean-square norm of bf16 rows, with the residual's addition where one is
+ * given:  s = x + residual (fp32; residual_out = bf16_RNE(s)),
+ *   y = bf16_RNE(s * rsqrt(mean(s^2) + eps) * w).
+ * x [M,K] and residual [M,K] with rows x_stride / residual_stride elements apart
+ * (multiples of 8, so a slice of a wider projection needs no copy), w bf16 [K],
+ * y and residual_out bf16 [M,K] packed.  residual and residual_out are both given
+ * or both NULL.  An output may stand exactly on x or residual (in place); any
+ * other overlap is rejected.  The reference has no norm; this is the library's own
+ * contract.  Requirements: M >= 1, K % 8 == 0, K <= 32768, eps >= 0; pointers on
+ * 16-byte bounds (FERRET_ERR_ALIGN).
+ */
+int ferret_rms_norm(const void* x, long long x_stride, const void* residual, long long residual_stride,
+                    const void* w, float eps, int M, int K, void* y, void* residual_out, void* stream);
+
+/*
+ * ferret_rms_norm with y as the e4m3 codes q [M,K] and fp32 scales [M,K/128] that
+ * every FP8 entry point above takes: the rule of ferret_quant_act_e4m3 on the
+ * fp32 y (not on its bf16 rounding).  Requirements: as ferret_rms_norm, with
+ * K % 128 == 0; q on an 8-byte bound.
+ */
+int ferret_rms_norm_e4m3(const void* x, long long x_stride, const void* residual, long long residual_stride,
+                         const void* w, float eps, int M, int K, void* q, float* scale, void* residual_out,
+                         void* stream);
+
+/*
+ * The paged latent cache of the entry points below: `pages` pages of `page_size`
+ * rows (a multiple of 16), one row per token: 512 normed key-value latents and 64
+ * rotary key values.
+ *   scales == NULL: data bf16 [pages, page_size, 576];
+ *   else:           data bytes [pages, page_size, 640], 512 e4m3 codes, then the
+ *                   rotary values as bf16, and scales bytes [pages, page_size, 4],
+ *                   one per 128 latents: byte b stands for 2^(b - 127).
+ * page_table int32 [B, max_pages]: the pages of each sequence in order.  An entry
+ * outside [0, pages) stands for no page: nothing is written to it, zeros are read
+ * from it, attention leaves its keys out.  Lengths past max_pages * page_size are
+ * cut.  cu_q / cu_k int32 [B + 1] ascend from 0: the rows of sequence b among the
+ * packed new tokens or keys; packed rows behind the last sequence are left alone,
+ * on the input and on the output side.  lens int32 [B]: keys of a sequence, its new
+ * tokens included, which are the last of them.  All of these are device arrays and
+ * are read by the kernels only: a captured graph replays with other lengths.
+ *
+ * ferret_latent_cache_write: new token i of sequence b to position
+ * lens[b] - n + i (n = its number of new tokens; negative positions are dropped).
+ * latent bf16 [T,512], rotary bf16 [T,64], rows *_stride elements apart (multiples
+ * of 8).  e4m3: per 128 latents byte = max(127 + ceil(log2(max|x| / 448)), 16) over
+ * the finite values, code = e4m3_RNE(x * 2^(127 - byte)); Inf and NaN give the NaN
+ * code.  A row that two tokens of one call write (a page named by two sequences)
+ * ends as a mix of both: the pages that are written belong to one sequence.
+ *
+ * ferret_latent_cache_read: positions 0 .. cu_k[b+1] - cu_k[b] of every sequence to
+ * latent bf16 [rows,512] and rotary bf16 [rows,64], exactly (a code times its
+ * scale is a bf16 value).
+ */
+int ferret_latent_cache_write(const void* latent, long long latent_stride, const void* rotary,
+                              long long rotary_stride, const int32_t* page_table, const int32_t* lens,
+                              const int32_t* cu_q, int B, int max_pages, int T, void* data, void* scales,
+                              int pages, int page_size, void* stream);
+int ferret_latent_cache_read(const void* data, const void* scales, int pages, int page_size,
+                             const int32_t* page_table, const int32_t* cu_k, int B, int max_pages, int rows,
+                             void* latent, void* rotary, void* stream);
+
+/*
+ * Latent attention in its absorbed form over the paged cache:
+ *   s_ij = scale * (q_latent_i . latent_j + q_rotary_i . rotary_j),
+ *   out_i = sum_j softmax_j(s_ij) latent_j      (bf16 [T,H,512]),
+ * for every head of every new token i, over keys j <= lens[b] - n + i of its sequence
+ * (causal != 0) or all lens[b].  lse (optional) fp32 [T,H]: the logarithm of the
+ * sum of exp(s).  A token that sees no key gets zeros and -inf.  q_latent bf16
+ * [T,H,512] and q_rotary bf16 [T,H,64] with token and head strides in elements
+ * (multiples of 8).  Inf or NaN in rows that a token does not see do not reach it; a
+ * key whose score is -inf (an Inf among its latents) has no weight.
+ * ws: ferret_latent_attention_workspace(B, T, H) bytes, on a 16-byte bound; two
+ * calls that overlap in time need one each.  The result depends on the batch only
+ * through the order of fp32 additions; the same call gives the same bits.
+ * Requirements: T >= 1, 1 <= H <= 1024, 0 < scale < 1e30.
+ */
+size_t ferret_latent_attention_workspace(int B, int T, int H);
+int ferret_latent_attention(const void* q_latent, long long ql_token, long long ql_head, const void* q_rotary,
+                            long long qr_token, long long qr_head, const void* data, const void* scales,
+                            int pages, int page_size, const int32_t* page_table, const int32_t* lens,
+                            const int32_t* cu_q, int B, int max_pages, int T, int H, float scale, int causal,
+                            void* out, float* lse, void* ws, size_t ws_bytes, void* stream);
+
+/*
+ * Latent attention in its expanded form, for ragged prompts:
+ *   s_ij = scale * (q_nope_i . k_nope_j + q_rotary_i . k_rotary_j),
+ *   out_i = sum_j softmax_j(s_ij) v_j           (bf16 [T,H,128]),
+ * per head, over keys j <= len - n + i of the token's sequence (causal != 0; len
+ * keys, n new tokens, the last of them) or all len.  q_nope bf16 [T,H,128], q_rotary
+ * [T,H,64], k_nope and v [S,H,128], k_rotary [S,64] (one for all heads), with strides
+ * in elements (multiples of 8, < 2^24), so the key-value projection is taken as it
+ * is.  cu_q and cu_k int32 [B + 1] as above; rows behind the last sequence are left
+ * alone.  lse, tokens that see no key, and Inf or NaN that a token does not see: as
+ * ferret_latent_attention.  Requirements: B, T, S >= 1, 1 <= H <= 1024,
+ * 0 < scale < 1e30.
+ */
+int ferret_latent_attention_expanded(const void* q_nope, long long qn_token, long long qn_head,
+                                     const void* q_rotary, long long qr_token, long long qr_head,
+                                     const void* k_nope, long long kn_key, long long kn_head,
+                                     const void* k_rotary, long long kr_key, const void* v, long long v_key,
+                                     long long v_head, const int32_t* cu_q, const int32_t* cu_k, int B, int T,
+                                     int S, int H, float scale, int causal, void* out, float* lse, void* stream);
 
 /*
  * Flags of the FP8 *_ex entry points below.  FERRET_FP8_MMA_E4M3 multiplies
