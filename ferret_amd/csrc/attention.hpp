@@ -29,14 +29,15 @@ __device__ __forceinline__ u32x2 lds_tr8(const uint8_t* p) {
 // (an LDS address, the same in all lanes) from base + off.  Written as assembly
 // because the compiler, which tracks the builtin's loads, waits for all of them
 // before every transposing LDS read; the waits here are the kernel's own
-// (wait_vmcnt).  No register is loaded, so nothing of theirs can be reused early.
+// (wait_vmcnt).  No register is loaded, so nothing of theirs can be reused early; M0,
+// a register that the compiler reserves, has no other user in these kernels.
 __device__ __forceinline__ void dma_16(const uint8_t* base, int off, uint32_t lds_at) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds_at)
-               : "memory", "m0");
+               : "memory");
 }
 __device__ __forceinline__ void dma_4(const uint32_t* base, int off, uint32_t lds_at) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(lds_at)
-               : "memory", "m0");
+               : "memory");
 }
 __device__ __forceinline__ uint32_t lds_address(const uint8_t* p) { return (uint32_t)(uintptr_t)(FERRET_LDS uint8_t*)p; }
 

@@ -39,6 +39,7 @@ namespace ferret {
 namespace {
 
 constexpr int kKeys = kLatentKeys, kUnits = kLatentUnits;
+constexpr int kJoinRows = 256;  // rows up to which a row's pieces are joined by several work-groups
 constexpr int kAhead = 4;      // LDS fragments read ahead
 constexpr int kFence = 4;      // fragments between scheduling fences
 
@@ -53,11 +54,12 @@ struct Args {
   float scale_log2;  // scale * log2(e)
   int causal;
   int min_steps;
+  int side_by_side;  // row tiles of a sequence taken at the same time
   uint16_t* out;  // [T, H, 512]
   float* lse;     // [T, H] or null
   // The workspace: rows [T * H] (int4), then ml [2 * kUnits][MR] (m and l), then the
-  // partial outputs [2 * kUnits][MR][512].  A row's record is {first work-group,
-  // pieces, first slot odd, row in tile}.
+  // partial outputs [2 * kUnits][MR][512].  A row's record is {first slot, pieces, row
+  // in tile, -}.
   uint8_t* ws;
   __host__ __device__ int4* rows() const { return reinterpret_cast<int4*>(ws); }
   __host__ __device__ float2* ml() const {
@@ -68,7 +70,8 @@ struct Args {
 
 template <int MR>
 __device__ __forceinline__ LatentSeq sequence(const Args& a, int b) {
-  return latent_seq(a.cu_q[b], a.cu_q[b + 1], a.lens[b], a.T, a.H, MR, a.pages.max_pages * a.pages.page_size);
+  return latent_seq(a.cu_q[b], a.cu_q[b + 1], a.lens[b], a.T, a.H, MR, a.side_by_side,
+                    a.pages.max_pages * a.pages.page_size);
 }
 
 template <bool F8>
@@ -83,20 +86,52 @@ struct Tile {
   static constexpr int kVmem = 2 * kLoads + (F8 ? 1 : 0);  // loads of a wave per step
 };
 
-// What only the ends of a piece need, kept in LDS: scalar registers are short.
+// What only the ends of a piece need, the arguments among it, kept in LDS: scalar
+// registers are short.
 struct Side {
-  uint16_t* out;
-  float* lse;
-  float2* ml;
-  float* part;
-  int4* rows;
-  const uint16_t *ql, *qr;
-  int ql_t, ql_h, qr_t, qr_h;
+  Args args;
   int chunk, seq_at, b;  // the deal, the sequence at hand and its place on the line
+  LatentSeq seq;
   int first_row;         // the tile's first row among all [T * H]
   int slot;              // of the partial result, -1 for a whole tile
   int end;               // of this work-group's share of the line
 };
+
+// By fields: a struct's copy would stand in scratch memory.
+__device__ __forceinline__ void put_seq(LatentSeq* to, const LatentSeq& s) {
+  to->q0 = s.q0;
+  to->n = s.n;
+  to->len = s.len;
+  to->rows = s.rows;
+  to->groups = s.groups;
+  to->steps = s.steps;
+}
+__device__ __forceinline__ LatentSeq get_seq(const LatentSeq* from) {
+  return LatentSeq{from->q0, from->n, from->len, from->rows, from->groups, from->steps};
+}
+
+__device__ __forceinline__ void put_args(Args* to, const Args& a) {
+  to->ql = a.ql;
+  to->qr = a.qr;
+  to->ql_t = a.ql_t;
+  to->ql_h = a.ql_h;
+  to->qr_t = a.qr_t;
+  to->qr_h = a.qr_h;
+  to->pages.table = a.pages.table;
+  to->pages.max_pages = a.pages.max_pages;
+  to->pages.pages = a.pages.pages;
+  to->pages.page_size = a.pages.page_size;
+  to->lens = a.lens;
+  to->cu_q = a.cu_q;
+  to->B = a.B;
+  to->T = a.T;
+  to->H = a.H;
+  to->causal = a.causal;
+  to->side_by_side = a.side_by_side;
+  to->out = a.out;
+  to->lse = a.lse;
+  to->ws = a.ws;
+}
 
 // LDS after the tile buffers.
 template <int MR, bool F8>
@@ -132,14 +167,21 @@ __global__ __launch_bounds__(256, 1) void latent_attention_kernel(Args a) {
   float* const tops = reinterpret_cast<float*>(lds + M::kTop);
   Side* const side = reinterpret_cast<Side*>(lds + M::kSide);
 
-  // ---- this work-group's piece [start, end) of the line
+  // ---- this work-group's share of the line
+  const LatentPlace place = latent_place(blockIdx.x, a.side_by_side);
   int cur;
   {
-    int* tot = reinterpret_cast<int*>(lds);  // wave totals, then the sequence found and its place
+    // The page table's first lines come under the loads of the lengths.
+    const int near = a.pages.table[(long long)(place.unit * a.B / (kUnits / a.side_by_side)) * a.pages.max_pages];
+    int* tot = reinterpret_cast<int*>(lds);  // wave totals
     const int per = (a.B + 255) / 256;
     const int b0 = threadIdx.x * per;
+    LatentSeq s{};
     int mine = 0;
-    for (int i = 0; i < per && b0 + i < a.B; ++i) mine += sequence<MR>(a, b0 + i).work();
+    for (int i = 0; i < per && b0 + i < a.B; ++i) {
+      s = sequence<MR>(a, b0 + i);
+      mine += s.work();
+    }
     int incl = mine;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
@@ -148,44 +190,40 @@ __global__ __launch_bounds__(256, 1) void latent_attention_kernel(Args a) {
     }
     if (lane == 63) tot[wave] = incl;
     __syncthreads();
+    asm volatile("" ::"v"(near));
     int before = 0, total = 0;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       if (w < wave) before += tot[w];
       total += tot[w];
     }
-    const int chunk = latent_chunk(total, a.min_steps);
-    const int start = (int)min((long long)blockIdx.x * chunk, (long long)total);
+    const int chunk = latent_chunk(total, kUnits / a.side_by_side, a.min_steps);
+    const int start = (int)min((long long)place.unit * chunk, (long long)total);
     const int excl = before + incl - mine;
     if (start >= total) return;
     if (excl <= start && start < excl + mine) {
-      int at = excl;
-      for (int i = 0; i < per; ++i) {
-        const int w = sequence<MR>(a, b0 + i).work();
-        if (start < at + w) {
-          side->b = b0 + i;
-          side->seq_at = at;
-          side->chunk = chunk;
-          side->end = min(start + chunk, total);
-          side->out = a.out;
-          side->lse = a.lse;
-          side->rows = a.rows();
-          side->ml = a.ml();
-          side->part = a.part(MR);
-          side->ql = a.ql;
-          side->qr = a.qr;
-          side->ql_t = a.ql_t;
-          side->ql_h = a.ql_h;
-          side->qr_t = a.qr_t;
-          side->qr_h = a.qr_h;
-          break;
+      int at = excl, i = 0;
+      if (per > 1)
+        for (;; ++i) {
+          s = sequence<MR>(a, b0 + i);
+          if (start < at + s.work() || i + 1 == per) break;
+          at += s.work();
         }
-        at += w;
-      }
+      side->b = b0 + i;
+      put_seq(&side->seq, s);
+      side->seq_at = at;
+      side->chunk = chunk;
+      side->end = min(start + chunk, total);
+      put_args(&side->args, a);
     }
     cur = uniform(start);
     __syncthreads();
   }
+
+  const Args& in = side->args;
+  const uint8_t* const data = a.data;
+  const uint32_t* const scales = a.scales;
+  const float scale_log2 = a.scale_log2;
 
   // ---- lane constants
   int load_off[L::kLoads];  // source bytes within a group of 8 rows, even group
@@ -197,32 +235,37 @@ __global__ __launch_bounds__(256, 1) void latent_attention_kernel(Args a) {
 
   while (cur < uniform(side->end)) {
     int b = uniform(side->b), seq_at = uniform(side->seq_at);
-    LatentSeq s = sequence<MR>(a, b);
-    while (cur >= seq_at + s.work() && b + 1 < a.B) {  // the next sequence with rows
+    LatentSeq s = get_seq(&side->seq);
+    while (cur >= seq_at + s.work() && b + 1 < in.B) {  // the next sequence with rows
       seq_at += s.work();
-      s = sequence<MR>(a, ++b);
+      s = sequence<MR>(in, ++b);
     }
     b = uniform(b);
     const int len = uniform(s.len), steps = uniform(s.steps), q0 = uniform(s.q0);
-    const int tile = uniform((cur - seq_at) / steps), s0 = uniform(cur - seq_at - tile * steps);
+    const int group = uniform((cur - seq_at) / steps), s0 = uniform(cur - seq_at - group * steps);
     const int s1 = uniform(min(steps, s0 + (side->end - cur)));
-    const int row0 = tile * MR, row_last = uniform(min(row0 + MR, s.rows) - 1);
+    const int row0 = (group * in.side_by_side + place.lane) * MR, row_last = uniform(min(row0 + MR, s.rows) - 1);
+    if (row_last < row0) {  // fewer tiles than work-groups side by side
+      cur += s1 - s0;
+      continue;
+    }
     // keys seen by the first and by the last token of the tile
     const int past = len - uniform(s.n) + 1;
-    const int see_all = uniform(max(a.causal ? past + row0 / a.H : len, 0));
-    const int see_any = uniform(max(a.causal ? past + row_last / a.H : len, 0));
+    const int see_all = uniform(max(in.causal ? past + row0 / in.H : len, 0));
+    const int see_any = uniform(max(in.causal ? past + row_last / in.H : len, 0));
     const int last = min(s1, (see_any + kKeys - 1) / kKeys);
-    const int chunk = side->chunk, first_row = q0 * a.H + row0;
+    const int chunk = side->chunk, first_row = q0 * in.H + row0;
     __syncthreads();  // the piece before is done with its record and buffers
     if (threadIdx.x == 0) {
       side->b = b;
+      put_seq(&side->seq, s);
       side->seq_at = seq_at;
       side->first_row = first_row;
-      side->slot = s0 == 0 && s1 == steps ? -1 : latent_slot(blockIdx.x, cur, chunk);
+      side->slot = s0 == 0 && s1 == steps ? -1 : latent_slot(place.unit, place.lane, in.side_by_side, cur, chunk);
     }
     if (s0 == 0 && (int)threadIdx.x <= row_last - row0) {  // where the pieces of this tile's rows stand
-      const LatentRecord r = latent_record(blockIdx.x, cur, steps, chunk);
-      side->rows[first_row + threadIdx.x] = make_int4(r.block, r.pieces, r.odd, threadIdx.x);
+      const LatentRecord r = latent_record(place.unit, place.lane, in.side_by_side, cur, steps, chunk);
+      in.rows()[first_row + threadIdx.x] = make_int4(r.slot0, r.pieces, threadIdx.x, 0);
     }
 
     f32x4 o[CT][MF];
@@ -237,21 +280,30 @@ __global__ __launch_bounds__(256, 1) void latent_attention_kernel(Args a) {
 #pragma unroll
       for (int c = 0; c < CT; ++c) o[c][f] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    // Step t's rows into its buffer: this wave's 16 of the 64.  The page table is read
-    // by scalar loads, which the count of vector loads in flight does not see.
-    const auto* table = (const __attribute__((address_space(4))) int32_t*)(a.pages.table +
-                                                                          (long long)b * a.pages.max_pages);
-    auto issue = [&](int t) {
+    // The page table, 64 steps at a time: lane i holds where the wave's 16 rows of step
+    // held + i stand, in units of 16 rows, -1 where they have no page.
+    const int32_t* table = in.pages.table + (long long)b * in.pages.max_pages;
+    int held = s0, where;
+    const auto look_up = [&]() __attribute__((always_inline)) {
+      const int pos = min(held + lane, last - 1) * kKeys + wave * 16;  // last > s0, or nothing is issued
+      const int page = pos / in.pages.page_size;
+      const int id = pos >= 0 && page < in.pages.max_pages ? table[page] : -1;
+      const long long row = page_row(id, in.pages.pages, in.pages.page_size, pos - page * in.pages.page_size);
+      where = row < 0 ? -1 : (int)(row >> 4);
+    };
+    look_up();
+
+    const auto issue = [&](int t) __attribute__((always_inline)) {
       uint8_t* buf = lds + (t % L::kBufs) * L::kBytes;
-      const int pos = t * kKeys + wave * 16;
-      const int page = uniform(pos / a.pages.page_size);
-      int id = -1;
-      if (page < a.pages.max_pages) id = table[page];
-      const long long at = page_row(id, a.pages.pages, a.pages.page_size, pos - page * a.pages.page_size);
+      if (t == held + 64) {
+        held = t;
+        look_up();
+      }
+      const int at = __builtin_amdgcn_readlane(where, t - held);
       const bool ok = at >= 0;
-      const long long row = ok ? at : 0;  // some row: masked
+      const long long row = ok ? (long long)at << 4 : 0;  // some row: masked
       if (lane == 0) lds[M::kValid + (t % L::kBufs) * 4 + wave] = ok ? 1 : 0;
-      const uint8_t* src = a.data + row * L::kRowB;
+      const uint8_t* src = data + row * L::kRowB;
       const uint32_t dst = uniform(lds_address(buf) + wave * 16 * L::kRowB);
 #pragma unroll
       for (int j = 0; j < L::kLoads; ++j) dma_16(src, load_off[j], dst + j * 1024);
@@ -259,14 +311,8 @@ __global__ __launch_bounds__(256, 1) void latent_attention_kernel(Args a) {
       for (int j = 0; j < L::kLoads; ++j)  // the odd group: one bit of the swizzle differs
         dma_16(src + 8 * L::kRowB, load_off[j] ^ 64, dst + 8 * L::kRowB + j * 1024);
       if constexpr (F8)
-        if (lane < 16) dma_4(a.scales + row, lane * 4, uniform(lds_address(buf) + L::kData + wave * 64));
+        if (lane < 16) dma_4(scales + row, lane * 4, uniform(lds_address(buf) + L::kData + wave * 64));
     };
-
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int i = 0; i < L::kBufs - 1; ++i)
-      if (s0 + i < last) issue(s0 + i);
-    __builtin_amdgcn_sched_barrier(0);
 
     // ---- queries: B fragments (rows past the tile's repeat its last one)
     u32x4 qf[QF][18];
@@ -274,16 +320,21 @@ __global__ __launch_bounds__(256, 1) void latent_attention_kernel(Args a) {
 #pragma unroll
     for (int f = 0; f < QF; ++f) {
       const int r = row0 + (wq * QF + f) * 16 + r16;
-      const int rc = min(r, row_last), tok = rc / a.H, head = rc - tok * a.H;
-      sees[f] = r <= row_last ? max(a.causal ? past + tok : len, 0) : 0;
-      const uint16_t* ql = side->ql + (long long)(q0 + tok) * side->ql_t + (long long)head * side->ql_h;
-      const uint16_t* qr = side->qr + (long long)(q0 + tok) * side->qr_t + (long long)head * side->qr_h;
+      const int rc = min(r, row_last), tok = rc / in.H, head = rc - tok * in.H;
+      sees[f] = r <= row_last ? max(in.causal ? past + tok : len, 0) : 0;
+      const uint16_t* ql = in.ql + (long long)(q0 + tok) * in.ql_t + (long long)head * in.ql_h;
+      const uint16_t* qr = in.qr + (long long)(q0 + tok) * in.qr_t + (long long)head * in.qr_h;
 #pragma unroll
       for (int k = 0; k < 16; ++k)
         qf[f][k] = ld_u32x4(ql + (F8 ? 64 * (k >> 1) + 16 * g + 8 * (k & 1) : 32 * k + 8 * g));
 #pragma unroll
       for (int k = 0; k < 2; ++k) qf[f][16 + k] = ld_u32x4(qr + 32 * k + 8 * g);
     }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < L::kBufs - 1; ++i)
+      if (s0 + i < last) issue(s0 + i);
+    __builtin_amdgcn_sched_barrier(0);
     wait_vmcnt<0>();  // the queries, so that no wait for them stands in the loop; the first steps come with them
     __builtin_amdgcn_sched_barrier(0);
 
@@ -405,7 +456,7 @@ __global__ __launch_bounds__(256, 1) void latent_attention_kernel(Args a) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) v = fmaxf(v, sc[k][f][i]);
         v = fmaxf(v, __shfl_xor(v, 16, 64));
-        v = fmaxf(v, __shfl_xor(v, 32, 64)) * a.scale_log2;
+        v = fmaxf(v, __shfl_xor(v, 32, 64)) * scale_log2;
         move = move || v > m[f] + kLazy;  // from -inf: any finite score
         if (g == 0) tops[wk * MR + (wq * QF + f) * 16 + r16] = v;
       }
@@ -423,7 +474,7 @@ __global__ __launch_bounds__(256, 1) void latent_attention_kernel(Args a) {
             f32x4 p;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              p[i] = __builtin_amdgcn_exp2f(fmaf(sc[k][f][i], a.scale_log2, -base));
+              p[i] = __builtin_amdgcn_exp2f(fmaf(sc[k][f][i], scale_log2, -base));
               pend[f] += p[i];
             }
             const int kb = wk * KT + k;  // 16-key block of the step: 2 chunks
@@ -542,18 +593,18 @@ __global__ __launch_bounds__(256, 1) void latent_attention_kernel(Args a) {
         if (slot < 0) {
           const long long at = side->first_row + r;
           const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          uint16_t* to = side->out + at * kLatent + col;
+          uint16_t* to = in.out + at * kLatent + col;
 #pragma unroll
           for (int c = 0; c < CT; ++c)
             *reinterpret_cast<u32x2*>(to + c * 16) =
                 u32x2{pack_bf16x2(o[c][f][0] * inv, o[c][f][1] * inv), pack_bf16x2(o[c][f][2] * inv, o[c][f][3] * inv)};
-          if (wave == 0 && g == 0 && side->lse != nullptr)
-            side->lse[at] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+          if (wave == 0 && g == 0 && in.lse != nullptr)
+            in.lse[at] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
         } else {
           const long long at = (long long)slot * MR + r;
-          if (wave == 0 && g == 0) side->ml[at] = make_float2(top, sum);
+          if (wave == 0 && g == 0) in.ml()[at] = make_float2(top, sum);
           if (last > s0) {
-            float* to = side->part + at * kLatent + col;
+            float* to = in.part(MR) + at * kLatent + col;
 #pragma unroll
             for (int c = 0; c < CT; ++c) *reinterpret_cast<f32x4*>(to + c * 16) = o[c][f];
           }
@@ -565,60 +616,107 @@ __global__ __launch_bounds__(256, 1) void latent_attention_kernel(Args a) {
   }
 }
 
-// Joins the pieces of the query rows that were cut.  COLS columns of a row per
-// 256 threads: COLS / 4 lanes across, the pieces dealt to 1024 / COLS groups.
-template <int COLS>
-__global__ __launch_bounds__(256) void latent_join_kernel(Args a, int mr) {
-  constexpr int LANES = COLS / 4, GROUPS = 256 / LANES;
-  __shared__ f32x4 red[256];
-  __shared__ float stat[8];
-  const long long row = blockIdx.x;
-  // rows behind the last sequence have no record
-  if (row < (long long)max(a.cu_q[0], 0) * a.H || row >= (long long)min(a.cu_q[a.B], a.T) * a.H) return;
-  const int4 rec = a.rows()[row];
-  const float2* ml = a.ml();
-  const float* part = a.part(mr);
-  const LatentRecord where{rec.x, rec.y, rec.z};
-  const int pieces = rec.y;
-  if (!latent_record_joins(where) || (unsigned)rec.w >= (unsigned)mr) return;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const auto slot_row = [&](int j) { return (long long)latent_record_slot(where, j) * mr + rec.w; };
-  float top = -INFINITY;
-  for (int j = threadIdx.x; j < pieces; j += 256) top = fmaxf(top, ml[slot_row(j)].x);
+// Joins the pieces of the query rows that were cut, in the order of the keys.
+
+// The record of a row; false where nothing is to be joined.
+__device__ __forceinline__ bool to_join(const Args& a, int mr, long long row, LatentRecord* where, int* r) {
+  const int4 rec = a.rows()[row];  // rows behind the last sequence have none: whatever stands there
+  *where = LatentRecord{rec.x, rec.y};
+  *r = rec.z;
+  return row >= (long long)max(a.cu_q[0], 0) * a.H && row < (long long)min(a.cu_q[a.B], a.T) * a.H &&
+         latent_record_joins(*where, a.side_by_side) && (unsigned)rec.z < (unsigned)mr;
+}
+
+__device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  for (int off = 32; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+  return v;
+}
+__device__ __forceinline__ float wave_add(float v) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+
+// Many rows, few pieces each: a wave per row, 8 columns per lane, the pieces' weights
+// 64 at a time in the lanes.
+__global__ __launch_bounds__(256) void latent_join_kernel(Args a, int mr, int rows) {
+  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (row >= rows) return;
+  LatentRecord where;
+  int r;
+  if (!to_join(a, mr, row, &where, &r)) return;
+  const float2* ml = a.ml();
+  const float* part = a.part(mr) + lane * 4;
+  const auto at = [&](int j) { return (long long)latent_record_slot(where, a.side_by_side, j) * mr + r; };
+  float top = -INFINITY;
+  for (int j = lane; j < where.pieces; j += 64) top = fmaxf(top, ml[at(j)].x);
+  top = wave_max(top);
+  const float base = top == -INFINITY ? 0.f : top;
+  f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  float sum = 0.f;
+  for (int j0 = 0; j0 < where.pieces; j0 += 64) {
+    const float2 v = j0 + lane < where.pieces ? ml[at(j0 + lane)] : make_float2(-INFINITY, 0.f);
+    // l may be NaN where the maximum is -inf; there and only there O is not written, or zero
+    sum += v.y != 0.f ? v.y * __builtin_amdgcn_exp2f(v.x - base) : 0.f;
+    const float w = v.x > -INFINITY ? __builtin_amdgcn_exp2f(v.x - base) : 0.f;
+#pragma unroll 4
+    for (int j = 0; j < min(where.pieces - j0, 64); ++j) {
+      const float wj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), j));
+      if (wj != 0.f) {
+        const float* from = part + at(j0 + j) * kLatent;
+        acc[0] += *reinterpret_cast<const f32x4*>(from) * wj;
+        acc[1] += *reinterpret_cast<const f32x4*>(from + 256) * wj;
+      }
+    }
+  }
+  sum = wave_add(sum);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    *reinterpret_cast<u32x2*>(a.out + (long long)row * kLatent + h * 256 + lane * 4) =
+        u32x2{pack_bf16x2(acc[h][0] * inv, acc[h][1] * inv), pack_bf16x2(acc[h][2] * inv, acc[h][3] * inv)};
+  if (a.lse != nullptr && lane == 0)
+    a.lse[row] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+// Few rows, up to kUnits pieces each: a work-group per row and 64 columns, 16 lanes
+// across and the pieces dealt to 16 groups of lanes.
+__global__ __launch_bounds__(256) void latent_join_long_kernel(Args a, int mr) {
+  __shared__ f32x4 red[256];
+  __shared__ float weight[kUnits], stat[8];
+  const int row = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  LatentRecord where;
+  int r;
+  if (!to_join(a, mr, row, &where, &r)) return;
+  const auto at = [&](int j) { return (long long)latent_record_slot(where, a.side_by_side, j) * mr + r; };
+  const float2 v = (int)threadIdx.x < where.pieces ? a.ml()[at(threadIdx.x)] : make_float2(-INFINITY, 0.f);
+  float top = wave_max(v.x);
   if (lane == 0) stat[wave] = top;
   __syncthreads();
   top = fmaxf(fmaxf(stat[0], stat[1]), fmaxf(stat[2], stat[3]));
-  float sum = 0.f;
   const float base = top == -INFINITY ? 0.f : top;
-  for (int j = threadIdx.x; j < pieces; j += 256) {
-    const float2 v = ml[slot_row(j)];
-    if (v.y != 0.f) sum += v.y * __builtin_amdgcn_exp2f(v.x - base);  // NaN too: its maximum may be -inf
-  }
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+  // l may be NaN where the maximum is -inf; there and only there O is not written, or zero
+  float sum = wave_add(v.y != 0.f ? v.y * __builtin_amdgcn_exp2f(v.x - base) : 0.f);
+  weight[threadIdx.x] = v.x > -INFINITY ? __builtin_amdgcn_exp2f(v.x - base) : 0.f;
   if (lane == 0) stat[4 + wave] = sum;
   __syncthreads();
   sum = (stat[4] + stat[5]) + (stat[6] + stat[7]);
-  const int across = threadIdx.x % LANES, group = threadIdx.x / LANES;
-  const int col = blockIdx.y * COLS + across * 4;
+  const int across = threadIdx.x & 15, group = threadIdx.x >> 4, col = blockIdx.y * 64 + across * 4;
+  const float* part = a.part(mr) + col;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  if (top > -INFINITY) {
-#pragma unroll 4
-    for (int j = group; j < pieces; j += GROUPS) {
-      const long long at = slot_row(j);
-      const float mj = ml[at].x;
-      if (mj > -INFINITY) acc += *reinterpret_cast<const f32x4*>(part + at * kLatent + col) *
-                                 __builtin_amdgcn_exp2f(mj - top);
-    }
+#pragma unroll 8
+  for (int j = group; j < where.pieces; j += 16) {
+    const float w = weight[j];
+    if (w != 0.f) acc += *reinterpret_cast<const f32x4*>(part + at(j) * kLatent) * w;
   }
   red[threadIdx.x] = acc;
   __syncthreads();
   if (group != 0) return;
-  for (int i = 1; i < GROUPS; ++i) acc += red[i * LANES + across];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) acc += red[i * 16 + across];
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  *reinterpret_cast<u32x2*>(a.out + row * kLatent + col) =
+  *reinterpret_cast<u32x2*>(a.out + (long long)row * kLatent + col) =
       u32x2{pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv)};
   if (a.lse != nullptr && col == 0)
     a.lse[row] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
@@ -631,10 +729,10 @@ int launch(const Args& a, hipStream_t st) {
   hipLaunchKernelGGL((latent_attention_kernel<QF, WQ, F8>), dim3(kUnits), dim3(256), lds, st, a);
   FERRET_HIP_CHECK(hipGetLastError());
   const unsigned rows = (unsigned)((long long)a.T * a.H);
-  if (rows <= 1024)
-    hipLaunchKernelGGL((latent_join_kernel<128>), dim3(rows, 4), dim3(256), 0, st, a, mr);
+  if (rows <= kJoinRows)
+    hipLaunchKernelGGL(latent_join_long_kernel, dim3(rows, kLatent / 64), dim3(256), 0, st, a, mr);
   else
-    hipLaunchKernelGGL((latent_join_kernel<512>), dim3(rows, 1), dim3(256), 0, st, a, mr);
+    hipLaunchKernelGGL(latent_join_kernel, dim3((rows + 3) / 4), dim3(256), 0, st, a, mr, (int)rows);
   return (int)hipGetLastError();
 }
 
@@ -651,6 +749,12 @@ int launch_rows(int mr, const Args& a, hipStream_t st) {
 int tile_rows(int T, int B, int H) {
   const long long rows = (long long)T * H / B;
   return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+}
+
+// Row tiles side by side by the tiles that a sequence has on average.
+int side_by_side(int T, int B, int H) {
+  const long long tiles = (long long)T * H / B / 64;
+  return tiles < 2 ? 1 : tiles < 4 ? 2 : tiles < 8 ? 4 : 8;
 }
 
 }  // namespace
@@ -685,6 +789,7 @@ extern "C" int ferret_latent_attention(const void* q_latent, long long ql_token,
                  FERRET_ERR_ALIGN);
   const int mr = tile_rows(T, B, H);
   // steps of the whole batch are counted in 32 bits
+  FERRET_REQUIRE((long long)pages * page_size < (1LL << 35), FERRET_ERR_SHAPE);
   const long long tiles = (long long)T * H / mr + B, most = ((long long)max_pages * page_size + kKeys - 1) / kKeys;
   FERRET_REQUIRE(tiles * most < (1LL << 31), FERRET_ERR_SHAPE);
   FERRET_REQUIRE(ws != nullptr && ws_bytes >= ferret_latent_attention_workspace(B, T, H) && (bits(ws) & 15) == 0,
@@ -707,6 +812,7 @@ extern "C" int ferret_latent_attention(const void* q_latent, long long ql_token,
   a.scale_log2 = scale * kLog2e;
   a.causal = causal != 0;
   a.min_steps = 2;
+  a.side_by_side = side_by_side(T, B, H);
   a.out = static_cast<uint16_t*>(out);
   a.lse = lse;
   a.ws = static_cast<uint8_t*>(ws);

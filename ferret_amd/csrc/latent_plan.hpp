@@ -26,47 +26,62 @@ FERRET_HD long long page_row(int id, int pages, int page_size, int offset) {
 }
 
 // The work of one sequence: query rows (token-major, then heads) in tiles of `mr`,
-// keys in steps.  Index values outside the tensors are cut to them.
+// `side` of which are taken side by side (each by a work-group of its own, over the
+// same keys at the same time) as one group; keys in steps.  Index values outside the
+// tensors are cut to them.
 struct LatentSeq {
-  int q0, n, len, rows, tiles, steps;
-  FERRET_HD int work() const { return tiles * steps; }
+  int q0, n, len, rows, groups, steps;
+  FERRET_HD int work() const { return groups * steps; }
 };
 
-FERRET_HD LatentSeq latent_seq(int start, int end, int len, int T, int H, int mr, int most_keys) {
+FERRET_HD LatentSeq latent_seq(int start, int end, int len, int T, int H, int mr, int side, int most_keys) {
   LatentSeq s;
   s.q0 = plan_min(plan_max(start, 0), T);
   s.n = plan_min(plan_max(end, s.q0), T) - s.q0;
   s.len = plan_min(plan_max(len, 0), most_keys);
   s.rows = s.n * H;
-  s.tiles = (s.rows + mr - 1) / mr;
+  s.groups = (s.rows + mr * side - 1) / (mr * side);
   s.steps = plan_max((s.len + kLatentKeys - 1) / kLatentKeys, 1);  // an empty sequence's rows are written too
   return s;
 }
 
-// Steps per work-group of a line of `total`.
-FERRET_HD int latent_chunk(int total, int min_steps) {
-  return plan_max(min_steps, (total + kLatentUnits - 1) / kLatentUnits);
+// The line of all (sequence, group, step) is dealt in equal shares to `units` =
+// kLatentUnits / side units of `side` work-groups.  Steps per unit of a line of `total`:
+FERRET_HD int latent_chunk(int total, int units, int min_steps) {
+  return plan_max(min_steps, (total + units - 1) / units);
 }
 
-// The slot of the partial result that work-group `block` takes up at `cur` of the
-// line: its share may start and end inside a tile, so it has two.
-FERRET_HD int latent_slot(int block, int cur, int chunk) { return 2 * block + (cur > block * chunk ? 1 : 0); }
-
-// Where the pieces of a tile stand that work-group `block` begins at `cur`: the first
-// in its slot `odd`, the others each in the even slot of the next work-group.
-struct LatentRecord {
-  int block, pieces, odd;
+// The unit and the place in it of a work-group.  Work-groups are dealt to the 8 XCDs
+// in turn; a unit's stay on one, so that its keys come from memory once.
+struct LatentPlace {
+  int unit, lane;
 };
-FERRET_HD LatentRecord latent_record(int block, int cur, int steps, int chunk) {
-  return LatentRecord{block, (cur + steps - 1) / chunk - block + 1, cur > block * chunk ? 1 : 0};
+FERRET_HD LatentPlace latent_place(int block, int side) {
+  return LatentPlace{block / (8 * side) * 8 + block % 8, block / 8 % side};
 }
-FERRET_HD int latent_record_slot(const LatentRecord& r, int piece) {
-  return 2 * (r.block + piece) + (piece == 0 && r.odd != 0 ? 1 : 0);
+
+// The slot of the partial result that a unit's work-group takes up at `cur` of the
+// line: the share may start and end inside a tile, so there are two each.
+FERRET_HD int latent_slot(int unit, int lane, int side, int cur, int chunk) {
+  return 2 * (unit * side + lane) + (cur > unit * chunk ? 1 : 0);
+}
+
+// Where the pieces of a tile stand that `unit` begins at `cur`: the first in its slot
+// `odd`, the others each in the even slot of the next unit.  slot0 is the first's.
+struct LatentRecord {
+  int slot0, pieces;
+};
+FERRET_HD LatentRecord latent_record(int unit, int lane, int side, int cur, int steps, int chunk) {
+  return LatentRecord{latent_slot(unit, lane, side, cur, chunk), (cur + steps - 1) / chunk - unit + 1};
+}
+FERRET_HD int latent_record_slot(const LatentRecord& r, int side, int piece) {
+  return piece == 0 ? r.slot0 : (r.slot0 & ~1) + 2 * side * piece;
 }
 // More than one piece, all of them inside the workspace (a row that no sequence
 // covers has no record, and whatever stands there must lead nowhere else).
-FERRET_HD bool latent_record_joins(const LatentRecord& r) {
-  return r.pieces >= 2 && r.pieces <= kLatentUnits && (unsigned)r.block <= (unsigned)(kLatentUnits - r.pieces);
+FERRET_HD bool latent_record_joins(const LatentRecord& r, int side) {
+  return r.pieces >= 2 && r.pieces <= kLatentUnits && (unsigned)r.slot0 < (unsigned)(2 * kLatentUnits) &&
+         (r.slot0 | 1) + 2 * side * (r.pieces - 1) < 2 * kLatentUnits;
 }
 
 }  // namespace ferret

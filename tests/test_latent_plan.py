@@ -18,6 +18,7 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "ferret_amd", "csrc")
 
 WALKER = r"""
+#include <algorithm>
 #include <cstdio>
 #include <cstdlib>
 #include <map>
@@ -31,23 +32,29 @@ using namespace ferret;
 static long long bad = 0, walked = 0;
 #define CHECK(c) do { if (!(c) && bad++ < 20) std::printf("line %d: %s\n", __LINE__, #c); } while (0)
 
-static void walk(const std::vector<int>& cu, const std::vector<int>& lens, int T, int H, int mr, int most, int min_steps) {
-  const int B = (int)lens.size();
-  auto seq = [&](int b) { return latent_seq(cu[b], cu[b + 1], lens[b], T, H, mr, most); };
+static void walk(const std::vector<int>& cu, const std::vector<int>& lens, int T, int H, int mr, int side, int most,
+                 int min_steps) {
+  const int B = (int)lens.size(), units = kLatentUnits / side;
+  auto seq = [&](int b) { return latent_seq(cu[b], cu[b + 1], lens[b], T, H, mr, side, most); };
   int total = 0;
   for (int b = 0; b < B; ++b) {
     const LatentSeq s = seq(b);
     CHECK(s.q0 >= 0 && s.n >= 0 && s.q0 + s.n <= T && s.len >= 0 && s.len <= most && s.steps >= 1);
-    CHECK((long long)s.tiles * mr >= s.rows && (s.tiles == 0 || (s.tiles - 1) * mr < s.rows));
+    CHECK((long long)s.groups * mr * side >= s.rows && (s.groups == 0 || (s.groups - 1) * mr * side < s.rows));
     total += s.work();
   }
-  const int chunk = latent_chunk(total, min_steps);
+  const int chunk = latent_chunk(total, units, min_steps);
+  long long expected = 0;
   std::set<std::tuple<int, int, int>> done;
   std::map<std::pair<int, int>, std::vector<std::pair<int, int>>> pieces;  // tile -> (first step, slot)
   std::map<std::pair<int, int>, LatentRecord> records;
   std::set<int> slots;
+  std::set<std::pair<int, int>> places;
   for (int block = 0; block < kLatentUnits; ++block) {
-    const int start = (int)((long long)block * chunk < total ? (long long)block * chunk : total);
+    const LatentPlace at = latent_place(block, side);
+    CHECK(at.unit >= 0 && at.unit < units && at.lane >= 0 && at.lane < side && places.insert({at.unit, at.lane}).second);
+    CHECK(at.unit % 8 == block % 8);  // one XCD
+    const int start = (int)((long long)at.unit * chunk < total ? (long long)at.unit * chunk : total);
     if (start >= total) continue;
     const int end = plan_min(start + chunk, total);
     int b = 0, seq_at = 0, cur = start;
@@ -58,34 +65,42 @@ static void walk(const std::vector<int>& cu, const std::vector<int>& lens, int T
         seq_at += s.work();
         s = seq(++b);
       }
-      const int tile = (cur - seq_at) / s.steps, s0 = cur - seq_at - tile * s.steps, s1 = plan_min(s.steps, s0 + end - cur);
-      CHECK(tile >= 0 && tile < s.tiles && s0 >= 0 && s1 > s0);
+      const int group = (cur - seq_at) / s.steps, s0 = cur - seq_at - group * s.steps, s1 = plan_min(s.steps, s0 + end - cur);
+      const int tile = group * side + at.lane;
+      CHECK(group >= 0 && group < s.groups && s0 >= 0 && s1 > s0);
       const int row0 = tile * mr, row_last = plan_min(row0 + mr, s.rows) - 1;
+      if (row_last < row0) {
+        cur += s1 - s0;
+        continue;
+      }
       CHECK(row_last >= row0 && (long long)s.q0 * H + row_last < (long long)T * H);
       for (int t = s0; t < s1; ++t) CHECK(done.insert({b, tile, t}).second);
       if (!(s0 == 0 && s1 == s.steps)) {
-        const int slot = latent_slot(block, cur, chunk);
+        const int slot = latent_slot(at.unit, at.lane, side, cur, chunk);
         CHECK(slot >= 0 && slot < 2 * kLatentUnits && slots.insert(slot).second);
         pieces[{b, tile}].push_back({s0, slot});
       }
-      if (s0 == 0) records[{b, tile}] = latent_record(block, cur, s.steps, chunk);
+      if (s0 == 0) records[{b, tile}] = latent_record(at.unit, at.lane, side, cur, s.steps, chunk);
       cur += s1 - s0;
     }
   }
-  CHECK((long long)done.size() == total);
   for (int b = 0; b < B; ++b)
-    for (int tile = 0; tile < seq(b).tiles; ++tile) {
+    for (int tile = 0; tile * mr < seq(b).rows; ++tile) {
+      expected += seq(b).steps;
       CHECK(records.count({b, tile}) == 1);
       const LatentRecord r = records[{b, tile}];
-      const auto& p = pieces[{b, tile}];
-      CHECK(latent_record_joins(r) == (p.size() > 0));
+      auto& p = pieces[{b, tile}];
+      std::sort(p.begin(), p.end());
+      CHECK(latent_record_joins(r, side) == (p.size() > 0));
       if (p.empty()) {
         CHECK(r.pieces == 1);
         continue;
       }
-      CHECK((int)p.size() == r.pieces);  // blocks ascend, so do the steps
-      for (int j = 0; j < r.pieces; ++j) CHECK(p[j].second == latent_record_slot(r, j) && (j == 0) == (p[j].first == 0));
+      CHECK((int)p.size() == r.pieces);  // units ascend, so do the steps
+      for (int j = 0; j < r.pieces && j < (int)p.size(); ++j)
+        CHECK(p[j].second == latent_record_slot(r, side, j) && (j == 0) == (p[j].first == 0));
     }
+  CHECK((long long)done.size() == expected);
   ++walked;
 }
 
@@ -103,9 +118,10 @@ int main() {
     }
     const int T = cu.back() + pick(0, 3) > 0 ? cu.back() + pick(1, 3) : 1;
     if (k % 10 == 9) for (auto& c : cu) if (!pick(0, 4)) c = pick(-5, T + 40) * (pick(0, 1) ? 1 : INT_MAX / (T + 60));
-    if (k % 10 != 9) walk(cu, lens, T, H, mr, most, pick(1, 9));
+    const int side = 1 << pick(0, 3);
+    if (k % 10 != 9) walk(cu, lens, T, H, mr, side, most, pick(1, 9));
     else for (int b = 0; b < B; ++b) {  // not ascending: rows stay inside all the same
-      const LatentSeq s = latent_seq(cu[b], cu[b + 1], lens[b], T, H, mr, most);
+      const LatentSeq s = latent_seq(cu[b], cu[b + 1], lens[b], T, H, mr, side, most);
       CHECK(s.q0 >= 0 && s.n >= 0 && s.q0 + s.n <= T && s.len >= 0 && s.len <= most);
     }
   }
@@ -114,12 +130,14 @@ int main() {
       const long long r = page_row(id, pages, 64, 63);
       CHECK(r == (id >= 0 && id < pages ? (long long)id * 64 + 63 : -1));
     }
-  for (int v : {INT_MIN, -1, 0, 1, 255, 256, 257, INT_MAX})
-    for (int n : {INT_MIN, 0, 1, 2, 255, 256, 257, INT_MAX}) {
-      const LatentRecord r{v, n, 1};
-      if (latent_record_joins(r))
-        for (int j = 0; j < n; ++j) CHECK(latent_record_slot(r, j) >= 0 && latent_record_slot(r, j) < 2 * kLatentUnits);
-    }
+  for (int side : {1, 2, 4, 8})
+    for (int v : {INT_MIN, -1, 0, 1, 254, 255, 256, 510, 511, 512, INT_MAX})
+      for (int n : {INT_MIN, -1, 0, 1, 2, 31, 32, 33, 255, 256, 257, INT_MAX}) {
+        const LatentRecord r{v, n};
+        if (latent_record_joins(r, side))
+          for (int j = 0; j < n; ++j)
+            CHECK(latent_record_slot(r, side, j) >= 0 && latent_record_slot(r, side, j) < 2 * kLatentUnits);
+      }
   std::printf("%lld walked, %lld violations\n", walked, bad);
   return bad != 0;
 }
