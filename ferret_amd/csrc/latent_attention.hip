@@ -83,7 +83,7 @@ struct Tile {
   static constexpr int kData = kKeys * kRowB;
   static constexpr int kBytes = kData + (F8 ? kKeys * 4 : 0);  // then the scale words
   static constexpr int kBufs = F8 ? 3 : 2;
-  static constexpr int kVmem = 2 * kLoads + (F8 ? 1 : 0);  // loads of a wave per step
+  static constexpr int vmem(int waves) { return 8 / waves * kLoads + (F8 ? 1 : 0); }  // loads of a wave per step
 };
 
 // What only the ends of a piece need, the arguments among it, kept in LDS: scalar
@@ -134,32 +134,41 @@ __device__ __forceinline__ void put_args(Args* to, const Args& a) {
 }
 
 // LDS after the tile buffers.
-template <int MR, bool F8>
+template <int MR, int WK, bool F8>
 struct Lds {
   static constexpr int kCopies = F8 ? 4 : 1;
   static constexpr int kP = Tile<F8>::kBufs * Tile<F8>::kBytes;  // P [copy][query][64 keys] bf16
-  static constexpr int kTop = kP + kCopies * MR * 128;           // maxima [4][MR], then factors [MR]
-  static constexpr int kValid = kTop + 5 * MR * 4;               // validity of the 16-row blocks, per buffer
+  static constexpr int kTop = kP + kCopies * MR * 128;           // maxima [WK][MR], then factors [MR]
+  static constexpr int kValid = kTop + (WK + 1) * MR * 4;        // validity of the 16-row blocks, per buffer
   static constexpr int kMove = kValid + 16;                      // which waves saw the maximum move
   static constexpr int kSide = kMove + 16;
   static constexpr int kBytes = kSide + sizeof(Side);
 };
-static_assert(Lds<64, true>::kBytes <= 160 * 1024 && Lds<64, false>::kBytes <= 160 * 1024, "LDS of a CU");
+static_assert(Lds<64, 2, true>::kBytes <= 160 * 1024 && Lds<64, 2, false>::kBytes <= 160 * 1024, "LDS of a CU");
+
+// Maximum over lanes l, l ^ 16, l ^ 32, l ^ 48, in all of them.
+__device__ __forceinline__ float rows_max(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 
 // Chunk c (16 bytes) of row r stands at chunk c ^ swz(r): the 16 rows of a key
 // fragment, and the rows of two transposed blocks (4 rows of two chunks each, or 8 of
 // one), fall on distinct banks (a row is 32 banks past a multiple of 64).
 __device__ __forceinline__ int swz(int r) { return ((r >> 1) & 4) | (r & 2) | ((r >> 2) & 1); }
 
-// QF 16-query fragments per wave of the first product, WQ x WK waves over queries x keys.
-template <int QF, int WQ, bool F8>
-__global__ __launch_bounds__(256, 1) void latent_attention_kernel(Args a) {
+// WQ x WK waves: 16 queries x 64 / WK keys each for the scores, all queries x
+// 512 / (WQ WK) columns for the output.
+template <int WQ, int WK, bool F8>
+__global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void latent_attention_kernel(Args a) {
   using L = Tile<F8>;
-  constexpr int MR = 16 * QF * WQ, MF = QF * WQ;
-  using M = Lds<MR, F8>;
-  constexpr int WK = 4 / WQ;
+  constexpr int MR = 16 * WQ, NW = WQ * WK, NT = 64 * NW;
+  using M = Lds<MR, WK, F8>;
   constexpr int KT = kKeys / 16 / WK;     // 16-key blocks of a wave's scores
-  constexpr int CT = kLatent / 16 / 4;    // 16-column blocks of a wave's output
+  constexpr int CT = kLatent / 16 / NW;   // 16-column blocks of a wave's output
+  constexpr int RG = 8 / NW;              // groups of 8 rows that a wave loads
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int r16 = lane & 15, g = lane >> 4;
@@ -174,7 +183,7 @@ __global__ __launch_bounds__(256, 1) void latent_attention_kernel(Args a) {
     // The page table's first lines come under the loads of the lengths.
     const int near = a.pages.table[(long long)(place.unit * a.B / (kUnits / a.side_by_side)) * a.pages.max_pages];
     int* tot = reinterpret_cast<int*>(lds);  // wave totals
-    const int per = (a.B + 255) / 256;
+    const int per = (a.B + NT - 1) / NT;
     const int b0 = threadIdx.x * per;
     LatentSeq s{};
     int mine = 0;
@@ -193,7 +202,7 @@ __global__ __launch_bounds__(256, 1) void latent_attention_kernel(Args a) {
     asm volatile("" ::"v"(near));
     int before = 0, total = 0;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < NW; ++w) {
       if (w < wave) before += tot[w];
       total += tot[w];
     }
@@ -226,11 +235,11 @@ __global__ __launch_bounds__(256, 1) void latent_attention_kernel(Args a) {
   const float scale_log2 = a.scale_log2;
 
   // ---- lane constants
-  int load_off[L::kLoads];  // source bytes within a group of 8 rows, even group
+  int load_off[L::kLoads];  // source bytes within a group of 8 rows; the swizzle differs in odd groups
 #pragma unroll
   for (int j = 0; j < L::kLoads; ++j) {
     const int slot = j * 64 + lane, row = slot / L::kChunks, pos = slot % L::kChunks;
-    load_off[j] = row * L::kRowB + ((pos ^ swz(row)) << 4);
+    load_off[j] = row * L::kRowB + ((pos ^ swz(RG == 1 ? (wave & 1) * 8 + row : row)) << 4);
   }
 
   while (cur < uniform(side->end)) {
@@ -268,24 +277,19 @@ __global__ __launch_bounds__(256, 1) void latent_attention_kernel(Args a) {
       in.rows()[first_row + threadIdx.x] = make_int4(r.slot0, r.pieces, threadIdx.x, 0);
     }
 
-    f32x4 o[CT][MF];
-    float m[QF], l[QF];
+    f32x4 o[CT][WQ];
+    float m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int f = 0; f < QF; ++f) {
-      m[f] = -INFINITY;
-      l[f] = 0.f;
-    }
-#pragma unroll
-    for (int f = 0; f < MF; ++f)
+    for (int f = 0; f < WQ; ++f)
 #pragma unroll
       for (int c = 0; c < CT; ++c) o[c][f] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    // The page table, 64 steps at a time: lane i holds where the wave's 16 rows of step
-    // held + i stand, in units of 16 rows, -1 where they have no page.
+    // The page table, 64 steps at a time: lane i holds where the 16 rows that the wave
+    // loads from (RG groups of 8 of them) in step held + i stand, in units of 16 rows, -1 where they have no page.
     const int32_t* table = in.pages.table + (long long)b * in.pages.max_pages;
     int held = s0, where;
     const auto look_up = [&]() __attribute__((always_inline)) {
-      const int pos = min(held + lane, last - 1) * kKeys + wave * 16;  // last > s0, or nothing is issued
+      const int pos = min(held + lane, last - 1) * kKeys + wave * RG / 2 * 16;  // last > s0, or nothing is issued
       const int page = pos / in.pages.page_size;
       const int id = pos >= 0 && page < in.pages.max_pages ? table[page] : -1;
       const long long row = page_row(id, in.pages.pages, in.pages.page_size, pos - page * in.pages.page_size);
@@ -293,69 +297,84 @@ __global__ __launch_bounds__(256, 1) void latent_attention_kernel(Args a) {
     };
     look_up();
 
-    const auto issue = [&](int t) __attribute__((always_inline)) {
-      uint8_t* buf = lds + (t % L::kBufs) * L::kBytes;
+    // Step t's rows into its buffer, load by load.
+    const uint8_t* src;
+    const uint32_t* src_scales;
+    uint32_t dst, dst_scales;
+    const auto aim = [&](int t) __attribute__((always_inline)) {
       if (t == held + 64) {
         held = t;
         look_up();
       }
       const int at = __builtin_amdgcn_readlane(where, t - held);
       const bool ok = at >= 0;
-      const long long row = ok ? (long long)at << 4 : 0;  // some row: masked
-      if (lane == 0) lds[M::kValid + (t % L::kBufs) * 4 + wave] = ok ? 1 : 0;
-      const uint8_t* src = data + row * L::kRowB;
-      const uint32_t dst = uniform(lds_address(buf) + wave * 16 * L::kRowB);
-#pragma unroll
-      for (int j = 0; j < L::kLoads; ++j) dma_16(src, load_off[j], dst + j * 1024);
-#pragma unroll
-      for (int j = 0; j < L::kLoads; ++j)  // the odd group: one bit of the swizzle differs
-        dma_16(src + 8 * L::kRowB, load_off[j] ^ 64, dst + 8 * L::kRowB + j * 1024);
-      if constexpr (F8)
-        if (lane < 16) dma_4(scales + row, lane * 4, uniform(lds_address(buf) + L::kData + wave * 64));
+      const long long row = (ok ? (long long)at << 4 : 0) + (RG == 1 ? (wave & 1) * 8 : 0);  // no page: some row, masked
+      if (lane == 0) lds[M::kValid + (t % L::kBufs) * 4 + wave * RG / 2] = ok ? 1 : 0;
+      src = data + row * L::kRowB;
+      dst = uniform(lds_address(lds) + (t % L::kBufs) * L::kBytes + wave * RG * 8 * L::kRowB);
+      if constexpr (F8) {
+        src_scales = scales + row;
+        dst_scales = uniform(lds_address(lds) + (t % L::kBufs) * L::kBytes + L::kData + wave * RG * 32);
+      }
+    };
+    constexpr int LD = L::vmem(NW);
+    const auto load = [&](int i) __attribute__((always_inline)) {
+      if (F8 && i == LD - 1) {
+        if (lane < RG * 8) dma_4(src_scales, lane * 4, dst_scales);
+      } else if (i < L::kLoads) {
+        dma_16(src, load_off[i], dst + i * 1024);
+      } else {  // the odd group: one bit of the swizzle differs
+        dma_16(src + 8 * L::kRowB, load_off[i - L::kLoads] ^ 64, dst + 8 * L::kRowB + (i - L::kLoads) * 1024);
+      }
     };
 
     // ---- queries: B fragments (rows past the tile's repeat its last one)
-    u32x4 qf[QF][18];
-    int sees[QF];
-#pragma unroll
-    for (int f = 0; f < QF; ++f) {
-      const int r = row0 + (wq * QF + f) * 16 + r16;
+    u32x4 qf[18];
+    int sees;
+    {
+      const int r = row0 + wq * 16 + r16;
       const int rc = min(r, row_last), tok = rc / in.H, head = rc - tok * in.H;
-      sees[f] = r <= row_last ? max(in.causal ? past + tok : len, 0) : 0;
+      sees = r <= row_last ? max(in.causal ? past + tok : len, 0) : 0;
       const uint16_t* ql = in.ql + (long long)(q0 + tok) * in.ql_t + (long long)head * in.ql_h;
       const uint16_t* qr = in.qr + (long long)(q0 + tok) * in.qr_t + (long long)head * in.qr_h;
 #pragma unroll
       for (int k = 0; k < 16; ++k)
-        qf[f][k] = ld_u32x4(ql + (F8 ? 64 * (k >> 1) + 16 * g + 8 * (k & 1) : 32 * k + 8 * g));
+        qf[k] = ld_u32x4(ql + (F8 ? 64 * (k >> 1) + 16 * g + 8 * (k & 1) : 32 * k + 8 * g));
 #pragma unroll
-      for (int k = 0; k < 2; ++k) qf[f][16 + k] = ld_u32x4(qr + 32 * k + 8 * g);
+      for (int k = 0; k < 2; ++k) qf[16 + k] = ld_u32x4(qr + 32 * k + 8 * g);
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < L::kBufs - 1; ++i)
-      if (s0 + i < last) issue(s0 + i);
+      if (s0 + i < last) {
+        aim(s0 + i);
+#pragma unroll
+        for (int j = 0; j < LD; ++j) load(j);
+      }
     __builtin_amdgcn_sched_barrier(0);
     wait_vmcnt<0>();  // the queries, so that no wait for them stands in the loop; the first steps come with them
     __builtin_amdgcn_sched_barrier(0);
 
     for (int t = s0; t < last; ++t) {
       // Step t has landed for every wave, and the buffer refilled below has been read.
-      if (L::kBufs == 3 && t + 1 < last) wait_vmcnt<L::kVmem>();
+      if (L::kBufs == 3 && t + 1 < last) wait_vmcnt<LD>();
       else wait_vmcnt<0>();
       lds_barrier();
-      if (t + L::kBufs - 1 < last) issue(t + L::kBufs - 1);
+      const bool more = t + L::kBufs - 1 < last;
+      if (more) aim(t + L::kBufs - 1);
       __builtin_amdgcn_sched_barrier(0);
       uint8_t* buf = lds + (t % L::kBufs) * L::kBytes;
       const uint32_t* words = reinterpret_cast<const uint32_t*>(buf + L::kData);
 
       // ---- S^T: 16 keys x 16 queries per block.  Key fragments are read kAhead
       // fragments before their use; the scheduling fences keep the compiler from
-      // hoisting more of them than the registers hold.
-      f32x4 sc[KT][QF];
+      // hoisting more of them than the registers hold.  The next step's loads are
+      // issued in between: in one go they would hold the wave up for as long as the
+      // products take.
+      constexpr int CH = KT == 1 ? 2 : 1;  // chains of accumulation per block
+      f32x4 sc[KT * CH];
 #pragma unroll
-      for (int k = 0; k < KT; ++k)
-#pragma unroll
-        for (int f = 0; f < QF; ++f) sc[k][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int k = 0; k < KT * CH; ++k) sc[k] = f32x4{0.f, 0.f, 0.f, 0.f};
       {
         // chunk 4j + g: the swizzle touches 8 chunks at most, j >> 1 is an offset
         const uint8_t* row = buf + (wk * KT * 16 + r16) * L::kRowB;
@@ -364,48 +383,48 @@ __global__ __launch_bounds__(256, 1) void latent_attention_kernel(Args a) {
         if constexpr (F8)
 #pragma unroll
           for (int k = 0; k < KT; ++k) word[k] = words[(wk * KT + k) * 16 + r16];
-        const auto frag = [&](int i) {
-          const int k = i / L::kFrags, j = i % L::kFrags;
+        constexpr int NF = KT * L::kFrags;
+        const auto frag = [&](int i) {  // i = (chunk, block)
+          const int j = i / KT, k = i % KT;
           return ld_u32x4(at[j & 1] + k * 16 * L::kRowB + (j >> 1) * 128);
         };
         u32x4 ring[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) ring[i] = frag(i);
-        static_for<0, KT * L::kFrags>([&](auto ic) {
-          constexpr int i = decltype(ic)::value, k = i / L::kFrags, j = i % L::kFrags;
+        static_for<0, NF>([&](auto ic) {
+          constexpr int i = decltype(ic)::value, j = i / KT, k = i % KT;
           const u32x4 c = ring[i % kAhead];
-          if constexpr (i + kAhead < KT * L::kFrags) ring[i % kAhead] = frag(i + kAhead);
+          if constexpr (i + kAhead < NF) ring[i % kAhead] = frag(i + kAhead);
           if constexpr (F8 && j < 8) {
             const float e = __uint_as_float(((word[k] >> (8 * (j >> 1))) & 255u) << 23);
             const bf16x8 lo = e4m3x8_to_bf16x8_scaled(c[0], c[1], e), hi = e4m3x8_to_bf16x8_scaled(c[2], c[3], e);
-#pragma unroll
-            for (int f = 0; f < QF; ++f) sc[k][f] = mfma_bf16(lo, __builtin_bit_cast(bf16x8, qf[f][2 * j]), sc[k][f]);
-#pragma unroll
-            for (int f = 0; f < QF; ++f)
-              sc[k][f] = mfma_bf16(hi, __builtin_bit_cast(bf16x8, qf[f][2 * j + 1]), sc[k][f]);
+            sc[k] = mfma_bf16(lo, __builtin_bit_cast(bf16x8, qf[2 * j]), sc[k]);
+            sc[k + (CH - 1)] = mfma_bf16(hi, __builtin_bit_cast(bf16x8, qf[2 * j + 1]), sc[k + (CH - 1)]);
           } else {
-#pragma unroll
-            for (int f = 0; f < QF; ++f)
-              sc[k][f] = mfma_bf16_16x16x32(c, qf[f][F8 ? j + 8 : j], sc[k][f]);
+            constexpr int at = CH == 2 ? j & 1 : k;
+            sc[at] = mfma_bf16_16x16x32(c, qf[F8 ? j + 8 : j], sc[at]);
           }
-          if constexpr (i % kFence == kFence - 1) __builtin_amdgcn_sched_barrier(0);
+          if constexpr (i % kFence == kFence - 1) {
+            constexpr int x0 = (i + 1 - kFence) * LD / NF, x1 = (i + 1) * LD / NF;
+            if (more) static_for<x0, x1>([&](auto x) { load(decltype(x)::value); });
+            __builtin_amdgcn_sched_barrier(0);
+          }
         });
+        constexpr int rest = NF / kFence * kFence * LD / NF;
+        if (more) static_for<rest, LD>([&](auto x) { load(decltype(x)::value); });
+        if constexpr (CH == 2) sc[0] += sc[1];
       }
       __builtin_amdgcn_sched_barrier(0);
 
       // ---- masks: only where the step passes what some row sees, or misses a page
       const uint32_t ok = uniform(*reinterpret_cast<const uint32_t*>(lds + M::kValid + (t % L::kBufs) * 4));
       if ((t + 1) * kKeys > see_all || ok != 0x01010101u) {
+        const int left = sees - (t * kKeys + wk * KT * 16 + 4 * g);
 #pragma unroll
-        for (int f = 0; f < QF; ++f) {
-          const int left = sees[f] - (t * kKeys + wk * KT * 16 + 4 * g);
+        for (int k = 0; k < KT; ++k) {
+          const int upto = (ok >> (8 * (wk * KT + k))) & 1 ? left - k * 16 : 0;
 #pragma unroll
-          for (int k = 0; k < KT; ++k) {
-            const int upto = (ok >> (8 * (wk * KT + k))) & 1 ? left - k * 16 : 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sc[k][f][i] = i < upto ? sc[k][f][i] : -INFINITY;
-          }
-          __builtin_amdgcn_sched_barrier(0);
+          for (int i = 0; i < 4; ++i) sc[k][i] = i < upto ? sc[k][i] : -INFINITY;
         }
         // A value that a row does not see must not reach it as 0 * NaN: rows that
         // no query sees become zeros, and Inf and NaN of rows that some do not see
@@ -414,7 +433,7 @@ __global__ __launch_bounds__(256, 1) void latent_attention_kernel(Args a) {
         lds_barrier();  // the keys have been read
         constexpr int VC = F8 ? kLatent / 16 : kLatent / 8;  // chunks of a row's values
 #pragma unroll 1
-        for (int i = threadIdx.x; i < kKeys * VC; i += 256) {
+        for (int i = threadIdx.x; i < kKeys * VC; i += NT) {
           const int r = i / VC, key = t * kKeys + r;
           const bool none = key >= see_any || !((ok >> (8 * (r >> 4))) & 1);
           if (!none && key < see_all) continue;
@@ -445,103 +464,98 @@ __global__ __launch_bounds__(256, 1) void latent_attention_kernel(Args a) {
         }
       }
 
-      // ---- softmax terms of the lane's queries (column r16 of each fragment), with
-      // the maximum of the steps before
-      bool move = false;
+      // ---- softmax terms of the lane's query (column r16), with the maximum of the
+      // steps before
+      float top = sc[0][0];
 #pragma unroll
-      for (int f = 0; f < QF; ++f) {
-        float v = sc[0][f][0];
+      for (int k = 0; k < KT; ++k)
 #pragma unroll
-        for (int k = 0; k < KT; ++k)
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[k][i]);
+      top = rows_max(top) * scale_log2;
+      const bool move = __any(top > m + kLazy);  // from -inf: any finite score
+      const int q = wq * 16 + r16;
+      if (g == 0) tops[wk * MR + q] = top;
+      if (lane == 0) lds[M::kMove + wave] = move ? 1 : 0;
+      float pend;  // this step's part of l
+      const auto put_p = [&]() __attribute__((always_inline)) {
+        const float base = m == -INFINITY ? 0.f : m;
+        pend = 0.f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v = fmaxf(v, sc[k][f][i]);
-        v = fmaxf(v, __shfl_xor(v, 16, 64));
-        v = fmaxf(v, __shfl_xor(v, 32, 64)) * scale_log2;
-        move = move || v > m[f] + kLazy;  // from -inf: any finite score
-        if (g == 0) tops[wk * MR + (wq * QF + f) * 16 + r16] = v;
-      }
-      const bool mine = __any(move);
-      if (lane == 0) lds[M::kMove + wave] = mine ? 1 : 0;
-      float pend[QF];  // this step's part of l
-      const auto put_p = [&]() {
+        for (int k = 0; k < KT; ++k) {
+          f32x4 p;
 #pragma unroll
-        for (int f = 0; f < QF; ++f) {
-          const float base = m[f] == -INFINITY ? 0.f : m[f];
-          const int q = (wq * QF + f) * 16 + r16;
-          pend[f] = 0.f;
-#pragma unroll
-          for (int k = 0; k < KT; ++k) {
-            f32x4 p;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              p[i] = __builtin_amdgcn_exp2f(fmaf(sc[k][f][i], scale_log2, -base));
-              pend[f] += p[i];
-            }
-            const int kb = wk * KT + k;  // 16-key block of the step: 2 chunks
-            uint8_t* to = lds + M::kP + q * 128 + (((2 * kb + (g >> 1)) ^ (r16 >> 1)) << 4) + (g & 1) * 8;
-            if constexpr (F8) {
-              const u32x4 w4 = *reinterpret_cast<const u32x4*>(words + kb * 16 + 4 * g);
-#pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                float e[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) e[i] = p[i] * __uint_as_float(((w4[i] >> (8 * c)) & 255u) << 23);
-                *reinterpret_cast<u32x2*>(to + c * MR * 128) = u32x2{pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3])};
-              }
-            } else {
-              *reinterpret_cast<u32x2*>(to) = u32x2{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3])};
-            }
+          for (int i = 0; i < 4; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(fmaf(sc[k][i], scale_log2, -base));
+            pend += p[i];
           }
-          __builtin_amdgcn_sched_barrier(0);
+          const int kb = wk * KT + k;  // 16-key block of the step: 2 chunks
+          uint8_t* to = lds + M::kP + q * 128 + (((2 * kb + (g >> 1)) ^ (r16 >> 1)) << 4) + (g & 1) * 8;
+          if constexpr (F8) {
+            const u32x4 w4 = *reinterpret_cast<const u32x4*>(words + kb * 16 + 4 * g);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              float e[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) e[i] = p[i] * __uint_as_float(((w4[i] >> (8 * c)) & 255u) << 23);
+              *reinterpret_cast<u32x2*>(to + c * MR * 128) = u32x2{pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3])};
+            }
+          } else {
+            *reinterpret_cast<u32x2*>(to) = u32x2{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3])};
+          }
         }
       };
       put_p();
       lds_barrier();
-      if (uniform(*reinterpret_cast<const uint32_t*>(lds + M::kMove)) != 0) {
+      const u32x2 moves = *reinterpret_cast<const u32x2*>(lds + M::kMove);
+
+      // ---- O^T += V^T P^T, 32 keys at a time: lane (column r16, key octet g)
+      const uint8_t* pbuf = lds + M::kP + (F8 ? wave * CT / 8 * MR * 128 : 0) + r16 * 128;
+      const uint8_t* const pat[2] = {pbuf + ((g ^ (r16 >> 1)) << 4), pbuf + (((4 + g) ^ (r16 >> 1)) << 4)};
+      u32x4 p[WQ];
+      const auto get_p = [&](int h) __attribute__((always_inline)) {
+#pragma unroll
+        for (int f = 0; f < WQ; ++f) p[f] = ld_u32x4(pat[h] + f * 16 * 128);
+      };
+      get_p(0);
+      if (uniform(NW == 8 ? moves[0] | moves[1] : moves[0]) != 0) {
         // The maximum of some query moves: again with the new one, O follows.
+        float to = m;
 #pragma unroll
-        for (int f = 0; f < QF; ++f) {
-          const int q = (wq * QF + f) * 16 + r16;
-          float to = m[f];
-#pragma unroll
-          for (int w = 0; w < WK; ++w) to = fmaxf(to, tops[w * MR + q]);
-          const float by = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[f] - to);
-          m[f] = to;
-          l[f] *= by;
-          if (wk == 0 && g == 0) tops[4 * MR + q] = by;
-        }
+        for (int w = 0; w < WK; ++w) to = fmaxf(to, tops[w * MR + q]);
+        const float by = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to);
+        m = to;
+        l *= by;
+        if (wk == 0 && g == 0) tops[WK * MR + q] = by;
+        lds_barrier();  // P has been read
         put_p();
         lds_barrier();
+        get_p(0);
 #pragma unroll
-        for (int f = 0; f < MF; ++f) {
-          const float by = tops[4 * MR + f * 16 + r16];
+        for (int f = 0; f < WQ; ++f) {
+          const float by = tops[WK * MR + f * 16 + r16];
 #pragma unroll
           for (int c = 0; c < CT; ++c) o[c][f] *= by;
           __builtin_amdgcn_sched_barrier(0);
         }
       }
-#pragma unroll
-      for (int f = 0; f < QF; ++f) l[f] += pend[f];
-
-      // ---- O^T += V^T P^T, 32 keys at a time: lane (column r16, key octet g)
+      l += pend;
       __builtin_amdgcn_sched_barrier(0);
       {
-        const uint8_t* pbuf = lds + M::kP + (F8 ? wave * MR * 128 : 0) + r16 * 128;
-        const uint8_t* const pat[2] = {pbuf + ((g ^ (r16 >> 1)) << 4), pbuf + (((4 + g) ^ (r16 >> 1)) << 4)};
-        // The wave's columns start on a multiple of 8 chunks, so the swizzled block
-        // is an exclusive-or into the address, whose low bits are the swizzle's.
+        // An exclusive-or of the block into the address is the swizzle: a wave's columns
+        // start on a multiple of its chunks, and the bits below belong to the swizzle.
+        constexpr int WB = CT * (F8 ? 16 : 32);  // a wave's bytes of a row
         const int row = 8 * g + (F8 ? r16 >> 1 : r16 >> 2);
-        const uint32_t at = (uint32_t)(t % L::kBufs) * L::kBytes + row * L::kRowB + wave * (F8 ? 128 : 256) +
-                            ((swz(row) ^ (F8 ? 0 : (lane >> 1) & 1)) << 4) + 8 * (lane & 1);
+        const int z = ((swz(row) ^ (F8 ? 0 : (lane >> 1) & 1)) << 4) ^ (wave * WB & 127);
+        const uint32_t at = (uint32_t)(t % L::kBufs) * L::kBytes + row * L::kRowB + (wave * WB & ~127) + z + 8 * (lane & 1);
         const auto frag = [&](int i) {  // i = (half, block)
           const int h = i / CT, c = i % CT;
           if constexpr (F8) {
             const u32x2 v = lds_tr8(lds + (at ^ (c << 4)) + h * 32 * L::kRowB);
             return u32x4{v[0], v[1], 0u, 0u};
           } else {  // rows 4 further: the lowest bit of the swizzle flips
-            const uint8_t* p = lds + (at ^ ((c & 3) << 5)) + (c >> 2) * 128 + h * 32 * L::kRowB;
-            const uint8_t* p4 = lds + (at ^ ((c & 3) << 5) ^ 16) + (c >> 2) * 128 + (h * 32 + 4) * L::kRowB;
-            const u32x2 v0 = lds_tr16(p), v1 = lds_tr16(p4);
+            const uint8_t* x = lds + (at ^ ((c & 3) << 5)) + (c >> 2) * 128 + h * 32 * L::kRowB;
+            const uint8_t* x4 = lds + (at ^ ((c & 3) << 5) ^ 16) + (c >> 2) * 128 + (h * 32 + 4) * L::kRowB;
+            const u32x2 v0 = lds_tr16(x), v1 = lds_tr16(x4);
             return u32x4{v0[0], v0[1], v1[0], v1[1]};
           }
         };
@@ -550,43 +564,38 @@ __global__ __launch_bounds__(256, 1) void latent_attention_kernel(Args a) {
         for (int i = 0; i < kAhead; ++i) ring[i] = frag(i);
         static_for<0, kKeys / 32>([&](auto hc) {
           constexpr int h = decltype(hc)::value;
-          u32x4 p[MF];
-#pragma unroll
-          for (int f = 0; f < MF; ++f) {
-            p[f] = ld_u32x4(pat[h] + f * 16 * 128);
-          }
+          if constexpr (h > 0) get_p(h);
           static_for<0, CT>([&](auto cc) {
             constexpr int c = decltype(cc)::value, i = h * CT + c;
             const u32x4 v = ring[i % kAhead];
             if constexpr (i + kAhead < kKeys / 32 * CT) ring[i % kAhead] = frag(i + kAhead);
             const bf16x8 vb = F8 ? e4m3x8_to_bf16x8(v[0], v[1]) : __builtin_bit_cast(bf16x8, v);
 #pragma unroll
-            for (int f = 0; f < MF; ++f) o[c][f] = mfma_bf16(vb, __builtin_bit_cast(bf16x8, p[f]), o[c][f]);
+            for (int f = 0; f < WQ; ++f) o[c][f] = mfma_bf16(vb, __builtin_bit_cast(bf16x8, p[f]), o[c][f]);
             if constexpr (i % kFence == kFence - 1) __builtin_amdgcn_sched_barrier(0);
           });
         });
       }
     }
 
-    // ---- the piece's result: l of all waves, then a quarter of the columns per wave
+    // ---- the piece's result: l of all waves, then each wave's columns
     __syncthreads();  // the last step's maxima and factors have been read
-#pragma unroll
-    for (int f = 0; f < QF; ++f) {
-      float sum = l[f];
+    {
+      float sum = l;
       sum += __shfl_xor(sum, 16, 64);
       sum += __shfl_xor(sum, 32, 64);
-      const int q = (wq * QF + f) * 16 + r16;
+      const int q = wq * 16 + r16;
       if (g == 0) tops[wk * MR + q] = sum;
-      if (wk == 0 && g == 0) tops[4 * MR + q] = m[f];
+      if (wk == 0 && g == 0) tops[WK * MR + q] = m;
     }
     __syncthreads();
 #pragma unroll
-    for (int f = 0; f < MF; ++f) {
+    for (int f = 0; f < WQ; ++f) {
       const int r = f * 16 + r16;
       float sum = tops[r];
 #pragma unroll
       for (int w = 1; w < WK; ++w) sum += tops[w * MR + r];
-      const float top = tops[4 * MR + r];
+      const float top = tops[WK * MR + r];
       const int col = wave * CT * 16 + 4 * g;
       if (row0 + r <= row_last) {
         const int slot = uniform(side->slot);
@@ -722,11 +731,11 @@ __global__ __launch_bounds__(256) void latent_join_long_kernel(Args a, int mr) {
     a.lse[row] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
-template <int QF, int WQ, bool F8>
+template <int WQ, int WK, bool F8>
 int launch(const Args& a, hipStream_t st) {
-  constexpr int mr = 16 * QF * WQ, lds = Lds<mr, F8>::kBytes;
-  FERRET_HIP_CHECK((set_lds_limit_once<latent_attention_kernel<QF, WQ, F8>>(lds)));
-  hipLaunchKernelGGL((latent_attention_kernel<QF, WQ, F8>), dim3(kUnits), dim3(256), lds, st, a);
+  constexpr int mr = 16 * WQ, lds = Lds<mr, WK, F8>::kBytes;
+  FERRET_HIP_CHECK((set_lds_limit_once<latent_attention_kernel<WQ, WK, F8>>(lds)));
+  hipLaunchKernelGGL((latent_attention_kernel<WQ, WK, F8>), dim3(kUnits), dim3(64 * WQ * WK), lds, st, a);
   FERRET_HIP_CHECK(hipGetLastError());
   const unsigned rows = (unsigned)((long long)a.T * a.H);
   if (rows <= kJoinRows)
@@ -739,9 +748,9 @@ int launch(const Args& a, hipStream_t st) {
 template <bool F8>
 int launch_rows(int mr, const Args& a, hipStream_t st) {
   switch (mr) {
-    case 16: return launch<1, 1, F8>(a, st);
-    case 32: return launch<2, 1, F8>(a, st);
-    default: return launch<2, 2, F8>(a, st);
+    case 16: return launch<1, 4, F8>(a, st);
+    case 32: return launch<2, 4, F8>(a, st);
+    default: return launch<4, 2, F8>(a, st);
   }
 }
 
