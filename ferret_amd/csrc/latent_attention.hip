@@ -144,7 +144,7 @@ struct Lds {
   static constexpr int kSide = kMove + 16;
   static constexpr int kBytes = kSide + sizeof(Side);
 };
-static_assert(Lds<64, 2, true>::kBytes <= 160 * 1024 && Lds<64, 2, false>::kBytes <= 160 * 1024, "LDS of a CU");
+static_assert(Lds<32, 4, true>::kBytes <= 160 * 1024 && Lds<32, 4, false>::kBytes <= 160 * 1024, "LDS of a CU");
 
 // Maximum over lanes l, l ^ 16, l ^ 32, l ^ 48, in all of them.
 __device__ __forceinline__ float rows_max(float v) {
@@ -158,6 +158,173 @@ __device__ __forceinline__ float rows_max(float v) {
 // fragment, and the rows of two transposed blocks (4 rows of two chunks each, or 8 of
 // one), fall on distinct banks (a row is 32 banks past a multiple of 64).
 __device__ __forceinline__ int swz(int r) { return ((r >> 1) & 4) | (r & 2) | ((r >> 2) & 1); }
+
+// The start of a work-group's share of the line: false where it has none.  The page
+// table's first lines come under the loads of the lengths.  tot: 8 words of LDS.
+template <int MR, int NT>
+__device__ __forceinline__ bool take_share(const Args& a, LatentPlace place, Side* side, int* tot, int* cur) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int near = a.pages.table[(long long)(place.unit * a.B / (kUnits / a.side_by_side)) * a.pages.max_pages];
+  const int per = (a.B + NT - 1) / NT;
+  const int b0 = threadIdx.x * per;
+  LatentSeq s{};
+  int mine = 0;
+  for (int i = 0; i < per && b0 + i < a.B; ++i) {
+    s = sequence<MR>(a, b0 + i);
+    mine += s.work();
+  }
+  int incl = mine;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int o = __shfl_up(incl, off, 64);
+    if (lane >= off) incl += o;
+  }
+  if (lane == 63) tot[wave] = incl;
+  __syncthreads();
+  asm volatile("" ::"v"(near));
+  int before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) {
+    if (w < wave) before += tot[w];
+    total += tot[w];
+  }
+  const int chunk = latent_chunk(total, kUnits / a.side_by_side, a.min_steps);
+  const int start = (int)min((long long)place.unit * chunk, (long long)total);
+  const int excl = before + incl - mine;
+  if (start >= total) return false;
+  if (excl <= start && start < excl + mine) {
+    int at = excl, i = 0;
+    if (per > 1)
+      for (;; ++i) {
+        s = sequence<MR>(a, b0 + i);
+        if (start < at + s.work() || i + 1 == per) break;
+        at += s.work();
+      }
+    side->b = b0 + i;
+    put_seq(&side->seq, s);
+    side->seq_at = at;
+    side->chunk = chunk;
+    side->end = min(start + chunk, total);
+    put_args(&side->args, a);
+  }
+  *cur = uniform(start);
+  __syncthreads();
+  return true;
+}
+
+// A piece of a row tile: steps s0 .. s1 of sequence b.
+struct Piece {
+  int b, s0, s1, len, past, q0;
+  int row0, row_last;     // query rows of the sequence
+  int see_all, see_any;   // keys that the first and the last token of the tile see
+};
+
+// The piece at `cur`, its place noted in LDS and its rows' record in the workspace;
+// false for a tile that is not there (fewer tiles than work-groups side by side).
+template <int MR>
+__device__ __forceinline__ bool next_piece(LatentPlace place, Side* side, int cur, Piece* p) {
+  const Args& in = side->args;
+  int b = uniform(side->b), seq_at = uniform(side->seq_at);
+  LatentSeq s = get_seq(&side->seq);
+  while (cur >= seq_at + s.work() && b + 1 < in.B) {  // the next sequence with rows
+    seq_at += s.work();
+    s = sequence<MR>(in, ++b);
+  }
+  p->b = b = uniform(b);
+  p->len = uniform(s.len);
+  p->q0 = uniform(s.q0);
+  const int steps = uniform(s.steps), group = uniform((cur - seq_at) / steps);
+  p->s0 = uniform(cur - seq_at - group * steps);
+  p->s1 = uniform(min(steps, p->s0 + (side->end - cur)));
+  p->row0 = (group * in.side_by_side + place.lane) * MR;
+  p->row_last = uniform(min(p->row0 + MR, s.rows) - 1);
+  if (p->row_last < p->row0) return false;
+  p->past = p->len - uniform(s.n) + 1;
+  p->see_all = uniform(max(in.causal ? p->past + p->row0 / in.H : p->len, 0));
+  p->see_any = uniform(max(in.causal ? p->past + p->row_last / in.H : p->len, 0));
+  const int chunk = side->chunk, first_row = p->q0 * in.H + p->row0;
+  __syncthreads();  // the piece before is done with its record and buffers
+  if (threadIdx.x == 0) {
+    side->b = b;
+    put_seq(&side->seq, s);
+    side->seq_at = seq_at;
+    side->first_row = first_row;
+    side->slot =
+        p->s0 == 0 && p->s1 == steps ? -1 : latent_slot(place.unit, place.lane, in.side_by_side, cur, chunk);
+  }
+  if (p->s0 == 0 && (int)threadIdx.x <= p->row_last - p->row0) {
+    const LatentRecord r = latent_record(place.unit, place.lane, in.side_by_side, cur, steps, chunk);
+    in.rows()[first_row + threadIdx.x] = make_int4(r.slot0, r.pieces, threadIdx.x, 0);
+  }
+  return true;
+}
+
+// Where 16-row block `block` (of the sequence) of the wave's lanes stands in the cache, in
+// units of 16 rows, -1 where it has no page.
+__device__ __forceinline__ int find_block(const Pages& pages, const int32_t* table, int block) {
+  const int pos = block * 16, page = pos / pages.page_size;
+  const int id = pos >= 0 && page < pages.max_pages ? table[page] : -1;
+  const long long row = page_row(id, pages.pages, pages.page_size, pos - page * pages.page_size);
+  return row < 0 ? -1 : (int)(row >> 4);
+}
+
+// A fragment of queries (column r16 = row `r` of the sequence), and the keys that it sees.
+template <bool F8>
+__device__ __forceinline__ int get_queries(const Args& in, const Piece& p, int r, int g, u32x4 (&qf)[18]) {
+  const int rc = min(r, p.row_last), tok = rc / in.H, head = rc - tok * in.H;  // past the tile: its last row
+  const uint16_t* ql = in.ql + (long long)(p.q0 + tok) * in.ql_t + (long long)head * in.ql_h;
+  const uint16_t* qr = in.qr + (long long)(p.q0 + tok) * in.qr_t + (long long)head * in.qr_h;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) qf[k] = ld_u32x4(ql + (F8 ? 64 * (k >> 1) + 16 * g + 8 * (k & 1) : 32 * k + 8 * g));
+#pragma unroll
+  for (int k = 0; k < 2; ++k) qf[16 + k] = ld_u32x4(qr + 32 * k + 8 * g);
+  return r <= p.row_last ? max(in.causal ? p.past + tok : p.len, 0) : 0;
+}
+
+// Inf and NaN among 16 bytes of values become zeros.
+template <bool F8>
+__device__ __forceinline__ u32x4 only_finite(u32x4 v) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if constexpr (F8) {
+      const uint32_t nan = (((v[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
+      v[w] &= ~(nan * 255u);
+    } else {
+      if ((v[w] & 0x7f80u) == 0x7f80u) v[w] &= 0xffff0000u;
+      if ((v[w] & 0x7f800000u) == 0x7f800000u) v[w] &= 0x0000ffffu;
+    }
+  }
+  return v;
+}
+
+// Row r of the tile done: its output, or its part of a piece.  o: blocks of 16 columns
+// from `col` on, 4 of each per lane.
+template <int MR, int CT, int WQ>
+__device__ __forceinline__ void put_rows(const Side* side, const Piece& p, int steps_taken, int f, int r16, int col,
+                                         bool stats, float top, float sum, const f32x4 (&o)[CT][WQ]) {
+  const Args& in = side->args;
+  const int r = f * 16 + r16, slot = uniform(side->slot);
+  if (p.row0 + r > p.row_last) return;
+  if (slot < 0) {
+    const long long at = side->first_row + r;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    uint16_t* to = in.out + at * kLatent + col;
+#pragma unroll
+    for (int c = 0; c < CT; ++c)
+      *reinterpret_cast<u32x2*>(to + c * 16) =
+          u32x2{pack_bf16x2(o[c][f][0] * inv, o[c][f][1] * inv), pack_bf16x2(o[c][f][2] * inv, o[c][f][3] * inv)};
+    if (stats && in.lse != nullptr)
+      in.lse[at] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+  } else {
+    const long long at = (long long)slot * MR + r;
+    if (stats) in.ml()[at] = make_float2(top, sum);
+    if (steps_taken > 0) {
+      float* to = in.part(MR) + at * kLatent + col;
+#pragma unroll
+      for (int c = 0; c < CT; ++c) *reinterpret_cast<f32x4*>(to + c * 16) = o[c][f];
+    }
+  }
+}
 
 // WQ x WK waves: 16 queries x 64 / WK keys each for the scores, all queries x
 // 512 / (WQ WK) columns for the output.
@@ -176,59 +343,9 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void latent_attention_ke
   float* const tops = reinterpret_cast<float*>(lds + M::kTop);
   Side* const side = reinterpret_cast<Side*>(lds + M::kSide);
 
-  // ---- this work-group's share of the line
   const LatentPlace place = latent_place(blockIdx.x, a.side_by_side);
   int cur;
-  {
-    // The page table's first lines come under the loads of the lengths.
-    const int near = a.pages.table[(long long)(place.unit * a.B / (kUnits / a.side_by_side)) * a.pages.max_pages];
-    int* tot = reinterpret_cast<int*>(lds);  // wave totals
-    const int per = (a.B + NT - 1) / NT;
-    const int b0 = threadIdx.x * per;
-    LatentSeq s{};
-    int mine = 0;
-    for (int i = 0; i < per && b0 + i < a.B; ++i) {
-      s = sequence<MR>(a, b0 + i);
-      mine += s.work();
-    }
-    int incl = mine;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int o = __shfl_up(incl, off, 64);
-      if (lane >= off) incl += o;
-    }
-    if (lane == 63) tot[wave] = incl;
-    __syncthreads();
-    asm volatile("" ::"v"(near));
-    int before = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      if (w < wave) before += tot[w];
-      total += tot[w];
-    }
-    const int chunk = latent_chunk(total, kUnits / a.side_by_side, a.min_steps);
-    const int start = (int)min((long long)place.unit * chunk, (long long)total);
-    const int excl = before + incl - mine;
-    if (start >= total) return;
-    if (excl <= start && start < excl + mine) {
-      int at = excl, i = 0;
-      if (per > 1)
-        for (;; ++i) {
-          s = sequence<MR>(a, b0 + i);
-          if (start < at + s.work() || i + 1 == per) break;
-          at += s.work();
-        }
-      side->b = b0 + i;
-      put_seq(&side->seq, s);
-      side->seq_at = at;
-      side->chunk = chunk;
-      side->end = min(start + chunk, total);
-      put_args(&side->args, a);
-    }
-    cur = uniform(start);
-    __syncthreads();
-  }
-
+  if (!take_share<MR, NT>(a, place, side, reinterpret_cast<int*>(lds), &cur)) return;
   const Args& in = side->args;
   const uint8_t* const data = a.data;
   const uint32_t* const scales = a.scales;
@@ -243,39 +360,12 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void latent_attention_ke
   }
 
   while (cur < uniform(side->end)) {
-    int b = uniform(side->b), seq_at = uniform(side->seq_at);
-    LatentSeq s = get_seq(&side->seq);
-    while (cur >= seq_at + s.work() && b + 1 < in.B) {  // the next sequence with rows
-      seq_at += s.work();
-      s = sequence<MR>(in, ++b);
-    }
-    b = uniform(b);
-    const int len = uniform(s.len), steps = uniform(s.steps), q0 = uniform(s.q0);
-    const int group = uniform((cur - seq_at) / steps), s0 = uniform(cur - seq_at - group * steps);
-    const int s1 = uniform(min(steps, s0 + (side->end - cur)));
-    const int row0 = (group * in.side_by_side + place.lane) * MR, row_last = uniform(min(row0 + MR, s.rows) - 1);
-    if (row_last < row0) {  // fewer tiles than work-groups side by side
-      cur += s1 - s0;
-      continue;
-    }
-    // keys seen by the first and by the last token of the tile
-    const int past = len - uniform(s.n) + 1;
-    const int see_all = uniform(max(in.causal ? past + row0 / in.H : len, 0));
-    const int see_any = uniform(max(in.causal ? past + row_last / in.H : len, 0));
-    const int last = min(s1, (see_any + kKeys - 1) / kKeys);
-    const int chunk = side->chunk, first_row = q0 * in.H + row0;
-    __syncthreads();  // the piece before is done with its record and buffers
-    if (threadIdx.x == 0) {
-      side->b = b;
-      put_seq(&side->seq, s);
-      side->seq_at = seq_at;
-      side->first_row = first_row;
-      side->slot = s0 == 0 && s1 == steps ? -1 : latent_slot(place.unit, place.lane, in.side_by_side, cur, chunk);
-    }
-    if (s0 == 0 && (int)threadIdx.x <= row_last - row0) {  // where the pieces of this tile's rows stand
-      const LatentRecord r = latent_record(place.unit, place.lane, in.side_by_side, cur, steps, chunk);
-      in.rows()[first_row + threadIdx.x] = make_int4(r.slot0, r.pieces, threadIdx.x, 0);
-    }
+    Piece pc;
+    const bool there = next_piece<MR>(place, side, cur, &pc);
+    const int s0 = pc.s0, see_all = pc.see_all, see_any = pc.see_any;
+    cur += pc.s1 - s0;
+    if (!there) continue;
+    const int last = min(pc.s1, (see_any + kKeys - 1) / kKeys);
 
     f32x4 o[CT][WQ];
     float m = -INFINITY, l = 0.f;
@@ -284,16 +374,12 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void latent_attention_ke
 #pragma unroll
       for (int c = 0; c < CT; ++c) o[c][f] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    // The page table, 64 steps at a time: lane i holds where the 16 rows that the wave
-    // loads from (RG groups of 8 of them) in step held + i stand, in units of 16 rows, -1 where they have no page.
-    const int32_t* table = in.pages.table + (long long)b * in.pages.max_pages;
+    // The page table, 64 steps at a time: lane i holds where the 16 rows stand that the
+    // wave loads from (RG groups of 8 of them) in step held + i.
+    const int32_t* table = in.pages.table + (long long)pc.b * in.pages.max_pages;
     int held = s0, where;
     const auto look_up = [&]() __attribute__((always_inline)) {
-      const int pos = min(held + lane, last - 1) * kKeys + wave * RG / 2 * 16;  // last > s0, or nothing is issued
-      const int page = pos / in.pages.page_size;
-      const int id = pos >= 0 && page < in.pages.max_pages ? table[page] : -1;
-      const long long row = page_row(id, in.pages.pages, in.pages.page_size, pos - page * in.pages.page_size);
-      where = row < 0 ? -1 : (int)(row >> 4);
+      where = find_block(in.pages, table, min(held + lane, last - 1) * (kKeys / 16) + wave * RG / 2);
     };
     look_up();
 
@@ -328,21 +414,8 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void latent_attention_ke
       }
     };
 
-    // ---- queries: B fragments (rows past the tile's repeat its last one)
-    u32x4 qf[18];
-    int sees;
-    {
-      const int r = row0 + wq * 16 + r16;
-      const int rc = min(r, row_last), tok = rc / in.H, head = rc - tok * in.H;
-      sees = r <= row_last ? max(in.causal ? past + tok : len, 0) : 0;
-      const uint16_t* ql = in.ql + (long long)(q0 + tok) * in.ql_t + (long long)head * in.ql_h;
-      const uint16_t* qr = in.qr + (long long)(q0 + tok) * in.qr_t + (long long)head * in.qr_h;
-#pragma unroll
-      for (int k = 0; k < 16; ++k)
-        qf[k] = ld_u32x4(ql + (F8 ? 64 * (k >> 1) + 16 * g + 8 * (k & 1) : 32 * k + 8 * g));
-#pragma unroll
-      for (int k = 0; k < 2; ++k) qf[16 + k] = ld_u32x4(qr + 32 * k + 8 * g);
-    }
+    u32x4 qf[18];  // queries: B fragments
+    const int sees = get_queries<F8>(in, pc, pc.row0 + wq * 16 + r16, g, qf);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < L::kBufs - 1; ++i)
@@ -439,19 +512,7 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void latent_attention_ke
           if (!none && key < see_all) continue;
           u32x4* p = reinterpret_cast<u32x4*>(buf + r * L::kRowB + (((i % VC) ^ swz(r)) << 4));
           u32x4 v = {0u, 0u, 0u, 0u};
-          if (!none) {
-            v = *p;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              if constexpr (F8) {
-                const uint32_t nan = (((v[w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
-                v[w] &= ~(nan * 255u);
-              } else {
-                if ((v[w] & 0x7f80u) == 0x7f80u) v[w] &= 0xffff0000u;
-                if ((v[w] & 0x7f800000u) == 0x7f800000u) v[w] &= 0x0000ffffu;
-              }
-            }
-          }
+          if (!none) v = only_finite<F8>(*p);
           *p = v;
         }
         if constexpr (F8) {
@@ -591,37 +652,361 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void latent_attention_ke
     __syncthreads();
 #pragma unroll
     for (int f = 0; f < WQ; ++f) {
-      const int r = f * 16 + r16;
-      float sum = tops[r];
+      float sum = tops[f * 16 + r16];
 #pragma unroll
-      for (int w = 1; w < WK; ++w) sum += tops[w * MR + r];
-      const float top = tops[WK * MR + r];
-      const int col = wave * CT * 16 + 4 * g;
-      if (row0 + r <= row_last) {
-        const int slot = uniform(side->slot);
-        if (slot < 0) {
-          const long long at = side->first_row + r;
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          uint16_t* to = in.out + at * kLatent + col;
-#pragma unroll
-          for (int c = 0; c < CT; ++c)
-            *reinterpret_cast<u32x2*>(to + c * 16) =
-                u32x2{pack_bf16x2(o[c][f][0] * inv, o[c][f][1] * inv), pack_bf16x2(o[c][f][2] * inv, o[c][f][3] * inv)};
-          if (wave == 0 && g == 0 && in.lse != nullptr)
-            in.lse[at] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
-        } else {
-          const long long at = (long long)slot * MR + r;
-          if (wave == 0 && g == 0) in.ml()[at] = make_float2(top, sum);
-          if (last > s0) {
-            float* to = in.part(MR) + at * kLatent + col;
-#pragma unroll
-            for (int c = 0; c < CT; ++c) *reinterpret_cast<f32x4*>(to + c * 16) = o[c][f];
-          }
-        }
-      }
+      for (int w = 1; w < WK; ++w) sum += tops[w * MR + f * 16 + r16];
+      put_rows<MR>(side, pc, last - s0, f, r16, wave * CT * 16 + 4 * g, wave == 0 && g == 0, tops[WK * MR + f * 16 + r16],
+                   sum, o);
       __builtin_amdgcn_sched_barrier(0);
     }
-    cur += s1 - s0;
+  }
+}
+
+// ---- 64 query rows: two products at a time
+
+// LDS: four buffers of 32 keys, P twice, and the small records.
+template <bool F8>
+struct Wide {
+  static constexpr int kRows = 64, kStep = 32, kBufs = 4;
+  static constexpr int kData = kStep * Tile<F8>::kRowB, kBytes = kData + (F8 ? kStep * 4 : 0);
+  static constexpr int kCopies = F8 ? 4 : 1, kPCopy = kRows * kStep * 2, kPBytes = kCopies * kPCopy;
+  static constexpr int kP = kBufs * kBytes;             // P [2][copy][query][32 keys] bf16
+  static constexpr int kTop = kP + 2 * kPBytes;         // maxima [2][64], factors [64]
+  static constexpr int kFin = kTop + 3 * kRows * 4;     // sums [2][64], maxima [64] of the piece
+  static constexpr int kValid = kFin + 3 * kRows * 4;   // validity of the 16-row blocks, per buffer
+  static constexpr int kMove = kValid + 16;             // [2][4]: which waves saw the maximum move
+  static constexpr int kSide = kMove + 16;
+  static constexpr int kLds = kSide + sizeof(Side);
+  static constexpr int kLoad = Tile<F8>::kLoads + (F8 ? 1 : 0);  // loads of a wave per step
+};
+static_assert(Wide<true>::kLds <= 160 * 1024 && Wide<false>::kLds <= 160 * 1024, "LDS of a CU");
+
+// Waves 0 - 3 take the scores of 32 keys (32 queries x 16 keys each) while waves 4 - 7,
+// one of them on every SIMD beside one of the others, add the 32 keys before to the
+// output (64 queries x 128 columns each) and load the keys to come: the matrix unit
+// is fed by one while the other is at its softmax, at a barrier or at its loads, and
+// neither holds more than half of the registers (Q is 144, O 128 of 256).
+template <bool F8>
+__global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
+  using L = Tile<F8>;
+  using M = Wide<F8>;
+  constexpr int MR = M::kRows;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int r16 = lane & 15, g = lane >> 4;
+  float* const tops = reinterpret_cast<float*>(lds + M::kTop);
+  float* const fin = reinterpret_cast<float*>(lds + M::kFin);
+  Side* const side = reinterpret_cast<Side*>(lds + M::kSide);
+
+  const LatentPlace place = latent_place(blockIdx.x, a.side_by_side);
+  int cur;
+  if (!take_share<MR, 512>(a, place, side, reinterpret_cast<int*>(lds), &cur)) return;
+  const Args& in = side->args;
+  const float scale_log2 = a.scale_log2;
+  const auto moved = [&](int u) {
+    return uniform(*reinterpret_cast<const int*>(lds + M::kMove + (u & 1) * 4)) != 0;
+  };
+
+  if (wave < 4) {
+    // ================ scores
+    const int wq = wave >> 1, wk = wave & 1;
+    while (cur < uniform(side->end)) {
+      Piece pc;
+      const bool there = next_piece<MR>(place, side, cur, &pc);
+      cur += pc.s1 - pc.s0;
+      if (!there) continue;
+      const int u0 = 2 * pc.s0, end = min(2 * pc.s1, (pc.see_any + M::kStep - 1) / M::kStep);
+      u32x4 qf[2][18];
+      int sees[2];
+#pragma unroll
+      for (int f = 0; f < 2; ++f) sees[f] = get_queries<F8>(in, pc, pc.row0 + (wq * 2 + f) * 16 + r16, g, qf[f]);
+      float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, pend[2] = {0.f, 0.f};
+      f32x4 sc[2];
+
+      // P of step u, from its scores and the maxima so far; `edge`: masked keys may have any scale
+      const auto put_p = [&](int u, bool edge) __attribute__((always_inline)) {
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(lds + (u & 3) * M::kBytes + M::kData);
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+          const float base = m[f] == -INFINITY ? 0.f : m[f];
+          f32x4 p;
+          pend[f] = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(fmaf(sc[f][i], scale_log2, -base));
+            pend[f] += p[i];
+          }
+          const int q = (wq * 2 + f) * 16 + r16;
+          uint8_t* to = lds + M::kP + (u & 1) * M::kPBytes + q * 64 + (((2 * wk + (g >> 1)) ^ (r16 >> 2)) << 4) + (g & 1) * 8;
+          if constexpr (F8) {
+            const u32x4 w4 = *reinterpret_cast<const u32x4*>(words + wk * 16 + 4 * g);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              float e[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                e[i] = p[i] * __uint_as_float(((w4[i] >> (8 * c)) & 255u) << 23);
+                if (edge && p[i] == 0.f) e[i] = 0.f;
+              }
+              *reinterpret_cast<u32x2*>(to + c * M::kPCopy) = u32x2{pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3])};
+            }
+          } else {
+            *reinterpret_cast<u32x2*>(to) = u32x2{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3])};
+          }
+        }
+      };
+
+      bool edge = false;
+      for (int u = u0; u <= end && end > u0; ++u) {
+        lds_barrier();  // step u has landed, P of the step before is there
+        if (u > u0) {
+          if (moved(u - 1)) {  // the maximum of some query moves: again with the new one, O follows
+#pragma unroll
+            for (int f = 0; f < 2; ++f) {
+              const int q = (wq * 2 + f) * 16 + r16;
+              const float to = fmaxf(m[f], fmaxf(tops[q], tops[MR + q]));
+              const float by = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[f] - to);
+              m[f] = to;
+              l[f] *= by;
+              if (wk == 0 && g == 0) tops[2 * MR + q] = by;
+            }
+            put_p(u - 1, edge);
+            lds_barrier();
+          }
+          l[0] += pend[0];
+          l[1] += pend[1];
+        }
+        if (u == end) break;
+        __builtin_amdgcn_sched_barrier(0);
+        const uint8_t* buf = lds + (u & 3) * M::kBytes;
+
+        // ---- S^T: key fragments read kAhead before their use, two chains per block
+        f32x4 part[2][2];
+#pragma unroll
+        for (int f = 0; f < 2; ++f) part[f][0] = part[f][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        {
+          const uint8_t* row = buf + (wk * 16 + r16) * L::kRowB;
+          const uint8_t* const at[2] = {row + ((g ^ swz(r16)) << 4), row + (((4 + g) ^ swz(r16)) << 4)};
+          uint32_t word = 0;
+          if constexpr (F8) word = reinterpret_cast<const uint32_t*>(buf + M::kData)[wk * 16 + r16];
+          const auto frag = [&](int j) { return ld_u32x4(at[j & 1] + (j >> 1) * 128); };
+          u32x4 ring[kAhead];
+#pragma unroll
+          for (int j = 0; j < kAhead; ++j) ring[j] = frag(j);
+          static_for<0, L::kFrags>([&](auto jc) {
+            constexpr int j = decltype(jc)::value;
+            const u32x4 c = ring[j % kAhead];
+            if constexpr (j + kAhead < L::kFrags) ring[j % kAhead] = frag(j + kAhead);
+            if constexpr (F8 && j < 8) {
+              const float e = __uint_as_float(((word >> (8 * (j >> 1))) & 255u) << 23);
+              const bf16x8 lo = e4m3x8_to_bf16x8_scaled(c[0], c[1], e), hi = e4m3x8_to_bf16x8_scaled(c[2], c[3], e);
+#pragma unroll
+              for (int f = 0; f < 2; ++f) part[f][0] = mfma_bf16(lo, __builtin_bit_cast(bf16x8, qf[f][2 * j]), part[f][0]);
+#pragma unroll
+              for (int f = 0; f < 2; ++f)
+                part[f][1] = mfma_bf16(hi, __builtin_bit_cast(bf16x8, qf[f][2 * j + 1]), part[f][1]);
+            } else {
+#pragma unroll
+              for (int f = 0; f < 2; ++f)
+                part[f][j & 1] = mfma_bf16_16x16x32(c, qf[f][F8 ? j + 8 : j], part[f][j & 1]);
+            }
+            if constexpr (j % kFence == kFence - 1) __builtin_amdgcn_sched_barrier(0);
+          });
+        }
+#pragma unroll
+        for (int f = 0; f < 2; ++f) sc[f] = part[f][0] + part[f][1];
+        __builtin_amdgcn_sched_barrier(0);
+
+        // ---- masks: only where the step passes what some row sees, or misses a page
+        const int have = uniform(lds[M::kValid + (u & 3) * 2 + wk]);
+        edge = (u + 1) * M::kStep > pc.see_all || have == 0;
+        if (edge) {
+#pragma unroll
+          for (int f = 0; f < 2; ++f) {
+            const int upto = have ? sees[f] - (u * M::kStep + wk * 16 + 4 * g) : 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[f][i] = i < upto ? sc[f][i] : -INFINITY;
+          }
+        }
+        bool move = false;
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+          const float top = rows_max(fmaxf(fmaxf(sc[f][0], sc[f][1]), fmaxf(sc[f][2], sc[f][3]))) * scale_log2;
+          move = move || top > m[f] + kLazy;  // from -inf: any finite score
+          if (g == 0) tops[wk * MR + (wq * 2 + f) * 16 + r16] = top;
+        }
+        const bool any = __any(move);
+        if (lane == 0) lds[M::kMove + (u & 1) * 4 + wave] = any ? 1 : 0;
+        put_p(u, edge);
+      }
+#pragma unroll
+      for (int f = 0; f < 2; ++f) {
+        float sum = l[f];
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        const int q = (wq * 2 + f) * 16 + r16;
+        if (g == 0) fin[wk * MR + q] = sum;
+        if (wk == 0 && g == 0) fin[2 * MR + q] = m[f];
+      }
+      lds_barrier();
+    }
+  } else {
+    // ================ output, and the loads
+    const int w = wave - 4;
+    constexpr int CT = 8;
+    int load_off[L::kLoads];  // source bytes within the wave's group of 8 rows
+#pragma unroll
+    for (int j = 0; j < L::kLoads; ++j) {
+      const int slot = j * 64 + lane, row = slot / L::kChunks, pos = slot % L::kChunks;
+      load_off[j] = row * L::kRowB + ((pos ^ swz((w & 1) * 8 + row)) << 4);
+    }
+    while (cur < uniform(side->end)) {
+      Piece pc;
+      const bool there = next_piece<MR>(place, side, cur, &pc);
+      cur += pc.s1 - pc.s0;
+      if (!there) continue;
+      const int u0 = 2 * pc.s0, end = min(2 * pc.s1, (pc.see_any + M::kStep - 1) / M::kStep);
+
+      // Where the group's 16-row block stands in steps held .. held + 63, a lane each.
+      const int32_t* table = in.pages.table + (long long)pc.b * in.pages.max_pages;
+      int held = u0, where;
+      const auto look_up = [&]() __attribute__((always_inline)) {
+        where = find_block(in.pages, table, min(held + lane, end - 1) * 2 + (w >> 1));
+      };
+      look_up();
+      const uint8_t* src;
+      const uint32_t* src_scales;
+      uint32_t dst, dst_scales;
+      const auto aim = [&](int u) __attribute__((always_inline)) {
+        if (u == held + 64) {
+          held = u;
+          look_up();
+        }
+        const int at = __builtin_amdgcn_readlane(where, u - held);
+        const long long row = (at >= 0 ? (long long)at << 4 : 0) + (w & 1) * 8;  // no page: some row, masked
+        if (lane == 0) lds[M::kValid + (u & 3) * 2 + (w >> 1)] = at >= 0 ? 1 : 0;
+        src = a.data + row * L::kRowB;
+        dst = uniform(lds_address(lds) + (u & 3) * M::kBytes + w * 8 * L::kRowB);
+        if constexpr (F8) {
+          src_scales = a.scales + row;
+          dst_scales = uniform(lds_address(lds) + (u & 3) * M::kBytes + M::kData + w * 32);
+        }
+      };
+      const auto load = [&](int i) __attribute__((always_inline)) {
+        if (i < L::kLoads) {
+          dma_16(src, load_off[i], dst + i * 1024);
+        } else if (lane < 8) {
+          dma_4(src_scales, lane * 4, dst_scales);
+        }
+      };
+      f32x4 o[CT][4];
+#pragma unroll
+      for (int f = 0; f < 4; ++f)
+#pragma unroll
+        for (int c = 0; c < CT; ++c) o[c][f] = f32x4{0.f, 0.f, 0.f, 0.f};
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (u0 + i < end) {
+          aim(u0 + i);
+#pragma unroll
+          for (int j = 0; j < M::kLoad; ++j) load(j);
+        }
+      __builtin_amdgcn_sched_barrier(0);
+
+      if (end > u0) {  // the first step has its scores taken
+        if (u0 + 1 < end) wait_vmcnt<M::kLoad>();
+        else wait_vmcnt<0>();
+        lds_barrier();
+        if (u0 + 2 < end) {
+          aim(u0 + 2);
+#pragma unroll
+          for (int j = 0; j < M::kLoad; ++j) load(j);
+        }
+      }
+      for (int u = u0 + 1; u <= end; ++u) {
+        if (u + 1 < end) wait_vmcnt<M::kLoad>();
+        else wait_vmcnt<0>();
+        lds_barrier();  // step u has landed, P of the step before is there, and the step before that is done with
+        const bool more = u + 2 < end;
+        if (more) aim(u + 2);
+        const int v = u - 1;  // the step that is added
+        if (moved(v)) {
+          lds_barrier();
+#pragma unroll
+          for (int f = 0; f < 4; ++f) {
+            const float by = tops[2 * MR + f * 16 + r16];
+#pragma unroll
+            for (int c = 0; c < CT; ++c) o[c][f] *= by;
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+        uint8_t* buf = lds + (v & 3) * M::kBytes;
+        const int ok = uniform(*reinterpret_cast<const uint16_t*>(lds + M::kValid + (v & 3) * 2));
+        if ((v + 1) * M::kStep > pc.see_all || ok != 0x0101) {
+          // A value that a row does not see must not reach it as 0 * NaN: rows that no
+          // query sees become zeros, and Inf and NaN of rows that some do not see are
+          // cleared.  A query that sees such a row has NaN in its l: its key is the
+          // same row.  Each wave does so for its own columns.
+          constexpr int VC = F8 ? 8 : 16;  // chunks of a row's values in 128 columns
+#pragma unroll 1
+          for (int i = lane; i < M::kStep * VC; i += 64) {
+            const int r = i / VC, key = v * M::kStep + r;
+            const bool none = key >= pc.see_any || !((ok >> (8 * (r >> 4))) & 1);
+            if (!none && key < pc.see_all) continue;
+            u32x4* x = reinterpret_cast<u32x4*>(buf + r * L::kRowB + (((w * VC + i % VC) ^ swz(r)) << 4));
+            *x = none ? u32x4{0u, 0u, 0u, 0u} : only_finite<F8>(*x);
+          }
+          asm volatile("" ::: "memory");
+        }
+        __builtin_amdgcn_sched_barrier(0);
+
+        // ---- O^T += V^T P^T: lane (column r16, key octet g)
+        {
+          const uint8_t* pbuf = lds + M::kP + (v & 1) * M::kPBytes + (F8 ? w * M::kPCopy : 0) + r16 * 64 + ((g ^ (r16 >> 2)) << 4);
+          u32x4 p[4];
+#pragma unroll
+          for (int f = 0; f < 4; ++f) p[f] = ld_u32x4(pbuf + f * 16 * 64);
+          // An exclusive-or of the block into the address is the swizzle.
+          const int row = 8 * g + (F8 ? r16 >> 1 : r16 >> 2);
+          const uint32_t at = (uint32_t)(v & 3) * M::kBytes + row * L::kRowB + w * (F8 ? 128 : 256) +
+                              ((swz(row) ^ (F8 ? 0 : (lane >> 1) & 1)) << 4) + 8 * (lane & 1);
+          const auto frag = [&](int c) {
+            if constexpr (F8) {
+              const u32x2 x = lds_tr8(lds + (at ^ (c << 4)));
+              return u32x4{x[0], x[1], 0u, 0u};
+            } else {  // rows 4 further: the lowest bit of the swizzle flips
+              const u32x2 x0 = lds_tr16(lds + (at ^ ((c & 3) << 5)) + (c >> 2) * 128);
+              const u32x2 x1 = lds_tr16(lds + (at ^ ((c & 3) << 5) ^ 16) + (c >> 2) * 128 + 4 * L::kRowB);
+              return u32x4{x0[0], x0[1], x1[0], x1[1]};
+            }
+          };
+          u32x4 ring[kAhead];
+#pragma unroll
+          for (int c = 0; c < kAhead; ++c) ring[c] = frag(c);
+          static_for<0, CT>([&](auto cc) {
+            constexpr int c = decltype(cc)::value;
+            const u32x4 x = ring[c % kAhead];
+            if constexpr (c + kAhead < CT) ring[c % kAhead] = frag(c + kAhead);
+            const bf16x8 xb = F8 ? e4m3x8_to_bf16x8(x[0], x[1]) : __builtin_bit_cast(bf16x8, x);
+#pragma unroll
+            for (int f = 0; f < 4; ++f) o[c][f] = mfma_bf16(xb, __builtin_bit_cast(bf16x8, p[f]), o[c][f]);
+            if constexpr (c % 2 == 1) {
+              constexpr int x0 = (c - 1) * M::kLoad / CT, x1 = (c + 1) * M::kLoad / CT;
+              if (more) static_for<x0, x1>([&](auto y) { load(decltype(y)::value); });
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          });
+        }
+      }
+      lds_barrier();  // sums and maxima
+#pragma unroll
+      for (int f = 0; f < 4; ++f) {
+        const int q = f * 16 + r16;
+        put_rows<MR>(side, pc, end - u0, f, r16, w * 128 + 4 * g, w == 0 && g == 0, fin[2 * MR + q], fin[q] + fin[MR + q], o);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
   }
 }
 
@@ -731,12 +1116,7 @@ __global__ __launch_bounds__(256) void latent_join_long_kernel(Args a, int mr) {
     a.lse[row] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
-template <int WQ, int WK, bool F8>
-int launch(const Args& a, hipStream_t st) {
-  constexpr int mr = 16 * WQ, lds = Lds<mr, WK, F8>::kBytes;
-  FERRET_HIP_CHECK((set_lds_limit_once<latent_attention_kernel<WQ, WK, F8>>(lds)));
-  hipLaunchKernelGGL((latent_attention_kernel<WQ, WK, F8>), dim3(kUnits), dim3(64 * WQ * WK), lds, st, a);
-  FERRET_HIP_CHECK(hipGetLastError());
+int launch_join(const Args& a, int mr, hipStream_t st) {
   const unsigned rows = (unsigned)((long long)a.T * a.H);
   if (rows <= kJoinRows)
     hipLaunchKernelGGL(latent_join_long_kernel, dim3(rows, kLatent / 64), dim3(256), 0, st, a, mr);
@@ -745,12 +1125,30 @@ int launch(const Args& a, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
+template <int WQ, int WK, bool F8>
+int launch(const Args& a, hipStream_t st) {
+  constexpr int mr = 16 * WQ, lds = Lds<mr, WK, F8>::kBytes;
+  FERRET_HIP_CHECK((set_lds_limit_once<latent_attention_kernel<WQ, WK, F8>>(lds)));
+  hipLaunchKernelGGL((latent_attention_kernel<WQ, WK, F8>), dim3(kUnits), dim3(64 * WQ * WK), lds, st, a);
+  FERRET_HIP_CHECK(hipGetLastError());
+  return launch_join(a, mr, st);
+}
+
+template <bool F8>
+int launch_wide(const Args& a, hipStream_t st) {
+  constexpr int lds = Wide<F8>::kLds;
+  FERRET_HIP_CHECK((set_lds_limit_once<latent_attention_wide_kernel<F8>>(lds)));
+  hipLaunchKernelGGL((latent_attention_wide_kernel<F8>), dim3(kUnits), dim3(512), lds, st, a);
+  FERRET_HIP_CHECK(hipGetLastError());
+  return launch_join(a, Wide<F8>::kRows, st);
+}
+
 template <bool F8>
 int launch_rows(int mr, const Args& a, hipStream_t st) {
   switch (mr) {
     case 16: return launch<1, 4, F8>(a, st);
     case 32: return launch<2, 4, F8>(a, st);
-    default: return launch<4, 2, F8>(a, st);
+    default: return launch_wide<F8>(a, st);
   }
 }
 
