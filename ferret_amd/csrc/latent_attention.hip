@@ -90,7 +90,8 @@ struct Tile {
 // registers are short.
 struct Side {
   Args args;
-  int chunk, seq_at, b;  // the deal, the sequence at hand and its place on the line
+  int chunk, extra;      // the deal
+  int seq_at, b;         // the sequence at hand and its place on the line
   LatentSeq seq;
   int first_row;         // the tile's first row among all [T * H]
   int slot;              // of the partial result, -1 for a whole tile
@@ -160,7 +161,7 @@ __device__ __forceinline__ float rows_max(float v) {
 __device__ __forceinline__ int swz(int r) { return ((r >> 1) & 4) | (r & 2) | ((r >> 2) & 1); }
 
 // The start of a work-group's share of the line: false where it has none.  The page
-// table's first lines come under the loads of the lengths.  tot: 8 words of LDS.
+// table's first lines come under the loads of the lengths.  tot: 24 words of LDS.
 template <int MR, int NT>
 __device__ __forceinline__ bool take_share(const Args& a, LatentPlace place, Side* side, int* tot, int* cur) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -168,42 +169,68 @@ __device__ __forceinline__ bool take_share(const Args& a, LatentPlace place, Sid
   const int per = (a.B + NT - 1) / NT;
   const int b0 = threadIdx.x * per;
   LatentSeq s{};
-  int mine = 0;
+  int mine = 0, my_groups = 0;
   for (int i = 0; i < per && b0 + i < a.B; ++i) {
     s = sequence<MR>(a, b0 + i);
-    mine += s.work();
+    mine += s.work(0);
+    my_groups += s.groups;
   }
-  int incl = mine;
+  int incl = mine, incl_groups = my_groups;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
-    const int o = __shfl_up(incl, off, 64);
-    if (lane >= off) incl += o;
+    const int o = __shfl_up(incl, off, 64), og = __shfl_up(incl_groups, off, 64);
+    if (lane >= off) {
+      incl += o;
+      incl_groups += og;
+    }
   }
-  if (lane == 63) tot[wave] = incl;
+  constexpr int NW = NT / 64;
+  if (lane == 63) {
+    tot[wave] = incl;
+    tot[NW + wave] = incl_groups;
+  }
   __syncthreads();
   asm volatile("" ::"v"(near));
-  int before = 0, total = 0;
+  int before = 0, total = 0, groups_before = 0, groups = 0;
 #pragma unroll
-  for (int w = 0; w < NT / 64; ++w) {
-    if (w < wave) before += tot[w];
+  for (int w = 0; w < NW; ++w) {
+    if (w < wave) {
+      before += tot[w];
+      groups_before += tot[NW + w];
+    }
     total += tot[w];
+    groups += tot[NW + w];
   }
-  const int chunk = latent_chunk(total, kUnits / a.side_by_side, a.min_steps);
+  const int units = kUnits / a.side_by_side;
+  int chunk = latent_chunk(total, units, a.min_steps), extra = kLatentExtra;
+  if (per == 1) {  // more sequences than threads do not all fit
+    const bool fits = latent_fits(s, chunk);
+    if (lane == 0) tot[2 * NW + wave] = 0;
+    if (__any(!fits) && lane == 0) tot[2 * NW + wave] = 1;
+    __syncthreads();
+    int misfits = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) misfits |= tot[2 * NW + w];
+    if (misfits == 0) extra = 0;
+  }
+  total += extra * groups;
+  if (extra != 0) chunk = latent_chunk(total, units, a.min_steps);
   const int start = (int)min((long long)place.unit * chunk, (long long)total);
-  const int excl = before + incl - mine;
+  const int excl = before + incl - mine + extra * (groups_before + incl_groups - my_groups);
   if (start >= total) return false;
-  if (excl <= start && start < excl + mine) {
+  if (excl <= start && start < excl + mine + extra * my_groups) {
     int at = excl, i = 0;
     if (per > 1)
       for (;; ++i) {
         s = sequence<MR>(a, b0 + i);
-        if (start < at + s.work() || i + 1 == per) break;
-        at += s.work();
+        if (start < at + s.work(extra) || i + 1 == per) break;
+        at += s.work(extra);
       }
     side->b = b0 + i;
     put_seq(&side->seq, s);
     side->seq_at = at;
     side->chunk = chunk;
+    side->extra = extra;
     side->end = min(start + chunk, total);
     put_args(&side->args, a);
   }
@@ -215,33 +242,39 @@ __device__ __forceinline__ bool take_share(const Args& a, LatentPlace place, Sid
 // A piece of a row tile: steps s0 .. s1 of sequence b.
 struct Piece {
   int b, s0, s1, len, past, q0;
+  bool one;               // the sequence has one new token
   int row0, row_last;     // query rows of the sequence
   int see_all, see_any;   // keys that the first and the last token of the tile see
 };
 
 // The piece at `cur`, its place noted in LDS and its rows' record in the workspace;
-// false for a tile that is not there (fewer tiles than work-groups side by side).
+// false where there are no keys (the extra steps) or no rows (fewer tiles than
+// work-groups side by side).
 template <int MR>
 __device__ __forceinline__ bool next_piece(LatentPlace place, Side* side, int cur, Piece* p) {
   const Args& in = side->args;
+  const int extra = side->extra;
   int b = uniform(side->b), seq_at = uniform(side->seq_at);
   LatentSeq s = get_seq(&side->seq);
-  while (cur >= seq_at + s.work() && b + 1 < in.B) {  // the next sequence with rows
-    seq_at += s.work();
+  while (cur >= seq_at + s.work(extra) && b + 1 < in.B) {  // the next sequence with rows
+    seq_at += s.work(extra);
     s = sequence<MR>(in, ++b);
   }
   p->b = b = uniform(b);
   p->len = uniform(s.len);
   p->q0 = uniform(s.q0);
-  const int steps = uniform(s.steps), group = uniform((cur - seq_at) / steps);
-  p->s0 = uniform(cur - seq_at - group * steps);
-  p->s1 = uniform(min(steps, p->s0 + (side->end - cur)));
-  p->row0 = (group * in.side_by_side + place.lane) * MR;
+  const int steps = uniform(s.steps), line = uniform(s.steps + extra), n = uniform(s.n);
+  const int group = s.groups > 1 ? uniform((cur - seq_at) / line) : 0;
+  p->s0 = uniform(cur - seq_at - group * line);
+  p->s1 = uniform(min(line, p->s0 + (side->end - cur)));
+  p->row0 = uniform((group * in.side_by_side + place.lane) * MR);
   p->row_last = uniform(min(p->row0 + MR, s.rows) - 1);
-  if (p->row_last < p->row0) return false;
-  p->past = p->len - uniform(s.n) + 1;
-  p->see_all = uniform(max(in.causal ? p->past + p->row0 / in.H : p->len, 0));
-  p->see_any = uniform(max(in.causal ? p->past + p->row_last / in.H : p->len, 0));
+  if (p->row_last < p->row0 || p->s0 >= steps) return false;
+  p->past = p->len - n + 1;
+  const bool causal = in.causal && n > 1;  // one token sees all
+  p->see_all = causal ? uniform(max(p->past + p->row0 / in.H, 0)) : p->len;
+  p->see_any = causal ? uniform(max(p->past + p->row_last / in.H, 0)) : p->len;
+  p->one = n == 1;
   const int chunk = side->chunk, first_row = p->q0 * in.H + p->row0;
   __syncthreads();  // the piece before is done with its record and buffers
   if (threadIdx.x == 0) {
@@ -250,7 +283,7 @@ __device__ __forceinline__ bool next_piece(LatentPlace place, Side* side, int cu
     side->seq_at = seq_at;
     side->first_row = first_row;
     side->slot =
-        p->s0 == 0 && p->s1 == steps ? -1 : latent_slot(place.unit, place.lane, in.side_by_side, cur, chunk);
+        p->s0 == 0 && p->s1 >= steps ? -1 : latent_slot(place.unit, place.lane, in.side_by_side, cur, chunk);
   }
   if (p->s0 == 0 && (int)threadIdx.x <= p->row_last - p->row0) {
     const LatentRecord r = latent_record(place.unit, place.lane, in.side_by_side, cur, steps, chunk);
@@ -271,7 +304,7 @@ __device__ __forceinline__ int find_block(const Pages& pages, const int32_t* tab
 // A fragment of queries (column r16 = row `r` of the sequence), and the keys that it sees.
 template <bool F8>
 __device__ __forceinline__ int get_queries(const Args& in, const Piece& p, int r, int g, u32x4 (&qf)[18]) {
-  const int rc = min(r, p.row_last), tok = rc / in.H, head = rc - tok * in.H;  // past the tile: its last row
+  const int rc = min(r, p.row_last), tok = p.one ? 0 : rc / in.H, head = rc - tok * in.H;  // past the tile: its last row
   const uint16_t* ql = in.ql + (long long)(p.q0 + tok) * in.ql_t + (long long)head * in.ql_h;
   const uint16_t* qr = in.qr + (long long)(p.q0 + tok) * in.qr_t + (long long)head * in.qr_h;
 #pragma unroll
@@ -300,7 +333,7 @@ __device__ __forceinline__ u32x4 only_finite(u32x4 v) {
 // Row r of the tile done: its output, or its part of a piece.  o: blocks of 16 columns
 // from `col` on, 4 of each per lane.
 template <int MR, int CT, int WQ>
-__device__ __forceinline__ void put_rows(const Side* side, const Piece& p, int steps_taken, int f, int r16, int col,
+__device__ __forceinline__ void put_rows(const Side* side, const Piece& p, int f, int r16, int col,
                                          bool stats, float top, float sum, const f32x4 (&o)[CT][WQ]) {
   const Args& in = side->args;
   const int r = f * 16 + r16, slot = uniform(side->slot);
@@ -318,11 +351,9 @@ __device__ __forceinline__ void put_rows(const Side* side, const Piece& p, int s
   } else {
     const long long at = (long long)slot * MR + r;
     if (stats) in.ml()[at] = make_float2(top, sum);
-    if (steps_taken > 0) {
-      float* to = in.part(MR) + at * kLatent + col;
+    float* to = in.part(MR) + at * kLatent + col;
 #pragma unroll
-      for (int c = 0; c < CT; ++c) *reinterpret_cast<f32x4*>(to + c * 16) = o[c][f];
-    }
+    for (int c = 0; c < CT; ++c) *reinterpret_cast<f32x4*>(to + c * 16) = o[c][f];
   }
 }
 
@@ -655,7 +686,7 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void latent_attention_ke
       float sum = tops[f * 16 + r16];
 #pragma unroll
       for (int w = 1; w < WK; ++w) sum += tops[w * MR + f * 16 + r16];
-      put_rows<MR>(side, pc, last - s0, f, r16, wave * CT * 16 + 4 * g, wave == 0 && g == 0, tops[WK * MR + f * 16 + r16],
+      put_rows<MR>(side, pc, f, r16, wave * CT * 16 + 4 * g, wave == 0 && g == 0, tops[WK * MR + f * 16 + r16],
                    sum, o);
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -1003,7 +1034,7 @@ __global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
 #pragma unroll
       for (int f = 0; f < 4; ++f) {
         const int q = f * 16 + r16;
-        put_rows<MR>(side, pc, end - u0, f, r16, w * 128 + 4 * g, w == 0 && g == 0, fin[2 * MR + q], fin[q] + fin[MR + q], o);
+        put_rows<MR>(side, pc, f, r16, w * 128 + 4 * g, w == 0 && g == 0, fin[2 * MR + q], fin[q] + fin[MR + q], o);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -1032,8 +1063,15 @@ __device__ __forceinline__ float wave_add(float v) {
   return v;
 }
 
+// A piece's weight and part of the sum.  l may be NaN where the maximum is -inf (a NaN
+// that is a piece's only key), and the row is NaN then.
+__device__ __forceinline__ float piece_weight(float2 v, float base) { return __builtin_amdgcn_exp2f(v.x - base); }
+__device__ __forceinline__ float piece_sum(float2 v, float base) {
+  return v.y != 0.f ? v.y * piece_weight(v, base) : 0.f;
+}
+
 // Many rows, few pieces each: a wave per row, 8 columns per lane, the pieces' weights
-// 64 at a time in the lanes.
+// 64 at a time in the lanes, eight pieces' loads under way together.
 __global__ __launch_bounds__(256) void latent_join_kernel(Args a, int mr, int rows) {
   const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (row >= rows) return;
@@ -1051,16 +1089,24 @@ __global__ __launch_bounds__(256) void latent_join_kernel(Args a, int mr, int ro
   float sum = 0.f;
   for (int j0 = 0; j0 < where.pieces; j0 += 64) {
     const float2 v = j0 + lane < where.pieces ? ml[at(j0 + lane)] : make_float2(-INFINITY, 0.f);
-    // l may be NaN where the maximum is -inf; there and only there O is not written, or zero
-    sum += v.y != 0.f ? v.y * __builtin_amdgcn_exp2f(v.x - base) : 0.f;
-    const float w = v.x > -INFINITY ? __builtin_amdgcn_exp2f(v.x - base) : 0.f;
-#pragma unroll 4
-    for (int j = 0; j < min(where.pieces - j0, 64); ++j) {
-      const float wj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), j));
-      if (wj != 0.f) {
-        const float* from = part + at(j0 + j) * kLatent;
-        acc[0] += *reinterpret_cast<const f32x4*>(from) * wj;
-        acc[1] += *reinterpret_cast<const f32x4*>(from + 256) * wj;
+    sum += piece_sum(v, base);
+    const float w = piece_weight(v, base);
+    const int n = min(where.pieces - j0, 64);
+    for (int j = 0; j < n; j += 8) {
+      f32x4 x[8][2];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float* from = part + at(j0 + min(j + i, n - 1)) * kLatent;  // past the last: again, by weight 0
+        x[i][0] = *reinterpret_cast<const f32x4*>(from);
+        x[i][1] = *reinterpret_cast<const f32x4*>(from + 256);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float wi = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), min(j + i, 63)));
+        if (j + i < n) {
+          acc[0] += x[i][0] * wi;
+          acc[1] += x[i][1] * wi;
+        }
       }
     }
   }
@@ -1074,8 +1120,8 @@ __global__ __launch_bounds__(256) void latent_join_kernel(Args a, int mr, int ro
     a.lse[row] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
-// Few rows, up to kUnits pieces each: a work-group per row and 64 columns, 16 lanes
-// across and the pieces dealt to 16 groups of lanes.
+// Few rows, up to kUnits pieces each: a work-group per row and 32 columns, 8 lanes
+// across and the pieces dealt to 32 groups of lanes, at most 8 each.
 __global__ __launch_bounds__(256) void latent_join_long_kernel(Args a, int mr) {
   __shared__ f32x4 red[256];
   __shared__ float weight[kUnits], stat[8];
@@ -1083,32 +1129,35 @@ __global__ __launch_bounds__(256) void latent_join_long_kernel(Args a, int mr) {
   LatentRecord where;
   int r;
   if (!to_join(a, mr, row, &where, &r)) return;
+  const int across = threadIdx.x & 7, group = threadIdx.x >> 3, col = blockIdx.y * 32 + across * 4;
   const auto at = [&](int j) { return (long long)latent_record_slot(where, a.side_by_side, j) * mr + r; };
   const float2 v = (int)threadIdx.x < where.pieces ? a.ml()[at(threadIdx.x)] : make_float2(-INFINITY, 0.f);
+  const float* part = a.part(mr) + col;
+  f32x4 x[kUnits / 32];
+#pragma unroll
+  for (int i = 0; i < kUnits / 32; ++i) {
+    const int j = group + 32 * i;
+    x[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (j < where.pieces) x[i] = *reinterpret_cast<const f32x4*>(part + at(j) * kLatent);
+  }
   float top = wave_max(v.x);
   if (lane == 0) stat[wave] = top;
   __syncthreads();
   top = fmaxf(fmaxf(stat[0], stat[1]), fmaxf(stat[2], stat[3]));
   const float base = top == -INFINITY ? 0.f : top;
-  // l may be NaN where the maximum is -inf; there and only there O is not written, or zero
-  float sum = wave_add(v.y != 0.f ? v.y * __builtin_amdgcn_exp2f(v.x - base) : 0.f);
-  weight[threadIdx.x] = v.x > -INFINITY ? __builtin_amdgcn_exp2f(v.x - base) : 0.f;
+  float sum = wave_add(piece_sum(v, base));
+  weight[threadIdx.x] = piece_weight(v, base);
   if (lane == 0) stat[4 + wave] = sum;
   __syncthreads();
   sum = (stat[4] + stat[5]) + (stat[6] + stat[7]);
-  const int across = threadIdx.x & 15, group = threadIdx.x >> 4, col = blockIdx.y * 64 + across * 4;
-  const float* part = a.part(mr) + col;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-  for (int j = group; j < where.pieces; j += 16) {
-    const float w = weight[j];
-    if (w != 0.f) acc += *reinterpret_cast<const f32x4*>(part + at(j) * kLatent) * w;
-  }
+#pragma unroll
+  for (int i = 0; i < kUnits / 32; ++i) acc += x[i] * weight[group + 32 * i];
   red[threadIdx.x] = acc;
   __syncthreads();
   if (group != 0) return;
-#pragma unroll
-  for (int i = 1; i < 16; ++i) acc += red[i * 16 + across];
+#pragma unroll 8
+  for (int i = 1; i < 32; ++i) acc += red[i * 8 + across];
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   *reinterpret_cast<u32x2*>(a.out + (long long)row * kLatent + col) =
       u32x2{pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv)};
@@ -1119,7 +1168,7 @@ __global__ __launch_bounds__(256) void latent_join_long_kernel(Args a, int mr) {
 int launch_join(const Args& a, int mr, hipStream_t st) {
   const unsigned rows = (unsigned)((long long)a.T * a.H);
   if (rows <= kJoinRows)
-    hipLaunchKernelGGL(latent_join_long_kernel, dim3(rows, kLatent / 64), dim3(256), 0, st, a, mr);
+    hipLaunchKernelGGL(latent_join_long_kernel, dim3(rows, kLatent / 32), dim3(256), 0, st, a, mr);
   else
     hipLaunchKernelGGL(latent_join_kernel, dim3((rows + 3) / 4), dim3(256), 0, st, a, mr, (int)rows);
   return (int)hipGetLastError();
@@ -1197,7 +1246,7 @@ extern "C" int ferret_latent_attention(const void* q_latent, long long ql_token,
   const int mr = tile_rows(T, B, H);
   // steps of the whole batch are counted in 32 bits
   FERRET_REQUIRE((long long)pages * page_size < (1LL << 35), FERRET_ERR_SHAPE);
-  const long long tiles = (long long)T * H / mr + B, most = ((long long)max_pages * page_size + kKeys - 1) / kKeys;
+  const long long tiles = (long long)T * H / mr + B, most = ((long long)max_pages * page_size + kKeys - 1) / kKeys + kLatentExtra;
   FERRET_REQUIRE(tiles * most < (1LL << 31), FERRET_ERR_SHAPE);
   FERRET_REQUIRE(ws != nullptr && ws_bytes >= ferret_latent_attention_workspace(B, T, H) && (bits(ws) & 15) == 0,
                  FERRET_ERR_WORKSPACE);

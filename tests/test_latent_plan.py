@@ -29,21 +29,29 @@ WALKER = r"""
 #include "latent_plan.hpp"
 using namespace ferret;
 
-static long long bad = 0, walked = 0;
+static long long bad = 0, walked = 0, whole = 0, cut = 0;
 #define CHECK(c) do { if (!(c) && bad++ < 20) std::printf("line %d: %s\n", __LINE__, #c); } while (0)
 
 static void walk(const std::vector<int>& cu, const std::vector<int>& lens, int T, int H, int mr, int side, int most,
                  int min_steps) {
   const int B = (int)lens.size(), units = kLatentUnits / side;
   auto seq = [&](int b) { return latent_seq(cu[b], cu[b + 1], lens[b], T, H, mr, side, most); };
-  int total = 0;
+  int total = 0, groups = 0;
+  const int threads = mr == 16 ? 256 : 512;
   for (int b = 0; b < B; ++b) {
     const LatentSeq s = seq(b);
     CHECK(s.q0 >= 0 && s.n >= 0 && s.q0 + s.n <= T && s.len >= 0 && s.len <= most && s.steps >= 1);
     CHECK((long long)s.groups * mr * side >= s.rows && (s.groups == 0 || (s.groups - 1) * mr * side < s.rows));
-    total += s.work();
+    total += s.work(0);
+    groups += s.groups;
   }
-  const int chunk = latent_chunk(total, units, min_steps);
+  int chunk = latent_chunk(total, units, min_steps), extra = kLatentExtra;
+  bool fits = B <= threads;
+  for (int b = 0; b < B; ++b) fits = fits && latent_fits(seq(b), chunk);
+  if (fits) extra = 0;
+  total += extra * groups;
+  if (extra != 0) chunk = latent_chunk(total, units, min_steps);
+  (fits ? whole : cut) += 1;
   long long expected = 0;
   std::set<std::tuple<int, int, int>> done;
   std::map<std::pair<int, int>, std::vector<std::pair<int, int>>> pieces;  // tile -> (first step, slot)
@@ -58,24 +66,25 @@ static void walk(const std::vector<int>& cu, const std::vector<int>& lens, int T
     if (start >= total) continue;
     const int end = plan_min(start + chunk, total);
     int b = 0, seq_at = 0, cur = start;
-    while (seq_at + seq(b).work() <= start) seq_at += seq(b++).work();
+    while (seq_at + seq(b).work(extra) <= start) seq_at += seq(b++).work(extra);
     while (cur < end) {
       LatentSeq s = seq(b);
-      while (cur >= seq_at + s.work() && b + 1 < B) {
-        seq_at += s.work();
+      while (cur >= seq_at + s.work(extra) && b + 1 < B) {
+        seq_at += s.work(extra);
         s = seq(++b);
       }
-      const int group = (cur - seq_at) / s.steps, s0 = cur - seq_at - group * s.steps, s1 = plan_min(s.steps, s0 + end - cur);
+      const int line = s.steps + extra, group = s.groups > 1 ? (cur - seq_at) / line : 0;
+      const int s0 = cur - seq_at - group * line, s1 = plan_min(line, s0 + end - cur);
       const int tile = group * side + at.lane;
       CHECK(group >= 0 && group < s.groups && s0 >= 0 && s1 > s0);
       const int row0 = tile * mr, row_last = plan_min(row0 + mr, s.rows) - 1;
-      if (row_last < row0) {
+      if (row_last < row0 || s0 >= s.steps) {
         cur += s1 - s0;
         continue;
       }
       CHECK(row_last >= row0 && (long long)s.q0 * H + row_last < (long long)T * H);
-      for (int t = s0; t < s1; ++t) CHECK(done.insert({b, tile, t}).second);
-      if (!(s0 == 0 && s1 == s.steps)) {
+      for (int t = s0; t < plan_min(s1, s.steps); ++t) CHECK(done.insert({b, tile, t}).second);
+      if (!(s0 == 0 && s1 >= s.steps)) {
         const int slot = latent_slot(at.unit, at.lane, side, cur, chunk);
         CHECK(slot >= 0 && slot < 2 * kLatentUnits && slots.insert(slot).second);
         pieces[{b, tile}].push_back({s0, slot});
@@ -138,6 +147,13 @@ int main() {
           for (int j = 0; j < n; ++j)
             CHECK(latent_record_slot(r, side, j) >= 0 && latent_record_slot(r, side, j) < 2 * kLatentUnits);
       }
+  for (int k = 0; k < 200; ++k) {  // equal lengths, some of which fit the shares
+    const int B = 1 << pick(0, 8), n = pick(1, 4);
+    std::vector<int> cu{0}, lens(B, 64 * pick(1, 60));
+    for (int b = 0; b < B; ++b) cu.push_back(cu.back() + n);
+    walk(cu, lens, cu.back(), 16, 16 << pick(0, 2), 1 << pick(0, 3), 1 << 16, 2);
+  }
+  CHECK(whole > 20 && cut > 100);
   std::printf("%lld walked, %lld violations\n", walked, bad);
   return bad != 0;
 }
