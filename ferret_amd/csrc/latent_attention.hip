@@ -695,48 +695,49 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void latent_attention_ke
 
 // ---- 64 query rows: two products at a time
 
-// LDS: four buffers of 32 keys, P twice, and the small records.
+// A step is 32 keys (bf16) or 64 (e4m3).  LDS: the buffers (one step's values, one's
+// keys, the others on their way), P twice, and the small records.
 template <bool F8>
 struct Wide {
-  static constexpr int kRows = 64, kStep = 32, kBufs = 4;
+  static constexpr int kRows = 64, kStep = F8 ? 64 : 32, kBufs = F8 ? 3 : 4, kAway = kBufs - 2;
   static constexpr int kData = kStep * Tile<F8>::kRowB, kBytes = kData + (F8 ? kStep * 4 : 0);
-  static constexpr int kCopies = F8 ? 4 : 1, kPCopy = kRows * kStep * 2, kPBytes = kCopies * kPCopy;
-  static constexpr int kP = kBufs * kBytes;             // P [2][copy][query][32 keys] bf16
+  static constexpr int kPRow = kStep * 2, kPBytes = kRows * kPRow;
+  static constexpr int kP = kBufs * kBytes;             // P [2][query][keys] bf16
   static constexpr int kTop = kP + 2 * kPBytes;         // maxima [2][64], factors [64]
   static constexpr int kFin = kTop + 3 * kRows * 4;     // sums [2][64], maxima [64] of the piece
-  static constexpr int kValid = kFin + 3 * kRows * 4;   // validity of the 16-row blocks, per buffer
-  static constexpr int kMove = kValid + 16;             // [2][4]: which waves saw the maximum move
-  static constexpr int kSide = kMove + 16;
+  static constexpr int kFlags = kFin + 3 * kRows * 4;   // per step parity: which waves saw the maximum move [4],
+  static constexpr int kValid = kFlags + 16;            // per buffer: validity of its 16-row blocks [4]
+  static constexpr int kSide = kValid + 16;
   static constexpr int kLds = kSide + sizeof(Side);
-  static constexpr int kLoad = Tile<F8>::kLoads + (F8 ? 1 : 0);  // loads of a wave per step
+  static constexpr int kGroups = kStep / 32;                                  // groups of 8 rows that a wave loads
+  static constexpr int kLoad = kGroups * Tile<F8>::kLoads + (F8 ? 1 : 0);     // its loads per step
 };
 static_assert(Wide<true>::kLds <= 160 * 1024 && Wide<false>::kLds <= 160 * 1024, "LDS of a CU");
 
-// Waves 0 - 3 take the scores of 32 keys (32 queries x 16 keys each) while waves 4 - 7,
-// one of them on every SIMD beside one of the others, add the 32 keys before to the
-// output (64 queries x 128 columns each) and load the keys to come: the matrix unit
-// is fed by one while the other is at its softmax, at a barrier or at its loads, and
-// neither holds more than half of the registers (Q is 144, O 128 of 256).
+// Waves 0 - 3 take the scores of one step (32 queries and half of the keys each) while
+// waves 4 - 7, one of them on every SIMD beside one of the others, add the step before
+// to the output (64 queries x 128 columns each) and load the keys to come: the matrix
+// unit is fed by one while the other is at its softmax, at a barrier or at its loads,
+// and neither holds more than half of the registers (Q is 144, O 128 of 256).
 template <bool F8>
 __global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
   using L = Tile<F8>;
   using M = Wide<F8>;
-  constexpr int MR = M::kRows;
+  constexpr int MR = M::kRows, KT = M::kStep / 32;  // 16-key blocks of a wave's scores
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int r16 = lane & 15, g = lane >> 4;
   float* const tops = reinterpret_cast<float*>(lds + M::kTop);
   float* const fin = reinterpret_cast<float*>(lds + M::kFin);
   Side* const side = reinterpret_cast<Side*>(lds + M::kSide);
+  // P of a query: chunk c of 8 keys stands at c ^ swz_p(query)
+  const int zp = M::kStep == 64 ? r16 >> 1 : r16 >> 2;
 
   const LatentPlace place = latent_place(blockIdx.x, a.side_by_side);
   int cur;
   if (!take_share<MR, 512>(a, place, side, reinterpret_cast<int*>(lds), &cur)) return;
   const Args& in = side->args;
   const float scale_log2 = a.scale_log2;
-  const auto moved = [&](int u) {
-    return uniform(*reinterpret_cast<const int*>(lds + M::kMove + (u & 1) * 4)) != 0;
-  };
 
   if (wave < 4) {
     // ================ scores
@@ -746,52 +747,60 @@ __global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
       const bool there = next_piece<MR>(place, side, cur, &pc);
       cur += pc.s1 - pc.s0;
       if (!there) continue;
-      const int u0 = 2 * pc.s0, end = min(2 * pc.s1, (pc.see_any + M::kStep - 1) / M::kStep);
+      const int u0 = pc.s0 * (64 / M::kStep);
+      const int end = min(pc.s1 * (64 / M::kStep), (pc.see_any + M::kStep - 1) / M::kStep);
       u32x4 qf[2][18];
       int sees[2];
 #pragma unroll
       for (int f = 0; f < 2; ++f) sees[f] = get_queries<F8>(in, pc, pc.row0 + (wq * 2 + f) * 16 + r16, g, qf[f]);
       float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, pend[2] = {0.f, 0.f};
-      f32x4 sc[2];
+      f32x4 sc[KT][2];
 
-      // P of step u, from its scores and the maxima so far; `edge`: masked keys may have any scale
-      const auto put_p = [&](int u, bool edge) __attribute__((always_inline)) {
-        const uint32_t* words = reinterpret_cast<const uint32_t*>(lds + (u & 3) * M::kBytes + M::kData);
+      // P of step u from its scores and the maxima so far
+      const auto put_p = [&](int u) __attribute__((always_inline)) {
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
           const float base = m[f] == -INFINITY ? 0.f : m[f];
-          f32x4 p;
           pend[f] = 0.f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            p[i] = __builtin_amdgcn_exp2f(fmaf(sc[f][i], scale_log2, -base));
-            pend[f] += p[i];
-          }
-          const int q = (wq * 2 + f) * 16 + r16;
-          uint8_t* to = lds + M::kP + (u & 1) * M::kPBytes + q * 64 + (((2 * wk + (g >> 1)) ^ (r16 >> 2)) << 4) + (g & 1) * 8;
-          if constexpr (F8) {
-            const u32x4 w4 = *reinterpret_cast<const u32x4*>(words + wk * 16 + 4 * g);
+          for (int k = 0; k < KT; ++k) {
+            f32x4 p;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              float e[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                e[i] = p[i] * __uint_as_float(((w4[i] >> (8 * c)) & 255u) << 23);
-                if (edge && p[i] == 0.f) e[i] = 0.f;
-              }
-              *reinterpret_cast<u32x2*>(to + c * M::kPCopy) = u32x2{pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3])};
+            for (int i = 0; i < 4; ++i) {
+              p[i] = __builtin_amdgcn_exp2f(fmaf(sc[k][f][i], scale_log2, -base));
+              pend[f] += p[i];
             }
-          } else {
-            *reinterpret_cast<u32x2*>(to) = u32x2{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3])};
+            const int q = (wq * 2 + f) * 16 + r16, chunk = 2 * (wk * KT + k) + (g >> 1);
+            *reinterpret_cast<u32x2*>(lds + M::kP + (u & 1) * M::kPBytes + q * M::kPRow + ((chunk ^ zp) << 4) + (g & 1) * 8) =
+                u32x2{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3])};
           }
         }
       };
 
-      bool edge = false;
       for (int u = u0; u <= end && end > u0; ++u) {
         lds_barrier();  // step u has landed, P of the step before is there
+        // Everything that the step reads first goes out before anything is waited for.
+        const int buffer = u % M::kBufs;
+        const int flags = *reinterpret_cast<const int*>(lds + M::kFlags + ((u & 1) ^ 1) * 4);
+        const uint32_t valid = *reinterpret_cast<const uint32_t*>(lds + M::kValid + buffer * 4);
+        const uint8_t* buf = lds + buffer * M::kBytes;
+        const uint8_t* row = buf + (wk * KT * 16 + r16) * L::kRowB;
+        const uint8_t* const at[2] = {row + ((g ^ swz(r16)) << 4), row + (((4 + g) ^ swz(r16)) << 4)};
+        uint32_t word[KT];
+        if constexpr (F8)
+#pragma unroll
+          for (int k = 0; k < KT; ++k)
+            word[k] = reinterpret_cast<const uint32_t*>(buf + M::kData)[(wk * KT + k) * 16 + r16];
+        constexpr int NF = KT * L::kFrags;
+        const auto frag = [&](int i) {  // i = (chunk, block)
+          const int j = i / KT, k = i % KT;
+          return ld_u32x4(at[j & 1] + k * 16 * L::kRowB + (j >> 1) * 128);
+        };
+        u32x4 ring[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) ring[i] = frag(i);
         if (u > u0) {
-          if (moved(u - 1)) {  // the maximum of some query moves: again with the new one, O follows
+          if (uniform(flags) != 0) {  // the maximum of some query moves: again with the new one, O follows
 #pragma unroll
             for (int f = 0; f < 2; ++f) {
               const int q = (wq * 2 + f) * 16 + r16;
@@ -801,7 +810,7 @@ __global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
               l[f] *= by;
               if (wk == 0 && g == 0) tops[2 * MR + q] = by;
             }
-            put_p(u - 1, edge);
+            put_p(u - 1);
             lds_barrier();
           }
           l[0] += pend[0];
@@ -809,66 +818,70 @@ __global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
         }
         if (u == end) break;
         __builtin_amdgcn_sched_barrier(0);
-        const uint8_t* buf = lds + (u & 3) * M::kBytes;
 
-        // ---- S^T: key fragments read kAhead before their use, two chains per block
+        // ---- S^T: key fragments read kAhead before their use, four chains of accumulation
         f32x4 part[2][2];
 #pragma unroll
         for (int f = 0; f < 2; ++f) part[f][0] = part[f][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-        {
-          const uint8_t* row = buf + (wk * 16 + r16) * L::kRowB;
-          const uint8_t* const at[2] = {row + ((g ^ swz(r16)) << 4), row + (((4 + g) ^ swz(r16)) << 4)};
-          uint32_t word = 0;
-          if constexpr (F8) word = reinterpret_cast<const uint32_t*>(buf + M::kData)[wk * 16 + r16];
-          const auto frag = [&](int j) { return ld_u32x4(at[j & 1] + (j >> 1) * 128); };
-          u32x4 ring[kAhead];
+        static_for<0, NF>([&](auto ic) {
+          constexpr int i = decltype(ic)::value, j = i / KT, k = i % KT;
+          const u32x4 c = ring[i % kAhead];
+          if constexpr (i + kAhead < NF) ring[i % kAhead] = frag(i + kAhead);
+          if constexpr (F8 && j < 8) {
+            constexpr int lo_at = KT == 2 ? k : 0, hi_at = KT == 2 ? k : 1;
+            const float e = __uint_as_float(((word[k] >> (8 * (j >> 1))) & 255u) << 23);
+            const bf16x8 lo = e4m3x8_to_bf16x8_scaled(c[0], c[1], e), hi = e4m3x8_to_bf16x8_scaled(c[2], c[3], e);
 #pragma unroll
-          for (int j = 0; j < kAhead; ++j) ring[j] = frag(j);
-          static_for<0, L::kFrags>([&](auto jc) {
-            constexpr int j = decltype(jc)::value;
-            const u32x4 c = ring[j % kAhead];
-            if constexpr (j + kAhead < L::kFrags) ring[j % kAhead] = frag(j + kAhead);
-            if constexpr (F8 && j < 8) {
-              const float e = __uint_as_float(((word >> (8 * (j >> 1))) & 255u) << 23);
-              const bf16x8 lo = e4m3x8_to_bf16x8_scaled(c[0], c[1], e), hi = e4m3x8_to_bf16x8_scaled(c[2], c[3], e);
+            for (int f = 0; f < 2; ++f)
+              part[f][lo_at] = mfma_bf16(lo, __builtin_bit_cast(bf16x8, qf[f][2 * j]), part[f][lo_at]);
 #pragma unroll
-              for (int f = 0; f < 2; ++f) part[f][0] = mfma_bf16(lo, __builtin_bit_cast(bf16x8, qf[f][2 * j]), part[f][0]);
+            for (int f = 0; f < 2; ++f)
+              part[f][hi_at] = mfma_bf16(hi, __builtin_bit_cast(bf16x8, qf[f][2 * j + 1]), part[f][hi_at]);
+          } else {
+            constexpr int to = KT == 2 ? k : j & 1;
 #pragma unroll
-              for (int f = 0; f < 2; ++f)
-                part[f][1] = mfma_bf16(hi, __builtin_bit_cast(bf16x8, qf[f][2 * j + 1]), part[f][1]);
-            } else {
+            for (int f = 0; f < 2; ++f) part[f][to] = mfma_bf16_16x16x32(c, qf[f][F8 ? j + 8 : j], part[f][to]);
+          }
+          if constexpr (i % kFence == kFence - 1) __builtin_amdgcn_sched_barrier(0);
+        });
 #pragma unroll
-              for (int f = 0; f < 2; ++f)
-                part[f][j & 1] = mfma_bf16_16x16x32(c, qf[f][F8 ? j + 8 : j], part[f][j & 1]);
-            }
-            if constexpr (j % kFence == kFence - 1) __builtin_amdgcn_sched_barrier(0);
-          });
+        for (int f = 0; f < 2; ++f) {
+          if constexpr (KT == 2) {
+            sc[0][f] = part[f][0];
+            sc[KT - 1][f] = part[f][1];
+          } else {
+            sc[0][f] = part[f][0] + part[f][1];
+          }
         }
-#pragma unroll
-        for (int f = 0; f < 2; ++f) sc[f] = part[f][0] + part[f][1];
         __builtin_amdgcn_sched_barrier(0);
 
         // ---- masks: only where the step passes what some row sees, or misses a page
-        const int have = uniform(lds[M::kValid + (u & 3) * 2 + wk]);
-        edge = (u + 1) * M::kStep > pc.see_all || have == 0;
-        if (edge) {
+        const uint32_t have = (uint32_t)uniform(valid) >> (8 * wk * KT);
+        if ((u + 1) * M::kStep > pc.see_all || (have & (KT == 2 ? 0x0101u : 1u)) != (KT == 2 ? 0x0101u : 1u)) {
 #pragma unroll
-          for (int f = 0; f < 2; ++f) {
-            const int upto = have ? sees[f] - (u * M::kStep + wk * 16 + 4 * g) : 0;
+          for (int f = 0; f < 2; ++f)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sc[f][i] = i < upto ? sc[f][i] : -INFINITY;
-          }
+            for (int k = 0; k < KT; ++k) {
+              const int upto = (have >> (8 * k)) & 1 ? sees[f] - (u * M::kStep + (wk * KT + k) * 16 + 4 * g) : 0;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) sc[k][f][i] = i < upto ? sc[k][f][i] : -INFINITY;
+            }
         }
         bool move = false;
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
-          const float top = rows_max(fmaxf(fmaxf(sc[f][0], sc[f][1]), fmaxf(sc[f][2], sc[f][3]))) * scale_log2;
+          float top = sc[0][f][0];
+#pragma unroll
+          for (int k = 0; k < KT; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, sc[k][f][i]);
+          top = rows_max(top) * scale_log2;
           move = move || top > m[f] + kLazy;  // from -inf: any finite score
           if (g == 0) tops[wk * MR + (wq * 2 + f) * 16 + r16] = top;
         }
         const bool any = __any(move);
-        if (lane == 0) lds[M::kMove + (u & 1) * 4 + wave] = any ? 1 : 0;
-        put_p(u, edge);
+        if (lane == 0) lds[M::kFlags + (u & 1) * 4 + wave] = any ? 1 : 0;
+        put_p(u);
       }
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
@@ -884,25 +897,26 @@ __global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
   } else {
     // ================ output, and the loads
     const int w = wave - 4;
-    constexpr int CT = 8;
-    int load_off[L::kLoads];  // source bytes within the wave's group of 8 rows
+    constexpr int CT = 8, RG = M::kGroups;
+    int load_off[L::kLoads];  // source bytes within a group of 8 rows; the swizzle differs in odd groups
 #pragma unroll
     for (int j = 0; j < L::kLoads; ++j) {
       const int slot = j * 64 + lane, row = slot / L::kChunks, pos = slot % L::kChunks;
-      load_off[j] = row * L::kRowB + ((pos ^ swz((w & 1) * 8 + row)) << 4);
+      load_off[j] = row * L::kRowB + ((pos ^ swz(RG == 1 ? (w & 1) * 8 + row : row)) << 4);
     }
     while (cur < uniform(side->end)) {
       Piece pc;
       const bool there = next_piece<MR>(place, side, cur, &pc);
       cur += pc.s1 - pc.s0;
       if (!there) continue;
-      const int u0 = 2 * pc.s0, end = min(2 * pc.s1, (pc.see_any + M::kStep - 1) / M::kStep);
+      const int u0 = pc.s0 * (64 / M::kStep);
+      const int end = min(pc.s1 * (64 / M::kStep), (pc.see_any + M::kStep - 1) / M::kStep);
 
-      // Where the group's 16-row block stands in steps held .. held + 63, a lane each.
+      // Where the wave's 16-row block stands in steps held .. held + 63, a lane each.
       const int32_t* table = in.pages.table + (long long)pc.b * in.pages.max_pages;
       int held = u0, where;
       const auto look_up = [&]() __attribute__((always_inline)) {
-        where = find_block(in.pages, table, min(held + lane, end - 1) * 2 + (w >> 1));
+        where = find_block(in.pages, table, min(held + lane, end - 1) * (M::kStep / 16) + w * RG / 2);
       };
       look_up();
       const uint8_t* src;
@@ -913,22 +927,36 @@ __global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
           held = u;
           look_up();
         }
-        const int at = __builtin_amdgcn_readlane(where, u - held);
-        const long long row = (at >= 0 ? (long long)at << 4 : 0) + (w & 1) * 8;  // no page: some row, masked
-        if (lane == 0) lds[M::kValid + (u & 3) * 2 + (w >> 1)] = at >= 0 ? 1 : 0;
+        const int at = __builtin_amdgcn_readlane(where, u - held), buffer = u % M::kBufs;
+        const long long row = (at >= 0 ? (long long)at << 4 : 0) + (RG == 1 ? (w & 1) * 8 : 0);  // no page: some row, masked
+        if (lane == 0) lds[M::kValid + buffer * 4 + w * RG / 2] = at >= 0 ? 1 : 0;
         src = a.data + row * L::kRowB;
-        dst = uniform(lds_address(lds) + (u & 3) * M::kBytes + w * 8 * L::kRowB);
+        dst = uniform(lds_address(lds) + buffer * M::kBytes + w * RG * 8 * L::kRowB);
         if constexpr (F8) {
           src_scales = a.scales + row;
-          dst_scales = uniform(lds_address(lds) + (u & 3) * M::kBytes + M::kData + w * 32);
+          dst_scales = uniform(lds_address(lds) + buffer * M::kBytes + M::kData + w * RG * 32);
         }
       };
       const auto load = [&](int i) __attribute__((always_inline)) {
-        if (i < L::kLoads) {
+        if (F8 && i == M::kLoad - 1) {
+          if (lane < RG * 8) dma_4(src_scales, lane * 4, dst_scales);
+        } else if (i < L::kLoads) {
           dma_16(src, load_off[i], dst + i * 1024);
-        } else if (lane < 8) {
-          dma_4(src_scales, lane * 4, dst_scales);
+        } else {
+          dma_16(src + 8 * L::kRowB, load_off[i - L::kLoads] ^ 64, dst + 8 * L::kRowB + (i - L::kLoads) * 1024);
         }
+      };
+      const auto load_all = [&](int u) __attribute__((always_inline)) {
+        if (u < end) {
+          aim(u);
+#pragma unroll
+          for (int j = 0; j < M::kLoad; ++j) load(j);
+        }
+      };
+      // Step u has landed; the steps after it may be on their way.
+      const auto landed = [&](int u) __attribute__((always_inline)) {
+        if (M::kAway == 2 && u + 1 < end) wait_vmcnt<M::kLoad>();
+        else wait_vmcnt<0>();
       };
       f32x4 o[CT][4];
 #pragma unroll
@@ -937,33 +965,40 @@ __global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
         for (int c = 0; c < CT; ++c) o[c][f] = f32x4{0.f, 0.f, 0.f, 0.f};
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        if (u0 + i < end) {
-          aim(u0 + i);
-#pragma unroll
-          for (int j = 0; j < M::kLoad; ++j) load(j);
-        }
+      for (int i = 0; i < M::kAway; ++i) load_all(u0 + i);
       __builtin_amdgcn_sched_barrier(0);
 
       if (end > u0) {  // the first step has its scores taken
-        if (u0 + 1 < end) wait_vmcnt<M::kLoad>();
-        else wait_vmcnt<0>();
+        landed(u0);
         lds_barrier();
-        if (u0 + 2 < end) {
-          aim(u0 + 2);
-#pragma unroll
-          for (int j = 0; j < M::kLoad; ++j) load(j);
-        }
+        load_all(u0 + M::kAway);
       }
       for (int u = u0 + 1; u <= end; ++u) {
-        if (u + 1 < end) wait_vmcnt<M::kLoad>();
-        else wait_vmcnt<0>();
-        lds_barrier();  // step u has landed, P of the step before is there, and the step before that is done with
-        const bool more = u + 2 < end;
-        if (more) aim(u + 2);
-        const int v = u - 1;  // the step that is added
-        if (moved(v)) {
+        landed(u);
+        lds_barrier();  // step u has landed, P of step v is there, and the step before that is done with
+        const int v = u - 1, buffer = v % M::kBufs;  // the step that is added
+        // ---- O^T += V^T P^T: lane (column r16, key octet g).  What is read first goes
+        // out before anything is waited for.
+        const int flags = *reinterpret_cast<const int*>(lds + M::kFlags + (v & 1) * 4);
+        const uint32_t valid = *reinterpret_cast<const uint32_t*>(lds + M::kValid + buffer * 4);
+        const uint8_t* pbuf = lds + M::kP + (v & 1) * M::kPBytes + r16 * M::kPRow;
+        u32x4 p[4];
+        u32x4 words[2];
+        const auto get_p = [&](int h) __attribute__((always_inline)) {
+          if constexpr (F8) {
+            const uint8_t* from = lds + buffer * M::kBytes + M::kData + (h * 32 + 8 * g) * 4;
+            words[0] = ld_u32x4(from);
+            words[1] = ld_u32x4(from + 16);
+          }
+#pragma unroll
+          for (int f = 0; f < 4; ++f) p[f] = ld_u32x4(pbuf + f * 16 * M::kPRow + (((4 * h + g) ^ zp) << 4));
+        };
+        get_p(0);
+        const bool more = u + M::kAway < end;
+        if (more) aim(u + M::kAway);
+        if (uniform(flags) != 0) {
           lds_barrier();
+          get_p(0);
 #pragma unroll
           for (int f = 0; f < 4; ++f) {
             const float by = tops[2 * MR + f * 16 + r16];
@@ -972,9 +1007,11 @@ __global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
             __builtin_amdgcn_sched_barrier(0);
           }
         }
-        uint8_t* buf = lds + (v & 3) * M::kBytes;
-        const int ok = uniform(*reinterpret_cast<const uint16_t*>(lds + M::kValid + (v & 3) * 2));
-        if ((v + 1) * M::kStep > pc.see_all || ok != 0x0101) {
+        uint8_t* buf = lds + buffer * M::kBytes;
+        constexpr uint32_t kAll = M::kStep == 64 ? 0x01010101u : 0x0101u;
+        const uint32_t ok = (uint32_t)uniform(valid) & kAll;
+        const bool edge = (v + 1) * M::kStep > pc.see_all || ok != kAll;
+        if (edge) {
           // A value that a row does not see must not reach it as 0 * NaN: rows that no
           // query sees become zeros, and Inf and NaN of rows that some do not see are
           // cleared.  A query that sees such a row has NaN in its l: its key is the
@@ -992,43 +1029,64 @@ __global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
         }
         __builtin_amdgcn_sched_barrier(0);
 
-        // ---- O^T += V^T P^T: lane (column r16, key octet g)
-        {
-          const uint8_t* pbuf = lds + M::kP + (v & 1) * M::kPBytes + (F8 ? w * M::kPCopy : 0) + r16 * 64 + ((g ^ (r16 >> 2)) << 4);
-          u32x4 p[4];
+        // An exclusive-or of the block into the address is the swizzle.
+        const int row = 8 * g + (F8 ? r16 >> 1 : r16 >> 2);
+        const uint32_t at = (uint32_t)buffer * M::kBytes + row * L::kRowB + w * (F8 ? 128 : 256) +
+                            ((swz(row) ^ (F8 ? 0 : (lane >> 1) & 1)) << 4) + 8 * (lane & 1);
+        constexpr int NF = M::kStep / 32 * CT;
+        const auto frag = [&](int i) {  // i = (half, block)
+          const int h = i / CT, c = i % CT;
+          if constexpr (F8) {
+            const u32x2 x = lds_tr8(lds + (at ^ (c << 4)) + h * 32 * L::kRowB);
+            return u32x4{x[0], x[1], 0u, 0u};
+          } else {  // rows 4 further: the lowest bit of the swizzle flips
+            const u32x2 x0 = lds_tr16(lds + (at ^ ((c & 3) << 5)) + (c >> 2) * 128);
+            const u32x2 x1 = lds_tr16(lds + (at ^ ((c & 3) << 5) ^ 16) + (c >> 2) * 128 + 4 * L::kRowB);
+            return u32x4{x0[0], x0[1], x1[0], x1[1]};
+          }
+        };
+        u32x4 ring[kAhead];
 #pragma unroll
-          for (int f = 0; f < 4; ++f) p[f] = ld_u32x4(pbuf + f * 16 * 64);
-          // An exclusive-or of the block into the address is the swizzle.
-          const int row = 8 * g + (F8 ? r16 >> 1 : r16 >> 2);
-          const uint32_t at = (uint32_t)(v & 3) * M::kBytes + row * L::kRowB + w * (F8 ? 128 : 256) +
-                              ((swz(row) ^ (F8 ? 0 : (lane >> 1) & 1)) << 4) + 8 * (lane & 1);
-          const auto frag = [&](int c) {
-            if constexpr (F8) {
-              const u32x2 x = lds_tr8(lds + (at ^ (c << 4)));
-              return u32x4{x[0], x[1], 0u, 0u};
-            } else {  // rows 4 further: the lowest bit of the swizzle flips
-              const u32x2 x0 = lds_tr16(lds + (at ^ ((c & 3) << 5)) + (c >> 2) * 128);
-              const u32x2 x1 = lds_tr16(lds + (at ^ ((c & 3) << 5) ^ 16) + (c >> 2) * 128 + 4 * L::kRowB);
-              return u32x4{x0[0], x0[1], x1[0], x1[1]};
+        for (int i = 0; i < kAhead; ++i) ring[i] = frag(i);
+        // e4m3: a probability takes its key's power of two for the wave's columns (exact)
+        const auto scale_p = [&](int h) __attribute__((always_inline)) {
+          if constexpr (F8) {
+            float e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              e[i] = __uint_as_float(((words[i >> 2][i & 3] >> (8 * w)) & 255u) << 23);
+              if (edge) {  // the scale of a row that no query sees may be anything
+                const int r = h * 32 + 8 * g + i;
+                if (v * M::kStep + r >= pc.see_any || !((ok >> (8 * (r >> 4))) & 1)) e[i] = 1.f;
+              }
             }
-          };
-          u32x4 ring[kAhead];
 #pragma unroll
-          for (int c = 0; c < kAhead; ++c) ring[c] = frag(c);
-          static_for<0, CT>([&](auto cc) {
-            constexpr int c = decltype(cc)::value;
-            const u32x4 x = ring[c % kAhead];
-            if constexpr (c + kAhead < CT) ring[c % kAhead] = frag(c + kAhead);
-            const bf16x8 xb = F8 ? e4m3x8_to_bf16x8(x[0], x[1]) : __builtin_bit_cast(bf16x8, x);
+            for (int f = 0; f < 4; ++f)
 #pragma unroll
-            for (int f = 0; f < 4; ++f) o[c][f] = mfma_bf16(xb, __builtin_bit_cast(bf16x8, p[f]), o[c][f]);
-            if constexpr (c % 2 == 1) {
-              constexpr int x0 = (c - 1) * M::kLoad / CT, x1 = (c + 1) * M::kLoad / CT;
-              if (more) static_for<x0, x1>([&](auto y) { load(decltype(y)::value); });
-              __builtin_amdgcn_sched_barrier(0);
-            }
-          });
-        }
+              for (int i = 0; i < 4; ++i)
+                p[f][i] = pack_bf16x2(__uint_as_float(p[f][i] << 16) * e[2 * i],
+                                      __uint_as_float(p[f][i] & 0xffff0000u) * e[2 * i + 1]);
+          }
+        };
+        scale_p(0);
+        static_for<0, NF>([&](auto ic) {
+          constexpr int i = decltype(ic)::value, c = i % CT, h = i / CT;
+          const u32x4 x = ring[i % kAhead];
+          if constexpr (i + kAhead < NF) ring[i % kAhead] = frag(i + kAhead);
+          const bf16x8 xb = F8 ? e4m3x8_to_bf16x8(x[0], x[1]) : __builtin_bit_cast(bf16x8, x);
+#pragma unroll
+          for (int f = 0; f < 4; ++f) o[c][f] = mfma_bf16(xb, __builtin_bit_cast(bf16x8, p[f]), o[c][f]);
+          if constexpr (i % 2 == 1) {
+            constexpr int x0 = (i - 1) * M::kLoad / NF, x1 = (i + 1) * M::kLoad / NF;
+            if (more) static_for<x0, x1>([&](auto y) { load(decltype(y)::value); });
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          if constexpr (c == CT - 1 && h + 1 < M::kStep / 32) {
+            get_p(h + 1);
+            scale_p(h + 1);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        });
       }
       lds_barrier();  // sums and maxima
 #pragma unroll
