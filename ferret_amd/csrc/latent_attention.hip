@@ -995,7 +995,7 @@ __global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
         };
         get_p(0);
         const bool more = u + M::kAway < end;
-        if (more) aim(u + M::kAway);
+        load_all(u + M::kAway);  // at once: between the products they held the wave up for longer
         if (uniform(flags) != 0) {
           lds_barrier();
           get_p(0);
@@ -1077,8 +1077,6 @@ __global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
 #pragma unroll
           for (int f = 0; f < 4; ++f) o[c][f] = mfma_bf16(xb, __builtin_bit_cast(bf16x8, p[f]), o[c][f]);
           if constexpr (i % 2 == 1) {
-            constexpr int x0 = (i - 1) * M::kLoad / NF, x1 = (i + 1) * M::kLoad / NF;
-            if (more) static_for<x0, x1>([&](auto y) { load(decltype(y)::value); });
             __builtin_amdgcn_sched_barrier(0);
           }
           if constexpr (c == CT - 1 && h + 1 < M::kStep / 32) {
