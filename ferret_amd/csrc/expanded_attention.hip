@@ -4,19 +4,27 @@
 // for one head; token i of n new ones sees the keys j <= len - n + i of its sequence
 // (causal) or all len.  A token that sees none gives zeros and lse -inf.
 //
-// A work-group takes 128 tokens of one head, 32 per wave, and walks the keys in steps
-// of 64, which come into LDS by asynchronous loads, one step ahead.  S^T = K Q^T has
-// the keys as MFMA rows: a lane holds the scores of one query and, per block, four
-// consecutive keys, which is the operand that O^T = V^T P^T needs (the order of the
-// keys within the contraction is free as long as V^T follows it), so P never leaves
-// its registers.  V^T comes from row-major V by transposing LDS reads.  80 KB of LDS
-// and half the registers leave room for two work-groups per CU: one's softmax runs
-// under the other's products.  Tiles of a sequence go longest first, and a head's
-// tiles to one XCD where the number of heads is a multiple of 8 (keys from its L2).
+// A work-group takes 128 tokens of one head, 32 per wave, and walks the keys in steps of
+// 64.  Either one team of four waves walks them all and two work-groups share a CU, or
+// two teams take steps in turn and join their outputs at the end.  Both put two waves on
+// each SIMD, so that one's softmax runs under the other's products, and both fill the
+// 160 KB of a CU; two teams halve the time of a long tile, one needs no join. Keys and
+// values come into LDS by asynchronous loads, one step ahead.  S^T = K Q^T has the keys
+// as MFMA rows: a lane holds the scores of one query and, per block, four consecutive
+// keys, which is the operand that O^T = V^T P^T needs (the order of the keys within the
+// contraction is free as long as V^T follows it), so P never leaves its registers.  V^T
+// comes from row-major V by transposing LDS reads.  Tiles go longest first
+// (expanded_plan.hpp), and a head's tiles to one XCD where the number of heads is a
+// multiple of 8 (keys from its L2).
 //
-// MFMA-bound: 2 * (192 + 128) operations per query, visible key and head.  S, m, l and
-// O are fp32; P is rounded to bf16 (half an ulp, 2^-9), l sums the unrounded terms.
+// Bound by the matrix and vector pipes together: 2 * (192 + 128) operations per query,
+// visible key and head keep the first busy for 43% of a long prompt's time,
+// exponentials, packing and masks the second for a third, with no LDS bank conflicts.
+// 16 heads, 4096 new tokens after 4096 others: 255 us, 1010 TFLOP/s (counting visible
+// pairs).  S, m, l and O are fp32; P is rounded to bf16 (half a step, 2^-8 relative), l sums the
+// unrounded terms.
 #include "attention.hpp"
+#include "expanded_plan.hpp"
 
 #include <initializer_list>
 
@@ -24,12 +32,12 @@ namespace ferret {
 namespace {
 
 constexpr int kNope = 128, kRope = 64, kValue = 128;
-constexpr int kStep = 64;                              // keys per step
-constexpr int kTokens = 128;                           // per work-group
+constexpr int kStep = kTileKeys, kTokens = kTileTokens;
 constexpr int kKn = 0, kKr = kStep * kNope * 2;        // a buffer: keys, rotary keys, values
 constexpr int kV = kKr + kStep * kRope * 2, kBuf = kV + kStep * kValue * 2;
-constexpr int kLdsBytes = 2 * kBuf;
-static_assert(2 * kLdsBytes <= 160 * 1024, "two work-groups per CU");
+static_assert(4 * kBuf <= 160 * 1024, "LDS of a CU: two work-groups, or one of two teams");
+
+constexpr int kCus = 256, kOneTeamGroups = 576;
 
 struct Args {
   const uint16_t *qn, *qr, *kn, *kr, *v;
@@ -48,36 +56,76 @@ __device__ __forceinline__ int swz_kn(int r) { return r & 15; }
 __device__ __forceinline__ int swz_kr(int r) { return (r >> 1) & 7; }
 __device__ __forceinline__ int swz_v(int r) { return 2 * (r & 7); }
 
-__global__ __launch_bounds__(256, 2) void expanded_attention_kernel(Args a) {
+// Index values outside the tensors are cut to them.
+__device__ __forceinline__ TileSeq tiles_of(const Args& a, int b) {
+  const int q0 = min(max(a.cu_q[b], 0), a.T), k0 = min(max(a.cu_k[b], 0), a.S);
+  return TileSeq{min(max(a.cu_q[b + 1], q0), a.T) - q0, min(max(a.cu_k[b + 1], k0), a.S) - k0, a.causal};
+}
+
+template <int TEAMS>
+__global__ __launch_bounds__(256 * TEAMS, 2) void expanded_attention_kernel(Args a) {
   constexpr int QF = 2, KT = kStep / 16, CT = kValue / 16;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6) & 3, team = TEAMS == 2 ? uniform(threadIdx.x >> 8) : 0;
   const int r16 = lane & 15, g = lane >> 4;
   const int head = blockIdx.x % a.H;
 
   // ---- the tile: every wave finds it by itself
-  int b = -1, tile = 0, left = blockIdx.x / a.H;
-  for (int base = 0; base < a.B; base += 64) {
-    int tiles = 0;
-    if (base + lane < a.B) {
-      const int q0 = min(max(a.cu_q[base + lane], 0), a.T), q1 = min(max(a.cu_q[base + lane + 1], q0), a.T);
-      tiles = (q1 - q0 + kTokens - 1) / kTokens;
+  int b = -1, tile = 0;
+  const int slot = blockIdx.x / a.H;
+  if (a.B <= kOrderedBatch) {
+    // The longest tiles of the batch first: the length of the rank-th, 64 lengths at a
+    // time, a lane each; then the tile among those of that length.
+    const TileSeq mine = lane < a.B ? tiles_of(a, lane) : TileSeq{0, 0, 0};  // one load deep
+    const auto seq = [&](int i) __attribute__((always_inline)) {
+      return TileSeq{__builtin_amdgcn_readlane(mine.n, i), __builtin_amdgcn_readlane(mine.len, i), a.causal};
+    };
+    int all = 0;
+    for (int i = 0; i < a.B; ++i) all += seq(i).tiles();
+    if (slot >= all) return;
+    const int rank = TEAMS == 2 ? slot : paired_rank(slot, all, kCus / a.H);
+    int base = 0, stride = (a.S + kStep - 1) / kStep / 64 + 1;
+    for (;;) {
+      int count = 0;
+      for (int i = 0; i < a.B; ++i) count += seq(i).at_least(base + lane * stride);
+      const unsigned long long enough = __ballot(count > rank);
+      base += (63 - __clzll((long long)enough)) * stride;  // lane 0's are enough
+      if (stride == 1) break;
+      stride = (stride + 63) / 64;
     }
-    int incl = tiles;
+    int before = 0;
+    for (int i = 0; i < a.B; ++i) before += seq(i).at_least(base + 1);
+    int among = rank - before;
+    for (int i = 0; i < a.B && b < 0; ++i) {
+      const TileSeq s = seq(i);
+      const int from = s.first_of(base), count = s.first_of(base + 1) - from;
+      if (among < count) {
+        b = i;
+        tile = from + among;
+      }
+      among -= count;
+    }
+  } else {
+    // Sequence by sequence, each from its longest tile on.
+    int left = slot;
+    for (int base = 0; base < a.B; base += 64) {
+      const int tiles = base + lane < a.B ? tiles_of(a, base + lane).tiles() : 0;
+      int incl = tiles;
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int o = __shfl_up(incl, off, 64);
-      if (lane >= off) incl += o;
+      for (int off = 1; off < 64; off <<= 1) {
+        const int o = __shfl_up(incl, off, 64);
+        if (lane >= off) incl += o;
+      }
+      const unsigned long long past = __ballot(left < incl);
+      if (past != 0) {
+        const int at = __ffsll((long long)past) - 1;
+        b = base + at;
+        const int count = __shfl(tiles, at, 64), before = __shfl(incl, at, 64) - count;
+        tile = count - 1 - (left - before);
+        break;
+      }
+      left -= __shfl(incl, 63, 64);
     }
-    const unsigned long long past = __ballot(left < incl);
-    if (past != 0) {
-      const int at = __ffsll((long long)past) - 1;
-      b = base + at;
-      const int count = __shfl(tiles, at, 64), before = __shfl(incl, at, 64) - count;
-      tile = count - 1 - (left - before);
-      break;
-    }
-    left -= __shfl(incl, 63, 64);
   }
   b = uniform(b);
   if (b < 0) return;
@@ -91,12 +139,14 @@ __global__ __launch_bounds__(256, 2) void expanded_attention_kernel(Args a) {
   const int see_any = a.causal ? max(past + row_last, 0) : len;    // and of the last
   const int last = (min(see_any, len) + kStep - 1) / kStep;
 
-  // ---- steps into LDS: this wave's 16 rows of each array (4, 8 and 4 rows per load)
+  // ---- steps into LDS: this wave's 16 rows of each array (4, 8 and 4 rows per load).
+  // The team takes steps team, team + TEAMS, ...
+  uint8_t* const own = lds + team * 2 * kBuf;
   const uint8_t* kn = reinterpret_cast<const uint8_t*>(a.kn + (long long)k0 * a.kn_s + (long long)head * a.kn_h);
   const uint8_t* kr = reinterpret_cast<const uint8_t*>(a.kr + (long long)k0 * a.kr_s);
   const uint8_t* vv = reinterpret_cast<const uint8_t*>(a.v + (long long)k0 * a.v_s + (long long)head * a.v_h);
   const auto issue = [&](int t) {
-    const uint32_t buf = uniform(lds_address(lds) + (t & 1) * kBuf);
+    const uint32_t buf = uniform(lds_address(own) + (t / TEAMS & 1) * kBuf);
     const int most = len - 1 - t * kStep;  // rows past the sequence repeat its last one
     const uint8_t* kn_t = kn + (long long)t * kStep * a.kn_s * 2;
     const uint8_t* kr_t = kr + (long long)t * kStep * a.kr_s * 2;
@@ -117,7 +167,7 @@ __global__ __launch_bounds__(256, 2) void expanded_attention_kernel(Args a) {
       dma_16(v_t, min(r, most) * a.v_s * 2 + ((r16 ^ swz_v(r)) << 4), buf + kV + (wave * 16 + j * 4) * 256);
     }
   };
-  if (last > 0) issue(0);
+  if (team < last) issue(team);
 
   // ---- queries (rows past the tile's repeat its last one)
   u32x4 qf[QF][6];
@@ -146,12 +196,15 @@ __global__ __launch_bounds__(256, 2) void expanded_attention_kernel(Args a) {
     for (int c = 0; c < CT; ++c) o[c][f] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  for (int t = 0; t < last; ++t) {
+  for (int turn = 0; turn < last; turn += TEAMS) {
+    const int t = turn + team;
+    const bool live = TEAMS == 1 || t < last;
     wait_vmcnt<0>();
-    lds_barrier();  // the step has landed for every wave, and the other buffer has been read
-    if (t + 1 < last) issue(t + 1);
+    lds_barrier();  // the steps have landed for every wave, and the other buffers have been read
+    if (t + TEAMS < last) issue(t + TEAMS);
     __builtin_amdgcn_sched_barrier(0);
-    uint8_t* buf = lds + (t & 1) * kBuf;
+    const int buffer = (team * 2 + (t / TEAMS & 1)) * kBuf;
+    uint8_t* buf = lds + buffer;
 
     // ---- S^T: 16 keys x 16 queries per block
     f32x4 sc[KT][QF];
@@ -159,7 +212,7 @@ __global__ __launch_bounds__(256, 2) void expanded_attention_kernel(Args a) {
     for (int k = 0; k < KT; ++k)
 #pragma unroll
       for (int f = 0; f < QF; ++f) sc[k][f] = f32x4{0.f, 0.f, 0.f, 0.f};
-    {
+    if (live) {
       const uint8_t* nope = buf + kKn + r16 * 256;
       const uint8_t* rope = buf + kKr + r16 * 128;
       const int zn = (g ^ (r16 & 3)) << 4, zr = (g ^ (swz_kr(r16) & 3)) << 4;
@@ -182,7 +235,7 @@ __global__ __launch_bounds__(256, 2) void expanded_attention_kernel(Args a) {
 
     // ---- masks: only where the step passes what some token of the tile sees
     unsigned long long odd = 0;  // rows with Inf or NaN among the values that not all tokens see
-    if ((t + 1) * kStep > see_all) {
+    if ((turn + TEAMS) * kStep > see_all) {  // of either team: the barriers are for both
 #pragma unroll
       for (int f = 0; f < QF; ++f) {
         const int upto = sees[f] - t * kStep - 4 * g;
@@ -196,10 +249,10 @@ __global__ __launch_bounds__(256, 2) void expanded_attention_kernel(Args a) {
       // added below to those that do.  The record of such rows takes the keys' place.
       lds_barrier();  // the keys have been read
       unsigned* found = reinterpret_cast<unsigned*>(buf + kKn);
-      if (threadIdx.x < 2) found[threadIdx.x] = 0;
+      if ((threadIdx.x & 255) < 2) found[threadIdx.x & 1] = 0;
       lds_barrier();
 #pragma unroll 1
-      for (int i = threadIdx.x; i < kStep * 16; i += 256) {
+      for (int i = threadIdx.x & 255; i < kStep * 16 && live; i += 256) {
         const int r = i >> 4, key = t * kStep + r;
         if (key < see_all) continue;
         u32x4* p = reinterpret_cast<u32x4*>(buf + kV + r * 256 + (((i & 15) ^ swz_v(r)) << 4));
@@ -222,6 +275,7 @@ __global__ __launch_bounds__(256, 2) void expanded_attention_kernel(Args a) {
       odd = (unsigned long long)(unsigned)uniform(found[1]) << 32 | (unsigned)uniform(found[0]);
     }
 
+    if (!live) continue;
     // ---- softmax of the lane's queries
     float top[QF];
     bool move = false;
@@ -268,7 +322,7 @@ __global__ __launch_bounds__(256, 2) void expanded_attention_kernel(Args a) {
     // 16-key blocks; lane 4j + i reads elements 4i of key row 4g + j
     {
       const int row = 4 * g + (r16 >> 2);
-      const uint32_t at = (uint32_t)((t & 1) * kBuf + kV) + row * 256 + (lane & 1) * 8 +
+      const uint32_t at = (uint32_t)(buffer + kV) + row * 256 + (lane & 1) * 8 +
                           ((((lane >> 1) & 1) ^ swz_v(row)) << 4);
 #pragma unroll
       for (int h = 0; h < KT / 2; ++h)
@@ -301,20 +355,59 @@ __global__ __launch_bounds__(256, 2) void expanded_attention_kernel(Args a) {
 
 #pragma unroll
   for (int f = 0; f < QF; ++f) {
-    float sum = l[f];
-    sum += __shfl_xor(sum, 16, 64);
-    sum += __shfl_xor(sum, 32, 64);
-    const int r = row0 + (wave * QF + f) * 16 + r16;
-    if (r > row_last) continue;
-    const long long at = (long long)(q0 + r) * a.H + head;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    uint16_t* to = a.out + at * kValue + 4 * g;
-#pragma unroll
-    for (int c = 0; c < CT; ++c)
-      *reinterpret_cast<u32x2*>(to + c * 16) =
-          u32x2{pack_bf16x2(o[c][f][0] * inv, o[c][f][1] * inv), pack_bf16x2(o[c][f][2] * inv, o[c][f][3] * inv)};
-    if (a.lse != nullptr && g == 0) a.lse[at] = sum == 0.f ? -INFINITY : (m[f] + __builtin_amdgcn_logf(sum)) * kLn2;
+    l[f] += __shfl_xor(l[f], 16, 64);
+    l[f] += __shfl_xor(l[f], 32, 64);
   }
+  const auto put = [&](int f, float top, float sum, auto&& value) __attribute__((always_inline)) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int r = row0 + (wave * QF + f) * 16 + r16;
+    if (r > row_last) return;
+    const long long at = (long long)(q0 + r) * a.H + head;
+    uint16_t* out = a.out + at * kValue + 4 * g;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      const f32x4 x = value(c) * inv;
+      *reinterpret_cast<u32x2*>(out + c * 16) = u32x2{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+    }
+    if (a.lse != nullptr && g == 0) a.lse[at] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+  };
+  if constexpr (TEAMS == 1) {
+#pragma unroll
+    for (int f = 0; f < QF; ++f) put(f, m[f], l[f], [&](int c) { return o[c][f]; });
+  } else {
+    // Each team finishes one of the two fragments of its queries.
+    lds_barrier();  // the last steps have been read
+    const auto finish = [&](auto kc) __attribute__((always_inline)) {
+      constexpr int keep = decltype(kc)::value, send = 1 - keep;
+      f32x4* to = reinterpret_cast<f32x4*>(lds) + (send * 4 + wave) * CT * 64 + lane;
+      float2* stat = reinterpret_cast<float2*>(lds + TEAMS * 4 * CT * 64 * sizeof(f32x4));
+#pragma unroll
+      for (int c = 0; c < CT; ++c) to[c * 64] = o[c][send];
+      stat[(send * 4 + wave) * 64 + lane] = make_float2(m[send], l[send]);
+      lds_barrier();
+      const f32x4* from = reinterpret_cast<const f32x4*>(lds) + (keep * 4 + wave) * CT * 64 + lane;
+      const float2 other = stat[(keep * 4 + wave) * 64 + lane];
+      const float top = fmaxf(m[keep], other.x), base = top == -INFINITY ? 0.f : top;
+      const float mine = __builtin_amdgcn_exp2f(m[keep] - base), theirs = __builtin_amdgcn_exp2f(other.x - base);
+      // l may be NaN where the maximum is -inf (a NaN that is the team's only key), and so is the sum then
+      const float sum = (l[keep] != 0.f ? l[keep] * mine : 0.f) + (other.y != 0.f ? other.y * theirs : 0.f);
+      put(keep, top, sum, [&](int c) { return o[c][keep] * mine + from[c * 64] * theirs; });
+    };
+    if (team == 0) finish(IntC<0>{});
+    else finish(IntC<1>{});
+  }
+}
+
+// The kernel's variant.  Up to about one round of work-groups the longest tile decides, and
+// two teams halve it; beyond, single teams pack better and save the join.  One / two teams,
+// causal, us: 16 heads, one prompt of 2048 (272 work-groups) 59.5 / 48.8, of 4096 (528)
+// 115 / 102, two of 2048 (544) 64.6 / 62.2; 128 heads of 512 (640) 27.2 / 34.3; 16 heads,
+// five prompts of 1024 (720) 51.3 / 64.7, eight (1152) 77.0 / 104.
+template <int TEAMS>
+hipError_t launch(const Args& a, unsigned groups, hipStream_t stream) {
+  if (const hipError_t e = set_lds_limit_once<expanded_attention_kernel<TEAMS>>(TEAMS * 2 * kBuf); e != hipSuccess) return e;
+  hipLaunchKernelGGL(expanded_attention_kernel<TEAMS>, dim3(groups), dim3(256 * TEAMS), TEAMS * 2 * kBuf, stream, a);
+  return hipGetLastError();
 }
 
 }  // namespace
@@ -367,8 +460,7 @@ extern "C" int ferret_latent_attention_expanded(const void* q_nope, long long qn
   a.causal = causal != 0;
   a.out = static_cast<uint16_t*>(out);
   a.lse = lse;
-  FERRET_HIP_CHECK((set_lds_limit_once<expanded_attention_kernel>(kLdsBytes)));
-  hipLaunchKernelGGL(expanded_attention_kernel, dim3((unsigned)(tiles * H)), dim3(256), kLdsBytes,
-                     (hipStream_t)stream, a);
-  return (int)hipGetLastError();
+  const hipStream_t on = (hipStream_t)stream;
+  return (int)(tiles * H > kOneTeamGroups ? launch<1>(a, (unsigned)(tiles * H), on)
+                                          : launch<2>(a, (unsigned)(tiles * H), on));
 }

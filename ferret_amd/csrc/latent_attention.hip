@@ -994,7 +994,6 @@ __global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
           for (int f = 0; f < 4; ++f) p[f] = ld_u32x4(pbuf + f * 16 * M::kPRow + (((4 * h + g) ^ zp) << 4));
         };
         get_p(0);
-        const bool more = u + M::kAway < end;
         load_all(u + M::kAway);  // at once: between the products they held the wave up for longer
         if (uniform(flags) != 0) {
           lds_barrier();
