@@ -20,7 +20,7 @@
 // Bound by the matrix and vector pipes together: 2 * (192 + 128) operations per query,
 // visible key and head keep the first busy for 43% of a long prompt's time,
 // exponentials, packing and masks the second for a third, with no LDS bank conflicts.
-// 16 heads, 4096 new tokens after 4096 others: 255 us, 1010 TFLOP/s (counting visible
+// 16 heads, 4096 new tokens after 4096 others: 247 us, 1045 TFLOP/s (counting visible
 // pairs).  S, m, l and O are fp32; P is rounded to bf16 (half a step, 2^-8 relative), l sums the
 // unrounded terms.
 #include "attention.hpp"
@@ -37,6 +37,11 @@ constexpr int kKn = 0, kKr = kStep * kNope * 2;        // a buffer: keys, rotary
 constexpr int kV = kKr + kStep * kRope * 2, kBuf = kV + kStep * kValue * 2;
 static_assert(4 * kBuf <= 160 * 1024, "LDS of a CU: two work-groups, or one of two teams");
 
+// Key and value fragments are read ahead of their products in rings that scheduling
+// fences keep: 245.8 us for the long prompt above against 252.7 where the compiler
+// places the reads, two at a time; 4 and 4, or 8 and 4, with a fence per 4 products: 248.0
+// and 246.9.
+constexpr int kAheadK = 6, kAheadV = 4, kFence = 2;
 constexpr int kCus = 256, kOneTeamGroups = 576;
 
 struct Args {
@@ -216,21 +221,22 @@ __global__ __launch_bounds__(256 * TEAMS, 2) void expanded_attention_kernel(Args
       const uint8_t* nope = buf + kKn + r16 * 256;
       const uint8_t* rope = buf + kKr + r16 * 128;
       const int zn = (g ^ (r16 & 3)) << 4, zr = (g ^ (swz_kr(r16) & 3)) << 4;
+      const auto frag = [&](int i) __attribute__((always_inline)) {  // i = (block, chunk)
+        const int k = i / 6, j = i % 6;
+        return j < 4 ? ld_u32x4(nope + k * 16 * 256 + (zn | ((j ^ (r16 >> 2)) << 6)))
+                     : ld_u32x4(rope + k * 16 * 128 + (zr | (((j - 4) ^ (swz_kr(r16) >> 2)) << 6)));
+      };
+      u32x4 ring[kAheadK];
 #pragma unroll
-      for (int k = 0; k < KT; ++k) {
+      for (int i = 0; i < kAheadK; ++i) ring[i] = frag(i);
+      static_for<0, KT * 6>([&](auto ic) __attribute__((always_inline)) {
+        constexpr int i = decltype(ic)::value, k = i / 6, j = i % 6;
+        const u32x4 c = ring[i % kAheadK];
+        if constexpr (i + kAheadK < KT * 6) ring[i % kAheadK] = frag(i + kAheadK);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const u32x4 c = ld_u32x4(nope + k * 16 * 256 + (zn | ((j ^ (r16 >> 2)) << 6)));
-#pragma unroll
-          for (int f = 0; f < QF; ++f) sc[k][f] = mfma_bf16_16x16x32(c, qf[f][j], sc[k][f]);
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const u32x4 c = ld_u32x4(rope + k * 16 * 128 + (zr | ((j ^ (swz_kr(r16) >> 2)) << 6)));
-#pragma unroll
-          for (int f = 0; f < QF; ++f) sc[k][f] = mfma_bf16_16x16x32(c, qf[f][4 + j], sc[k][f]);
-        }
-      }
+        for (int f = 0; f < QF; ++f) sc[k][f] = mfma_bf16_16x16x32(c, qf[f][j], sc[k][f]);
+        if constexpr (i % kFence == kFence - 1) __builtin_amdgcn_sched_barrier(0);
+      });
     }
 
     // ---- masks: only where the step passes what some token of the tile sees
@@ -276,6 +282,20 @@ __global__ __launch_bounds__(256 * TEAMS, 2) void expanded_attention_kernel(Args
     }
 
     if (!live) continue;
+    // ---- the first values are read under the softmax; 32 keys at a time: the lane's keys are 4g .. 4g + 3 of both
+    // 16-key blocks; lane 4j + i reads elements 4i of key row 4g + j
+    const int row = 4 * g + (r16 >> 2);
+    const uint32_t at = (uint32_t)(buffer + kV) + row * 256 + (lane & 1) * 8 +
+                        ((((lane >> 1) & 1) ^ swz_v(row)) << 4);
+    const auto frag = [&](int i) __attribute__((always_inline)) {  // i = (half, block)
+      const uint8_t* x = lds + (at ^ (i % CT << 5)) + i / CT * 32 * 256;
+      const u32x2 v0 = lds_tr16(x), v1 = lds_tr16(x + 16 * 256);
+      return u32x4{v0[0], v0[1], v1[0], v1[1]};
+    };
+    u32x4 ring[kAheadV];
+#pragma unroll
+    for (int i = 0; i < kAheadV; ++i) ring[i] = frag(i);
+    __builtin_amdgcn_sched_barrier(0);
     // ---- softmax of the lane's queries
     float top[QF];
     bool move = false;
@@ -286,8 +306,7 @@ __global__ __launch_bounds__(256 * TEAMS, 2) void expanded_attention_kernel(Args
       for (int k = 0; k < KT; ++k)
 #pragma unroll
         for (int i = 0; i < 4; ++i) x = fmaxf(x, sc[k][f][i]);
-      x = fmaxf(x, __shfl_xor(x, 16, 64));
-      top[f] = fmaxf(x, __shfl_xor(x, 32, 64)) * a.scale_log2;
+      top[f] = rows_max(x) * a.scale_log2;
       move = move || top[f] > m[f] + kLazy;
     }
     if (__any(move)) {
@@ -318,23 +337,15 @@ __global__ __launch_bounds__(256 * TEAMS, 2) void expanded_attention_kernel(Args
       }
     }
 
-    // ---- O^T += V^T P^T, 32 keys at a time: the lane's keys are 4g .. 4g + 3 of both
-    // 16-key blocks; lane 4j + i reads elements 4i of key row 4g + j
-    {
-      const int row = 4 * g + (r16 >> 2);
-      const uint32_t at = (uint32_t)(buffer + kV) + row * 256 + (lane & 1) * 8 +
-                          ((((lane >> 1) & 1) ^ swz_v(row)) << 4);
+    // ---- O^T += V^T P^T
+    static_for<0, KT / 2 * CT>([&](auto ic) __attribute__((always_inline)) {
+      constexpr int i = decltype(ic)::value, h = i / CT, c = i % CT;
+      const u32x4 v = ring[i % kAheadV];
+      if constexpr (i + kAheadV < KT / 2 * CT) ring[i % kAheadV] = frag(i + kAheadV);
 #pragma unroll
-      for (int h = 0; h < KT / 2; ++h)
-#pragma unroll
-        for (int c = 0; c < CT; ++c) {
-          const uint8_t* x = lds + (at ^ (c << 5)) + h * 32 * 256;
-          const u32x2 v0 = lds_tr16(x), v1 = lds_tr16(x + 16 * 256);
-          const u32x4 v = {v0[0], v0[1], v1[0], v1[1]};
-#pragma unroll
-          for (int f = 0; f < QF; ++f) o[c][f] = mfma_bf16_16x16x32(v, p[h][f], o[c][f]);
-        }
-    }
+      for (int f = 0; f < QF; ++f) o[c][f] = mfma_bf16_16x16x32(v, p[h][f], o[c][f]);
+      if constexpr (i % kFence == kFence - 1) __builtin_amdgcn_sched_barrier(0);
+    });
     while (odd != 0) {  // Inf and NaN to the tokens that see them
       const int r = __ffsll((long long)odd) - 1, key = t * kStep + r;
       odd &= odd - 1;

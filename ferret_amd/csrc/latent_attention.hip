@@ -147,14 +147,6 @@ struct Lds {
 };
 static_assert(Lds<32, 4, true>::kBytes <= 160 * 1024 && Lds<32, 4, false>::kBytes <= 160 * 1024, "LDS of a CU");
 
-// Maximum over lanes l, l ^ 16, l ^ 32, l ^ 48, in all of them.
-__device__ __forceinline__ float rows_max(float v) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-
 // Chunk c (16 bytes) of row r stands at chunk c ^ swz(r): the rows of two transposed
 // blocks (4 rows of two chunks each, or 8 of one) fall on distinct banks (a row is 32
 // banks past a multiple of 64), and so do the 16 lanes of a key fragment that are read
