@@ -8,7 +8,9 @@
 // 64.  Either one team of four waves walks them all and two work-groups share a CU, or
 // two teams take steps in turn and join their outputs at the end.  Both put two waves on
 // each SIMD, so that one's softmax runs under the other's products, and both fill the
-// 160 KB of a CU; two teams halve the time of a long tile, one needs no join. Keys and
+// 160 KB of a CU; two teams halve the time of a long tile, one needs no join.  Where
+// there are fewer tiles than CUs, parts of a tile's keys go to work-groups of their own
+// (two teams each), whose fp32 partials a second kernel joins in order.  Keys and
 // values come into LDS by asynchronous loads, one step ahead.  S^T = K Q^T has the keys
 // as MFMA rows: a lane holds the scores of one query and, per block, four consecutive
 // keys, which is the operand that O^T = V^T P^T needs (the order of the keys within the
@@ -26,6 +28,7 @@
 #include "attention.hpp"
 #include "expanded_plan.hpp"
 
+#include <algorithm>
 #include <initializer_list>
 
 namespace ferret {
@@ -43,6 +46,7 @@ static_assert(4 * kBuf <= 160 * 1024, "LDS of a CU: two work-groups, or one of t
 // and 246.9.
 constexpr int kAheadK = 6, kAheadV = 4, kFence = 2;
 constexpr int kCus = 256, kOneTeamGroups = 576;
+constexpr int kMaxParts = 16, kPartSteps = 6;
 
 struct Args {
   const uint16_t *qn, *qr, *kn, *kr, *v;
@@ -53,6 +57,9 @@ struct Args {
   int causal;
   uint16_t* out;  // [T, H, 128]
   float* lse;     // [T, H] or null
+  int parts;      // of a tile's keys
+  float2* ml;     // [parts][T * H]: maxima and sums, and then the outputs [parts][T * H][128]
+  __host__ __device__ float* part() const { return reinterpret_cast<float*>(ml + (size_t)parts * T * H); }
 };
 
 // The swizzles: 16-byte chunk c of row r stands at c ^ swizzle(r).  Rows of 256
@@ -67,7 +74,7 @@ __device__ __forceinline__ TileSeq tiles_of(const Args& a, int b) {
   return TileSeq{min(max(a.cu_q[b + 1], q0), a.T) - q0, min(max(a.cu_k[b + 1], k0), a.S) - k0, a.causal};
 }
 
-template <int TEAMS>
+template <int TEAMS, bool SPLIT>
 __global__ __launch_bounds__(256 * TEAMS, 2) void expanded_attention_kernel(Args a) {
   constexpr int QF = 2, KT = kStep / 16, CT = kValue / 16;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
@@ -77,7 +84,7 @@ __global__ __launch_bounds__(256 * TEAMS, 2) void expanded_attention_kernel(Args
 
   // ---- the tile: every wave finds it by itself
   int b = -1, tile = 0;
-  const int slot = blockIdx.x / a.H;
+  const int in_line = blockIdx.x / a.H, slot = SPLIT ? in_line / a.parts : in_line;
   if (a.B <= kOrderedBatch) {
     // The longest tiles of the batch first: the length of the rank-th, 64 lengths at a
     // time, a lane each; then the tile among those of that length.
@@ -142,7 +149,10 @@ __global__ __launch_bounds__(256 * TEAMS, 2) void expanded_attention_kernel(Args
   const int past = len - n + 1;
   const int see_all = a.causal ? max(past + row0, 0) : len;        // keys of the first token
   const int see_any = a.causal ? max(past + row_last, 0) : len;    // and of the last
-  const int last = (min(see_any, len) + kStep - 1) / kStep;
+  const int steps = (min(see_any, len) + kStep - 1) / kStep;
+  const int part = SPLIT ? uniform(in_line - slot * a.parts) : 0;
+  const int share = SPLIT ? (steps + 2 * a.parts - 1) / (2 * a.parts) * 2 : steps;  // whole turns of both teams
+  const int first = part * share, last = min(first + share, steps);
 
   // ---- steps into LDS: this wave's 16 rows of each array (4, 8 and 4 rows per load).
   // The team takes steps team, team + TEAMS, ...
@@ -172,7 +182,7 @@ __global__ __launch_bounds__(256 * TEAMS, 2) void expanded_attention_kernel(Args
       dma_16(v_t, min(r, most) * a.v_s * 2 + ((r16 ^ swz_v(r)) << 4), buf + kV + (wave * 16 + j * 4) * 256);
     }
   };
-  if (team < last) issue(team);
+  if (first + team < last) issue(first + team);
 
   // ---- queries (rows past the tile's repeat its last one)
   u32x4 qf[QF][6];
@@ -201,7 +211,7 @@ __global__ __launch_bounds__(256 * TEAMS, 2) void expanded_attention_kernel(Args
     for (int c = 0; c < CT; ++c) o[c][f] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  for (int turn = 0; turn < last; turn += TEAMS) {
+  for (int turn = first; turn < last; turn += TEAMS) {
     const int t = turn + team;
     const bool live = TEAMS == 1 || t < last;
     wait_vmcnt<0>();
@@ -370,10 +380,17 @@ __global__ __launch_bounds__(256 * TEAMS, 2) void expanded_attention_kernel(Args
     l[f] += __shfl_xor(l[f], 32, 64);
   }
   const auto put = [&](int f, float top, float sum, auto&& value) __attribute__((always_inline)) {
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const int r = row0 + (wave * QF + f) * 16 + r16;
     if (r > row_last) return;
     const long long at = (long long)(q0 + r) * a.H + head;
+    if constexpr (SPLIT) {
+      const long long to = (long long)part * a.T * a.H + at;
+#pragma unroll
+      for (int c = 0; c < CT; ++c) *reinterpret_cast<f32x4*>(a.part() + to * kValue + c * 16 + 4 * g) = value(c);
+      if (g == 0) a.ml[to] = make_float2(top, sum);
+      return;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
     uint16_t* out = a.out + at * kValue + 4 * g;
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
@@ -409,15 +426,68 @@ __global__ __launch_bounds__(256 * TEAMS, 2) void expanded_attention_kernel(Args
   }
 }
 
+// Joins the parts of a row, 32 lanes of 4 columns each; rows behind the last sequence
+// have none.
+__global__ __launch_bounds__(256) void expanded_join_kernel(Args a) {
+  const long long rows = (long long)a.T * a.H, row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (row < (long long)max(a.cu_q[0], 0) * a.H || row >= (long long)min(a.cu_q[a.B], a.T) * a.H) return;
+  const float* part = a.part() + row * kValue + (threadIdx.x & 31) * 4;
+  float2 ml[kMaxParts];
+  f32x4 x[kMaxParts];
+#pragma unroll
+  for (int i = 0; i < kMaxParts; ++i) {
+    ml[i] = make_float2(-INFINITY, 0.f);
+    x[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (i < a.parts) {
+      ml[i] = a.ml[i * rows + row];
+      x[i] = *reinterpret_cast<const f32x4*>(part + i * rows * kValue);
+    }
+  }
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kMaxParts; ++i) top = fmaxf(top, ml[i].x);
+  const float base = top == -INFINITY ? 0.f : top;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kMaxParts; ++i) {
+    const float by = __builtin_amdgcn_exp2f(ml[i].x - base);
+    acc += x[i] * by;
+    sum += ml[i].y != 0.f ? ml[i].y * by : 0.f;  // NaN where a NaN is a part's only key
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  acc *= inv;
+  *reinterpret_cast<u32x2*>(a.out + row * kValue + (threadIdx.x & 31) * 4) =
+      u32x2{pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3])};
+  if (a.lse != nullptr && (threadIdx.x & 31) == 0)
+    a.lse[row] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+// Tiles that B sequences with T tokens can have.
+long long tiles_of(int B, int T) { return std::min<long long>(T, (T + (kTokens - 1LL) * B) / kTokens); }
+
+// Parts of a tile's keys: as many as there are CUs for, of kPartSteps steps or more by the
+// keys that a token sees on average, as though all were causal.  One part / as here, us: 8
+// heads, 100 tokens of 8192 keys 146 / 26.9 (16 parts), 1024 of 8192 146 / 57.0 (4), 2048
+// of 8192 147 / 93.5 (2), 2048 of 2048 45.2 / 39.3 (2).  Against it: 16 heads, 1024 of
+// 1024, 28.4 in one and 31.3 in two parts of 4 steps, whose partials cost more than
+// they gain; 8 heads, 2048 of 8192, 123 in parts for four times as many CUs.
+int parts_of(int B, int T, int S, int H) {
+  const long long wide = kCus / (tiles_of(B, T) * H), deep = (S - T / 2) / B / (kStep * kPartSteps);
+  return (int)std::max(1LL, std::min({wide, deep, (long long)kMaxParts}));
+}
+
 // The kernel's variant.  Up to about one round of work-groups the longest tile decides, and
 // two teams halve it; beyond, single teams pack better and save the join.  One / two teams,
-// causal, us: 16 heads, one prompt of 2048 (272 work-groups) 59.5 / 48.8, of 4096 (528)
-// 115 / 102, two of 2048 (544) 64.6 / 62.2; 128 heads of 512 (640) 27.2 / 34.3; 16 heads,
-// five prompts of 1024 (720) 51.3 / 64.7, eight (1152) 77.0 / 104.
-template <int TEAMS>
-hipError_t launch(const Args& a, unsigned groups, hipStream_t stream) {
-  if (const hipError_t e = set_lds_limit_once<expanded_attention_kernel<TEAMS>>(TEAMS * 2 * kBuf); e != hipSuccess) return e;
-  hipLaunchKernelGGL(expanded_attention_kernel<TEAMS>, dim3(groups), dim3(256 * TEAMS), TEAMS * 2 * kBuf, stream, a);
+// causal, us: 16 heads, one prompt of 2048 (256 work-groups) 56.0 / 47.0, of 4096 (512)
+// 109 / 98.6, two of 2048 (512) 61.8 / 60.0; 128 heads of 512 (512) 26.2 / 33.6; 16 heads,
+// five prompts of 1024 (640) 50.2 / 63.3, eight (1024) 72.5 / 98.2.
+template <int TEAMS, bool SPLIT>
+hipError_t launch(const Args& a, long long groups, hipStream_t stream) {
+  constexpr int lds = TEAMS * 2 * kBuf;
+  if (const hipError_t e = set_lds_limit_once<expanded_attention_kernel<TEAMS, SPLIT>>(lds); e != hipSuccess) return e;
+  hipLaunchKernelGGL((expanded_attention_kernel<TEAMS, SPLIT>), dim3((unsigned)groups), dim3(256 * TEAMS), lds, stream,
+                     a);
   return hipGetLastError();
 }
 
@@ -426,13 +496,19 @@ hipError_t launch(const Args& a, unsigned groups, hipStream_t stream) {
 
 using namespace ferret;
 
+extern "C" size_t ferret_latent_attention_expanded_workspace(int B, int T, int S, int H) {
+  if (B < 1 || T < 1 || S < 1 || H < 1 || H > 1024) return 0;
+  const int parts = parts_of(B, T, S, H);
+  return parts > 1 ? (size_t)parts * T * H * (sizeof(float2) + kValue * sizeof(float)) : 0;
+}
+
 extern "C" int ferret_latent_attention_expanded(const void* q_nope, long long qn_token, long long qn_head,
                                                 const void* q_rotary, long long qr_token, long long qr_head,
                                                 const void* k_nope, long long kn_key, long long kn_head,
                                                 const void* k_rotary, long long kr_key, const void* v, long long v_key,
                                                 long long v_head, const int32_t* cu_q, const int32_t* cu_k, int B,
                                                 int T, int S, int H, float scale, int causal, void* out, float* lse,
-                                                void* stream) {
+                                                void* ws, size_t ws_bytes, void* stream) {
   FERRET_REQUIRE(q_nope && q_rotary && k_nope && k_rotary && v && cu_q && cu_k && out, FERRET_ERR_NULL);
   FERRET_REQUIRE(B >= 1 && T >= 1 && S >= 1 && H >= 1 && H <= 1024, FERRET_ERR_SHAPE);
   FERRET_REQUIRE(scale > 0.f && scale < 1e30f, FERRET_ERR_SHAPE);
@@ -444,8 +520,12 @@ extern "C" int ferret_latent_attention_expanded(const void* q_nope, long long qn
   FERRET_REQUIRE(((bits(q_nope) | bits(q_rotary) | bits(k_nope) | bits(k_rotary) | bits(v) | bits(out)) & 15) == 0 &&
                      (bits(lse) & 3) == 0,
                  FERRET_ERR_ALIGN);
-  const long long tiles = T / kTokens + (B < T ? B : T);
-  FERRET_REQUIRE(tiles * H < (1LL << 31), FERRET_ERR_SHAPE);
+  const int parts = parts_of(B, T, S, H);
+  const long long groups = tiles_of(B, T) * H * parts;
+  FERRET_REQUIRE(groups < (1LL << 31), FERRET_ERR_SHAPE);
+  FERRET_REQUIRE(parts == 1 || (ws != nullptr && (bits(ws) & 15) == 0 &&
+                                ws_bytes >= ferret_latent_attention_expanded_workspace(B, T, S, H)),
+                 FERRET_ERR_WORKSPACE);
   Args a;
   a.qn = static_cast<const uint16_t*>(q_nope);
   a.qr = static_cast<const uint16_t*>(q_rotary);
@@ -471,7 +551,14 @@ extern "C" int ferret_latent_attention_expanded(const void* q_nope, long long qn
   a.causal = causal != 0;
   a.out = static_cast<uint16_t*>(out);
   a.lse = lse;
+  a.parts = parts;
+  a.ml = static_cast<float2*>(ws);
   const hipStream_t on = (hipStream_t)stream;
-  return (int)(tiles * H > kOneTeamGroups ? launch<1>(a, (unsigned)(tiles * H), on)
-                                          : launch<2>(a, (unsigned)(tiles * H), on));
+  if (parts > 1) {
+    FERRET_HIP_CHECK((launch<2, true>(a, groups, on)));
+    const long long rows = (long long)T * H;
+    hipLaunchKernelGGL(expanded_join_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, on, a);
+    return (int)hipGetLastError();
+  }
+  return (int)(groups > kOneTeamGroups ? launch<1, false>(a, groups, on) : launch<2, false>(a, groups, on));
 }

@@ -595,8 +595,8 @@ NATIVE(latent_attention, 12) {
   return Py_BuildValue("(NN)", wrap(o), wrap(lse));
 }
 
-// q_nope, q_rotary, k_nope, k_rotary, v, cu_q, cu_k, scale, causal, return_lse, out -> out, or (out, lse)
-NATIVE(latent_attention_expanded, 11) {
+// q_nope, q_rotary, k_nope, k_rotary, v, cu_q, cu_k, scale, causal, return_lse, out, workspace -> out, or (out, lse)
+NATIVE(latent_attention_expanded, 12) {
   Call c;
   float scale;
   const auto* qn = c.rows(a[0], 3, kBf16);
@@ -614,6 +614,8 @@ NATIVE(latent_attention_expanded, 11) {
   c.require_current();
   const bool causal = a[8] == Py_True, with_lse = a[9] == Py_True;
   const at::Tensor o = c.out(a[10], {T, H, 128}, kBf16);
+  const size_t need = c.ok() ? ferret_latent_attention_expanded_workspace(B, T, S, H) : 0;
+  const at::Tensor ws = c.workspace(a[11], need);
   if (!c.ok()) Py_RETURN_NONE;
   const at::Tensor lse = with_lse ? c.fresh({T, H}, kF32) : at::Tensor();
   void* st = stream();
@@ -621,7 +623,7 @@ NATIVE(latent_attention_expanded, 11) {
         return ferret_latent_attention_expanded(
             ptr(qn), step(qn, 0), step(qn, 1), ptr(qr), step(qr, 0), step(qr, 1), ptr(kn), step(kn, 0), step(kn, 1),
             ptr(kr), step(kr, 0), ptr(v), step(v, 0), step(v, 1), ptr_as<int32_t>(cu_q), ptr_as<int32_t>(cu_k), B, T,
-            S, H, scale, causal, ptr(o), ptr_as<float>(lse), st);
+            S, H, scale, causal, ptr(o), ptr_as<float>(lse), ptr(ws), need, st);
       }))
     return declined();
   if (!with_lse) return wrap(o);

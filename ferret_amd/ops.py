@@ -724,10 +724,16 @@ def latent_attention(q_latent: torch.Tensor, q_rotary: torch.Tensor, cache: Late
     return (out, lse) if return_lse else out
 
 
+def latent_attention_expanded_workspace_bytes(num_sequences: int, num_tokens: int, num_keys: int,
+                                              num_heads: int) -> int:
+    """Bytes of the partial results that latent_attention_expanded joins: 0 unless few tokens attend many keys."""
+    return int(_lib.load().ferret_latent_attention_expanded_workspace(num_sequences, num_tokens, num_keys, num_heads))
+
+
 def latent_attention_expanded(q_nope: torch.Tensor, q_rotary: torch.Tensor, k_nope: torch.Tensor,
                               k_rotary: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
                               scale: float, causal: bool = True, return_lse: bool = False,
-                              out: torch.Tensor | None = None):
+                              out: torch.Tensor | None = None, workspace: torch.Tensor | None = None):
     """out bf16 [T, H, 128] (or (out, lse fp32 [T, H])): latent attention in its expanded form over ragged prompts.
 
     q_nope bf16 [T, H, 128], q_rotary [T, H, 64], k_nope and v [S, H, 128] (the two
@@ -736,10 +742,11 @@ def latent_attention_expanded(q_nope: torch.Tensor, q_rotary: torch.Tensor, k_no
     int32 [B+1], keys by cu_k; the n new tokens of a sequence are the last of its
     keys, each seeing the keys up to its own (causal) or all.  Tokens that see
     no key get zeros (lse -inf); rows behind the last sequence are left as they
-    were (unset where `out` is new).
+    were (unset where `out` is new).  `workspace` of
+    latent_attention_expanded_workspace_bytes as latent_attention's.
     """
     r = _lib.native().latent_attention_expanded(q_nope, q_rotary, k_nope, k_rotary, v, cu_q, cu_k, float(scale),
-                                                bool(causal), bool(return_lse), out)
+                                                bool(causal), bool(return_lse), out, workspace)
     if r is not None:
         return r
     qp, qt, qh = _rows(q_nope, "q_nope", (None, None, 128))
@@ -753,15 +760,18 @@ def latent_attention_expanded(q_nope: torch.Tensor, q_rotary: torch.Tensor, k_no
     B = cu_q.shape[0] - 1
     if B < 1 or cu_k.shape[0] != B + 1:
         raise ValueError(f"cu_q and cu_k must both be [B + 1], got {tuple(cu_q.shape)}, {tuple(cu_k.shape)}")
-    _same_device(q_nope, q_rotary, k_nope, k_rotary, v, cu_q, cu_k, out)
+    _same_device(q_nope, q_rotary, k_nope, k_rotary, v, cu_q, cu_k, out, workspace)
     dev = q_nope.device
     if out is None:
         out = torch.empty((T, H, 128), dtype=torch.bfloat16, device=dev)
     op = _out(out, "out", (T, H, 128), torch.bfloat16, dev)
     lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
+    need = latent_attention_expanded_workspace_bytes(B, T, S, H)
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     with _on(q_nope):
         rc = _lib.load().ferret_latent_attention_expanded(
             qp, qt, qh, rp, rt, rh, kp, ks, kh, krp, krs, vp, vs, vh, cqp, ckp, B, T, S, H, scale, int(causal), op,
-            lse.data_ptr() if lse is not None else 0, _stream())
+            lse.data_ptr() if lse is not None else 0, _dev(workspace, "workspace"), need, _stream())
     _lib.check("ferret_latent_attention_expanded", rc)
     return (out, lse) if return_lse else out

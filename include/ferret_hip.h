@@ -363,13 +363,17 @@ int ferret_latent_attention(const void* q_latent, long long ql_token, long long 
  * alone.  lse, tokens that see no key, and Inf or NaN that a token does not see: as
  * ferret_latent_attention.  Requirements: B, T, S >= 1, 1 <= H <= 1024,
  * 0 < scale < 1e30.
+ * ws: ferret_latent_attention_expanded_workspace(B, T, S, H) bytes, on a 16-byte
+ * bound; none (0, ws may be NULL) unless few tokens attend many keys.
  */
+size_t ferret_latent_attention_expanded_workspace(int B, int T, int S, int H);
 int ferret_latent_attention_expanded(const void* q_nope, long long qn_token, long long qn_head,
                                      const void* q_rotary, long long qr_token, long long qr_head,
                                      const void* k_nope, long long kn_key, long long kn_head,
                                      const void* k_rotary, long long kr_key, const void* v, long long v_key,
                                      long long v_head, const int32_t* cu_q, const int32_t* cu_k, int B, int T,
-                                     int S, int H, float scale, int causal, void* out, float* lse, void* stream);
+                                     int S, int H, float scale, int causal, void* out, float* lse, void* ws,
+                                     size_t ws_bytes, void* stream);
 
 /*
  * Flags of the FP8 *_ex entry points below.  FERRET_FP8_MMA_E4M3 multiplies

@@ -73,14 +73,21 @@ def test_absorbed(L):
 
 
 def test_expanded(L):
-    #       qn    t     h    qr   t    h   kn   s     h   kr  s   v   s     h   cu cu B  T  S  H scale causal out lse st
-    good = [P, 3008, 192, P, 3008, 192, P, 4096, 256, P, 64, P, 4096, 256, P, P, 2, 9, 30, 16, 0.07, 1, P, None, None]
+    #       qn    t     h    qr   t    h   kn   s     h   kr  s   v   s     h   cu cu B  T  S  H scale causal out lse ws bytes st
+    good = [P, 3008, 192, P, 3008, 192, P, 4096, 256, P, 64, P, 4096, 256, P, P, 2, 9, 30, 16, 0.07, 1, P, None, None, 0,
+            None]
     f = L.ferret_latent_attention_expanded
     for at, v, rc in [(0, None, -1), (3, None, -1), (6, None, -1), (9, None, -1), (11, None, -1), (14, None, -1),
                       (15, None, -1), (22, None, -1), (16, 0, -2), (17, 0, -2), (18, 0, -2), (19, 0, -2), (19, 1025, -2),
                       (20, 0.0, -2), (20, float("nan"), -2), (7, 1 << 24, -2), (10, -8, -2), (1, 3010, -4), (13, 260, -4),
                       (6, P + 4, -4), (22, P + 2, -4), (23, P + 1, -4)]:
         assert f(*_swap(good, **{f"_{at}": v})) == rc, (at, v)
+    need = L.ferret_latent_attention_expanded_workspace(2, 9, 8000, 16)
+    assert need == 8 * 9 * 16 * (8 + 512) and L.ferret_latent_attention_expanded_workspace(2, 9, 30, 16) == 0
+    assert L.ferret_latent_attention_expanded_workspace(0, 9, 8000, 16) == 0
+    split = _swap(good, _18=8000, _24=P, _25=need)
+    for at, v in [(24, None), (24, P + 8), (25, need - 1)]:
+        assert f(*_swap(split, **{f"_{at}": v})) == -3, (at, v)
 
 
 def test_python_layer_refuses_cpu_tensors_and_other_caches():

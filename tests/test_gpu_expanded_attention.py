@@ -183,3 +183,54 @@ def test_refusals(ops):
         ops.latent_attention_expanded(qn, qr, kn.float(), kr, v, cu, cu, SCALE)
     with pytest.raises(RuntimeError, match="code -2"):
         ops.latent_attention_expanded(qn, qr, kn, kr, v, cu, cu, 0.0)
+
+
+@pytest.mark.parametrize("lens,new,H", [([5000], [3], 1), ([2100, 1500], [130, 7], 3), ([6000, 10], [20, 10], 2),
+                                        ([1600, 0, 1700], [200, 0, 1], 4), ([1100, 1040], [1100, 2], 8)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_few_tokens_over_many_keys(ops, lens, new, H, causal):
+    """The keys are cut into parts that are joined."""
+    print(f"[case] expanded in parts lens={lens} new={new} H={H} causal={causal}", flush=True)
+    assert ops.latent_attention_expanded_workspace_bytes(len(lens), sum(new), sum(lens), H) > 0
+    c = Case(lens, new, H)
+    c.check(*c.run(ops, causal=causal), causal=causal)
+
+
+def test_parts_leave_padded_rows_and_replay(ops):
+    print("[case] expanded in parts, padded, graph", flush=True)
+    c = Case([2000, 1500], [60, 20], 4, spare=9)
+    ws = torch.full((ops.latent_attention_expanded_workspace_bytes(2, 89, 3509, 4) // 4,), float("nan"), device="cuda")
+    out = torch.full((89, 4, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+    _, lse = c.run(ops, out=out, workspace=ws)
+    assert (out[80:] == 7).all()
+    c.check(out, lse)
+    args, cu_q, cu_k = c.tensors(), i32(starts(c.new)), i32(starts(c.lens))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = ops.latent_attention_expanded(*args, cu_q, cu_k, SCALE)
+    for new, lens in (([60, 20], [2000, 1500]), ([1, 70], [0, 3400]), ([80, 0], [500, 3000]), ([60, 20], [2000, 1500])):
+        cu_q.copy_(i32(starts(new)))
+        cu_k.copy_(i32(starts(lens)))
+        g.replay()
+        want = ops.latent_attention_expanded(*args, cu_q, cu_k, SCALE)
+        torch.cuda.synchronize()
+        assert torch.equal(got[:sum(new)], want[:sum(new)])
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_parts_and_values_that_a_token_does_not_see(ops, value):
+    print(f"[case] expanded in parts {value}", flush=True)
+    c = Case([2100, 1400], [140, 40], 2)
+    clean, _ = c.run(ops)
+    c.v[1960 + 90, 1, 17] = value                 # new token 90's own key
+    c.v[2100 + 5, 0, 3] = value                   # a key that all of the second sequence see
+    out, _ = c.run(ops)
+    got, want = out.float(), clean.float()
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    hit[90:140, 1, 17] = True
+    hit[140:, 0, 3] = True
+    assert torch.equal(got[~hit], want[~hit])
+    if value != value:
+        assert got[hit].isnan().all()
+    else:
+        assert (got[hit] == value).all()
