@@ -39,7 +39,7 @@ namespace ferret {
 namespace {
 
 constexpr int kKeys = kLatentKeys, kUnits = kLatentUnits;
-constexpr int kJoinRows = 256;  // rows up to which a row's pieces are joined by several work-groups
+constexpr int kJoinRows = 512;  // rows up to which four work-groups join a row's pieces
 constexpr int kAhead = 4;      // LDS fragments read ahead
 constexpr int kFence = 4;      // fragments between scheduling fences
 
@@ -1170,26 +1170,32 @@ __global__ __launch_bounds__(256) void latent_join_kernel(Args a, int mr, int ro
     a.lse[row] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
-// Few rows, up to kUnits pieces each: a work-group per row and 32 columns, 8 lanes
-// across and the pieces dealt to 32 groups of lanes, at most 8 each.
+// Few rows, up to kUnits pieces each: a work-group per row and 128 columns, 32 lanes
+// across and the pieces dealt to 8 groups of lanes, 8 in flight each.  A wave per row /
+// this, whole call, us: 16 heads, e4m3, one sequence of 100001 53.5 / 27.7, 32 of 6000 (512
+// rows) 39.5 / 38.9, 64 of 600 to 8000 (1024 rows) 49.2 / 51.6.
 __global__ __launch_bounds__(256) void latent_join_long_kernel(Args a, int mr) {
+  constexpr int ACROSS = 32, GROUPS = 256 / ACROSS;
   __shared__ f32x4 red[256];
   __shared__ float weight[kUnits], stat[8];
   const int row = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   LatentRecord where;
   int r;
   if (!to_join(a, mr, row, &where, &r)) return;
-  const int across = threadIdx.x & 7, group = threadIdx.x >> 3, col = blockIdx.y * 32 + across * 4;
+  const int across = threadIdx.x % ACROSS, group = threadIdx.x / ACROSS, col = (blockIdx.y * ACROSS + across) * 4;
   const auto at = [&](int j) { return (long long)latent_record_slot(where, a.side_by_side, j) * mr + r; };
   const float2 v = (int)threadIdx.x < where.pieces ? a.ml()[at(threadIdx.x)] : make_float2(-INFINITY, 0.f);
   const float* part = a.part(mr) + col;
-  f32x4 x[kUnits / 32];
+  f32x4 x[8];
+  const auto load = [&](int j0) __attribute__((always_inline)) {
 #pragma unroll
-  for (int i = 0; i < kUnits / 32; ++i) {
-    const int j = group + 32 * i;
-    x[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (j < where.pieces) x[i] = *reinterpret_cast<const f32x4*>(part + at(j) * kLatent);
-  }
+    for (int i = 0; i < 8; ++i) {
+      const int j = j0 + group + GROUPS * i;
+      x[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (j < where.pieces) x[i] = *reinterpret_cast<const f32x4*>(part + at(j) * kLatent);
+    }
+  };
+  load(0);  // under the weights
   float top = wave_max(v.x);
   if (lane == 0) stat[wave] = top;
   __syncthreads();
@@ -1201,13 +1207,18 @@ __global__ __launch_bounds__(256) void latent_join_long_kernel(Args a, int mr) {
   __syncthreads();
   sum = (stat[4] + stat[5]) + (stat[6] + stat[7]);
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int j0 = 0;;) {
 #pragma unroll
-  for (int i = 0; i < kUnits / 32; ++i) acc += x[i] * weight[group + 32 * i];
+    for (int i = 0; i < 8; ++i) acc += x[i] * weight[j0 + group + GROUPS * i];
+    j0 += 8 * GROUPS;
+    if (j0 >= where.pieces) break;
+    load(j0);
+  }
   red[threadIdx.x] = acc;
   __syncthreads();
   if (group != 0) return;
-#pragma unroll 8
-  for (int i = 1; i < 32; ++i) acc += red[i * 8 + across];
+#pragma unroll
+  for (int i = 1; i < GROUPS; ++i) acc += red[i * ACROSS + across];
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   *reinterpret_cast<u32x2*>(a.out + (long long)row * kLatent + col) =
       u32x2{pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv)};
@@ -1218,7 +1229,7 @@ __global__ __launch_bounds__(256) void latent_join_long_kernel(Args a, int mr) {
 int launch_join(const Args& a, int mr, hipStream_t st) {
   const unsigned rows = (unsigned)((long long)a.T * a.H);
   if (rows <= kJoinRows)
-    hipLaunchKernelGGL(latent_join_long_kernel, dim3(rows, kLatent / 32), dim3(256), 0, st, a, mr);
+    hipLaunchKernelGGL(latent_join_long_kernel, dim3(rows, kLatent / 128), dim3(256), 0, st, a, mr);
   else
     hipLaunchKernelGGL(latent_join_kernel, dim3((rows + 3) / 4), dim3(256), 0, st, a, mr, (int)rows);
   return (int)hipGetLastError();

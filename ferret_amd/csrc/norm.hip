@@ -11,7 +11,9 @@
 // One pass: a row stays in the registers of the WPR waves that own it (CH
 // 16-byte chunks per lane), so it is read once, and a row may be written in
 // place: every lane's loads have returned before its row's sum is known.
-// HBM-bound: 2 bytes read per element (4 with the residual) and 1 to 4 written.
+// HBM-bound: 2 bytes read per element (4 with the residual) and 1 to 4 written.  8192
+// rows of 7168 with residual and codes: 70 us, 5.9 TB/s; 64 rows of 512: 4.5 us, the
+// launch.
 #include "common.hpp"
 
 namespace ferret {
@@ -142,8 +144,11 @@ static int launch_norm(const NormArgs& a, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
-// Waves per row by the chunks of a row: one wave up to 192 chunks (four rows
-// per work-group), then the fewest waves that hold the row at four chunks per lane.
+// Waves per row by the chunks of a row.  One up to 192 chunks, four rows per work-group
+// (8192 rows, codes out, us: K = 1024 8.0 against 10.6 with four waves, 1536 9.2 against
+// 10.4 with two and 12.5 with four), two up to 256 (2048: 11.4 against 13.3 with four),
+// eight up to 2048 (4096 and the residual 40.8 against 41.3 with four, 7168 70.0 against
+// 71.5 with four and 74.8 with sixteen), and sixteen for the rows that those do not hold.
 template <bool RES, bool F8>
 static int pick_norm(const NormArgs& a, hipStream_t st) {
   const int chunks = a.K / 8;
@@ -151,8 +156,8 @@ static int pick_norm(const NormArgs& a, hipStream_t st) {
   if (chunks <= 128) return launch_norm<1, 2, RES, F8>(a, st);
   if (chunks <= 192) return launch_norm<1, 3, RES, F8>(a, st);
   if (chunks <= 256) return launch_norm<2, 2, RES, F8>(a, st);
-  if (chunks <= 512) return launch_norm<4, 2, RES, F8>(a, st);
-  if (chunks <= 1024) return launch_norm<4, 4, RES, F8>(a, st);
+  if (chunks <= 512) return launch_norm<8, 1, RES, F8>(a, st);
+  if (chunks <= 1024) return launch_norm<8, 2, RES, F8>(a, st);
   if (chunks <= 2048) return launch_norm<8, 4, RES, F8>(a, st);
   return launch_norm<16, 4, RES, F8>(a, st);
 }
