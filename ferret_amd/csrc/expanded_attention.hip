@@ -22,9 +22,9 @@
 // Bound by the matrix and vector pipes together: 2 * (192 + 128) operations per query,
 // visible key and head keep the first busy for 43% of a long prompt's time,
 // exponentials, packing and masks the second for a third, with no LDS bank conflicts.
-// 16 heads, 4096 new tokens after 4096 others: 247 us, 1045 TFLOP/s (counting visible
-// pairs).  S, m, l and O are fp32; P is rounded to bf16 (half a step, 2^-8 relative), l sums the
-// unrounded terms.
+// 16 heads, 4096 new tokens after 4096 others: 244 us, 1060 TFLOP/s (counting visible
+// pairs), where a large product of the library reaches 1206.  S, m, l and O are fp32; P is
+// rounded to bf16 (half a step, 2^-8 relative), l sums the unrounded terms.
 #include "attention.hpp"
 #include "expanded_plan.hpp"
 
@@ -41,11 +41,11 @@ constexpr int kV = kKr + kStep * kRope * 2, kBuf = kV + kStep * kValue * 2;
 static_assert(4 * kBuf <= 160 * 1024, "LDS of a CU: two work-groups, or one of two teams");
 
 // Key and value fragments are read ahead of their products in rings that scheduling
-// fences keep: 245.8 us for the long prompt above against 252.7 where the compiler
-// places the reads, two at a time; 4 and 4, or 8 and 4, with a fence per 4 products: 248.0
-// and 246.9.
+// fences keep: 4096 after 4096 others, in one team: 245.8 us against 252.7 where the
+// compiler places the reads, two at a time; 4 and 4, or 8 and 4, with a fence per 4
+// products: 248.0 and 246.9.
 constexpr int kAheadK = 6, kAheadV = 4, kFence = 2;
-constexpr int kCus = 256, kOneTeamGroups = 576;
+constexpr int kCus = 256;
 constexpr int kMaxParts = 16, kPartSteps = 6;
 
 struct Args {
@@ -477,11 +477,19 @@ int parts_of(int B, int T, int S, int H) {
   return (int)std::max(1LL, std::min({wide, deep, (long long)kMaxParts}));
 }
 
-// The kernel's variant.  Up to about one round of work-groups the longest tile decides, and
-// two teams halve it; beyond, single teams pack better and save the join.  One / two teams,
-// causal, us: 16 heads, one prompt of 2048 (256 work-groups) 56.0 / 47.0, of 4096 (512)
-// 109 / 98.6, two of 2048 (512) 61.8 / 60.0; 128 heads of 512 (512) 26.2 / 33.6; 16 heads,
-// five prompts of 1024 (640) 50.2 / 63.3, eight (1024) 72.5 / 98.2.
+// One team or two, by the time that each is expected to take: either the longest tile
+// decides (1.6 us a step in one team that has a CU to itself, half of 2.5 in two), or the
+// sum over the card (2.45 us for two steps of a CU's two work-groups, 2.5 for two teams'
+// and about 3 us for each of their tiles' start and join, which nothing covers).  One / two,
+// causal, us: 16 heads, one prompt of 2048 56.0 / 47.0, of 4096 109 / 98.6, 4096 after 4096
+// others 243.6 / 250.1, two of 2048 61.8 / 60.0, five of 1024 50.2 / 63.3, eight 72.5 /
+// 98.2; 128 heads of 512 26.2 / 33.6.
+bool one_team(int B, int T, int S, long long groups) {
+  const float longest = (float)S / B / kStep, mean = fmaxf((float)S - 0.5f * T, 0.f) / B / kStep;
+  const float all = (float)groups * mean / (2 * kCus);
+  return fmaxf(1.6f * longest, 2.45f * all) < fmaxf(1.25f * longest, 2.5f * all + 3.f * (float)groups / kCus);
+}
+
 template <int TEAMS, bool SPLIT>
 hipError_t launch(const Args& a, long long groups, hipStream_t stream) {
   constexpr int lds = TEAMS * 2 * kBuf;
@@ -560,5 +568,5 @@ extern "C" int ferret_latent_attention_expanded(const void* q_nope, long long qn
     hipLaunchKernelGGL(expanded_join_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, on, a);
     return (int)hipGetLastError();
   }
-  return (int)(groups > kOneTeamGroups ? launch<1, false>(a, groups, on) : launch<2, false>(a, groups, on));
+  return (int)(one_team(B, T, S, groups) ? launch<1, false>(a, groups, on) : launch<2, false>(a, groups, on));
 }

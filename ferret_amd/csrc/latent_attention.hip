@@ -14,17 +14,25 @@
 // work-group finds its piece by itself from lens and cu_q: no host read, so the
 // call can be captured into a graph and replayed with other lengths.
 //
-// One step: the 64 cached rows come into LDS by asynchronous loads, once for key and
-// value.  S^T = K Q^T is dealt to the four waves by queries (WQ) and keys (WK), with
-// the keys as MFMA rows, so that a lane holds the scores of one query; its softmax
-// terms go through LDS as bf16, and for O^T = V^T P^T every wave takes all queries
-// and a quarter of the 512 columns.  So no product is done twice and a row is read
-// from LDS WQ times as key and once as value; the output tile stays in registers.
-// V^T is read with the transposing LDS loads (ds_read_b64_tr): 16 columns by key.
+// Up to 32 rows per tile (latent_attention_kernel), a step: the 64 cached rows come into
+// LDS by asynchronous loads, once for key and value.  S^T = K Q^T is dealt to the waves
+// by queries (WQ) and keys (WK), with the keys as MFMA rows, so that a lane holds the
+// scores of one query; its softmax terms go through LDS as bf16, and for O^T = V^T P^T
+// every wave takes all queries and a share of the 512 columns.  So no product is done
+// twice and a row is read from LDS WQ times as key and once as value; the output tile
+// stays in registers.  V^T is read with the transposing LDS loads (ds_read_b64_tr):
+// 16 columns by key.  64 rows (latent_attention_wide_kernel): scores and output are
+// done by waves of their own, side by side.
 // e4m3 rows stay e4m3 in LDS.  Keys are widened and scaled in one instruction (exact);
 // values are widened unscaled, and each probability is multiplied by its key's power
-// of two instead, before it is rounded to bf16 (exact, so nothing is lost): one copy
-// of P per block of 128 columns, that is per wave.
+// of two instead, before (16 and 32 rows: one copy of P per block of 128 columns) or
+// after (64 rows) it is rounded to bf16: exact, so nothing is lost by it.
+//
+// What bounds it.  16 heads, one token: the cache's bytes; 64 sequences of 600 to 8000
+// keys, e4m3, 49 us, 3.6 TB/s with launch and joins, of which the kernel takes 42.  64
+// rows: no one unit.  32 sequences of 8192, 128 heads, bf16, 100 us: the matrix units
+// are busy for 40% of the cycles, LDS for 27%, the vector units for 20% (e4m3: 43%, they
+// widen and scale), memory delivers 3.0 TB/s; the clock falls to 2.0 GHz under it.
 //
 // Numerics: S, m, l and O are fp32; P is rounded to bf16 for the MFMA (half a step,
 // 2^-8 relative, random over the keys), l sums the unrounded P.  The running
@@ -1262,13 +1270,19 @@ int launch_rows(int mr, const Args& a, hipStream_t st) {
   }
 }
 
-// Query rows per tile by the rows that a sequence has on average.
+// Query rows per tile by the rows that a sequence has on average.  Us, e4m3, 64 sequences
+// of 3000: 32 heads 45.7 in tiles of 32, 56.3 of 16, 51.1 of 64; 16 heads of 600 to 8000
+// 49.2 of 16, 53.7 of 32; 32 of 3000, 64 heads 40.9 of 64, 44.2 of 32; 128 heads, bf16,
+// 32 of 900 to 6000 67.2 of 64 against 83.0 of 32.
 int tile_rows(int T, int B, int H) {
   const long long rows = (long long)T * H / B;
   return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 }
 
-// Row tiles side by side by the tiles that a sequence has on average.
+// Row tiles side by side by the tiles that a sequence has on average: work-groups of one
+// XCD that walk the same keys at the same time.  128 heads, bf16, 32 sequences of 900 to
+// 6000: 58.5 us, one after another 65.1; 500 new tokens of two sequences, 16 heads: 172
+// us eight at a time, 194 two or one.
 int side_by_side(int T, int B, int H) {
   const long long tiles = (long long)T * H / B / 64;
   return tiles < 2 ? 1 : tiles < 4 ? 2 : tiles < 8 ? 4 : 8;
@@ -1328,7 +1342,9 @@ extern "C" int ferret_latent_attention(const void* q_latent, long long ql_token,
   a.H = H;
   a.scale_log2 = scale * kLog2e;
   a.causal = causal != 0;
-  a.min_steps = 2;
+  // Shares of one step where a step is short: 16 heads, 256 keys 13.4 us against 14.9 in
+  // shares of two; 128 heads, 8 sequences of 100 keys 21.1 in shares of two, 22.1 of one.
+  a.min_steps = mr == 64 ? 2 : 1;
   a.side_by_side = side_by_side(T, B, H);
   a.out = static_cast<uint16_t*>(out);
   a.lse = lse;

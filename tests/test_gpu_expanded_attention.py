@@ -234,3 +234,32 @@ def test_parts_and_values_that_a_token_does_not_see(ops, value):
         assert got[hit].isnan().all()
     else:
         assert (got[hit] == value).all()
+
+
+@pytest.mark.parametrize("lens,new,H,causal", [
+    ([300, 129, 64, 0, 257, 40], [129, 129, 64, 0, 200, 45], 96, True), ([200, 131], [200, 1], 256, True),
+    ([90, 190, 70], [130, 60, 70], 192, False), ([(7 * i) % 61 for i in range(40)], [(5 * i) % 23 for i in range(40)], 24, True)])
+def test_many_work_groups(ops, lens, new, H, causal):
+    """Short tiles of many heads: two work-groups per CU."""
+    print(f"[case] expanded {len(lens)} sequences, {H} heads, causal={causal}", flush=True)
+    c = Case(lens, new, H)
+    c.check(*c.run(ops, causal=causal), causal=causal)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_many_work_groups_and_values_that_a_token_does_not_see(ops, value):
+    print(f"[case] expanded 160 heads {value}", flush=True)
+    c = Case([250, 130], [240, 130], 160)
+    clean, _ = c.run(ops)
+    c.v[100, 101, 17] = value                     # new token 90
+    c.v[250 + 129, 3, 64] = value                 # the last token's own
+    out, _ = c.run(ops)
+    got, want = out.float(), clean.float()
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    hit[90:240, 101, 17] = True
+    hit[369, 3, 64] = True
+    assert torch.equal(got[~hit], want[~hit])
+    if value != value:
+        assert got[hit].isnan().all()
+    else:
+        assert (got[hit] == value).all()
