@@ -29,10 +29,11 @@
 // after (64 rows) it is rounded to bf16: exact, so nothing is lost by it.
 //
 // What bounds it.  16 heads, one token: the cache's bytes; 64 sequences of 600 to 8000
-// keys, e4m3, 49 us, 3.6 TB/s with launch and joins, of which the kernel takes 42.  64
+// keys, e4m3, 49 us, 3.6 TB/s with launch and joins, of which the kernel takes 44.  64
 // rows: no one unit.  32 sequences of 8192, 128 heads, bf16, 100 us: the matrix units
-// are busy for 40% of the cycles, LDS for 27%, the vector units for 20% (e4m3: 43%, they
-// widen and scale), memory delivers 3.0 TB/s; the clock falls to 2.0 GHz under it.
+// are busy for 40% of the cycles, LDS for 27%, the vector units for 20%, and memory
+// delivers 3.0 TB/s; the clock falls to 2.0 GHz under it.  e4m3, 93 us: the vector
+// units, which widen the keys twice and the values once.
 //
 // Numerics: S, m, l and O are fp32; P is rounded to bf16 for the MFMA (half a step,
 // 2^-8 relative, random over the keys), l sums the unrounded P.  The running
@@ -1050,24 +1051,35 @@ __global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
         u32x4 ring[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) ring[i] = frag(i);
-        // e4m3: a probability takes its key's power of two for the wave's columns (exact)
+        // e4m3: a probability takes its key's power of two for the wave's columns, by adding
+        // to the exponents of two at a time: 125.5 us for chunks of 200 to 500 tokens on
+        // 5000 keys, 137.7 by widening, two products and rounding.  Exact for normal numbers; a
+        // product below 2^-126 becomes some number below 2^-126, and a P of zero counts
+        // as 2^-127 (the largest P of a row is 1 or more).
         const auto scale_p = [&](int h) __attribute__((always_inline)) {
           if constexpr (F8) {
-            float e[8];
+            u16x2 add[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              e[i] = __uint_as_float(((words[i >> 2][i & 3] >> (8 * w)) & 255u) << 23);
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t w0 = words[i >> 1][2 * (i & 1)] >> (8 * w), w1 = words[i >> 1][2 * (i & 1) + 1] >> (8 * w);
+              add[i] = __builtin_bit_cast(u16x2, (w0 & 255u) | (w1 & 255u) << 16) * (uint16_t)128 - (uint16_t)(127 * 128);
               if (edge) {  // the scale of a row that no query sees may be anything
-                const int r = h * 32 + 8 * g + i;
-                if (v * M::kStep + r >= pc.see_any || !((ok >> (8 * (r >> 4))) & 1)) e[i] = 1.f;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                  const int r = h * 32 + 8 * g + 2 * i + k;
+                  if (v * M::kStep + r >= pc.see_any || !((ok >> (8 * (r >> 4))) & 1)) add[i][k] = 0;
+                }
               }
             }
 #pragma unroll
             for (int f = 0; f < 4; ++f)
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                p[f][i] = pack_bf16x2(__uint_as_float(p[f][i] << 16) * e[2 * i],
-                                      __uint_as_float(p[f][i] & 0xffff0000u) * e[2 * i + 1]);
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t pair = p[f][i];
+                const u16x2 sum = __builtin_bit_cast(u16x2, pair) + add[i];
+                p[f][i] = __builtin_bit_cast(uint32_t,
+                                             __builtin_elementwise_max(__builtin_bit_cast(s16x2, sum), s16x2{0, 0}));
+              }
           }
         };
         scale_p(0);

@@ -267,3 +267,17 @@ def test_refusals(ops):
     for scale in (0.0, -1.0, float("nan"), float("inf")):
         with pytest.raises(RuntimeError, match="code -2"):
             ops.latent_attention(ql, qr, b.cache, table, lens, cu, scale)
+
+
+@pytest.mark.parametrize("by", [80, -80])
+@pytest.mark.parametrize("H", [16, 32, 64, 128])
+def test_powers_of_two_go_through(ops, H, by):
+    """Latents times 2^by (in the scale bytes) under queries times 2^-by: outputs times 2^by, bit for bit."""
+    print(f"[case] absorbed e4m3, latents times 2^{by}, H={H}", flush=True)
+    b, cu_q = Batch([700, 65, 130], 64, True, 17), i32([0, 1, 2, 3])
+    (ql, qr), (table, lens) = _queries(3, H, 5), b.device()
+    want = ops.latent_attention(bf16_tensor(ql), bf16_tensor(qr), b.cache, table, lens, cu_q, SCALE)
+    moved = ops.LatentCache(b.cache.data, (b.cache.scales.int() + by).clamp(0, 254).to(torch.uint8))
+    got = ops.latent_attention(bf16_tensor(ql * np.float32(2.0 ** -by)), bf16_tensor(qr), moved, table, lens, cu_q, SCALE)
+    torch.cuda.synchronize()
+    assert torch.equal(got.float(), want.float() * 2.0 ** by)
