@@ -281,3 +281,40 @@ def test_powers_of_two_go_through(ops, H, by):
     got = ops.latent_attention(bf16_tensor(ql * np.float32(2.0 ** -by)), bf16_tensor(qr), moved, table, lens, cu_q, SCALE)
     torch.cuda.synchronize()
     assert torch.equal(got.float(), want.float() * 2.0 ** by)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("H", [16, 64])
+def test_pages_shared_by_sequences_and_named_twice(ops, H, e4m3):
+    print(f"[case] absorbed, shared pages e4m3={e4m3} H={H}", flush=True)
+    b = Batch([158, 200, 64], 64, e4m3, 23)
+    b.table[1, :2] = b.table[0, :2]               # a common prefix of 128 keys
+    b.table[1, 2] = b.table[0, 0]                 # and its first page once more
+    for x in (b.lat, b.rot):
+        x[1] = np.concatenate([x[0][:128], x[0][:64], x[1][192:]])
+    _run(ops, b, [3, 2, 1], H)
+
+
+def test_two_calls_at_once(ops):
+    """Calls that overlap on two streams, each with a workspace from the allocator, and one passed to both in turn."""
+    print("[case] absorbed, two streams", flush=True)
+    cases = [(Batch([3000, 900], 64, True, 31), 16), (Batch([500, 2000], 64, False, 32), 64)]
+    args, want = [], []
+    for b, H in cases:
+        (ql, qr), (table, lens) = _queries(2, H, 9), b.device()
+        args.append((bf16_tensor(ql), bf16_tensor(qr), b.cache, table, lens, i32([0, 1, 2]), SCALE))
+        want.append(ops.latent_attention(*args[-1]))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in args]
+    got = [[], []]
+    for _ in range(20):
+        for s, a, g in zip(streams, args, got):
+            with torch.cuda.stream(s):
+                g.append(ops.latent_attention(*a))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(x, w) for x in g)
+    ws = torch.empty(max(ops.latent_attention_workspace_bytes(2, 2, H) for _, H in cases), dtype=torch.uint8, device="cuda")
+    for _ in range(3):
+        for a, w in zip(args, want):
+            assert torch.equal(ops.latent_attention(*a, workspace=ws), w)
