@@ -434,6 +434,10 @@ bool as_float(PyObject* o, float* v) {
   return x >= 0.0;
 }
 
+// Elements from one row of a matrix to the next, the row's width where there is one row:
+// a stride of 0 over more rows (an expanded row) is left for the library to refuse.
+int64_t pitch(const at::Tensor* t) { return t->size(0) == 1 ? t->size(1) : t->stride(0); }
+
 // The stride of dimension d, 0 where it has one element.
 int64_t step(const at::Tensor* t, int d) { return t->size(d) == 1 ? 0 : t->stride(d); }
 
@@ -458,8 +462,8 @@ struct Norm {
     }
     c.require_current();
     if (r != nullptr) ro = c.out(out, {M, K}, kBf16);
-    xs = step(x, 0) != 0 ? step(x, 0) : K;
-    rs = r != nullptr && step(r, 0) != 0 ? step(r, 0) : K;
+    xs = pitch(x);
+    rs = r != nullptr ? pitch(r) : K;
     return c.ok();
   }
   PyObject* residual() const {
@@ -537,10 +541,9 @@ NATIVE(latent_cache_write, 7) {
   if (lat->size(1) != 512 || rot->size(0) != T || rot->size(1) != 64) Py_RETURN_NONE;
   void* st = stream();
   if (!run("ferret_latent_cache_write", [&] {
-        return ferret_latent_cache_write(ptr(lat), T > 1 ? step(lat, 0) : 512, ptr(rot), T > 1 ? step(rot, 0) : 64,
-                                         ptr_as<int32_t>(k.table), ptr_as<int32_t>(k.lens),
-                                         ptr_as<int32_t>(k.starts), k.B, k.max_pages, T, ptr(k.data), k.scale_ptr(),
-                                         k.pages, k.page_size, st);
+        return ferret_latent_cache_write(ptr(lat), pitch(lat), ptr(rot), pitch(rot), ptr_as<int32_t>(k.table),
+                                         ptr_as<int32_t>(k.lens), ptr_as<int32_t>(k.starts), k.B, k.max_pages, T,
+                                         ptr(k.data), k.scale_ptr(), k.pages, k.page_size, st);
       }))
     return declined();
   Py_RETURN_TRUE;

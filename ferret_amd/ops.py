@@ -485,6 +485,18 @@ def _rows(t: torch.Tensor, name: str, shape: tuple, dtype=torch.bfloat16) -> tup
     return (t.data_ptr(), *strides)
 
 
+def _pitched(t: torch.Tensor, name: str, shape: tuple) -> tuple:
+    """_rows of a 2-D tensor whose rows may not share storage: pointer, and the elements from one row to the
+    next (the row's own width where there is one row, whatever its stride)."""
+    at, pitch = _rows(t, name, shape)
+    if t.shape[0] == 1:
+        return at, t.shape[1]
+    if pitch < t.shape[1]:
+        raise ValueError(f"{name}'s rows must be {t.shape[1]} elements apart or more, got strides {t.stride()} "
+                         f"(an expanded row has to be copied)")
+    return at, pitch
+
+
 class _on:
     """The device of `t` as the current one (a no-op where it is already)."""
 
@@ -504,19 +516,19 @@ def _norm_args(x, w, residual, residual_out):
     if not isinstance(x, torch.Tensor) or x.dim() != 2:
         raise ValueError("x must be a 2-D tensor [M, K]")
     M, K = x.shape
-    xp, xs = _rows(x, "x", (None, None))
+    xp, xs = _pitched(x, "x", (None, None))
     wp = _dev(w, "w", torch.bfloat16, 1)
     if w.shape[0] != K:
         raise ValueError(f"w must be [{K}], got {tuple(w.shape)}")
-    rp, rs, ro = 0, 0, None
+    rp, rs, ro = 0, K, None
     if residual is not None:
-        rp, rs = _rows(residual, "residual", (M, K))
+        rp, rs = _pitched(residual, "residual", (M, K))
         ro = torch.empty((M, K), dtype=torch.bfloat16, device=x.device) if residual_out is None else residual_out
         _out(ro, "residual_out", (M, K), torch.bfloat16, x.device)
     elif residual_out is not None:
         raise ValueError("residual_out needs a residual")
     _same_device(x, w, residual)
-    return M, K, xp, xs or K, wp, rp, rs or K, ro
+    return M, K, xp, xs, wp, rp, rs, ro
 
 
 def rms_norm(x: torch.Tensor, w: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6,
@@ -525,7 +537,7 @@ def rms_norm(x: torch.Tensor, w: torch.Tensor, residual: torch.Tensor | None = N
 
     The sum and the norm are fp32 (the norm is of the sum, not of its bf16
     copy); residual_out is bf16(s), None without a residual.  x and residual
-    may be row slices of wider tensors; `out` may be x and `residual_out` the
+    may be row slices of wider tensors (not expanded rows); `out` may be x and `residual_out` the
     residual itself (in place).  K % 8 == 0, K <= 32768.
     """
     r = _lib.native().rms_norm(x, w, residual, float(eps), out, residual_out)
@@ -630,7 +642,7 @@ def _cache(cache: LatentCache, page_table: torch.Tensor, starts: torch.Tensor, n
 def latent_cache_write(cache: LatentCache, latent: torch.Tensor, rotary: torch.Tensor, page_table: torch.Tensor,
                        lens: torch.Tensor, cu_q: torch.Tensor) -> None:
     """Writes new tokens' rows into the cache: latent bf16 [T, 512] and rotary bf16 [T, 64]
-    (row slices of wider tensors allowed), packed by cu_q int32 [B+1], token i of
+    (row slices of wider tensors allowed, expanded rows not), packed by cu_q int32 [B+1], token i of
     sequence b to position lens[b] - n + i of the pages that page_table [B,
     max_pages] names.  Rows behind the last sequence, negative positions and
     entries that are no page are dropped.  Pages that are written must belong to
@@ -640,14 +652,13 @@ def latent_cache_write(cache: LatentCache, latent: torch.Tensor, rotary: torch.T
     if _lib.native().latent_cache_write(cache.data, cache.scales, latent, rotary, page_table, lens, cu_q):
         return
     dp, sp, pages, page_size, tp, B, max_pages = _cache(cache, page_table, cu_q, "cu_q", lens)
-    lp, ls = _rows(latent, "latent", (None, LATENT))
+    lp, ls = _pitched(latent, "latent", (None, LATENT))
     T = latent.shape[0]
-    rp, rs = _rows(rotary, "rotary", (T, ROTARY))
+    rp, rs = _pitched(rotary, "rotary", (T, ROTARY))
     _same_device(cache.data, latent, rotary)
     with _on(latent):
-        rc = _lib.load().ferret_latent_cache_write(lp, ls or LATENT, rp, rs or ROTARY, tp, lens.data_ptr(),
-                                                   cu_q.data_ptr(), B, max_pages, T, dp, sp, pages, page_size,
-                                                   _stream())
+        rc = _lib.load().ferret_latent_cache_write(lp, ls, rp, rs, tp, lens.data_ptr(), cu_q.data_ptr(), B, max_pages,
+                                                   T, dp, sp, pages, page_size, _stream())
     _lib.check("ferret_latent_cache_write", rc)
 
 

@@ -272,7 +272,7 @@ int ferret_moe_combine(const void* o, const float* w, int T, int topk, int N, vo
  * given:  s = x + residual (fp32; residual_out = bf16_RNE(s)),
  *   y = bf16_RNE(s * rsqrt(mean(s^2) + eps) * w).
  * x [M,K] and residual [M,K] with rows x_stride / residual_stride elements apart
- * (multiples of 8, so a slice of a wider projection needs no copy), w bf16 [K],
+ * (multiples of 8, K or more, so a slice of a wider projection needs no copy), w bf16 [K],
  * y and residual_out bf16 [M,K] packed.  residual and residual_out are both given
  * or both NULL.  An output may stand exactly on x or residual (in place); any
  * other overlap is rejected.  The reference has no norm; this is the library's own
@@ -312,7 +312,7 @@ int ferret_rms_norm_e4m3(const void* x, long long x_stride, const void* residual
  * ferret_latent_cache_write: new token i of sequence b to position
  * lens[b] - n + i (n = its number of new tokens; negative positions are dropped).
  * latent bf16 [T,512], rotary bf16 [T,64], rows *_stride elements apart (multiples
- * of 8).  e4m3: per 128 latents byte = max(127 + ceil(log2(max|x| / 448)), 16) over
+ * of 8, a row's width or more).  e4m3: per 128 latents byte = max(127 + ceil(log2(max|x| / 448)), 16) over
  * the finite values, code = e4m3_RNE(x * 2^(127 - byte)); Inf and NaN give the NaN
  * code.  A row that two tokens of one call write (a page named by two sequences)
  * ends as a mix of both: the pages that are written belong to one sequence.
