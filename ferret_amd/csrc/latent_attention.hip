@@ -334,6 +334,60 @@ __device__ __forceinline__ u32x4 only_finite(u32x4 v) {
   return v;
 }
 
+// A value that a row does not see must not reach it as 0 * NaN: before the products with a
+// step's values, rows of the step (the first of which is key `first`) that no query of the
+// tile sees become zeros, and Inf and NaN of rows that some do not see are cleared.  Each
+// wave does so for its own columns, CT blocks of 16 from chunk `chunk` on.  ok: which 16-row
+// blocks have a page.
+// A query that sees a cleared Inf or NaN has NaN in its l, as its key is the same row; but
+// a key of bf16 latents with an Inf may score -inf and have no weight, and 0 * Inf makes
+// that column NaN in the steps that all queries see: so it does here.
+template <bool F8, int STEP, int CT, int WQ>
+__device__ __forceinline__ void clear_unseen(const Args& in, const Piece& p, uint8_t* buf, int first, uint32_t ok,
+                                             int chunk, f32x4 (&o)[CT][WQ]) {
+  constexpr int VC = F8 ? CT : 2 * CT, ROW = F8 ? kRowE4m3 : kRowBf16;
+  const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
+  const auto place = [&](int r, int c) { return buf + r * ROW + (((chunk + c) ^ swz(r)) << 4); };
+#pragma unroll 1
+  for (int i0 = 0; i0 < STEP * VC; i0 += 64) {
+    const int r = (i0 + lane) / VC, key = first + r;
+    const bool none = key >= p.see_any || !((ok >> (8 * (r >> 4))) & 1), some = !none && key >= p.see_all;
+    u32x4* const at = reinterpret_cast<u32x4*>(place(r, lane % VC));
+    u32x4 x = {0u, 0u, 0u, 0u}, fine = x;
+    if (some) fine = only_finite<F8>(x = *at);
+    if constexpr (!F8) {
+      const bool bad = x[0] != fine[0] || x[1] != fine[1] || x[2] != fine[2] || x[3] != fine[3];
+      for (unsigned long long rest = __ballot(bad); rest != 0;) {
+        const int first_bad = __ffsll((long long)rest) - 1, row = (i0 + first_bad) / VC;
+        rest &= ~0ull << (first_bad / VC * VC + VC - 1) << 1;  // the row's other chunks are looked at with it
+        uint32_t sees[WQ];  // all bits where the lane's query sees the key
+#pragma unroll
+        for (int f = 0; f < WQ; ++f) {
+          const int tok = p.one ? 0 : min(p.row0 + f * 16 + r16, p.row_last) / in.H;
+          sees[f] = first + row < (in.causal ? p.past + tok : p.len) ? ~0u : 0u;
+        }
+#pragma unroll
+        for (int c = 0; c < CT; ++c) {  // the lane's columns c * 16 + 4g .. 4g + 3
+          const u32x2 w = *reinterpret_cast<const u32x2*>(place(row, 2 * c + (g >> 1)) + (g & 1) * 8);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t inf = j & 1 ? 0x7f800000u : 0x7f80u;
+            const uint32_t nan = (w[j >> 1] & inf) == inf ? 0x7fc00000u : 0u;
+#pragma unroll
+            for (int f = 0; f < WQ; ++f) {
+              const float v = o[c][f][j];  // copied first: a bit cast of a vector's element reads element 0
+              o[c][f][j] = __uint_as_float(__float_as_uint(v) | (nan & sees[f]));
+            }
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      asm volatile("" ::: "memory");
+    }
+    if (none || some) *at = fine;
+  }
+}
+
 // Row r of the tile done: its output, or its part of a piece.  o: blocks of 16 columns
 // from `col` on, 4 of each per lane.
 template <int MR, int CT, int WQ>
@@ -534,22 +588,8 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void latent_attention_ke
 #pragma unroll
           for (int i = 0; i < 4; ++i) sc[k][i] = i < upto ? sc[k][i] : -INFINITY;
         }
-        // A value that a row does not see must not reach it as 0 * NaN: rows that
-        // no query sees become zeros, and Inf and NaN of rows that some do not see
-        // are cleared.  A query that sees such a row has NaN in its l: its key is
-        // the same row.
         lds_barrier();  // the keys have been read
-        constexpr int VC = F8 ? kLatent / 16 : kLatent / 8;  // chunks of a row's values
-#pragma unroll 1
-        for (int i = threadIdx.x; i < kKeys * VC; i += NT) {
-          const int r = i / VC, key = t * kKeys + r;
-          const bool none = key >= see_any || !((ok >> (8 * (r >> 4))) & 1);
-          if (!none && key < see_all) continue;
-          u32x4* p = reinterpret_cast<u32x4*>(buf + r * L::kRowB + (((i % VC) ^ swz(r)) << 4));
-          u32x4 v = {0u, 0u, 0u, 0u};
-          if (!none) v = only_finite<F8>(*p);
-          *p = v;
-        }
+        clear_unseen<F8, kKeys>(in, pc, buf, t * kKeys, ok, wave * CT * (F8 ? 1 : 2), o);
         if constexpr (F8) {
           if (threadIdx.x < kKeys) {
             const int r = threadIdx.x;
@@ -1015,19 +1055,7 @@ __global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
         const uint32_t ok = (uint32_t)uniform(valid) & kAll;
         const bool edge = (v + 1) * M::kStep > pc.see_all || ok != kAll;
         if (edge) {
-          // A value that a row does not see must not reach it as 0 * NaN: rows that no
-          // query sees become zeros, and Inf and NaN of rows that some do not see are
-          // cleared.  A query that sees such a row has NaN in its l: its key is the
-          // same row.  Each wave does so for its own columns.
-          constexpr int VC = F8 ? 8 : 16;  // chunks of a row's values in 128 columns
-#pragma unroll 1
-          for (int i = lane; i < M::kStep * VC; i += 64) {
-            const int r = i / VC, key = v * M::kStep + r;
-            const bool none = key >= pc.see_any || !((ok >> (8 * (r >> 4))) & 1);
-            if (!none && key < pc.see_all) continue;
-            u32x4* x = reinterpret_cast<u32x4*>(buf + r * L::kRowB + (((w * VC + i % VC) ^ swz(r)) << 4));
-            *x = none ? u32x4{0u, 0u, 0u, 0u} : only_finite<F8>(*x);
-          }
+          clear_unseen<F8, M::kStep>(in, pc, buf, v * M::kStep, ok, w * (F8 ? 8 : 16), o);
           asm volatile("" ::: "memory");
         }
         __builtin_amdgcn_sched_barrier(0);

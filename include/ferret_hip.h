@@ -337,8 +337,9 @@ int ferret_latent_cache_read(const void* data, const void* scales, int pages, in
  * (causal != 0) or all lens[b].  lse (optional) fp32 [T,H]: the logarithm of the
  * sum of exp(s).  A token that sees no key gets zeros and -inf.  q_latent bf16
  * [T,H,512] and q_rotary bf16 [T,H,64] with token and head strides in elements
- * (multiples of 8).  Inf or NaN in rows that a token does not see do not reach it; a
- * key whose score is -inf (an Inf among its latents) has no weight.
+ * (multiples of 8).  Inf or NaN in rows that a token does not see do not reach it.  One
+ * among the latents of a key that it sees makes that column NaN for it, and the whole
+ * row unless the key's score is -inf, which has no weight.
  * ws: ferret_latent_attention_workspace(B, T, H) bytes, on a 16-byte bound; two
  * calls that overlap in time need one each.  The result depends on the batch only
  * through the order of fp32 additions; the same call gives the same bits.

@@ -4,7 +4,8 @@ import pytest
 import torch
 
 from ferret_amd import lib
-from tests.attention_helpers import bf16_tensor, bf16_values, i32
+from oracle import attention as A
+from tests.attention_helpers import SCALE, Batch, assert_near, bf16_tensor, bf16_values, i32, visible
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +40,34 @@ def test_expanded_rows_are_refused(ops, native, monkeypatch):
     assert (out == 7).all() and (cache.data == 0).all()
     # one row has any stride
     assert torch.equal(ops.rms_norm(x[0].expand(1, 512), w)[0], ops.rms_norm(x[:1], w)[0])
+
+
+@pytest.mark.parametrize("H,n,length", [(16, 1, 200), (24, 1, 200), (128, 1, 200), (16, 1, 5000), (3, 4, 200), (4, 5, 200),
+                                        (16, 5, 200), (1, 70, 200), (64, 3, 130), (16, 5, 5000)])
+def test_an_infinite_latent_under_a_score_of_minus_infinity(ops, H, n, length):
+    """bf16: such a key has no weight, and its Inf times that weight makes its column NaN for every token that
+    sees it: in a step that all rows of a tile see and at the causal edge, alone and among other tokens."""
+    print(f"[case] absorbed, Inf under -inf H={H} n={n} length={length}", flush=True)
+    rng = np.random.default_rng(H + n)
+    ql, qr = bf16_values(rng, n, H, 512), bf16_values(rng, n, H, 64)
+    ql[..., 5] = -0.5
+    for key in sorted({5, length - n, length - 2, length - 1}):
+        b = Batch([length], 64, False, 41)
+        table, lens = b.device()
+        b.cache.data.view(-1, 576)[int(b.slots[0][key]), 5] = float("inf")
+        out, lse = ops.latent_attention(bf16_tensor(ql), bf16_tensor(qr), b.cache, table, lens, i32([0, n]), SCALE,
+                                        return_lse=True)
+        torch.cuda.synchronize()
+        out, lse = out.float().cpu().numpy(), lse.cpu().numpy()
+        see = visible(n, length)
+        sees = see[:, key].copy()
+        assert np.isnan(out[sees][..., 5]).all(), key
+        see[:, key] = False
+        k = np.concatenate([b.lat[0], b.rot[0]], 1)
+        for h in range(H):
+            o, ref, spread, reach = A.attend(np.concatenate([ql[:, h], qr[:, h]], 1), k, b.lat[0], SCALE, see)
+            eo, el = A.bounds(o, ref, spread, reach, 576, length)
+            got = out[:, h].copy()
+            got[sees, 5] = o[sees, 5]
+            assert_near(got, o, eo, f"key {key} head {h}")
+            assert_near(lse[:, h], ref, el, f"lse key {key} head {h}")
