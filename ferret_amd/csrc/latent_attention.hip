@@ -1082,8 +1082,12 @@ __global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
         // e4m3: a probability takes its key's power of two for the wave's columns, by adding
         // to the exponents of two at a time: 125.5 us for chunks of 200 to 500 tokens on
         // 5000 keys, 137.7 by widening, two products and rounding.  Exact for normal numbers; a
-        // product below 2^-126 becomes some number below 2^-126, and a P of zero counts
-        // as 2^-127 (the largest P of a row is 1 or more).
+        // product below 2^-126 becomes some number below 2^-126.  Zeros stay zeros (P is zero
+        // or normal): a key that a query does not see, or whose term vanished, may have any scale.
+        // The pair of ones is kept from the compiler, which would make compares and selects of
+        // the minimum's product (8% more time).
+        uint32_t ones = 0x00010001u;
+        if constexpr (F8) asm("" : "+s"(ones));
         const auto scale_p = [&](int h) __attribute__((always_inline)) {
           if constexpr (F8) {
             u16x2 add[4];
@@ -1091,20 +1095,14 @@ __global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
             for (int i = 0; i < 4; ++i) {
               const uint32_t w0 = words[i >> 1][2 * (i & 1)] >> (8 * w), w1 = words[i >> 1][2 * (i & 1) + 1] >> (8 * w);
               add[i] = __builtin_bit_cast(u16x2, (w0 & 255u) | (w1 & 255u) << 16) * (uint16_t)128 - (uint16_t)(127 * 128);
-              if (edge) {  // the scale of a row that no query sees may be anything
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                  const int r = h * 32 + 8 * g + 2 * i + k;
-                  if (v * M::kStep + r >= pc.see_any || !((ok >> (8 * (r >> 4))) & 1)) add[i][k] = 0;
-                }
-              }
             }
 #pragma unroll
             for (int f = 0; f < 4; ++f)
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const uint32_t pair = p[f][i];
-                const u16x2 sum = __builtin_bit_cast(u16x2, pair) + add[i];
+                const u16x2 from = __builtin_bit_cast(u16x2, pair);
+                const u16x2 sum = add[i] * __builtin_elementwise_min(from, __builtin_bit_cast(u16x2, ones)) + from;
                 p[f][i] = __builtin_bit_cast(uint32_t,
                                              __builtin_elementwise_max(__builtin_bit_cast(s16x2, sum), s16x2{0, 0}));
               }

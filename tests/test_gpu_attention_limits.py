@@ -71,3 +71,40 @@ def test_an_infinite_latent_under_a_score_of_minus_infinity(ops, H, n, length):
             got[sees, 5] = o[sees, 5]
             assert_near(got, o, eo, f"key {key} head {h}")
             assert_near(lse[:, h], ref, el, f"lse key {key} head {h}")
+
+
+@pytest.mark.parametrize("H,n", [(16, 1), (3, 4), (4, 5), (16, 5), (1, 70), (128, 1), (64, 3)])
+@pytest.mark.parametrize("length", [200, 5000])
+def test_a_key_without_weight_adds_nothing_whatever_its_scale(ops, H, n, length):
+    """e4m3: a key that a token does not see, or whose term vanishes, counts as nothing, also where its latents
+    stand 2^110 above those of the others."""
+    print(f"[case] absorbed, scales 2^110 apart H={H} n={n} length={length}", flush=True)
+    rng = np.random.default_rng(H + n)
+    ql, qr = bf16_values(rng, n, H, 512), bf16_values(rng, n, H, 64)
+    ql[...] = -np.abs(ql)
+    k0 = Batch([length], 64, True, 43)
+    table, lens = k0.device()
+    want = ops.latent_attention(bf16_tensor(ql), bf16_tensor(qr), k0.cache, table, lens, i32([0, n]), SCALE)
+    hidden = length - 1 if n > 1 else None      # the last token's own key, which the others do not see
+    for key in (hidden, 7):
+        if key is None:
+            continue
+        b = Batch([length], 64, True, 43)
+        row = int(b.slots[0][key])
+        b.cache.data.view(-1, 640)[row, :512] = 0x38          # 1 in every column: the scores are below -2^110
+        b.cache.scales.view(-1, 4)[row] = 247
+        out, lse = ops.latent_attention(bf16_tensor(ql), bf16_tensor(qr), b.cache, table, lens, i32([0, n]), SCALE,
+                                        return_lse=True)
+        torch.cuda.synchronize()
+        assert torch.isfinite(out).all()
+        if key == hidden:
+            assert torch.equal(out[:n - 1], want[:n - 1])
+        out, lse = out.float().cpu().numpy(), lse.cpu().numpy()
+        see = visible(n, length)
+        see[:, key] = False
+        k = np.concatenate([b.lat[0], b.rot[0]], 1)
+        for h in range(H):
+            o, ref, spread, reach = A.attend(np.concatenate([ql[:, h], qr[:, h]], 1), k, b.lat[0], SCALE, see)
+            eo, el = A.bounds(o, ref, spread, reach, 576, length)
+            assert_near(out[:, h], o, eo, f"key {key} head {h}")
+            assert_near(lse[:, h], ref, el, f"lse key {key} head {h}")
