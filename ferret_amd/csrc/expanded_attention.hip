@@ -49,6 +49,9 @@ constexpr int kAheadK = 6, kAheadV = 4, kFence = 2;
 constexpr int kCus = 256;
 constexpr int kMaxParts = 16, kPartSteps = 6;
 
+// Bytes of the maxima and sums of so many rows: the outputs behind them are read 16 bytes at a time.
+__host__ __device__ constexpr size_t stat_bytes(size_t rows) { return (rows * sizeof(float2) + 15) & ~(size_t)15; }
+
 struct Args {
   const uint16_t *qn, *qr, *kn, *kr, *v;
   int qn_t, qn_h, qr_t, qr_h, kn_s, kn_h, kr_s, v_s, v_h;  // strides in elements
@@ -59,8 +62,10 @@ struct Args {
   uint16_t* out;  // [T, H, 128]
   float* lse;     // [T, H] or null
   int parts;      // of a tile's keys
-  float2* ml;     // [parts][T * H]: maxima and sums, and then the outputs [parts][T * H][128]
-  __host__ __device__ float* part() const { return reinterpret_cast<float*>(ml + (size_t)parts * T * H); }
+  float2* ml;     // [parts][T * H]: maxima and sums, then on a 16-byte bound the outputs [parts][T * H][128]
+  __host__ __device__ float* part() const {
+    return reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(ml) + stat_bytes((size_t)parts * T * H));
+  }
 };
 
 // The swizzles: 16-byte chunk c of row r stands at c ^ swizzle(r).  Rows of 256
@@ -508,7 +513,8 @@ using namespace ferret;
 extern "C" size_t ferret_latent_attention_expanded_workspace(int B, int T, int S, int H) {
   if (B < 1 || T < 1 || S < 1 || H < 1 || H > 1024) return 0;
   const int parts = parts_of(B, T, S, H);
-  return parts > 1 ? (size_t)parts * T * H * (sizeof(float2) + kValue * sizeof(float)) : 0;
+  const size_t rows = (size_t)parts * T * H;
+  return parts > 1 ? stat_bytes(rows) + rows * kValue * sizeof(float) : 0;
 }
 
 extern "C" int ferret_latent_attention_expanded(const void* q_nope, long long qn_token, long long qn_head,

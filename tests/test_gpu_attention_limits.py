@@ -6,6 +6,7 @@ import torch
 from ferret_amd import lib
 from oracle import attention as A
 from tests.attention_helpers import SCALE, Batch, assert_near, bf16_tensor, bf16_values, i32, visible
+from tests.test_gpu_expanded_attention import Case as Expanded
 
 pytestmark = pytest.mark.gpu
 
@@ -108,3 +109,10 @@ def test_a_key_without_weight_adds_nothing_whatever_its_scale(ops, H, n, length)
             eo, el = A.bounds(o, ref, spread, reach, 576, length)
             assert_near(out[:, h], o, eo, f"key {key} head {h}")
             assert_near(lse[:, h], ref, el, f"lse key {key} head {h}")
+
+
+@pytest.mark.parametrize("length,n,H", [(2000, 1, 1), (1200, 3, 1), (2700, 5, 3)])
+def test_expanded_in_an_odd_number_of_parts_of_odd_rows(ops, length, n, H):
+    print(f"[case] expanded in odd parts length={length} n={n} H={H}", flush=True)
+    c = Expanded([length], [n], H)
+    c.check(*c.run(ops))
