@@ -28,6 +28,7 @@
 // rounded to bf16 (half a step, 2^-8 relative), l sums the unrounded terms.
 #include "attention.hpp"
 #include "expanded_plan.hpp"
+#include "ranges.hpp"
 
 #include <algorithm>
 #include <initializer_list>
@@ -538,9 +539,18 @@ extern "C" int ferret_latent_attention_expanded(const void* q_nope, long long qn
   const int parts = parts_of(B, T, S, H);
   const long long groups = tiles_of(B, T) * H * parts;
   FERRET_REQUIRE(groups < (1LL << 31), FERRET_ERR_SHAPE);
-  FERRET_REQUIRE(parts == 1 || (ws != nullptr && (bits(ws) & 15) == 0 &&
-                                ws_bytes >= ferret_latent_attention_expanded_workspace(B, T, S, H)),
-                 FERRET_ERR_WORKSPACE);
+  const size_t need = ferret_latent_attention_expanded_workspace(B, T, S, H);
+  FERRET_REQUIRE(parts == 1 || (ws != nullptr && (bits(ws) & 15) == 0 && ws_bytes >= need), FERRET_ERR_WORKSPACE);
+  // In place is sound: a work-group writes the rows that it alone has read, or the join does.
+  const bool over = in_place(out, q_nope, T, qn_token, H, qn_head, kNope);
+  FERRET_REQUIRE(!clash({Range{out, (uint64_t)T * H * kValue * 2}, Range{lse, (uint64_t)T * H * 4},
+                         Range{ws, need}},
+                        {bf16_range(over ? nullptr : q_nope, T, qn_token, H, qn_head, kNope),
+                         bf16_range(q_rotary, T, qr_token, H, qr_head, kRope),
+                         bf16_range(k_nope, S, kn_key, H, kn_head, kNope), bf16_range(k_rotary, S, kr_key, 1, 0, kRope),
+                         bf16_range(v, S, v_key, H, v_head, kValue), Range{cu_q, 4 * (B + 1ULL)},
+                         Range{cu_k, 4 * (B + 1ULL)}}),
+                 FERRET_ERR_SHAPE);
   Args a;
   a.qn = static_cast<const uint16_t*>(q_nope);
   a.qr = static_cast<const uint16_t*>(q_rotary);

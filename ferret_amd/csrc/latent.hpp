@@ -15,6 +15,7 @@
 
 #include "common.hpp"
 #include "latent_plan.hpp"
+#include "ranges.hpp"
 
 namespace ferret {
 
@@ -27,6 +28,15 @@ struct Pages {
   const int32_t* table;  // [B, max_pages]
   int max_pages, pages, page_size;
 };
+
+// What the cache's two arrays and the page table span.
+inline Range data_range(const void* data, const void* scales, int pages, int page_size) {
+  return {data, (uint64_t)pages * page_size * (scales != nullptr ? kRowE4m3 : kRowBf16)};
+}
+inline Range scale_range(const void* scales, int pages, int page_size) {
+  return {scales, (uint64_t)pages * page_size * 4};
+}
+inline Range ints_range(const int32_t* at, uint64_t n) { return {at, 4 * n}; }
 
 // The row number of position `pos` of sequence b in the cache, -1 for no row.
 __device__ __forceinline__ long long cache_row(const Pages& p, int b, int pos) {

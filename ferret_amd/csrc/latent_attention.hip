@@ -1369,8 +1369,18 @@ extern "C" int ferret_latent_attention(const void* q_latent, long long ql_token,
   FERRET_REQUIRE((long long)pages * page_size < (1LL << 35), FERRET_ERR_SHAPE);
   const long long tiles = (long long)T * H / mr + B, most = ((long long)max_pages * page_size + kKeys - 1) / kKeys + kLatentExtra;
   FERRET_REQUIRE(tiles * most < (1LL << 31), FERRET_ERR_SHAPE);
-  FERRET_REQUIRE(ws != nullptr && ws_bytes >= ferret_latent_attention_workspace(B, T, H) && (bits(ws) & 15) == 0,
-                 FERRET_ERR_WORKSPACE);
+  const size_t need = ferret_latent_attention_workspace(B, T, H);
+  FERRET_REQUIRE(ws != nullptr && ws_bytes >= need && (bits(ws) & 15) == 0, FERRET_ERR_WORKSPACE);
+  // In place is sound: the work-group that has read a whole tile writes it, the join those
+  // that were cut.
+  const bool over = in_place(out, q_latent, T, ql_token, H, ql_head, kLatent);
+  FERRET_REQUIRE(!clash({Range{out, (uint64_t)T * H * kLatent * 2}, Range{lse, (uint64_t)T * H * 4}, Range{ws, need}},
+                        {bf16_range(over ? nullptr : q_latent, T, ql_token, H, ql_head, kLatent),
+                         bf16_range(q_rotary, T, qr_token, H, qr_head, kRotary),
+                         data_range(data, scales, pages, page_size), scale_range(scales, pages, page_size),
+                         ints_range(page_table, (uint64_t)B * max_pages), ints_range(lens, B),
+                         ints_range(cu_q, B + 1LL)}),
+                 FERRET_ERR_SHAPE);
   Args a;
   a.ql = static_cast<const uint16_t*>(q_latent);
   a.qr = static_cast<const uint16_t*>(q_rotary);

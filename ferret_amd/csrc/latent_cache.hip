@@ -138,6 +138,12 @@ extern "C" int ferret_latent_cache_write(const void* latent, long long latent_st
   FERRET_REQUIRE(((bits(latent) | bits(rotary) | bits(data)) & 15) == 0 && (bits(scales) & 3) == 0 &&
                      (T == 1 || (latent_stride % 8 == 0 && rotary_stride % 8 == 0)),
                  FERRET_ERR_ALIGN);
+  FERRET_REQUIRE(!clash({data_range(data, scales, pages, page_size), scale_range(scales, pages, page_size)},
+                        {bf16_range(latent, T, T == 1 ? 0 : latent_stride, 1, 0, kLatent),
+                         bf16_range(rotary, T, T == 1 ? 0 : rotary_stride, 1, 0, kRotary),
+                         ints_range(page_table, (uint64_t)B * max_pages), ints_range(lens, B),
+                         ints_range(cu_q, B + 1LL)}),
+                 FERRET_ERR_SHAPE);
   const Pages pg{page_table, max_pages, pages, page_size};
   const dim3 grid((unsigned)(((long long)T + 3) / 4));
   const auto* lat = static_cast<const uint16_t*>(latent);
@@ -160,6 +166,10 @@ extern "C" int ferret_latent_cache_read(const void* data, const void* scales, in
   if (rc != FERRET_OK) return rc;
   FERRET_REQUIRE(rows >= 1, FERRET_ERR_SHAPE);
   FERRET_REQUIRE(((bits(latent) | bits(rotary) | bits(data)) & 15) == 0 && (bits(scales) & 3) == 0, FERRET_ERR_ALIGN);
+  FERRET_REQUIRE(!clash({Range{latent, (uint64_t)rows * kLatent * 2}, Range{rotary, (uint64_t)rows * kRotary * 2}},
+                        {data_range(data, scales, pages, page_size), scale_range(scales, pages, page_size),
+                         ints_range(page_table, (uint64_t)B * max_pages), ints_range(cu_k, B + 1LL)}),
+                 FERRET_ERR_SHAPE);
   const Pages pg{page_table, max_pages, pages, page_size};
   const dim3 grid((unsigned)(((long long)rows + 3) / 4));
   if (scales != nullptr)

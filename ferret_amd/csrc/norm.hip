@@ -15,6 +15,7 @@
 // rows of 7168 with residual and codes: 70 us, 5.9 TB/s; 64 rows of 512: 4.5 us, the
 // launch.
 #include "common.hpp"
+#include "ranges.hpp"
 
 namespace ferret {
 
@@ -163,8 +164,7 @@ static int pick_norm(const NormArgs& a, hipStream_t st) {
 }
 
 static bool overlap(const void* a, long long a_bytes, const void* b, long long b_bytes) {
-  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-  return x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
+  return overlap(Range{a, (uint64_t)a_bytes}, Range{b, (uint64_t)b_bytes});
 }
 
 // Rows of `out` (K elements of `size` bytes, packed) over rows of `in`: only

@@ -646,8 +646,9 @@ def latent_cache_write(cache: LatentCache, latent: torch.Tensor, rotary: torch.T
     sequence b to position lens[b] - n + i of the pages that page_table [B,
     max_pages] names.  Rows behind the last sequence, negative positions and
     entries that are no page are dropped.  Pages that are written must belong to
-    one sequence.  e4m3 caches are quantised on the way (one power-of-two scale
-    per 128 latents, so that reading back is exact)."""
+    one sequence, and the new rows may not stand in the cache.  e4m3 caches are
+    quantised on the way (one power-of-two scale per 128 latents, so that reading
+    back is exact)."""
     _latent_cache(cache)
     if _lib.native().latent_cache_write(cache.data, cache.scales, latent, rotary, page_table, lens, cu_q):
         return
@@ -666,7 +667,8 @@ def latent_cache_read(cache: LatentCache, page_table: torch.Tensor, cu_k: torch.
                       latent: torch.Tensor | None = None, rotary: torch.Tensor | None = None):
     """(latent bf16 [total, 512], rotary bf16 [total, 64]): the first cu_k[b+1] - cu_k[b] rows of every
     sequence, packed, exactly.  Rows behind cu_k[B] are left as they were (unset where
-    the outputs are new); rows of entries that are no page are zeros."""
+    the outputs are new); rows of entries that are no page are zeros.  Outputs overlap neither each
+    other nor the cache."""
     _latent_cache(cache)
     r = _lib.native().latent_cache_read(cache.data, cache.scales, page_table, cu_k, total, latent, rotary)
     if r is not None:
@@ -706,7 +708,8 @@ def latent_attention(q_latent: torch.Tensor, q_rotary: torch.Tensor, cache: Late
     the lengths on the device: nothing is read back, a captured call replays
     with other lengths.  `workspace` of latent_attention_workspace_bytes is
     taken from torch's caching allocator unless one is passed; calls that
-    overlap in time (streams, graphs) need one each.
+    overlap in time (streams, graphs) need one each.  `out` may be q_latent
+    itself where that is packed, and overlaps nothing else.
     """
     _latent_cache(cache)
     r = _lib.native().latent_attention(q_latent, q_rotary, cache.data, cache.scales, page_table, lens, cu_q,
@@ -754,7 +757,8 @@ def latent_attention_expanded(q_nope: torch.Tensor, q_rotary: torch.Tensor, k_no
     keys, each seeing the keys up to its own (causal) or all.  Tokens that see
     no key get zeros (lse -inf); rows behind the last sequence are left as they
     were (unset where `out` is new).  `workspace` of
-    latent_attention_expanded_workspace_bytes as latent_attention's.
+    latent_attention_expanded_workspace_bytes as latent_attention's, `out` too (on a
+    packed q_nope).
     """
     r = _lib.native().latent_attention_expanded(q_nope, q_rotary, k_nope, k_rotary, v, cu_q, cu_k, float(scale),
                                                 bool(causal), bool(return_lse), out, workspace)

@@ -309,6 +309,10 @@ int ferret_rms_norm_e4m3(const void* x, long long x_stride, const void* residual
  * tokens included, which are the last of them.  All of these are device arrays and
  * are read by the kernels only: a captured graph replays with other lengths.
  *
+ * No entry point of the cache or the latent attention takes an output or workspace that
+ * overlaps another or anything that the call reads (FERRET_ERR_SHAPE), but for what is
+ * named as in place.
+ *
  * ferret_latent_cache_write: new token i of sequence b to position
  * lens[b] - n + i (n = its number of new tokens; negative positions are dropped).
  * latent bf16 [T,512], rotary bf16 [T,64], rows *_stride elements apart (multiples
@@ -343,6 +347,7 @@ int ferret_latent_cache_read(const void* data, const void* scales, int pages, in
  * ws: ferret_latent_attention_workspace(B, T, H) bytes, on a 16-byte bound; two
  * calls that overlap in time need one each.  The result depends on the batch only
  * through the order of fp32 additions; the same call gives the same bits.
+ * out may stand exactly on packed q_latent.
  * Requirements: T >= 1, 1 <= H <= 1024, 0 < scale < 1e30.
  */
 size_t ferret_latent_attention_workspace(int B, int T, int H);
@@ -362,8 +367,8 @@ int ferret_latent_attention(const void* q_latent, long long ql_token, long long 
  * in elements (multiples of 8, < 2^24), so the key-value projection is taken as it
  * is.  cu_q and cu_k int32 [B + 1] as above; rows behind the last sequence are left
  * alone.  lse, tokens that see no key, and Inf or NaN that a token does not see: as
- * ferret_latent_attention.  Requirements: B, T, S >= 1, 1 <= H <= 1024,
- * 0 < scale < 1e30.
+ * ferret_latent_attention.  out may stand exactly on packed q_nope.  Requirements:
+ * B, T, S >= 1, 1 <= H <= 1024, 0 < scale < 1e30.
  * ws: ferret_latent_attention_expanded_workspace(B, T, S, H) bytes, on a 16-byte
  * bound; none (0, ws may be NULL) unless few tokens attend many keys.
  */

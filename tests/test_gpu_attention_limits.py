@@ -116,3 +116,57 @@ def test_expanded_in_an_odd_number_of_parts_of_odd_rows(ops, length, n, H):
     print(f"[case] expanded in odd parts length={length} n={n} H={H}", flush=True)
     c = Expanded([length], [n], H)
     c.check(*c.run(ops))
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_overlapping_tensors_are_refused(ops, native, monkeypatch):
+    print(f"[case] overlaps, native={native}", flush=True)
+    if not native:
+        monkeypatch.setattr(lib, "native", lambda: lib._Absent())
+    rng = np.random.default_rng(2)
+    b = Batch([100, 30], 16, False, 1)
+    (table, lens), cu = b.device(), i32([0, 1, 2])
+    room = bf16_tensor(bf16_values(rng, 3, 4, 512))
+    ql, qr = room[:2], bf16_tensor(bf16_values(rng, 2, 4, 64))
+    before = b.cache.data.clone()
+    ws = torch.empty(ops.latent_attention_workspace_bytes(2, 2, 4), dtype=torch.uint8, device="cuda")
+    inside = b.cache.data.view(-1)[:100 * 576]
+    for call in (lambda: ops.latent_attention(ql, qr, b.cache, table, lens, cu, SCALE, out=room[1:]),
+                 lambda: ops.latent_attention(ql, qr, b.cache, table, lens, cu, SCALE, out=inside[:4096].view(2, 4, 512)),
+                 lambda: ops.latent_attention(ql, qr, b.cache, table, lens, cu, SCALE, workspace=ws,
+                                              out=ws[:8192].view(torch.bfloat16).view(2, 4, 512)),
+                 lambda: ops.latent_cache_read(b.cache, table, i32([0, 20, 40]), 40, inside[:40 * 512].view(40, 512)),
+                 lambda: ops.latent_cache_write(b.cache, inside.view(100, 576)[:2, :512], qr[:, 0].contiguous(), table, lens,
+                                                cu)):
+        with pytest.raises(RuntimeError, match="code -2"):
+            call()
+    torch.cuda.synchronize()
+    assert torch.equal(b.cache.data.view(torch.uint8), before.view(torch.uint8))
+
+
+@pytest.mark.parametrize("H,n,length", [(16, 1, 5000), (16, 40, 300), (128, 2, 3000), (3, 4, 70)])
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_absorbed_in_place(ops, H, n, length, e4m3):
+    """The output on its queries, in whole tiles and in tiles that are cut and joined."""
+    print(f"[case] absorbed in place H={H} n={n} length={length} e4m3={e4m3}", flush=True)
+    rng = np.random.default_rng(3)
+    b = Batch([length, n + 1], 64, e4m3, 5)
+    ql, qr = (bf16_tensor(bf16_values(rng, 2 * n, H, w)) for w in (512, 64))
+    args = (qr, b.cache, *b.device(), i32([0, n, 2 * n]), SCALE)
+    want = ops.latent_attention(ql, *args)
+    got = ops.latent_attention(ql, *args, out=ql)
+    torch.cuda.synchronize()
+    assert got.data_ptr() == ql.data_ptr() and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("lens,new,H", [([300, 129], [200, 129], 4), ([5000], [3], 2), ([200, 131], [200, 1], 256)])
+def test_expanded_in_place(ops, lens, new, H):
+    print(f"[case] expanded in place lens={lens} new={new} H={H}", flush=True)
+    c = Expanded(lens, new, H)
+    qn, *rest = c.tensors()
+    qn = qn.contiguous()
+    cu_q, cu_k = i32(np.cumsum([0, *new])), i32(np.cumsum([0, *lens]))
+    want = ops.latent_attention_expanded(qn, *rest, cu_q, cu_k, SCALE)
+    got = ops.latent_attention_expanded(qn, *rest, cu_q, cu_k, SCALE, out=qn)
+    torch.cuda.synchronize()
+    assert got.data_ptr() == qn.data_ptr() and torch.equal(got, want)
