@@ -176,16 +176,16 @@ __device__ __forceinline__ bool take_share(const Args& a, LatentPlace place, Sid
   int mine = 0, my_groups = 0;
   for (int i = 0; i < per && b0 + i < a.B; ++i) {
     s = sequence<MR>(a, b0 + i);
-    mine += s.work(0);
-    my_groups += s.groups;
+    mine = latent_add(mine, s.work(0));
+    my_groups = latent_add(my_groups, s.groups);
   }
   int incl = mine, incl_groups = my_groups;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
     const int o = __shfl_up(incl, off, 64), og = __shfl_up(incl_groups, off, 64);
     if (lane >= off) {
-      incl += o;
-      incl_groups += og;
+      incl = latent_add(incl, o);
+      incl_groups = latent_add(incl_groups, og);
     }
   }
   constexpr int NW = NT / 64;
@@ -195,33 +195,33 @@ __device__ __forceinline__ bool take_share(const Args& a, LatentPlace place, Sid
   }
   __syncthreads();
   asm volatile("" ::"v"(near));
-  int before = 0, total = 0, groups_before = 0, groups = 0;
+  int before = 0, all = 0, groups_before = 0, groups = 0;
 #pragma unroll
   for (int w = 0; w < NW; ++w) {
     if (w < wave) {
-      before += tot[w];
-      groups_before += tot[NW + w];
+      before = latent_add(before, tot[w]);
+      groups_before = latent_add(groups_before, tot[NW + w]);
     }
-    total += tot[w];
-    groups += tot[NW + w];
+    all = latent_add(all, tot[w]);
+    groups = latent_add(groups, tot[NW + w]);
   }
   const int units = kUnits / a.side_by_side;
-  int chunk = latent_chunk(total, units, a.min_steps), extra = kLatentExtra;
+  bool whole = false;
   if (per == 1) {  // more sequences than threads do not all fit
-    const bool fits = latent_fits(s, chunk);
+    const bool fits = latent_fits(s, latent_chunk(all, units, a.min_steps));
     if (lane == 0) tot[2 * NW + wave] = 0;
     if (__any(!fits) && lane == 0) tot[2 * NW + wave] = 1;
     __syncthreads();
     int misfits = 0;
 #pragma unroll
     for (int w = 0; w < NW; ++w) misfits |= tot[2 * NW + w];
-    if (misfits == 0) extra = 0;
+    whole = misfits == 0;
   }
-  total += extra * groups;
-  if (extra != 0) chunk = latent_chunk(total, units, a.min_steps);
+  const LatentDeal deal = latent_deal(all, groups, whole, units, a.min_steps);
+  const int total = deal.total, chunk = deal.chunk, extra = deal.extra;
   const int start = (int)min((long long)place.unit * chunk, (long long)total);
-  const int excl = before + incl - mine + extra * (groups_before + incl_groups - my_groups);
   if (start >= total) return false;
+  const int excl = before + incl - mine + extra * (groups_before + incl_groups - my_groups);
   if (excl <= start && start < excl + mine + extra * my_groups) {
     int at = excl, i = 0;
     if (per > 1)
@@ -1365,10 +1365,10 @@ extern "C" int ferret_latent_attention(const void* q_latent, long long ql_token,
                      ((bits(scales) | bits(lse)) & 3) == 0 && ((ql_token | ql_head | qr_token | qr_head) & 7) == 0,
                  FERRET_ERR_ALIGN);
   const int mr = tile_rows(T, B, H);
-  // steps of the whole batch are counted in 32 bits
+  // steps of the whole batch are counted in 32 bits, rounded up to whole shares
   FERRET_REQUIRE((long long)pages * page_size < (1LL << 35), FERRET_ERR_SHAPE);
   const long long tiles = (long long)T * H / mr + B, most = ((long long)max_pages * page_size + kKeys - 1) / kKeys + kLatentExtra;
-  FERRET_REQUIRE(tiles * most < (1LL << 31), FERRET_ERR_SHAPE);
+  FERRET_REQUIRE(tiles * most < (1LL << 31) - kUnits, FERRET_ERR_SHAPE);
   const size_t need = ferret_latent_attention_workspace(B, T, H);
   FERRET_REQUIRE(ws != nullptr && ws_bytes >= need && (bits(ws) & 15) == 0, FERRET_ERR_WORKSPACE);
   // In place is sound: the work-group that has read a whole tile writes it, the join those

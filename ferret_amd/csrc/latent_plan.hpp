@@ -6,6 +6,8 @@
 // outside the cache is named, whatever the index tensors hold.
 #pragma once
 
+#include <climits>
+
 #ifdef __HIPCC__
 #define FERRET_HD __host__ __device__ __forceinline__
 #else
@@ -54,10 +56,30 @@ FERRET_HD LatentSeq latent_seq(int start, int end, int len, int T, int H, int mr
 // sequences of 600 to 8000 keys: 62.5 us without, 51.5 with 5; 64 rows, bf16, 32 of
 // 2000: 47.9 us without, 55.0 with 5.  Steps per unit of a line of `total`:
 FERRET_HD int latent_chunk(int total, int units, int min_steps) {
-  return plan_max(min_steps, (total + units - 1) / units);
+  return plan_max(min_steps, total / units + (total % units != 0));
 }
 
 FERRET_HD bool latent_fits(const LatentSeq& s, int chunk) { return s.groups == 0 || s.steps % chunk == 0; }
+
+// Sums of work along the line, of numbers from 0 on; they stop at INT_MAX.  Starts that ascend
+// stay far below it (the caller checks T and the table's keys); where they do not, sequences
+// overlap, and a sum that went round would lead to shares that nobody or several name.
+FERRET_HD int latent_add(int a, int b) {
+  const unsigned sum = (unsigned)a + (unsigned)b;
+  return sum > (unsigned)INT_MAX ? INT_MAX : (int)sum;
+}
+
+// The deal of a line of `total` steps in `groups` groups to `units` units: total 0 where
+// there is nothing to do, or where it does not fit 32 bits.
+struct LatentDeal {
+  int total, chunk, extra;
+};
+FERRET_HD LatentDeal latent_deal(int total, int groups, bool fits, int units, int min_steps) {
+  const int extra = fits ? 0 : kLatentExtra;
+  const long long line = total + (long long)extra * groups;
+  if (line > INT_MAX - kLatentUnits) return LatentDeal{0, 1, 0};
+  return LatentDeal{(int)line, latent_chunk((int)line, units, min_steps), extra};
+}
 
 // The unit and the place in it of a work-group.  Work-groups are dealt to the 8 XCDs
 // in turn; a unit's stay on one, so that its keys come from memory once.

@@ -170,3 +170,18 @@ def test_expanded_in_place(ops, lens, new, H):
     got = ops.latent_attention_expanded(qn, *rest, cu_q, cu_k, SCALE, out=qn)
     torch.cuda.synchronize()
     assert got.data_ptr() == qn.data_ptr() and torch.equal(got, want)
+
+
+def test_overlapping_sequences_past_32_bits_of_steps_are_left_out(ops):
+    """Starts that do not ascend: 350 sequences over the same 64 tokens, 4.7e10 steps; nothing is written."""
+    print("[case] absorbed, overlapping sequences", flush=True)
+    B, T, H = 700, 64, 128
+    cache = ops.LatentCache.empty(1, 1 << 20)
+    table = torch.zeros((B, 16), dtype=torch.int32, device="cuda")
+    out = torch.full((T, H, 512), 7.0, dtype=torch.bfloat16, device="cuda")
+    cu = i32([T * (b % 2) for b in range(B)] + [T])
+    ws = torch.zeros(ops.latent_attention_workspace_bytes(B, T, H), dtype=torch.uint8, device="cuda")
+    ops.latent_attention(torch.zeros_like(out), out[..., :64].contiguous(), cache, table, i32([1 << 24] * B), cu, SCALE,
+                         out=out, workspace=ws)
+    torch.cuda.synchronize()
+    assert (out == 7).all()
