@@ -169,7 +169,8 @@ __device__ __forceinline__ int swz(int r) { return (((r >> 1) ^ r) & 4) | (r & 2
 template <int MR, int NT>
 __device__ __forceinline__ bool take_share(const Args& a, LatentPlace place, Side* side, int* tot, int* cur) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int near = a.pages.table[(long long)(place.unit * a.B / (kUnits / a.side_by_side)) * a.pages.max_pages];
+  const int near =
+      a.pages.table[(long long)latent_near(place.unit, kUnits / a.side_by_side, a.B) * a.pages.max_pages];
   const int per = (a.B + NT - 1) / NT;
   const int b0 = threadIdx.x * per;
   LatentSeq s{};

@@ -90,6 +90,10 @@ FERRET_HD LatentPlace latent_place(int block, int side) {
   return LatentPlace{block / (8 * side) * 8 + block % 8, block / 8 % side};
 }
 
+// A sequence that a unit's share may start in, were all alike: floor(unit * B / units),
+// without the product, which passes 32 bits from 2^23 sequences on.
+FERRET_HD int latent_near(int unit, int units, int B) { return unit * (B / units) + unit * (B % units) / units; }
+
 // The slot of the partial result that a unit's work-group takes up at `cur` of the
 // line: the share may start and end inside a tile, so there are two each.
 FERRET_HD int latent_slot(int unit, int lane, int side, int cur, int chunk) {

@@ -93,3 +93,32 @@ def test_a_share_is_named_once_or_there_is_none(tmp_path):
     res = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
     assert res.returncode == 0, res.stdout + res.stderr
     assert res.stdout.endswith(" 0 violations\n")
+
+
+NEAR = r"""
+#include <climits>
+#include <cstdio>
+#include <initializer_list>
+#include "latent_plan.hpp"
+using namespace ferret;
+int main() {
+  long long bad = 0;
+  for (int units : {32, 64, 128, 256})
+    for (int B : {1, 2, 31, 32, 33, 255, 256, 257, 600, 8421504, 8421505, 9000000, 1 << 28, INT_MAX})
+      for (int unit = 0; unit < units; ++unit) bad += latent_near(unit, units, B) != (long long)unit * B / units;
+  std::printf("%lld off\n", bad);
+  return bad != 0;
+}
+"""
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="g++ not installed")
+def test_the_sequence_looked_up_first_is_one_of_the_batch(tmp_path):
+    """Also where unit * B passes 32 bits (from 8421505 sequences on)."""
+    src = tmp_path / "near.cpp"
+    src.write_text(NEAR)
+    exe = tmp_path / "near"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover=all", f"-I{CSRC}",
+                    str(src), "-o", str(exe)], check=True, capture_output=True, text=True)
+    res = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert res.returncode == 0, res.stdout + res.stderr
