@@ -527,6 +527,7 @@ extern "C" int ferret_latent_attention_expanded(const void* q_nope, long long qn
                                                 void* ws, size_t ws_bytes, void* stream) {
   FERRET_REQUIRE(q_nope && q_rotary && k_nope && k_rotary && v && cu_q && cu_k && out, FERRET_ERR_NULL);
   FERRET_REQUIRE(B >= 1 && T >= 1 && S >= 1 && H >= 1 && H <= 1024, FERRET_ERR_SHAPE);
+  FERRET_REQUIRE(S <= 1 << 30, FERRET_ERR_SHAPE);  // the search for a tile looks some steps past S
   FERRET_REQUIRE(scale > 0.f && scale < 1e30f, FERRET_ERR_SHAPE);
   for (const long long stride : {qn_token, qn_head, qr_token, qr_head, kn_key, kn_head, kr_key, v_key, v_head}) {
     FERRET_REQUIRE(stride >= 0 && stride < (1LL << 24), FERRET_ERR_SHAPE);  // 64 rows stay within 32 bits

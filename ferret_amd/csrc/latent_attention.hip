@@ -1366,6 +1366,7 @@ extern "C" int ferret_latent_attention(const void* q_latent, long long ql_token,
                      ((bits(scales) | bits(lse)) & 3) == 0 && ((ql_token | ql_head | qr_token | qr_head) & 7) == 0,
                  FERRET_ERR_ALIGN);
   const int mr = tile_rows(T, B, H);
+  FERRET_REQUIRE((long long)max_pages * page_size <= (1LL << 31) - 2 * kKeys, FERRET_ERR_SHAPE);  // a step's end stays below 2^31
   // steps of the whole batch are counted in 32 bits, rounded up to whole shares
   FERRET_REQUIRE((long long)pages * page_size < (1LL << 35), FERRET_ERR_SHAPE);
   const long long tiles = (long long)T * H / mr + B, most = ((long long)max_pages * page_size + kKeys - 1) / kKeys + kLatentExtra;

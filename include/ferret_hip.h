@@ -348,7 +348,8 @@ int ferret_latent_cache_read(const void* data, const void* scales, int pages, in
  * calls that overlap in time need one each.  The result depends on the batch only
  * through the order of fp32 additions; the same call gives the same bits.
  * out may stand exactly on packed q_latent.
- * Requirements: T >= 1, 1 <= H <= 1024, 0 < scale < 1e30.
+ * Requirements: T >= 1, 1 <= H <= 1024, 0 < scale < 1e30, max_pages * page_size
+ * <= 2^31 - 128.
  */
 size_t ferret_latent_attention_workspace(int B, int T, int H);
 int ferret_latent_attention(const void* q_latent, long long ql_token, long long ql_head, const void* q_rotary,
@@ -368,7 +369,7 @@ int ferret_latent_attention(const void* q_latent, long long ql_token, long long 
  * is.  cu_q and cu_k int32 [B + 1] as above; rows behind the last sequence are left
  * alone.  lse, tokens that see no key, and Inf or NaN that a token does not see: as
  * ferret_latent_attention.  out may stand exactly on packed q_nope.  Requirements:
- * B, T, S >= 1, 1 <= H <= 1024, 0 < scale < 1e30.
+ * B, T >= 1, 1 <= S <= 2^30, 1 <= H <= 1024, 0 < scale < 1e30.
  * ws: ferret_latent_attention_expanded_workspace(B, T, S, H) bytes, on a 16-byte
  * bound; none (0, ws may be NULL) unless few tokens attend many keys.
  */

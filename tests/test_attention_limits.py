@@ -79,3 +79,17 @@ def test_expanded_outputs_and_workspace_stand_apart(L):
             if other != written:
                 assert _refused(f, args, written, args[other] + (16 if other == 0 else 0)), (written, other)
     assert _refused(f, [*args[:1], 2056, *args[2:]], 22, G)
+
+
+def test_keys_that_32_bits_do_not_count_are_refused(L):
+    """Steps of 64 keys end past 2^31 where a sequence may have more than 2^31 - 128 keys (a table may name a page
+    many times); the expanded form's search for a tile passes 2^31 from about 2.1e9 keys on (keys may have stride 0)."""
+    need = L.ferret_latent_attention_workspace(1, 1, 16)
+    args = [G, 8192, 512, 2 * G, 1024, 64, 3 * G, 4 * G, 100, 16, 5 * G, 6 * G, 7 * G, 1, 8, 1, 16, 0.07, 1, 8 * G, 9 * G,
+            10 * G, need, None]
+    for max_pages in ((1 << 27) - 1, (1 << 27) - 7):
+        assert _refused(L.ferret_latent_attention, args, 14, max_pages)
+    args = [G, 2048, 128, 2 * G, 1024, 64, 3 * G, 0, 0, 4 * G, 0, 5 * G, 0, 0, 6 * G, 7 * G, 1, 9, 8000, 16, 0.07, 1, 8 * G,
+            9 * G, 10 * G, 1 << 30, None]
+    for keys in ((1 << 30) + 1, (1 << 31) - 1):
+        assert _refused(L.ferret_latent_attention_expanded, args, 18, keys)
