@@ -44,7 +44,9 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const uint16_t* __rest
   if (lane < 8) rot = ld_u32x4_stream(rotary + t * rs + lane * 8);
   const int b = sequence_of(cu_q, B, t);
   if (b >= B || t < cu_q[b]) return;
-  const long long row = cache_row(pages, b, lens[b] - (cu_q[b + 1] - t));
+  const long long pos = (long long)lens[b] - cu_q[b + 1] + t;  // 32 bits would go round far below zero
+  if (pos < 0 || pos > INT_MAX) return;
+  const long long row = cache_row(pages, b, (int)pos);
   if (row < 0) return;
   if constexpr (!F8) {
     uint8_t* to = data + row * kRowBf16;

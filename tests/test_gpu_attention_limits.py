@@ -185,3 +185,17 @@ def test_overlapping_sequences_past_32_bits_of_steps_are_left_out(ops):
                          out=out, workspace=ws)
     torch.cuda.synchronize()
     assert (out == 7).all()
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_positions_far_below_zero_are_dropped(ops, e4m3):
+    """lens - n + i below -2^31 is a negative position like any other."""
+    print(f"[case] cache write far below zero e4m3={e4m3}", flush=True)
+    c = ops.LatentCache.empty(3, 16, torch.float8_e4m3fn if e4m3 else torch.bfloat16)
+    before = c.data.clone()
+    x, r = (torch.ones((20, w), dtype=torch.bfloat16, device="cuda") for w in (512, 64))
+    table = i32([0, 1, 2]).view(1, 3)
+    for length, end in ((-2 ** 31, 2 ** 31 - 1), (-2 ** 31 + 5, 2 ** 31 - 1), (-2 ** 31, 2 ** 31 - 20), (-1, 2 ** 31 - 1)):
+        ops.latent_cache_write(c, x, r, table, i32([length]), i32([0, end]))
+    torch.cuda.synchronize()
+    assert torch.equal(c.data, before)
