@@ -23,7 +23,7 @@
 // visible key and head keep the first busy for 52% of a long prompt's cycles,
 // exponentials, packing and masks the second for 36% or more, at a clock that falls
 // below 2 GHz; no LDS bank conflicts.
-// 16 heads, 4096 new tokens after 4096 others: 244 us, 1060 TFLOP/s (counting visible
+// 16 heads, 4096 new tokens after 4096 others: 240 us, 1070 TFLOP/s (counting visible
 // pairs), where a large product of the library reaches 1206.  S, m, l and O are fp32; P is
 // rounded to bf16 (half a step, 2^-8 relative), l sums the unrounded terms.
 #include "attention.hpp"
@@ -43,9 +43,9 @@ constexpr int kV = kKr + kStep * kRope * 2, kBuf = kV + kStep * kValue * 2;
 static_assert(4 * kBuf <= 160 * 1024, "LDS of a CU: two work-groups, or one of two teams");
 
 // Key and value fragments are read ahead of their products in rings that scheduling
-// fences keep: 4096 after 4096 others, in one team: 245.8 us against 252.7 where the
+// fences keep: 4096 after 4096 others, in one team: 240.2 us, 3% less than where the
 // compiler places the reads, two at a time; 4 and 4, or 8 and 4, with a fence per 4
-// products: 248.0 and 246.9.
+// products: 240.6 and 240.0.
 constexpr int kAheadK = 6, kAheadV = 4, kFence = 2;
 constexpr int kCus = 256;
 constexpr int kMaxParts = 16, kPartSteps = 6;
@@ -475,10 +475,10 @@ long long tiles_of(int B, int T) { return std::min<long long>(T, (T + (kTokens -
 
 // Parts of a tile's keys: as many as there are CUs for, of kPartSteps steps or more by the
 // keys that a token sees on average, as though all were causal.  One part / as here, us: 8
-// heads, 100 tokens of 8192 keys 146 / 26.9 (16 parts), 1024 of 8192 146 / 57.0 (4), 2048
-// of 8192 147 / 93.5 (2), 2048 of 2048 45.2 / 39.3 (2).  Against it: 16 heads, 1024 of
-// 1024, 28.4 in one and 31.3 in two parts of 4 steps, whose partials cost more than
-// they gain; 8 heads, 2048 of 8192, 123 in parts for four times as many CUs.
+// heads, 100 tokens of 8192 keys 148 / 26.7 (16 parts), 1024 of 8192 148 / 59.9 (4), 2048
+// of 8192 149 / 96.8 (2), 2048 of 2048 45.4 / 39.0 (2).  Against it: 16 heads, 1024 of
+// 1024, 28.6 in one and 31.1 in two parts of 4 steps, whose partials cost more than
+// they gain; 8 heads, 2048 of 8192, 128 in parts for four times as many CUs.
 int parts_of(int B, int T, int S, int H) {
   const long long wide = kCus / (tiles_of(B, T) * H), deep = (S - T / 2) / B / (kStep * kPartSteps);
   return (int)std::max(1LL, std::min({wide, deep, (long long)kMaxParts}));
@@ -488,9 +488,10 @@ int parts_of(int B, int T, int S, int H) {
 // decides (1.6 us a step in one team that has a CU to itself, half of 2.5 in two), or the
 // sum over the card (2.45 us for two steps of a CU's two work-groups, 2.5 for two teams'
 // and about 3 us for each of their tiles' start and join, which nothing covers).  One / two,
-// causal, us: 16 heads, one prompt of 2048 56.0 / 47.0, of 4096 109 / 98.6, 4096 after 4096
-// others 243.6 / 250.1, two of 2048 61.8 / 60.0, five of 1024 50.2 / 63.3, eight 72.5 /
-// 98.2; 128 heads of 512 26.2 / 33.6.
+// causal, us: 16 heads, one prompt of 2048 56.2 / 47.1, of 4096 109 / 97.6, 4096 after 4096
+// others 240 / 254, two of 2048 62.1 / 60.3, five of 1024 50.9 / 64.4, eight 74.1 / 102;
+// 128 heads of 512 27.2 / 34.4.  The longest prompt is taken to be as long as the mean: a ragged
+// batch's longest tile may count for more.
 bool one_team(int B, int T, int S, long long groups) {
   const float longest = (float)S / B / kStep, mean = fmaxf((float)S - 0.5f * T, 0.f) / B / kStep;
   const float all = (float)groups * mean / (2 * kCus);

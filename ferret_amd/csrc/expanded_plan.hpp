@@ -15,8 +15,8 @@ constexpr int kTileTokens = 128;   // query tokens per tile
 constexpr int kTileKeys = 64;      // keys per step
 // Sequences up to which tiles go by length over the whole batch: the search costs each
 // work-group about 0.15 us per sequence.  By length / sequence by sequence, 16 heads, us: four
-// prompts of 700 to 1900 64.3 / 75.7, eight of 300 to 1300 65.8 / 70.6, sixteen of 100 to 700
-// 50.8 / 41.5, forty of 50 to 300 77.8 / 42.5.
+// prompts of 700 to 1900 63.2 / 67.9, eight of 300 to 1300 63.7 / 71.3, sixteen of 100 to 700
+// 59.9 / 55.3, forty of 50 to 300 94.6 / 49.7.
 constexpr int kOrderedBatch = 8;
 
 // The tiles of one sequence: n new tokens, the last of len keys.
@@ -40,7 +40,7 @@ struct TileSeq {
 
 // Where two work-groups share a CU, the second `first` slots of a head (a CU's worth each)
 // go from short to long, so that the longest tiles do not meet the next longest (4096
-// tokens after 4096 others, 16 heads: 255 us, 265 without).
+// tokens after 4096 others, 16 heads: 240 us, 257 without).
 FERRET_XHD int paired_rank(int slot, int all, int first) {
   const int both = all < 2 * first ? all : 2 * first;
   return slot < first || slot >= both ? slot : both - 1 - (slot - first);

@@ -29,11 +29,11 @@
 // after (64 rows) it is rounded to bf16: exact, so nothing is lost by it.
 //
 // What bounds it.  16 heads, one token: the cache's bytes; 64 sequences of 600 to 8000
-// keys, e4m3, 49 us, 3.6 TB/s with launch and joins, of which the kernel takes 44.  64
+// keys, e4m3, 49 us, 3.6 TB/s with launch and joins, of which the kernel takes 45.  64
 // rows: no one unit.  32 sequences of 8192, 128 heads, bf16, 100 us: the matrix units
 // are busy for 40% of the cycles, LDS for 27%, the vector units for 20%, and memory
-// delivers 3.0 TB/s; the clock falls to 2.0 GHz under it.  e4m3, 93 us: the vector
-// units take 37%, widening the keys twice and the values once, beside 39% of products.
+// delivers 3.0 TB/s; the clock falls to 2.0 GHz under it.  e4m3, 92 us: the vector
+// units take 39%, widening the keys twice and the values once, beside 40% of products.
 //
 // Numerics: S, m, l and O are fp32; P is rounded to bf16 for the MFMA (half a step,
 // 2^-8 relative, random over the keys), l sums the unrounded P.  The running
@@ -1081,8 +1081,8 @@ __global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) ring[i] = frag(i);
         // e4m3: a probability takes its key's power of two for the wave's columns, by adding
-        // to the exponents of two at a time: 125.5 us for chunks of 200 to 500 tokens on
-        // 5000 keys, 137.7 by widening, two products and rounding.  Exact for normal numbers; a
+        // to the exponents of two at a time: 121.5 us for chunks of 200 and 500 tokens on 3500
+        // and 5000 keys, 125.7 by widening, two products and rounding.  Exact for normal numbers; a
         // product below 2^-126 becomes some number below 2^-126.  Zeros stay zeros (P is zero
         // or normal): a key that a query does not see, or whose term vanished, may have any scale.
         // The pair of ones is kept from the compiler, which would make compares and selects of
@@ -1168,7 +1168,7 @@ __device__ __forceinline__ float piece_sum(float2 v, float base) {
 }
 
 // Many rows, few pieces each: a wave per row, 8 columns per lane, the pieces' weights
-// 64 at a time in the lanes, eight pieces' loads under way together.
+// 64 at a time in the lanes, four pieces' loads under way together.
 __global__ __launch_bounds__(256) void latent_join_kernel(Args a, int mr, int rows) {
   const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (row >= rows) return;
@@ -1179,8 +1179,8 @@ __global__ __launch_bounds__(256) void latent_join_kernel(Args a, int mr, int ro
   const float* part = a.part(mr) + lane * 4;
   const auto at = [&](int j) { return (long long)latent_record_slot(where, a.side_by_side, j) * mr + r; };
   // The first pieces' outputs come under their maxima, four pieces at a time: 71 registers
-  // leave room for seven waves per SIMD (chunks of 200 to 500 tokens 122.7 us; eight at a
-  // time, after the maxima, 125.2).
+  // leave room for seven waves per SIMD (chunks of 200 to 500 tokens: 2% less time for the
+  // whole call than with eight at a time, after the maxima).
   f32x4 x[4][2];
   const auto load = [&](int j) __attribute__((always_inline)) {
 #pragma unroll
@@ -1227,8 +1227,8 @@ __global__ __launch_bounds__(256) void latent_join_kernel(Args a, int mr, int ro
 
 // Few rows, up to kUnits pieces each: a work-group per row and 128 columns, 32 lanes
 // across and the pieces dealt to 8 groups of lanes, 8 in flight each.  A wave per row /
-// this, whole call, us: 16 heads, e4m3, one sequence of 100001 53.5 / 27.7, 32 of 6000 (512
-// rows) 39.5 / 38.9, 64 of 600 to 8000 (1024 rows) 49.2 / 51.6.
+// this, whole call, us: 16 heads, e4m3, one sequence of 100001 69.4 / 28.2, 16 of 6000 28.7 /
+// 27.6, 32 of 6000 (512 rows) 40.1 / 40.3, 64 of 600 to 8000 (1024 rows) 50.4 / 53.1.
 __global__ __launch_bounds__(256) void latent_join_long_kernel(Args a, int mr) {
   constexpr int ACROSS = 32, GROUPS = 256 / ACROSS;
   __shared__ f32x4 red[256];
@@ -1318,18 +1318,18 @@ int launch_rows(int mr, const Args& a, hipStream_t st) {
 }
 
 // Query rows per tile by the rows that a sequence has on average.  Us, e4m3, 64 sequences
-// of 3000: 32 heads 45.7 in tiles of 32, 56.3 of 16, 51.1 of 64; 16 heads of 600 to 8000
-// 49.2 of 16, 53.7 of 32; 32 of 3000, 64 heads 40.9 of 64, 44.2 of 32; 128 heads, bf16,
-// 32 of 900 to 6000 67.2 of 64 against 83.0 of 32.
+// of 3000: 32 heads 46.9 in tiles of 32, 56.7 of 16, 48.7 of 64; 16 heads of 600 to 8000
+// 50.4 of 16, 54.6 of 32; 32 of 3000, 64 heads 39.8 of 64, 45.3 of 32; 128 heads, bf16,
+// 32 of 900 to 6000 58.8 of 64 against 80.6 of 32.
 int tile_rows(int T, int B, int H) {
   const long long rows = (long long)T * H / B;
   return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 }
 
 // Row tiles side by side by the tiles that a sequence has on average: work-groups of one
-// XCD that walk the same keys at the same time.  128 heads, bf16, 32 sequences of 900 to
-// 6000: 58.5 us, one after another 65.1; 500 new tokens of two sequences, 16 heads: 172
-// us eight at a time, 194 two or one.
+// XCD that walk the same keys at the same time.  128 heads (two tiles), bf16, 32 sequences of
+// 900 to 6000: 58.8 us two at a time, 66.0 one after another, 79.9 four; 500 new tokens of
+// two sequences of 4000, 16 heads, e4m3: 138 us eight at a time, 139 two, 158 one.
 int side_by_side(int T, int B, int H) {
   const long long tiles = (long long)T * H / B / 64;
   return tiles < 2 ? 1 : tiles < 4 ? 2 : tiles < 8 ? 4 : 8;
@@ -1400,8 +1400,8 @@ extern "C" int ferret_latent_attention(const void* q_latent, long long ql_token,
   a.H = H;
   a.scale_log2 = scale * kLog2e;
   a.causal = causal != 0;
-  // Shares of one step where a step is short: 16 heads, 256 keys 13.4 us against 14.9 in
-  // shares of two; 128 heads, 8 sequences of 100 keys 21.1 in shares of two, 22.1 of one.
+  // Shares of one step where a step is short: 16 heads, 256 keys 13.2 us against 14.8 in
+  // shares of two; 128 heads, e4m3, 8 sequences of 100 keys 20.4 in shares of two, 21.0 of one.
   a.min_steps = mr == 64 ? 2 : 1;
   a.side_by_side = side_by_side(T, B, H);
   a.out = static_cast<uint16_t*>(out);

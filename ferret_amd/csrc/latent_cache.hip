@@ -11,8 +11,9 @@
 // the rotary values.  HBM-bound: 1152 bytes on one side and 644 (e4m3) or 1152 on
 // the other; at decode sizes the launch and the two dependent loads (cu_q, page
 // table) are all there is.  48000 rows read from e4m3: 22.7 us, 3.8 TB/s (two and four
-// rows per wave, their loads in flight together: 23.3 and 30.5); 64 tokens written: 4
-// us with the launch.
+// rows per wave, their loads in flight together: 23.3 and 30.5); in a replayed graph 64
+// tokens written take 2.6 us and 9900 tokens 6.5, where their bytes take 3.6: a wave per
+// token, whose look-ups (cu_q, the length, the page table) follow one another.
 #include "latent.hpp"
 
 namespace ferret {

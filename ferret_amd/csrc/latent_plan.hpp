@@ -53,8 +53,8 @@ FERRET_HD LatentSeq latent_seq(int start, int end, int len, int T, int H, int mr
 // steps without keys, so that a unit that goes on to a second tile (its queries, and the
 // first keys' way from memory) is not the last to end: kLatentExtra, or none where
 // every sequence is a whole number of shares as it is (latent_fits).  16 rows, e4m3, 64
-// sequences of 600 to 8000 keys: 62.5 us without, 51.5 with 5; 64 rows, bf16, 32 of
-// 2000: 47.9 us without, 55.0 with 5.  Steps per unit of a line of `total`:
+// sequences of 600 to 8000 keys: 55.5 us without, 50.4 with 5; 64 rows, bf16, 32 of
+// 2000: 42.3 us without, 46.8 with 5.  Steps per unit of a line of `total`:
 FERRET_HD int latent_chunk(int total, int units, int min_steps) {
   return plan_max(min_steps, total / units + (total % units != 0));
 }

@@ -12,8 +12,8 @@
 // 16-byte chunks per lane), so it is read once, and a row may be written in
 // place: every lane's loads have returned before its row's sum is known.
 // HBM-bound: 2 bytes read per element (4 with the residual) and 1 to 4 written.  8192
-// rows of 7168 with residual and codes: 70 us, 5.9 TB/s; 64 rows of 512: 4.5 us, the
-// launch.
+// rows of 7168 with residual and codes: 71 us, 5.8 TB/s; 64 rows of 512: 2.3 us in a
+// replayed graph, 5.0 called from Python, the launch.
 #include "common.hpp"
 #include "ranges.hpp"
 

@@ -276,7 +276,8 @@ int ferret_moe_combine(const void* o, const float* w, int T, int topk, int N, vo
  * y and residual_out bf16 [M,K] packed.  residual and residual_out are both given
  * or both NULL.  An output may stand exactly on x or residual (in place); any
  * other overlap is rejected.  The reference has no norm; this is the library's own
- * contract.  Requirements: M >= 1, K % 8 == 0, K <= 32768, eps >= 0; pointers on
+ * contract.  The sum of the squares is fp32: rows whose squares add up past 2^128 come
+ * out as zeros.  Requirements: M >= 1, K % 8 == 0, K <= 32768, eps >= 0; pointers on
  * 16-byte bounds (FERRET_ERR_ALIGN).
  */
 int ferret_rms_norm(const void* x, long long x_stride, const void* residual, long long residual_stride,
@@ -302,24 +303,25 @@ int ferret_rms_norm_e4m3(const void* x, long long x_stride, const void* residual
  *                   one per 128 latents: byte b stands for 2^(b - 127).
  * page_table int32 [B, max_pages]: the pages of each sequence in order.  An entry
  * outside [0, pages) stands for no page: nothing is written to it, zeros are read
- * from it, attention leaves its keys out.  Lengths past max_pages * page_size are
- * cut.  cu_q / cu_k int32 [B + 1] ascend from 0: the rows of sequence b among the
- * packed new tokens or keys; packed rows behind the last sequence are left alone,
- * on the input and on the output side.  lens int32 [B]: keys of a sequence, its new
- * tokens included, which are the last of them.  All of these are device arrays and
- * are read by the kernels only: a captured graph replays with other lengths.
+ * from it, attention leaves its keys out.  The attention cuts lengths past max_pages *
+ * page_size to it; positions past it are not written, and read as zeros.  cu_q / cu_k
+ * int32 [B + 1] ascend from 0: the rows of sequence b among the packed new tokens or
+ * keys; packed rows behind the last sequence are left alone, on the input and on the
+ * output side.  lens int32 [B]: keys of a sequence, its new tokens included, which are
+ * the last of them.  All of these are device arrays and are read by the kernels only: a
+ * captured graph replays with other lengths.
  *
  * No entry point of the cache or the latent attention takes an output or workspace that
  * overlaps another or anything that the call reads (FERRET_ERR_SHAPE), but for what is
  * named as in place.
  *
  * ferret_latent_cache_write: new token i of sequence b to position
- * lens[b] - n + i (n = its number of new tokens; negative positions are dropped).
- * latent bf16 [T,512], rotary bf16 [T,64], rows *_stride elements apart (multiples
- * of 8, a row's width or more).  e4m3: per 128 latents byte = max(127 + ceil(log2(max|x| / 448)), 16) over
- * the finite values, code = e4m3_RNE(x * 2^(127 - byte)); Inf and NaN give the NaN
- * code.  A row that two tokens of one call write (a page named by two sequences)
- * ends as a mix of both: the pages that are written belong to one sequence.
+ * lens[b] - n + i (n = its number of new tokens; negative positions are dropped). latent
+ * bf16 [T,512], rotary bf16 [T,64], rows *_stride elements apart (multiples of 8, a
+ * row's width or more).  e4m3: per 128 latents byte = max(127 + ceil(log2(max|x| /
+ * 448)), 16) over the finite values, code = e4m3_RNE(x * 2^(127 - byte)); Inf and NaN
+ * give the NaN code.  A row that two tokens of one call write (a page named by two
+ * sequences) ends as a mix of both: the pages that are written belong to one sequence.
  *
  * ferret_latent_cache_read: positions 0 .. cu_k[b+1] - cu_k[b] of every sequence to
  * latent bf16 [rows,512] and rotary bf16 [rows,64], exactly (a code times its
@@ -346,7 +348,9 @@ int ferret_latent_cache_read(const void* data, const void* scales, int pages, in
  * row unless the key's score is -inf, which has no weight.
  * ws: ferret_latent_attention_workspace(B, T, H) bytes, on a 16-byte bound; two
  * calls that overlap in time need one each.  The result depends on the batch only
- * through the order of fp32 additions; the same call gives the same bits.
+ * through the order of fp32 additions and the maximum under which a softmax term is
+ * rounded to bf16; the same call gives the same bits.  Sums are fp32 and hold terms of
+ * up to 256 times the latents: finite where 256 * keys * max|latent| stays below 2^128.
  * out may stand exactly on packed q_latent.
  * Requirements: T >= 1, 1 <= H <= 1024, 0 < scale < 1e30, max_pages * page_size
  * <= 2^31 - 128.
@@ -362,14 +366,15 @@ int ferret_latent_attention(const void* q_latent, long long ql_token, long long 
  * Latent attention in its expanded form, for ragged prompts:
  *   s_ij = scale * (q_nope_i . k_nope_j + q_rotary_i . k_rotary_j),
  *   out_i = sum_j softmax_j(s_ij) v_j           (bf16 [T,H,128]),
- * per head, over keys j <= len - n + i of the token's sequence (causal != 0; len
- * keys, n new tokens, the last of them) or all len.  q_nope bf16 [T,H,128], q_rotary
- * [T,H,64], k_nope and v [S,H,128], k_rotary [S,64] (one for all heads), with strides
- * in elements (multiples of 8, < 2^24), so the key-value projection is taken as it
- * is.  cu_q and cu_k int32 [B + 1] as above; rows behind the last sequence are left
- * alone.  lse, tokens that see no key, and Inf or NaN that a token does not see: as
- * ferret_latent_attention.  out may stand exactly on packed q_nope.  Requirements:
- * B, T >= 1, 1 <= S <= 2^30, 1 <= H <= 1024, 0 < scale < 1e30.
+ * per head, over keys j <= len - n + i of the token's sequence (causal != 0; len keys, n
+ * new tokens, the last of them) or all len.  q_nope bf16 [T,H,128], q_rotary [T,H,64],
+ * k_nope and v [S,H,128], k_rotary [S,64] (one for all heads), with strides in elements
+ * (multiples of 8, < 2^24), so the key-value projection is taken as it is.  cu_q and
+ * cu_k int32 [B + 1] as above; rows behind the last sequence are left alone.  lse,
+ * tokens that see no key, Inf or NaN that a token does not see, and the range of the
+ * sums: as ferret_latent_attention.  An Inf or NaN among the values of a key that a
+ * token sees makes that column of it Inf or NaN.  out may stand exactly on packed
+ * q_nope.  Requirements: B, T >= 1, 1 <= S <= 2^30, 1 <= H <= 1024, 0 < scale < 1e30.
  * ws: ferret_latent_attention_expanded_workspace(B, T, S, H) bytes, on a 16-byte
  * bound; none (0, ws may be NULL) unless few tokens attend many keys.
  */
