@@ -349,6 +349,17 @@ __device__ __forceinline__ void clear_unseen(const Args& in, const Piece& p, uin
   constexpr int VC = F8 ? CT : 2 * CT, ROW = F8 ? kRowE4m3 : kRowBf16;
   const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
   const auto place = [&](int r, int c) { return buf + r * ROW + (((chunk + c) ^ swz(r)) << 4); };
+  // Every row seen by all or by none: a loop of its own where scalar registers are left for it
+  // (128 heads, bf16, 32 sequences of 900 to 6000: 58.5 us, 59.3 without).
+  if (WQ == 4 && p.see_all >= p.see_any) {
+#pragma unroll 1
+    for (int i0 = 0; i0 < STEP * VC; i0 += 64) {
+      const int r = (i0 + lane) / VC;
+      if (first + r >= p.see_any || !((ok >> (8 * (r >> 4))) & 1))
+        *reinterpret_cast<u32x4*>(place(r, lane % VC)) = u32x4{0u, 0u, 0u, 0u};
+    }
+    return;
+  }
 #pragma unroll 1
   for (int i0 = 0; i0 < STEP * VC; i0 += 64) {
     const int r = (i0 + lane) / VC, key = first + r;
@@ -356,7 +367,7 @@ __device__ __forceinline__ void clear_unseen(const Args& in, const Piece& p, uin
     u32x4* const at = reinterpret_cast<u32x4*>(place(r, lane % VC));
     u32x4 x = {0u, 0u, 0u, 0u}, fine = x;
     if (some) fine = only_finite<F8>(x = *at);
-    if constexpr (!F8) {
+    if (!F8 && p.see_all < p.see_any) {
       const bool bad = x[0] != fine[0] || x[1] != fine[1] || x[2] != fine[2] || x[3] != fine[3];
       for (unsigned long long rest = __ballot(bad); rest != 0;) {
         const int first_bad = __ffsll((long long)rest) - 1, row = (i0 + first_bad) / VC;
