@@ -36,6 +36,7 @@ constexpr auto kBf16 = at::kBFloat16;
 constexpr auto kF32 = at::kFloat;
 constexpr auto kI32 = at::kInt;
 constexpr auto kFp8 = at::kFloat8_e4m3fn;
+constexpr auto kI8 = at::kChar;
 
 // Transform wrappers (vmap, grad, functionalization): left to Python.
 const c10::DispatchKeySet kWrapped({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched,
@@ -441,6 +442,49 @@ int64_t pitch(const at::Tensor* t) { return t->size(0) == 1 ? t->size(1) : t->st
 // The stride of dimension d, 0 where it has one element.
 int64_t step(const at::Tensor* t, int d) { return t->size(d) == 1 ? 0 : t->stride(d); }
 
+// x, q, scale -> (q, scale)
+NATIVE(quant_act_int8, 3) {
+  Call c;
+  const auto* x = c.rows(a[0], 2, kBf16);
+  if (!c.ok()) Py_RETURN_NONE;
+  const int M = x->size(0), K = x->size(1);
+  c.require_current();
+  const at::Tensor q = c.out(a[1], {M, K}, kI8);
+  const at::Tensor s = c.out(a[2], {M}, kF32);
+  if (!c.ok()) Py_RETURN_NONE;
+  void* st = stream();
+  if (!run("ferret_quant_act_int8",
+           [&] { return ferret_quant_act_int8(ptr(x), pitch(x), M, K, ptr(q), ptr_as<float>(s), st); }))
+    return declined();
+  return Py_BuildValue("(NN)", wrap(q), wrap(s));
+}
+
+// a, sa, b, sb, residual, out, workspace
+NATIVE(int8_gemm, 7) {
+  Call c;
+  const auto* x = c.in(a[0], 2, kI8);
+  const auto* sx = c.in(a[1], 1, kF32);
+  const auto* w = c.in(a[2], 2, kI8);
+  const auto* sw = c.in(a[3], 1, kF32);
+  if (!c.ok()) Py_RETURN_NONE;
+  const int M = x->size(0), K = x->size(1), N = w->size(0);
+  c.require(w->size(1) == K && sx->size(0) == M && sw->size(0) == N);
+  c.require_current();
+  const at::Tensor* r = a[4] == Py_None ? nullptr : c.in(a[4], 2, kBf16);
+  if (!c.ok() || (r != nullptr && (r->size(0) != M || r->size(1) != N))) Py_RETURN_NONE;
+  const at::Tensor y = c.out(a[5], {M, N}, kBf16);
+  const size_t need = c.ok() ? ferret_int8_gemm_workspace(M, N, K) : 0;
+  const at::Tensor ws = c.workspace(a[6], need);
+  if (!c.ok()) Py_RETURN_NONE;
+  void* st = stream();
+  if (!run("ferret_int8_gemm", [&] {
+        return ferret_int8_gemm(ptr(x), ptr_as<float>(sx), ptr(w), ptr_as<float>(sw), r ? ptr(r) : nullptr, ptr(y), M,
+                                N, K, ptr(ws), need, st);
+      }))
+    return declined();
+  return wrap(y);
+}
+
 // x, w, residual, eps, residual_out of a norm.
 struct Norm {
   const at::Tensor *x, *w, *r = nullptr;
@@ -639,7 +683,7 @@ PyMethodDef kMethods[] = {METHOD(linear_bf16),   METHOD(fp8_gemm_blockscale), ME
                           METHOD(moe_w2_fp8),     METHOD(moe_w13_w4a16),       METHOD(quant_act_e4m3),
                           METHOD(moe_combine),    METHOD(rms_norm),            METHOD(rms_norm_e4m3),
                           METHOD(latent_cache_write), METHOD(latent_cache_read), METHOD(latent_attention),
-                          METHOD(latent_attention_expanded),
+                          METHOD(latent_attention_expanded), METHOD(quant_act_int8), METHOD(int8_gemm),
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", "Native call path of ferret_amd.ops.", -1, kMethods,
                        nullptr, nullptr, nullptr, nullptr};

@@ -50,6 +50,9 @@ SIGNATURES = {
     "ferret_moe_w2_fp8_ex": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int,
                                       _c_int, _vp, _c_int, _vp]),
     "ferret_workspace_bytes": (_c_size_t, [_c_int, _c_int, _c_int, _c_int, _c_int]),
+    "ferret_quant_act_int8": (_c_int, [_vp, _c_i64, _c_int, _c_int, _vp, _vp, _vp]),
+    "ferret_int8_gemm_workspace": (_c_size_t, [_c_int, _c_int, _c_int]),
+    "ferret_int8_gemm": (_c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _c_size_t, _vp]),
     "ferret_rms_norm": (_c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_float, _c_int, _c_int, _vp, _vp, _vp]),
     "ferret_rms_norm_e4m3": (_c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_float, _c_int, _c_int, _vp, _vp, _vp, _vp]),
     "ferret_latent_cache_write": (_c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _vp, _vp, _c_int, _c_int, _c_int, _vp, _vp,

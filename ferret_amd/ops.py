@@ -414,6 +414,73 @@ def quant_act_e4m3(x: torch.Tensor, q: torch.Tensor | None = None, scale: torch.
     return q, scale
 
 
+def quant_act_int8(x: torch.Tensor, q: torch.Tensor | None = None, scale: torch.Tensor | None = None):
+    """bf16 x [M, K] -> (int8 q [M, K], fp32 scale [M]): q = round(127 x / a), ties to even, scale = a / 127 with
+    a = max(max |x| of the row, 2^-100).
+
+    The activations of int8_gemm.  x may be a row slice of a wider tensor (not expanded rows); a row
+    with an Inf or NaN gets zeros and the scale NaN, so that its products are NaN.  K % 16 == 0,
+    K <= 32768; outputs overlap neither each other nor x.
+    """
+    r = _lib.native().quant_act_int8(x, q, scale)
+    if r is not None:
+        return r
+    if not isinstance(x, torch.Tensor) or x.dim() != 2:
+        raise ValueError("x must be a 2-D tensor [M, K]")
+    M, K = x.shape
+    xp, xs = _pitched(x, "x", (None, None))
+    _same_device(x, q, scale)
+    if q is None:
+        q = torch.empty((M, K), dtype=torch.int8, device=x.device)
+    if scale is None:
+        scale = torch.empty((M,), dtype=torch.float32, device=x.device)
+    qp, sp = _out(q, "q", (M, K), torch.int8, x.device), _out(scale, "scale", (M,), torch.float32, x.device)
+    with _on(x):
+        rc = _lib.load().ferret_quant_act_int8(xp, xs, M, K, qp, sp, _stream())
+    _lib.check("ferret_quant_act_int8", rc)
+    return q, scale
+
+
+def int8_gemm_workspace_bytes(M: int, N: int, K: int) -> int:
+    """Bytes of the partial sums that int8_gemm adds up for this shape (0: none)."""
+    return int(_lib.load().ferret_int8_gemm_workspace(M, N, K))
+
+
+def int8_gemm(a: torch.Tensor, sa: torch.Tensor, b: torch.Tensor, sb: torch.Tensor,
+              residual: torch.Tensor | None = None, out: torch.Tensor | None = None,
+              workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """y[M,N] (bf16) = (a[M,K] . b[N,K]^T) * sa[M] * sb[N] (+ residual): int8 codes, a scale per token and per channel.
+
+    The whole sum is exact, then fp32 and one rounding to bf16: a token's result has the same
+    bits whatever else is in the call.  Tokens from quant_act_int8, weights quantised the same way once at load.
+    N % 8 == 0, K % 16 == 0, K <= 65536.  `workspace` of int8_gemm_workspace_bytes is taken from
+    torch's caching allocator unless one is passed; calls that overlap in time (streams, graphs) need
+    one each.  `out` may be the residual itself and overlaps nothing else.
+    """
+    y = _lib.native().int8_gemm(a, sa, b, sb, residual, out, workspace)
+    if y is not None:
+        return y
+    ap, bp = _dev(a, "a", torch.int8, 2), _dev(b, "b", torch.int8, 2)
+    M, K = a.shape
+    N = b.shape[0]
+    if b.shape[1] != K:
+        raise ValueError(f"b must be [N, {K}], got {tuple(b.shape)}")
+    _same_device(a, sa, b, sb, residual, out, workspace)
+    sap, sbp = _out(sa, "sa", (M,), torch.float32, a.device), _out(sb, "sb", (N,), torch.float32, a.device)
+    rp = _out(residual, "residual", (M, N), torch.bfloat16, a.device) if residual is not None else 0
+    if out is None:
+        out = torch.empty((M, N), dtype=torch.bfloat16, device=a.device)
+    op = _out(out, "out", (M, N), torch.bfloat16, a.device)
+    need = int8_gemm_workspace_bytes(M, N, K)
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        workspace = torch.empty(need, dtype=torch.uint8, device=a.device)
+    with _on(a):
+        rc = _lib.load().ferret_int8_gemm(ap, sap, bp, sbp, rp, op, M, N, K,
+                                          _dev(workspace, "workspace") if need else None, need, _stream())
+    _lib.check("ferret_int8_gemm", rc)
+    return out
+
+
 def moe_w2_fp8(h: torch.Tensor, sh: torch.Tensor, w: torch.Tensor, sw: torch.Tensor, routing: Routing,
                out: torch.Tensor | None = None, mma: str = "bf16") -> torch.Tensor:
     """out[P, N] bf16 (pair order) = the FP8 block-scaled down projection of h [P, K] (pair order)."""

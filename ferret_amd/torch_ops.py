@@ -81,6 +81,30 @@ def _(x):
     return x.new_empty((M, K), dtype=FP8), x.new_empty((M, K // 128), dtype=torch.float32)
 
 
+@torch.library.custom_op(f"{_NS}::quant_act_int8", mutates_args=())
+def quant_act_int8(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """bf16 x[M,K] -> (int8 q[M,K], fp32 scale[M]), absmax/127 per token."""
+    return _ops.quant_act_int8(x)
+
+
+@quant_act_int8.register_fake
+def _(x):
+    M, K = x.shape
+    return x.new_empty((M, K), dtype=torch.int8), x.new_empty((M,), dtype=torch.float32)
+
+
+@torch.library.custom_op(f"{_NS}::int8_gemm", mutates_args=())
+def int8_gemm(a: torch.Tensor, sa: torch.Tensor, b: torch.Tensor, sb: torch.Tensor,
+              residual: torch.Tensor | None = None) -> torch.Tensor:
+    """y[M,N] bf16 of int8 a[M,K], b[N,K] with fp32 scales per token and channel (+ residual)."""
+    return _ops.int8_gemm(a, sa, b, sb, residual)
+
+
+@int8_gemm.register_fake
+def _(a, sa, b, sb, residual=None):
+    return a.new_empty((a.shape[0], b.shape[0]), dtype=torch.bfloat16)
+
+
 # ---- MoE routing ---------------------------------------------------------------------------------
 
 @torch.library.custom_op(f"{_NS}::moe_route_topk", mutates_args=())
@@ -311,4 +335,4 @@ def _(q_nope, q_rotary, k_nope, k_rotary, v, cu_q, cu_k, scale, causal=True):
 OPS = ("linear_bf16", "fp8_gemm_blockscale", "fp8_gemm_ue8m0", "quant_act_e4m3", "moe_route_topk", "moe_permute",
        "moe_w13_fp8", "moe_w13_w4a16", "int4_tile_weights", "moe_w2_fp8", "moe_combine", "rms_norm",
        "add_rms_norm", "rms_norm_e4m3", "add_rms_norm_e4m3", "latent_cache_write", "latent_cache_read",
-       "latent_attention", "latent_attention_expanded")
+       "latent_attention", "latent_attention_expanded", "quant_act_int8", "int8_gemm")

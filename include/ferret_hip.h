@@ -268,6 +268,33 @@ int ferret_moe_w2_fp8(const void* h, const float* sh, const void* w, const float
 int ferret_moe_combine(const void* o, const float* w, int T, int topk, int N, void* y, void* stream);
 
 /*
+ * bf16 rows to int8 codes with one fp32 scale per row, the tokens of ferret_int8_gemm:
+ *   a = max(max_k |x[m,k]|, 2^-100),  q[m,k] = RNE(127 x[m,k] / a)  (of the exact
+ *   quotient, ties to even),  scale[m] = a / 127.
+ * x [M,K] with rows x_stride elements apart (a multiple of 8, K or more), q int8 [M,K]
+ * packed, scale f32 [M].  A row with an Inf or NaN gets zeros and the scale NaN.  Outputs
+ * overlap nothing.  The reference has no 8-bit integer path; this and the product below
+ * are the library's own contract.  Requirements: M >= 1, K % 16 == 0, 16 <= K <= 32768;
+ * x and q on 16-byte bounds (FERRET_ERR_ALIGN).
+ */
+int ferret_quant_act_int8(const void* x, long long x_stride, int M, int K, void* q, float* scale, void* stream);
+
+/*
+ * int8 product with a scale per token and per output channel:
+ *   y[m,n] = bf16_RNE( float(sum_k a[m,k] b[n,k]) * sa[m] * sb[n] (+ residual[m,n]) ),
+ * a int8 [M,K], sa f32 [M], b int8 [N,K], sb f32 [N], residual and y bf16 [M,N].  The
+ * sum is exact; its conversion, the two products (in this order) and the addition round
+ * to fp32.  So the same bits come out whatever the other tokens of the call, and for
+ * every workspace.  ws: ferret_int8_gemm_workspace(M, N, K) bytes on a 16-byte bound (0:
+ * none, may be NULL); calls that overlap in time need one each.  y may be residual itself and
+ * overlaps nothing else.  Requirements: M >= 1, N >= 8, N % 8 == 0, 16 <= K <= 65536, K %
+ * 16 == 0, M * N < 2^40; pointers but sa on 16-byte bounds (FERRET_ERR_ALIGN).
+ */
+size_t ferret_int8_gemm_workspace(int M, int N, int K);
+int ferret_int8_gemm(const void* a, const float* sa, const void* b, const float* sb, const void* residual, void* y,
+                     int M, int N, int K, void* ws, size_t ws_bytes, void* stream);
+
+/*
  * Root-mean-square norm of bf16 rows, with the residual's addition where one is
  * given:  s = x + residual (fp32; residual_out = bf16_RNE(s)),
  *   y = bf16_RNE(s * rsqrt(mean(s^2) + eps) * w).
