@@ -43,6 +43,7 @@
 #include "latent.hpp"
 
 #include <initializer_list>
+#include <utility>
 
 namespace ferret {
 namespace {
@@ -66,6 +67,13 @@ struct Args {
   int side_by_side;  // row tiles of a sequence taken at the same time
   uint16_t* out;  // [T, H, 512]
   float* lse;     // [T, H] or null
+  // One of two passes over a row's keys (shared prefixes): where its whole tiles' m, l and
+  // outputs go instead of `out`, ml [T * H], then [T * H][512].  Null else.
+  uint8_t* whole;
+  __host__ __device__ float2* whole_ml() const { return reinterpret_cast<float2*>(whole); }
+  __host__ __device__ float* whole_part() const {
+    return reinterpret_cast<float*>(whole + (((size_t)T * H * sizeof(float2) + 255) & ~(size_t)255));
+  }
   // The workspace: rows [T * H] (int4), then ml [2 * kUnits][MR] (m and l), then the
   // partial outputs [2 * kUnits][MR][512].  A row's record is {first slot, pieces, row
   // in tile, -}.
@@ -140,6 +148,7 @@ __device__ __forceinline__ void put_args(Args* to, const Args& a) {
   to->side_by_side = a.side_by_side;
   to->out = a.out;
   to->lse = a.lse;
+  to->whole = a.whole;
   to->ws = a.ws;
 }
 
@@ -408,7 +417,7 @@ __device__ __forceinline__ void put_rows(const Side* side, const Piece& p, int f
   const Args& in = side->args;
   const int r = f * 16 + r16, slot = uniform(side->slot);
   if (p.row0 + r > p.row_last) return;
-  if (slot < 0) {
+  if (slot < 0 && in.whole == nullptr) {
     const long long at = side->first_row + r;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     uint16_t* to = in.out + at * kLatent + col;
@@ -419,9 +428,9 @@ __device__ __forceinline__ void put_rows(const Side* side, const Piece& p, int f
     if (stats && in.lse != nullptr)
       in.lse[at] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
   } else {
-    const long long at = (long long)slot * MR + r;
-    if (stats) in.ml()[at] = make_float2(top, sum);
-    float* to = in.part(MR) + at * kLatent + col;
+    const long long at = slot < 0 ? side->first_row + r : (long long)slot * MR + r;
+    if (stats) (slot < 0 ? in.whole_ml() : in.ml())[at] = make_float2(top, sum);
+    float* to = (slot < 0 ? in.whole_part() : in.part(MR)) + at * kLatent + col;
 #pragma unroll
     for (int c = 0; c < CT; ++c) *reinterpret_cast<f32x4*>(to + c * 16) = o[c][f];
   }
@@ -1301,13 +1310,96 @@ int launch_join(const Args& a, int mr, hipStream_t st) {
   return (int)hipGetLastError();
 }
 
+// ---- two passes over the keys: shared prefixes, then a sequence's own
+
+// The pieces of one row in one pass.
+struct Pieces {
+  const float2* ml;
+  const float* part;
+  long long first, rest, step;  // rows of `ml` and `part`: the first piece's; piece j > 0 at rest + j * step
+  int n;
+  __device__ __forceinline__ long long at(int j) const { return j == 0 ? first : rest + j * step; }
+};
+__device__ __forceinline__ Pieces pieces_of(const Args& a, int mr, long long row) {
+  Pieces p{a.whole_ml(), a.whole_part(), row, 0, 0, 0};
+  if (row < (long long)max(a.cu_q[0], 0) * a.H || row >= (long long)min(a.cu_q[a.B], a.T) * a.H) return p;  // no keys
+  const int4 rec = a.rows()[row];
+  const LatentRecord where{rec.x, rec.y};
+  p.n = 1;
+  if (latent_record_joins(where, a.side_by_side) && (unsigned)rec.z < (unsigned)mr) {
+    p.ml = a.ml();
+    p.part = a.part(mr);
+    p.n = where.pieces;
+    p.first = (long long)where.slot0 * mr + rec.z;
+    p.step = 2LL * a.side_by_side * mr;
+    p.rest = (long long)(where.slot0 & ~1) * mr + rec.z;
+  }
+  return p;
+}
+
+// Joins the pieces of both passes, the prefix's first: a wave per row, 8 columns per lane,
+// the pieces' weights 64 at a time in the lanes, four pieces' loads under way together.
+__global__ __launch_bounds__(256) void latent_shared_join_kernel(Args prefix, Args own, int prefix_mr, int own_mr) {
+  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (row < (long long)max(own.cu_q[0], 0) * own.H || row >= (long long)min(own.cu_q[own.B], own.T) * own.H) return;
+  const Pieces p0 = pieces_of(prefix, prefix_mr, row), p1 = pieces_of(own, own_mr, row);
+  const int n = p0.n + p1.n;
+  const auto stat = [&](int j) {
+    if (j >= n) return make_float2(-INFINITY, 0.f);
+    return j < p0.n ? p0.ml[p0.at(j)] : p1.ml[p1.at(j - p0.n)];
+  };
+  f32x4 x[4][2];
+  const auto load = [&](int j0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int j = min(j0 + i, n - 1);  // past the last: again, unused
+      const float* from = (j < p0.n ? p0.part + p0.at(j) * kLatent : p1.part + p1.at(j - p0.n) * kLatent) + lane * 4;
+      x[i][0] = *reinterpret_cast<const f32x4*>(from);
+      x[i][1] = *reinterpret_cast<const f32x4*>(from + 256);
+    }
+  };
+  load(0);
+  float2 v = stat(lane);
+  float top = v.x;
+  for (int j = lane + 64; j < n; j += 64) top = fmaxf(top, stat(j).x);
+  top = wave_max(top);
+  const float base = top == -INFINITY ? 0.f : top;
+  f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  float sum = 0.f, w = 0.f;
+  for (int j = 0; j < n; j += 4) {
+    if (j % 64 == 0) {
+      if (j > 0) v = stat(j + lane);
+      sum += piece_sum(v, base);
+      w = piece_weight(v, base);
+    }
+    if (j > 0) load(j);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float wi = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), j % 64 + i));
+      if (j + i < n) {
+        acc[0] += x[i][0] * wi;
+        acc[1] += x[i][1] * wi;
+      }
+    }
+  }
+  sum = wave_add(sum);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    *reinterpret_cast<u32x2*>(own.out + row * kLatent + h * 256 + lane * 4) =
+        u32x2{pack_bf16x2(acc[h][0] * inv, acc[h][1] * inv), pack_bf16x2(acc[h][2] * inv, acc[h][3] * inv)};
+  if (own.lse != nullptr && lane == 0)
+    own.lse[row] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
 template <int WQ, int WK, bool F8>
 int launch(const Args& a, hipStream_t st) {
   constexpr int mr = 16 * WQ, lds = Lds<mr, WK, F8>::kBytes;
   FERRET_HIP_CHECK((set_lds_limit_once<latent_attention_kernel<WQ, WK, F8>>(lds)));
   hipLaunchKernelGGL((latent_attention_kernel<WQ, WK, F8>), dim3(kUnits), dim3(64 * WQ * WK), lds, st, a);
   FERRET_HIP_CHECK(hipGetLastError());
-  return launch_join(a, mr, st);
+  return a.whole != nullptr ? FERRET_OK : launch_join(a, mr, st);
 }
 
 template <bool F8>
@@ -1316,7 +1408,7 @@ int launch_wide(const Args& a, hipStream_t st) {
   FERRET_HIP_CHECK((set_lds_limit_once<latent_attention_wide_kernel<F8>>(lds)));
   hipLaunchKernelGGL((latent_attention_wide_kernel<F8>), dim3(kUnits), dim3(512), lds, st, a);
   FERRET_HIP_CHECK(hipGetLastError());
-  return launch_join(a, Wide<F8>::kRows, st);
+  return a.whole != nullptr ? FERRET_OK : launch_join(a, Wide<F8>::kRows, st);
 }
 
 template <bool F8>
@@ -1344,6 +1436,55 @@ int tile_rows(int T, int B, int H) {
 int side_by_side(int T, int B, int H) {
   const long long tiles = (long long)T * H / B / 64;
   return tiles < 2 ? 1 : tiles < 4 ? 2 : tiles < 8 ? 4 : 8;
+}
+
+// Steps of a whole batch are counted in 32 bits, rounded up to whole shares; a step's
+// end stays below 2^31.
+int check_steps(int B, int max_pages, int pages, int page_size, int T, int H, int mr) {
+  FERRET_REQUIRE((long long)max_pages * page_size <= (1LL << 31) - 2 * kKeys, FERRET_ERR_SHAPE);
+  FERRET_REQUIRE((long long)pages * page_size < (1LL << 35), FERRET_ERR_SHAPE);
+  const long long tiles = (long long)T * H / mr + B, most = ((long long)max_pages * page_size + kKeys - 1) / kKeys + kLatentExtra;
+  FERRET_REQUIRE(tiles * most < (1LL << 31) - kUnits, FERRET_ERR_SHAPE);
+  return FERRET_OK;
+}
+
+// What the kernels of one pass over a batch's keys take; mr: query rows per tile.
+Args pass_args(const void* q_latent, long long ql_token, long long ql_head, const void* q_rotary, long long qr_token,
+               long long qr_head, const void* data, const void* scales, const Pages& pages, const int32_t* lens,
+               const int32_t* cu_q, int B, int T, int H, float scale, int causal, int mr, void* out, float* lse,
+               void* ws) {
+  Args a;
+  a.ql = static_cast<const uint16_t*>(q_latent);
+  a.qr = static_cast<const uint16_t*>(q_rotary);
+  a.ql_t = (int)ql_token;
+  a.ql_h = (int)ql_head;
+  a.qr_t = (int)qr_token;
+  a.qr_h = (int)qr_head;
+  a.data = static_cast<const uint8_t*>(data);
+  a.scales = static_cast<const uint32_t*>(scales);
+  a.pages = pages;
+  a.lens = lens;
+  a.cu_q = cu_q;
+  a.B = B;
+  a.T = T;
+  a.H = H;
+  a.scale_log2 = scale * kLog2e;
+  a.causal = causal != 0;
+  // Shares of one step where a step is short: 16 heads, 256 keys 13.2 us against 14.8 in
+  // shares of two; 128 heads, e4m3, 8 sequences of 100 keys 20.4 in shares of two, 21.0 of one.
+  a.min_steps = mr == 64 ? 2 : 1;
+  a.side_by_side = side_by_side(T, B, H);
+  a.out = static_cast<uint16_t*>(out);
+  a.lse = lse;
+  a.whole = nullptr;
+  a.ws = static_cast<uint8_t*>(ws);
+  return a;
+}
+
+// Bytes of m, l and outputs of all rows.
+size_t whole_bytes(int T, int H) {
+  const size_t rows = (size_t)T * H;
+  return ((rows * sizeof(float2) + 255) & ~(size_t)255) + rows * kLatent * sizeof(float);
 }
 
 }  // namespace
@@ -1377,11 +1518,8 @@ extern "C" int ferret_latent_attention(const void* q_latent, long long ql_token,
                      ((bits(scales) | bits(lse)) & 3) == 0 && ((ql_token | ql_head | qr_token | qr_head) & 7) == 0,
                  FERRET_ERR_ALIGN);
   const int mr = tile_rows(T, B, H);
-  FERRET_REQUIRE((long long)max_pages * page_size <= (1LL << 31) - 2 * kKeys, FERRET_ERR_SHAPE);  // a step's end stays below 2^31
-  // steps of the whole batch are counted in 32 bits, rounded up to whole shares
-  FERRET_REQUIRE((long long)pages * page_size < (1LL << 35), FERRET_ERR_SHAPE);
-  const long long tiles = (long long)T * H / mr + B, most = ((long long)max_pages * page_size + kKeys - 1) / kKeys + kLatentExtra;
-  FERRET_REQUIRE(tiles * most < (1LL << 31) - kUnits, FERRET_ERR_SHAPE);
+  const int steps = check_steps(B, max_pages, pages, page_size, T, H, mr);
+  if (steps != FERRET_OK) return steps;
   const size_t need = ferret_latent_attention_workspace(B, T, H);
   FERRET_REQUIRE(ws != nullptr && ws_bytes >= need && (bits(ws) & 15) == 0, FERRET_ERR_WORKSPACE);
   // In place is sound: the work-group that has read a whole tile writes it, the join those
@@ -1394,30 +1532,71 @@ extern "C" int ferret_latent_attention(const void* q_latent, long long ql_token,
                          ints_range(page_table, (uint64_t)B * max_pages), ints_range(lens, B),
                          ints_range(cu_q, B + 1LL)}),
                  FERRET_ERR_SHAPE);
-  Args a;
-  a.ql = static_cast<const uint16_t*>(q_latent);
-  a.qr = static_cast<const uint16_t*>(q_rotary);
-  a.ql_t = (int)ql_token;
-  a.ql_h = (int)ql_head;
-  a.qr_t = (int)qr_token;
-  a.qr_h = (int)qr_head;
-  a.data = static_cast<const uint8_t*>(data);
-  a.scales = static_cast<const uint32_t*>(scales);
-  a.pages = Pages{page_table, max_pages, pages, page_size};
-  a.lens = lens;
-  a.cu_q = cu_q;
-  a.B = B;
-  a.T = T;
-  a.H = H;
-  a.scale_log2 = scale * kLog2e;
-  a.causal = causal != 0;
-  // Shares of one step where a step is short: 16 heads, 256 keys 13.2 us against 14.8 in
-  // shares of two; 128 heads, e4m3, 8 sequences of 100 keys 20.4 in shares of two, 21.0 of one.
-  a.min_steps = mr == 64 ? 2 : 1;
-  a.side_by_side = side_by_side(T, B, H);
-  a.out = static_cast<uint16_t*>(out);
-  a.lse = lse;
-  a.ws = static_cast<uint8_t*>(ws);
+  const Args a = pass_args(q_latent, ql_token, ql_head, q_rotary, qr_token, qr_head, data, scales,
+                           Pages{page_table, max_pages, pages, page_size}, lens, cu_q, B, T, H, scale, causal, mr, out,
+                           lse, ws);
   return scales != nullptr ? launch_rows<true>(mr, a, (hipStream_t)stream)
                            : launch_rows<false>(mr, a, (hipStream_t)stream);
+}
+
+extern "C" size_t ferret_latent_attention_shared_workspace(int G, int B, int T, int H) {
+  const size_t prefix = ferret_latent_attention_workspace(G, T, H), own = ferret_latent_attention_workspace(B, T, H);
+  return prefix == 0 || own == 0 ? 0 : ((prefix + 255) & ~(size_t)255) + ((own + 255) & ~(size_t)255) + 2 * whole_bytes(T, H);
+}
+
+extern "C" int ferret_latent_attention_shared(const void* q_latent, long long ql_token, long long ql_head,
+                                              const void* q_rotary, long long qr_token, long long qr_head,
+                                              const void* data, const void* scales, int pages, int page_size,
+                                              const int32_t* prefix_table, const int32_t* prefix_lens,
+                                              const int32_t* cu_prefix, int G, int max_prefix_pages,
+                                              const int32_t* page_table, const int32_t* lens, const int32_t* cu_q, int B,
+                                              int max_pages, int T, int H, float scale, int causal, void* out,
+                                              float* lse, void* ws, size_t ws_bytes, void* stream) {
+  FERRET_REQUIRE(q_latent && q_rotary && data && prefix_lens && cu_prefix && lens && cu_q && out, FERRET_ERR_NULL);
+  int rc = ferret_check_pages(prefix_table, G, max_prefix_pages, pages, page_size);
+  if (rc == FERRET_OK) rc = ferret_check_pages(page_table, B, max_pages, pages, page_size);
+  if (rc != FERRET_OK) return rc;
+  FERRET_REQUIRE(T >= 1 && H >= 1 && H <= 1024 && (long long)T * H < (1LL << 31), FERRET_ERR_SHAPE);
+  FERRET_REQUIRE(scale > 0.f && scale < 1e30f, FERRET_ERR_SHAPE);
+  for (const long long stride : {ql_token, ql_head, qr_token, qr_head})
+    FERRET_REQUIRE(stride >= 0 && stride < (1LL << 31), FERRET_ERR_SHAPE);
+  const auto bits = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
+  FERRET_REQUIRE(((bits(q_latent) | bits(q_rotary) | bits(data) | bits(out)) & 15) == 0 &&
+                     ((bits(scales) | bits(lse)) & 3) == 0 && ((ql_token | ql_head | qr_token | qr_head) & 7) == 0,
+                 FERRET_ERR_ALIGN);
+  const int prefix_mr = tile_rows(T, G, H), own_mr = tile_rows(T, B, H);
+  rc = check_steps(G, max_prefix_pages, pages, page_size, T, H, prefix_mr);
+  if (rc == FERRET_OK) rc = check_steps(B, max_pages, pages, page_size, T, H, own_mr);
+  if (rc != FERRET_OK) return rc;
+  const size_t need = ferret_latent_attention_shared_workspace(G, B, T, H);
+  FERRET_REQUIRE(ws != nullptr && ws_bytes >= need && (bits(ws) & 15) == 0, FERRET_ERR_WORKSPACE);
+  // In place is sound: `out` is written by the join alone.
+  const bool over = in_place(out, q_latent, T, ql_token, H, ql_head, kLatent);
+  FERRET_REQUIRE(!clash({Range{out, (uint64_t)T * H * kLatent * 2}, Range{lse, (uint64_t)T * H * 4}, Range{ws, need}},
+                        {bf16_range(over ? nullptr : q_latent, T, ql_token, H, ql_head, kLatent),
+                         bf16_range(q_rotary, T, qr_token, H, qr_head, kRotary),
+                         data_range(data, scales, pages, page_size), scale_range(scales, pages, page_size),
+                         ints_range(prefix_table, (uint64_t)G * max_prefix_pages), ints_range(prefix_lens, G),
+                         ints_range(cu_prefix, G + 1LL), ints_range(page_table, (uint64_t)B * max_pages),
+                         ints_range(lens, B), ints_range(cu_q, B + 1LL)}),
+                 FERRET_ERR_SHAPE);
+  uint8_t* at = static_cast<uint8_t*>(ws);
+  const auto take = [&](size_t bytes) { uint8_t* p = at; at += (bytes + 255) & ~(size_t)255; return p; };
+  Args prefix = pass_args(q_latent, ql_token, ql_head, q_rotary, qr_token, qr_head, data, scales,
+                          Pages{prefix_table, max_prefix_pages, pages, page_size}, prefix_lens, cu_prefix, G, T, H,
+                          scale, 0, prefix_mr, nullptr, nullptr, take(ferret_latent_attention_workspace(G, T, H)));
+  Args own = pass_args(q_latent, ql_token, ql_head, q_rotary, qr_token, qr_head, data, scales,
+                       Pages{page_table, max_pages, pages, page_size}, lens, cu_q, B, T, H, scale, causal, own_mr, out,
+                       lse, take(ferret_latent_attention_workspace(B, T, H)));
+  prefix.whole = take(whole_bytes(T, H));
+  own.whole = take(whole_bytes(T, H));
+  const hipStream_t st = (hipStream_t)stream;
+  for (const auto& [pass, mr] : {std::pair<const Args&, int>(prefix, prefix_mr), {own, own_mr}}) {
+    rc = scales != nullptr ? launch_rows<true>(mr, pass, st) : launch_rows<false>(mr, pass, st);
+    if (rc != FERRET_OK) return rc;
+  }
+  const long long rows = (long long)T * H;
+  hipLaunchKernelGGL(latent_shared_join_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, prefix, own,
+                     prefix_mr, own_mr);
+  return (int)hipGetLastError();
 }

@@ -642,6 +642,38 @@ NATIVE(latent_attention, 12) {
   return Py_BuildValue("(NN)", wrap(o), wrap(lse));
 }
 
+// q_latent, q_rotary, data, scales, prefix_table, prefix_lens, cu_prefix, page_table, lens, cu_q, scale, causal,
+// return_lse, out, workspace -> out, or (out, lse)
+NATIVE(latent_attention_shared, 15) {
+  Call c;
+  Cache f, k;
+  float scale;
+  if (!f.read(c, a[2], a[3], a[4], a[6], a[5]) || !k.read(c, a[2], a[3], a[7], a[9], a[8])) Py_RETURN_NONE;
+  const auto* ql = c.rows(a[0], 3, kBf16);
+  const auto* qr = c.rows(a[1], 3, kBf16);
+  if (!c.ok() || !as_float(a[10], &scale)) Py_RETURN_NONE;
+  const int T = ql->size(0), H = ql->size(1);
+  c.require(ql->size(2) == 512 && qr->size(0) == T && qr->size(1) == H && qr->size(2) == 64);
+  const bool causal = a[11] == Py_True, with_lse = a[12] == Py_True;
+  const at::Tensor o = c.out(a[13], {T, H, 512}, kBf16);
+  const size_t need = ferret_latent_attention_shared_workspace(f.B, k.B, T, H);
+  if (!c.ok() || need == 0) Py_RETURN_NONE;
+  const at::Tensor ws = c.workspace(a[14], need);
+  if (!c.ok()) Py_RETURN_NONE;
+  const at::Tensor lse = with_lse ? c.fresh({T, H}, kF32) : at::Tensor();
+  void* st = stream();
+  if (!run("ferret_latent_attention_shared", [&] {
+        return ferret_latent_attention_shared(
+            ptr(ql), step(ql, 0), step(ql, 1), ptr(qr), step(qr, 0), step(qr, 1), ptr(k.data), k.scale_ptr(), k.pages,
+            k.page_size, ptr_as<int32_t>(f.table), ptr_as<int32_t>(f.lens), ptr_as<int32_t>(f.starts), f.B, f.max_pages,
+            ptr_as<int32_t>(k.table), ptr_as<int32_t>(k.lens), ptr_as<int32_t>(k.starts), k.B, k.max_pages, T, H, scale,
+            causal, ptr(o), ptr_as<float>(lse), ptr(ws), need, st);
+      }))
+    return declined();
+  if (!with_lse) return wrap(o);
+  return Py_BuildValue("(NN)", wrap(o), wrap(lse));
+}
+
 // q_nope, q_rotary, k_nope, k_rotary, v, cu_q, cu_k, scale, causal, return_lse, out, workspace -> out, or (out, lse)
 NATIVE(latent_attention_expanded, 12) {
   Call c;
@@ -684,6 +716,7 @@ PyMethodDef kMethods[] = {METHOD(linear_bf16),   METHOD(fp8_gemm_blockscale), ME
                           METHOD(moe_combine),    METHOD(rms_norm),            METHOD(rms_norm_e4m3),
                           METHOD(latent_cache_write), METHOD(latent_cache_read), METHOD(latent_attention),
                           METHOD(latent_attention_expanded), METHOD(quant_act_int8), METHOD(int8_gemm),
+                          METHOD(latent_attention_shared),
                           {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_native", "Native call path of ferret_amd.ops.", -1, kMethods,
                        nullptr, nullptr, nullptr, nullptr};

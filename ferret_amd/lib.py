@@ -63,6 +63,10 @@ SIGNATURES = {
                                                   _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _c_int, _c_int, _c_int,
                                                   _c_int, _c_float, _c_int, _vp, _vp, _vp, _c_size_t, _vp]),
     "ferret_latent_attention_expanded_workspace": (_c_size_t, [_c_int, _c_int, _c_int, _c_int]),
+    "ferret_latent_attention_shared_workspace": (_c_size_t, [_c_int, _c_int, _c_int, _c_int]),
+    "ferret_latent_attention_shared": (_c_int, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _c_int, _c_int,
+                                                _vp, _vp, _vp, _c_int, _c_int, _vp, _vp, _vp, _c_int, _c_int, _c_int,
+                                                _c_int, _c_float, _c_int, _vp, _vp, _vp, _c_size_t, _vp]),
     "ferret_latent_attention": (_c_int, [_vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _c_int, _c_int, _vp, _vp,
                                          _vp, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _vp, _vp, _vp,
                                          _c_size_t, _vp]),

@@ -682,7 +682,7 @@ def _latent_cache(cache) -> None:
         raise TypeError(f"cache must be a LatentCache, got {type(cache).__name__}")
 
 
-def _cache(cache: LatentCache, page_table: torch.Tensor, starts: torch.Tensor, name: str, lens=None):
+def _cache(cache: LatentCache, page_table: torch.Tensor, starts: torch.Tensor, name: str, lens=None, of=""):
     """Checks of the cache and of a batch's index tensors: data, scales, pages, page_size, table, B, max_pages."""
     data, scales = cache.data, cache.scales
     dp = _dev(data, "cache.data", torch.bfloat16 if scales is None else torch.uint8, 3)
@@ -694,14 +694,15 @@ def _cache(cache: LatentCache, page_table: torch.Tensor, starts: torch.Tensor, n
     sp = 0
     if scales is not None:
         sp = _out(scales, "cache.scales", (*data.shape[:2], LATENT // 128), torch.uint8, data.device)
-    tp = _dev(page_table, "page_table", torch.int32, 2)
+    table = f"{of}table" if of else "page_table"
+    tp = _dev(page_table, table, torch.int32, 2)
     _dev(starts, name, torch.int32, 1)
     B = starts.shape[0] - 1
     if B < 1 or page_table.shape[0] != B:
-        raise ValueError(f"page_table must be [B, max_pages] and {name} [B + 1], got {tuple(page_table.shape)}, "
+        raise ValueError(f"{table} must be [B, max_pages] and {name} [B + 1], got {tuple(page_table.shape)}, "
                          f"{tuple(starts.shape)}")
     if lens is not None:
-        _out(lens, "lens", (B,), torch.int32, data.device)
+        _out(lens, f"{of}lens", (B,), torch.int32, data.device)
     _same_device(data, scales, page_table, starts, lens)
     return dp, sp, data.shape[0], data.shape[1], tp, B, page_table.shape[1]
 
@@ -802,6 +803,58 @@ def latent_attention(q_latent: torch.Tensor, q_rotary: torch.Tensor, cache: Late
                                                  lse.data_ptr() if lse is not None else 0,
                                                  _dev(workspace, "workspace"), need, _stream())
     _lib.check("ferret_latent_attention", rc)
+    return (out, lse) if return_lse else out
+
+
+def latent_attention_shared_workspace_bytes(num_prefixes: int, num_sequences: int, num_tokens: int,
+                                            num_heads: int) -> int:
+    """Bytes of the partial results that latent_attention_shared joins."""
+    return int(_lib.load().ferret_latent_attention_shared_workspace(num_prefixes, num_sequences, num_tokens, num_heads))
+
+
+def latent_attention_shared(q_latent: torch.Tensor, q_rotary: torch.Tensor, cache: LatentCache,
+                            prefix_table: torch.Tensor, prefix_lens: torch.Tensor, cu_prefix: torch.Tensor,
+                            page_table: torch.Tensor, lens: torch.Tensor, cu_q: torch.Tensor, scale: float,
+                            causal: bool = True, return_lse: bool = False, out: torch.Tensor | None = None,
+                            workspace: torch.Tensor | None = None):
+    """latent_attention for a batch whose sequences share prefixes (a system prompt, a document, each prompt of
+    several samples): out bf16 [T, H, 512] (or (out, lse fp32 [T, H])).
+
+    A token sees all prefix_lens[g] keys of its prefix, in the pages that prefix_table
+    [G, max_prefix_pages] names, and then the keys of its own sequence as in latent_attention: page_table
+    [B, max_pages], lens and cu_q count the sequences' own keys and new tokens alone.  cu_prefix int32
+    [G+1] gives the packed new tokens of each prefix, whose sequences stand side by side; tokens outside
+    it see no prefix, and a prefix may be empty.  A prefix is read and multiplied once for all its
+    tokens.  Index tensors stay on the device (a captured call replays with other lengths);
+    `workspace` of latent_attention_shared_workspace_bytes, `out`, tokens that see no key and rows behind the
+    last sequence as in latent_attention.
+    """
+    _latent_cache(cache)
+    r = _lib.native().latent_attention_shared(q_latent, q_rotary, cache.data, cache.scales, prefix_table, prefix_lens,
+                                              cu_prefix, page_table, lens, cu_q, float(scale), bool(causal),
+                                              bool(return_lse), out, workspace)
+    if r is not None:
+        return r
+    *_, pp, G, max_prefix = _cache(cache, prefix_table, cu_prefix, "cu_prefix", prefix_lens, "prefix_")
+    dp, sp, pages, page_size, tp, B, max_pages = _cache(cache, page_table, cu_q, "cu_q", lens)
+    lp, lt, lh = _rows(q_latent, "q_latent", (None, None, LATENT))
+    T, H = q_latent.shape[:2]
+    rp, rt, rh = _rows(q_rotary, "q_rotary", (T, H, ROTARY))
+    _same_device(cache.data, q_latent, q_rotary, out, workspace)
+    dev = q_latent.device
+    if out is None:
+        out = torch.empty((T, H, LATENT), dtype=torch.bfloat16, device=dev)
+    op = _out(out, "out", (T, H, LATENT), torch.bfloat16, dev)
+    lse = torch.empty((T, H), dtype=torch.float32, device=dev) if return_lse else None
+    need = latent_attention_shared_workspace_bytes(G, B, T, H)
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    with _on(q_latent):
+        rc = _lib.load().ferret_latent_attention_shared(
+            lp, lt, lh, rp, rt, rh, dp, sp, pages, page_size, pp, prefix_lens.data_ptr(), cu_prefix.data_ptr(), G,
+            max_prefix, tp, lens.data_ptr(), cu_q.data_ptr(), B, max_pages, T, H, scale, int(causal), op,
+            lse.data_ptr() if lse is not None else 0, _dev(workspace, "workspace"), need, _stream())
+    _lib.check("ferret_latent_attention_shared", rc)
     return (out, lse) if return_lse else out
 
 

@@ -317,6 +317,24 @@ def _(q_latent, q_rotary, data, scales, page_table, lens, cu_q, scale, causal=Tr
             q_latent.new_empty((T, H), dtype=torch.float32))
 
 
+@torch.library.custom_op(f"{_NS}::latent_attention_shared", mutates_args=())
+def latent_attention_shared(q_latent: torch.Tensor, q_rotary: torch.Tensor, data: torch.Tensor,
+                            scales: torch.Tensor | None, prefix_table: torch.Tensor, prefix_lens: torch.Tensor,
+                            cu_prefix: torch.Tensor, page_table: torch.Tensor, lens: torch.Tensor, cu_q: torch.Tensor,
+                            scale: float, causal: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
+    """(out bf16 [T, H, 512], lse fp32 [T, H]): latent attention of a batch whose sequences share prefixes."""
+    return _ops.latent_attention_shared(q_latent, q_rotary, _ops.LatentCache(data, scales), prefix_table, prefix_lens,
+                                        cu_prefix, page_table, lens, cu_q, scale, causal=causal, return_lse=True)
+
+
+@latent_attention_shared.register_fake
+def _(q_latent, q_rotary, data, scales, prefix_table, prefix_lens, cu_prefix, page_table, lens, cu_q, scale,
+      causal=True):
+    T, H, _ = q_latent.shape
+    return (q_latent.new_empty((T, H, _ops.LATENT), dtype=torch.bfloat16),
+            q_latent.new_empty((T, H), dtype=torch.float32))
+
+
 @torch.library.custom_op(f"{_NS}::latent_attention_expanded", mutates_args=())
 def latent_attention_expanded(q_nope: torch.Tensor, q_rotary: torch.Tensor, k_nope: torch.Tensor,
                               k_rotary: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
@@ -335,4 +353,5 @@ def _(q_nope, q_rotary, k_nope, k_rotary, v, cu_q, cu_k, scale, causal=True):
 OPS = ("linear_bf16", "fp8_gemm_blockscale", "fp8_gemm_ue8m0", "quant_act_e4m3", "moe_route_topk", "moe_permute",
        "moe_w13_fp8", "moe_w13_w4a16", "int4_tile_weights", "moe_w2_fp8", "moe_combine", "rms_norm",
        "add_rms_norm", "rms_norm_e4m3", "add_rms_norm_e4m3", "latent_cache_write", "latent_cache_read",
-       "latent_attention", "latent_attention_expanded", "quant_act_int8", "int8_gemm")
+       "latent_attention", "latent_attention_expanded", "quant_act_int8", "int8_gemm",
+       "latent_attention_shared")

@@ -390,6 +390,28 @@ int ferret_latent_attention(const void* q_latent, long long ql_token, long long 
                             void* out, float* lse, void* ws, size_t ws_bytes, void* stream);
 
 /*
+ * ferret_latent_attention for a batch whose sequences share prefixes: a token sees all
+ * prefix_lens[g] keys of its prefix g, which are read once for all of its tokens, then
+ * keys of its own sequence as there (lens, causal and page_table count those alone, new
+ * tokens included).
+ * prefix_table int32 [G, max_prefix_pages], prefix_lens int32 [G] (0 for none) and
+ * cu_prefix int32 [G + 1], ascending: the packed new tokens that see prefix g (all tokens of
+ * its sequences, which stand side by side); tokens outside [cu_prefix[0], cu_prefix[G]) see
+ * no prefix.  Both tables are of the one cache.  Everything else, the softmax's statement, out in
+ * place, lse, tokens without keys, Inf and NaN, and the range of the sums, as
+ * ferret_latent_attention; requirements for both tables.
+ * ws: ferret_latent_attention_shared_workspace(G, B, T, H) bytes, on a 16-byte bound.
+ */
+size_t ferret_latent_attention_shared_workspace(int G, int B, int T, int H);
+int ferret_latent_attention_shared(const void* q_latent, long long ql_token, long long ql_head, const void* q_rotary,
+                                   long long qr_token, long long qr_head, const void* data, const void* scales,
+                                   int pages, int page_size, const int32_t* prefix_table, const int32_t* prefix_lens,
+                                   const int32_t* cu_prefix, int G, int max_prefix_pages, const int32_t* page_table,
+                                   const int32_t* lens, const int32_t* cu_q, int B, int max_pages, int T, int H,
+                                   float scale, int causal, void* out, float* lse, void* ws, size_t ws_bytes,
+                                   void* stream);
+
+/*
  * Latent attention in its expanded form, for ragged prompts:
  *   s_ij = scale * (q_nope_i . k_nope_j + q_rotary_i . k_rotary_j),
  *   out_i = sum_j softmax_j(s_ij) v_j           (bf16 [T,H,128]),
