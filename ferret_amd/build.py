@@ -24,7 +24,7 @@ LIB = os.path.join(PKG, "libferret_hip.so")
 NATIVE = os.path.join(PKG, "_native.so")
 SOURCES = ["skinny.hip", "bf16_tiled.hip", "fp8_mid.hip", "int4_moe.hip", "fp8_tiled.hip", "fp8_square.hip",
            "routing.hip", "moe_tail.hip", "ue8m0.hip", "norm.hip", "latent_cache.hip", "latent_attention.hip",
-           "expanded_attention.hip", "int8_quant.hip", "int8_gemm.hip",
+           "expanded_attention.hip", "int8_quant.hip", "int8_gemm.hip", "int8_square.hip",
            "dispatch.hip"]
 ARCH = "gfx950"
 

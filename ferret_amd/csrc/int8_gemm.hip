@@ -3,18 +3,24 @@
 // The sum is whole and exact in 32 bits (K <= 65536), so the result depends on
 // neither tile, split nor order: bit for bit the same from every variant.
 //
-// A work-group of 8 waves takes RT x 16 weight rows by TT x 16 tokens over one K
-// split; both operands go global -> LDS in stages of KS bytes of each row through a
-// ring of NS stages, one barrier per stage.  Rows past N or M repeat the last one
-// (never stored), 16-byte chunks past K the last one of their row, with the tokens'
-// as zeros.  v_mfma_i32_16x16x64_i8: weight rows are the A side, tokens the B side,
-// so a lane holds four outputs in a row of one token.
+// Here: the kernel for few tokens, the sum over K splits, and the entry points;
+// int8_square.hip: the kernel for more.  int8_plan.hpp chooses.
+//
+// Few tokens: the bytes of the weights bound it.  A work-group of four or eight waves takes
+// RT x 16 weight rows by all TT x 16 tokens over one K split; both operands go global ->
+// LDS in stages of KS bytes of each row through a ring of NS stages, one barrier per
+// stage.  The waves split the K of a stage as well as the tile (WK); the parts meet in
+// LDS once.  Rows past N or M repeat the last one (never stored), 16-byte chunks past K the
+// last one of their row, with the tokens' as zeros.  v_mfma_i32_16x16x64_i8: weight rows
+// are the A side, tokens the B side, so a lane holds four outputs in a row of one token.
+// Tiles of 16 rows and 512 bytes let 4096 rows fill the CUs in one launch: 4096 x 12288 at
+// 16 tokens 12.0 us, 13.5 in tiles of 64 rows and splits of K (two launches); 4096 x 4096 at 1
+// 6.1 against 8.4.  24576 x 4096 at 1 token, 96 rows, 17.5 us, 5.8 TB/s.
 //
 // Every work-group starts at another K step (row tile index modulo its steps) and wraps
 // around: in lockstep, all of them read the same columns of rows a power of two
 // apart, which sit on few of the memory channels.
-#include "common.hpp"
-#include "int8_plan.hpp"
+#include "int8_epilogue.hpp"
 #include "ranges.hpp"
 
 namespace ferret {
@@ -53,7 +59,7 @@ struct Cfg {
 // banks.
 template <int KS>
 __device__ __forceinline__ int swz(int row, int c) {
-  return KS == 256 ? c ^ row : c ^ ((((row >> 1) ^ row) & 4) | (row & 2) | ((row >> 2) & 1));
+  return KS >= 256 ? c ^ row : c ^ ((((row >> 1) ^ row) & 4) | (row & 2) | ((row >> 2) & 1));
 }
 
 // Wait until at most min(n, N) stages of L loads are in flight.
@@ -67,23 +73,8 @@ __device__ __forceinline__ void wait_younger(int n) {
   }
 }
 
-// Four outputs of token m from channel n on, each step rounded by itself.
 __device__ __forceinline__ void put_four(const Args& p, int m, int n, i32x4 sum) {
-#pragma clang fp contract(off)
-  const float sa = p.sa[m];
-  const f32x4 sb = *reinterpret_cast<const f32x4*>(p.sb + n);
-  const size_t at = (size_t)m * p.N + n;
-  f32x4 v;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = (float)sum[i] * sa * sb[i];
-  if (p.residual != nullptr) {
-    const u32x2 r = *reinterpret_cast<const u32x2*>(p.residual + at);
-    v[0] += __uint_as_float(r[0] << 16);
-    v[1] += __uint_as_float(r[0] & 0xffff0000u);
-    v[2] += __uint_as_float(r[1] << 16);
-    v[3] += __uint_as_float(r[1] & 0xffff0000u);
-  }
-  *reinterpret_cast<u32x2*>(p.out + at) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+  *reinterpret_cast<u32x2*>(p.out + (size_t)m * p.N + n) = four_outputs(p, m, n, p.sa[m], sum);
 }
 
 template <int RT, int TT, int KS, int NS, int WR, int WT, int WK>
@@ -189,22 +180,32 @@ __global__ __launch_bounds__(64 * WR * WT * WK) void int8_tiled_kernel(Args p) {
   }
 }
 
-// The sum over the K splits, four outputs per thread.
+// The sum over S K splits, four outputs per thread, all loads before the first sum.
+template <int S>
 __global__ __launch_bounds__(256) void int8_reduce_kernel(Args p) {
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x, quads = p.N / 4;
   if (i >= p.M * quads) return;
   const int m = (int)(i / quads), n = (int)(i % quads) * 4;
-  i32x4 v = {0, 0, 0, 0};
-  for (int s = 0; s < p.splits; ++s) v += *reinterpret_cast<const i32x4*>(p.partial + ((size_t)s * p.M + m) * p.N + n);
-  put_four(p, m, n, v);
+  i32x4 v[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s) v[s] = *reinterpret_cast<const i32x4*>(p.partial + ((size_t)s * p.M + m) * p.N + n);
+#pragma unroll
+  for (int s = 1; s < S; ++s) v[0] += v[s];
+  put_four(p, m, n, v[0]);
 }
 
-template <int I, int WR, int WT, int WK>
+template <int S>
+int launch_reduce(const Args& p, hipStream_t st) {
+  const long long quads = (long long)p.M * (p.N / 4);
+  hipLaunchKernelGGL(int8_reduce_kernel<S>, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, p);
+  return (int)hipGetLastError();
+}
+
+template <int RT, int TT, int KS, int NS, int WR, int WT, int WK>
 int launch(const Args& p, hipStream_t st) {
-  constexpr Tile t = kTiles[I];
-  using C = Cfg<t.rt, t.tt, t.ks, t.ns, WR, WT, WK>;
-  FERRET_HIP_CHECK((set_lds_limit_once<int8_tiled_kernel<t.rt, t.tt, t.ks, t.ns, WR, WT, WK>>(C::kLds)));
-  hipLaunchKernelGGL((int8_tiled_kernel<t.rt, t.tt, t.ks, t.ns, WR, WT, WK>),
+  using C = Cfg<RT, TT, KS, NS, WR, WT, WK>;
+  FERRET_HIP_CHECK((set_lds_limit_once<int8_tiled_kernel<RT, TT, KS, NS, WR, WT, WK>>(C::kLds)));
+  hipLaunchKernelGGL((int8_tiled_kernel<RT, TT, KS, NS, WR, WT, WK>),
                      dim3((unsigned)(cdiv(p.N, C::kRows) * p.tok_tiles * p.splits)), dim3(C::kThreads), C::kLds, st, p);
   return (int)hipGetLastError();
 }
@@ -213,28 +214,33 @@ int launch(const Args& p, hipStream_t st) {
 }  // namespace i8
 }  // namespace ferret
 
+int ferret_int8_square(int tile, const ferret::i8::Args& p, hipStream_t st);
+
 // The product by one plan.
 int ferret_int8_run(const ferret::i8::Plan& plan, ferret::i8::Args p, hipStream_t st) {
   using namespace ferret::i8;
   p.splits = plan.splits;
   p.tok_tiles = plan.tok_tiles;
   p.nt = plan.tok_tiles == 1;
-  static_assert(kNumTiles == 8, "one case per tile");
+  static_assert(kFirstSquare == 5 && kNumTiles == 12, "one case per tile");
   int rc = FERRET_ERR_SHAPE;
   switch (plan.tile) {
-    case 0: rc = launch<0, 2, 1, 4>(p, st); break;
-    case 1: rc = launch<1, 2, 1, 4>(p, st); break;
-    case 2: rc = launch<2, 2, 1, 4>(p, st); break;
-    case 3: rc = launch<3, 2, 1, 4>(p, st); break;
-    case 4: rc = launch<4, 2, 2, 2>(p, st); break;
-    case 5: rc = launch<5, 2, 2, 2>(p, st); break;
-    case 6: rc = launch<6, 2, 4, 1>(p, st); break;
-    case 7: rc = launch<7, 2, 4, 1>(p, st); break;
+    case 0: rc = launch<1, 1, 512, 4, 1, 1, 8>(p, st); break;
+    case 1: rc = launch<2, 1, 256, 6, 1, 1, 4>(p, st); break;
+    case 2: rc = launch<6, 1, 256, 5, 2, 1, 4>(p, st); break;
+    case 3: rc = launch<2, 2, 512, 4, 1, 1, 8>(p, st); break;
+    case 4: rc = launch<6, 4, 256, 4, 2, 2, 2>(p, st); break;
+    default: rc = ferret_int8_square(plan.tile, p, st); break;
   }
   if (rc != FERRET_OK || p.splits == 1) return rc;
-  const long long quads = (long long)p.M * (p.N / 4);
-  hipLaunchKernelGGL(int8_reduce_kernel, dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, st, p);
-  return (int)hipGetLastError();
+  switch (p.splits) {
+    case 2: return launch_reduce<2>(p, st);
+    case 3: return launch_reduce<3>(p, st);
+    case 4: return launch_reduce<4>(p, st);
+    case 6: return launch_reduce<6>(p, st);
+    case 8: return launch_reduce<8>(p, st);
+  }
+  return FERRET_ERR_SHAPE;
 }
 
 using namespace ferret;
@@ -245,8 +251,7 @@ static bool int8_shape(int M, int N, int K) {
 
 extern "C" size_t ferret_int8_gemm_workspace(int M, int N, int K) {
   if (!int8_shape(M, N, K)) return 0;
-  const i8::Plan plan = i8::plan(M, N, K, 256);
-  return plan.splits > 1 ? (size_t)plan.splits * M * N * 4 : 0;
+  return i8::workspace(i8::plan(M, N, K), M, N);
 }
 
 extern "C" int ferret_int8_gemm(const void* a, const float* sa, const void* b, const float* sb, const void* residual,
@@ -256,8 +261,8 @@ extern "C" int ferret_int8_gemm(const void* a, const float* sa, const void* b, c
   const auto bits = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
   FERRET_REQUIRE(((bits(a) | bits(b) | bits(sb) | bits(residual) | bits(y)) & 15) == 0 && (bits(sa) & 3) == 0,
                  FERRET_ERR_ALIGN);
-  const i8::Plan plan = i8::plan(M, N, K, 256);
-  const size_t need = plan.splits > 1 ? (size_t)plan.splits * M * N * 4 : 0;
+  const i8::Plan plan = i8::plan(M, N, K);
+  const size_t need = i8::workspace(plan, M, N);
   FERRET_REQUIRE(need == 0 || (ws != nullptr && ws_bytes >= need && (bits(ws) & 15) == 0), FERRET_ERR_WORKSPACE);
   const uint64_t m = M, n = N, k = K;
   FERRET_REQUIRE(!clash({Range{y, m * n * 2}, Range{need != 0 ? ws : nullptr, need}},

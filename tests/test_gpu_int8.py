@@ -106,6 +106,29 @@ def test_product_bits(hip, M, N, K, residual):
     assert np.array_equal(bits(y), I.product(*case))
 
 
+# A shape of each tile without and with K splits (tests/test_int8_plan.py checks that), most with K, N and M off the tile.
+TILES = [(1, 8, 1392), (1, 1352, 7632), (1, 16, 5984), (1, 8, 6896), (5, 8, 16), (1, 680, 5808), (1, 16808, 272),
+         (1, 2744, 12208), (21, 8, 32), (21, 4080, 7152), (19, 8, 4928), (17, 16712, 160), (33, 2912, 12272), (39, 8, 688),
+         (3, 5192, 10688), (33, 8, 5680), (51, 24, 16), (2703, 8, 3216), (33, 8, 2544), (65, 8480, 16), (65, 2704, 5920),
+         (2867, 8, 5664), (67, 17064, 16), (67, 5968, 8112), (3589, 2056, 16), (217, 21168, 16), (69, 10968, 1072),
+         (563, 19600, 16), (1025, 4104, 4112), (300, 24584, 528)]
+
+
+@pytest.mark.parametrize("M,N,K", TILES)
+def test_product_bits_of_every_tile(hip, M, N, K):
+    """Against whole numbers summed on the GPU in 64 bits (exact below 2^53), then rounded as the oracle rounds."""
+    print(f"[case] int8 product {M} x {N} x {K}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(M + N + K)
+    a, b = (torch.randint(-128, 128, (n, K), generator=g, device="cuda", dtype=torch.int8) for n in (M, N))
+    sa, sb = (torch.rand(n, generator=g, device="cuda") + 0.01 for n in (M, N))
+    r = torch.randn((M, N), generator=g, device="cuda").to(torch.bfloat16) if M % 4 == 1 else None
+    y = ops.int8_gemm(a, sa, b, sb, r)
+    total = (a.double() @ b.double().t()).float()
+    want = total * sa[:, None] * sb
+    want = (want if r is None else want + r.float()).to(torch.bfloat16)
+    assert torch.equal(y.view(torch.int16), want.view(torch.int16))
+
+
 def test_product_largest_sums(hip):
     """K = 65536 of -128 * -128: 2^30, and 127 * -128 beside it."""
     K = 65536
