@@ -43,13 +43,13 @@
 #include "latent.hpp"
 
 #include <initializer_list>
-#include <utility>
+#include <type_traits>
 
 namespace ferret {
 namespace {
 
 constexpr int kKeys = kLatentKeys, kUnits = kLatentUnits;
-constexpr int kJoinRows = 512;  // rows up to which four work-groups join a row's pieces
+constexpr int kWideRows = 64;   // query rows of the largest tile
 constexpr int kAhead = 4;      // LDS fragments read ahead
 constexpr int kFence = 4;      // fragments between scheduling fences
 
@@ -67,22 +67,22 @@ struct Args {
   int side_by_side;  // row tiles of a sequence taken at the same time
   uint16_t* out;  // [T, H, 512]
   float* lse;     // [T, H] or null
-  // One of two passes over a row's keys (shared prefixes): where its whole tiles' m, l and
-  // outputs go instead of `out`, ml [T * H], then [T * H][512].  Null else.
-  uint8_t* whole;
-  __host__ __device__ float2* whole_ml() const { return reinterpret_cast<float2*>(whole); }
-  __host__ __device__ float* whole_part() const {
-    return reinterpret_cast<float*>(whole + (((size_t)T * H * sizeof(float2) + 255) & ~(size_t)255));
-  }
-  // The workspace: rows [T * H] (int4), then ml [2 * kUnits][MR] (m and l), then the
-  // partial outputs [2 * kUnits][MR][512].  A row's record is {first slot, pieces, row
-  // in tile, -}.
+  // The workspace: rows [T * H] (int4), then ml [blocks][16] (m and l), then the partial
+  // outputs [blocks][32][64][4], `blocks` of 16 query rows: 2 * kUnits slots of a tile each,
+  // then, where there is a second pass over the rows' keys (shared prefixes), the whole
+  // tiles, which go to `out` else.  A block's outputs stand as the matrix units leave them, lane g * 16 +
+  // r holding columns 4g .. 4g + 3 of 16 of row r, so that a store or load of a wave is 1 KB
+  // in one piece: rows of 2 KB, 64 bytes at a time, took 4 us a tile.  A row's record is {first
+  // block of the tile in its first slot or as a whole, pieces, row in tile, -}.
   uint8_t* ws;
+  int whole;  // whether whole tiles go to the workspace
   __host__ __device__ int4* rows() const { return reinterpret_cast<int4*>(ws); }
+  __host__ __device__ int blocks(int mr) const { return 2 * kUnits * (mr / 16) + (whole ? whole_blocks() : 0); }
+  __host__ __device__ int whole_blocks() const { return T * H / 16 + B + kWideRows / 16; }
   __host__ __device__ float2* ml() const {
     return reinterpret_cast<float2*>(ws + (((size_t)T * H * sizeof(int4) + 255) & ~(size_t)255));
   }
-  __host__ __device__ float* part(int mr) const { return reinterpret_cast<float*>(ml() + 2 * kUnits * mr); }
+  __host__ __device__ float* part(int mr) const { return reinterpret_cast<float*>(ml() + (size_t)blocks(mr) * 16); }
 };
 
 template <int MR>
@@ -111,7 +111,7 @@ struct Side {
   int seq_at, b;         // the sequence at hand and its place on the line
   LatentSeq seq;
   int first_row;         // the tile's first row among all [T * H]
-  int slot;              // of the partial result, -1 for a whole tile
+  int block;             // of the partial result, -1 for a whole tile that goes to `out`
   int end;               // of this work-group's share of the line
 };
 
@@ -152,6 +152,33 @@ __device__ __forceinline__ void put_args(Args* to, const Args& a) {
   to->ws = a.ws;
 }
 
+// Where the cache's arrays are: in the kernel's own arguments, or, where scalar registers are
+// shorter still, in vector registers, read at each use (hidden from the compiler, which
+// would move the reading out of the loop and spill).
+struct Cache {
+  const uint8_t* data_;
+  const uint32_t* scales_;
+  __device__ __forceinline__ explicit Cache(const Args& a) : data_(a.data), scales_(a.scales) {}
+  __device__ __forceinline__ const uint8_t* data() const { return data_; }
+  __device__ __forceinline__ const uint32_t* scales() const { return scales_; }
+};
+struct CacheLate {
+  int at[4];
+  __device__ __forceinline__ explicit CacheLate(const Args& a) {
+    const uint64_t d = reinterpret_cast<uint64_t>(a.data), s = reinterpret_cast<uint64_t>(a.scales);
+    at[0] = (int)d;
+    at[1] = (int)(d >> 32);
+    at[2] = (int)s;
+    at[3] = (int)(s >> 32);
+  }
+  __device__ __forceinline__ uint64_t get(int i) {
+    asm volatile("" : "+v"(at[i]), "+v"(at[i + 1]));
+    return (uint64_t)(uint32_t)uniform(at[i + 1]) << 32 | (uint32_t)uniform(at[i]);
+  }
+  __device__ __forceinline__ const uint8_t* data() { return reinterpret_cast<const uint8_t*>(get(0)); }
+  __device__ __forceinline__ const uint32_t* scales() { return reinterpret_cast<const uint32_t*>(get(2)); }
+};
+
 // LDS after the tile buffers.
 template <int MR, int WK, bool F8>
 struct Lds {
@@ -176,10 +203,10 @@ __device__ __forceinline__ int swz(int r) { return (((r >> 1) ^ r) & 4) | (r & 2
 // The start of a work-group's share of the line: false where it has none.  The page
 // table's first lines come under the loads of the lengths.  tot: 24 words of LDS.
 template <int MR, int NT>
-__device__ __forceinline__ bool take_share(const Args& a, LatentPlace place, Side* side, int* tot, int* cur) {
+__device__ __forceinline__ bool take_share(const Args& a, int units, LatentPlace place, Side* side, int* tot, int* cur) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int near =
-      a.pages.table[(long long)latent_near(place.unit, kUnits / a.side_by_side, a.B) * a.pages.max_pages];
+      a.pages.table[(long long)latent_near(place.unit, units, a.B) * a.pages.max_pages];
   const int per = (a.B + NT - 1) / NT;
   const int b0 = threadIdx.x * per;
   LatentSeq s{};
@@ -215,7 +242,6 @@ __device__ __forceinline__ bool take_share(const Args& a, LatentPlace place, Sid
     all = latent_add(all, tot[w]);
     groups = latent_add(groups, tot[NW + w]);
   }
-  const int units = kUnits / a.side_by_side;
   bool whole = false;
   if (per == 1) {  // more sequences than threads do not all fit
     const bool fits = latent_fits(s, latent_chunk(all, units, a.min_steps));
@@ -229,7 +255,7 @@ __device__ __forceinline__ bool take_share(const Args& a, LatentPlace place, Sid
   }
   const LatentDeal deal = latent_deal(all, groups, whole, units, a.min_steps);
   const int total = deal.total, chunk = deal.chunk, extra = deal.extra;
-  const int start = (int)min((long long)place.unit * chunk, (long long)total);
+  const int start = uniform((int)min((long long)place.unit * chunk, (long long)total));
   if (start >= total) return false;
   const int excl = before + incl - mine + extra * (groups_before + incl_groups - my_groups);
   if (excl <= start && start < excl + mine + extra * my_groups) {
@@ -290,18 +316,21 @@ __device__ __forceinline__ bool next_piece(LatentPlace place, Side* side, int cu
   p->see_any = causal ? uniform(max(p->past + p->row_last / in.H, 0)) : p->len;
   p->one = n == 1;
   const int chunk = side->chunk, first_row = p->q0 * in.H + p->row0;
+  // A whole tile's place: sequences start on a block of their own.
+  const int whole = 2 * kUnits * (MR / 16) + (p->q0 * in.H >> 4) + b + (p->row0 >> 4);
   __syncthreads();  // the piece before is done with its record and buffers
   if (threadIdx.x == 0) {
     side->b = b;
     put_seq(&side->seq, s);
     side->seq_at = seq_at;
     side->first_row = first_row;
-    side->slot =
-        p->s0 == 0 && p->s1 >= steps ? -1 : latent_slot(place.unit, place.lane, in.side_by_side, cur, chunk);
+    side->block = p->s0 == 0 && p->s1 >= steps
+                      ? (in.whole ? whole : -1)
+                      : latent_slot(place.unit, place.lane, in.side_by_side, cur, chunk) * (MR / 16);
   }
   if (p->s0 == 0 && (int)threadIdx.x <= p->row_last - p->row0) {
     const LatentRecord r = latent_record(place.unit, place.lane, in.side_by_side, cur, steps, chunk);
-    in.rows()[first_row + threadIdx.x] = make_int4(r.slot0, r.pieces, threadIdx.x, 0);
+    in.rows()[first_row + threadIdx.x] = make_int4(r.pieces == 1 ? whole : r.slot0 * (MR / 16), r.pieces, threadIdx.x, 0);
   }
   return true;
 }
@@ -409,18 +438,18 @@ __device__ __forceinline__ void clear_unseen(const Args& in, const Piece& p, uin
   }
 }
 
-// Row r of the tile done: its output, or its part of a piece.  o: blocks of 16 columns
-// from `col` on, 4 of each per lane.
+// Row f * 16 + r16 of the tile done: its output, or its part of a piece.  o: blocks of 16
+// columns from column `first` on, 4 of each per lane, from 4 * g on.
 template <int MR, int CT, int WQ>
-__device__ __forceinline__ void put_rows(const Side* side, const Piece& p, int f, int r16, int col,
+__device__ __forceinline__ void put_rows(const Side* side, const Piece& p, int f, int r16, int g, int first,
                                          bool stats, float top, float sum, const f32x4 (&o)[CT][WQ]) {
   const Args& in = side->args;
-  const int r = f * 16 + r16, slot = uniform(side->slot);
+  const int r = f * 16 + r16, block = uniform(side->block);
   if (p.row0 + r > p.row_last) return;
-  if (slot < 0 && in.whole == nullptr) {
+  if (block < 0) {
     const long long at = side->first_row + r;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    uint16_t* to = in.out + at * kLatent + col;
+    uint16_t* to = in.out + at * kLatent + first + 4 * g;
 #pragma unroll
     for (int c = 0; c < CT; ++c)
       *reinterpret_cast<u32x2*>(to + c * 16) =
@@ -428,38 +457,34 @@ __device__ __forceinline__ void put_rows(const Side* side, const Piece& p, int f
     if (stats && in.lse != nullptr)
       in.lse[at] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
   } else {
-    const long long at = slot < 0 ? side->first_row + r : (long long)slot * MR + r;
-    if (stats) (slot < 0 ? in.whole_ml() : in.ml())[at] = make_float2(top, sum);
-    float* to = (slot < 0 ? in.whole_part() : in.part(MR)) + at * kLatent + col;
+    if (stats) in.ml()[(long long)(block + f) * 16 + r16] = make_float2(top, sum);
+    float* to = in.part(MR) + ((long long)(block + f) * 32 + first / 16) * 256 + (g * 16 + r16) * 4;
 #pragma unroll
-    for (int c = 0; c < CT; ++c) *reinterpret_cast<f32x4*>(to + c * 16) = o[c][f];
+    for (int c = 0; c < CT; ++c) *reinterpret_cast<f32x4*>(to + c * 256) = o[c][f];
   }
 }
 
 // WQ x WK waves: 16 queries x 64 / WK keys each for the scores, all queries x
 // 512 / (WQ WK) columns for the output.
-template <int WQ, int WK, bool F8>
-__global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void latent_attention_kernel(Args a) {
+template <int WQ, int WK, bool F8, typename Cache>
+__device__ __forceinline__ void attend_narrow(const Args& a, Cache cache, int units, LatentPlace place, uint8_t* lds) {
   using L = Tile<F8>;
   constexpr int MR = 16 * WQ, NW = WQ * WK, NT = 64 * NW;
   using M = Lds<MR, WK, F8>;
   constexpr int KT = kKeys / 16 / WK;     // 16-key blocks of a wave's scores
   constexpr int CT = kLatent / 16 / NW;   // 16-column blocks of a wave's output
   constexpr int RG = 8 / NW;              // groups of 8 rows that a wave loads
-  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int r16 = lane & 15, g = lane >> 4;
   const int wq = wave / WK, wk = wave % WK;
   float* const tops = reinterpret_cast<float*>(lds + M::kTop);
   Side* const side = reinterpret_cast<Side*>(lds + M::kSide);
 
-  const LatentPlace place = latent_place(blockIdx.x, a.side_by_side);
   int cur;
-  if (!take_share<MR, NT>(a, place, side, reinterpret_cast<int*>(lds), &cur)) return;
+  if (!take_share<MR, NT>(a, units, place, side, reinterpret_cast<int*>(lds), &cur)) return;
   const Args& in = side->args;
-  const uint8_t* const data = a.data;
-  const uint32_t* const scales = a.scales;
-  const float scale_log2 = a.scale_log2;
+  float scale_log2 = a.scale_log2;
+  asm("" : "+v"(scale_log2));  // not in a scalar register
 
   // ---- lane constants
   int load_off[L::kLoads];  // source bytes within a group of 8 rows; the swizzle differs in odd groups
@@ -506,10 +531,10 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void latent_attention_ke
       const bool ok = at >= 0;
       const long long row = (ok ? (long long)at << 4 : 0) + (RG == 1 ? (wave & 1) * 8 : 0);  // no page: some row, masked
       if (lane == 0) lds[M::kValid + (t % L::kBufs) * 4 + wave * RG / 2] = ok ? 1 : 0;
-      src = data + row * L::kRowB;
+      src = cache.data() + row * L::kRowB;
       dst = uniform(lds_address(lds) + (t % L::kBufs) * L::kBytes + wave * RG * 8 * L::kRowB);
       if constexpr (F8) {
-        src_scales = scales + row;
+        src_scales = cache.scales() + row;
         dst_scales = uniform(lds_address(lds) + (t % L::kBufs) * L::kBytes + L::kData + wave * RG * 32);
       }
     };
@@ -751,8 +776,7 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void latent_attention_ke
       float sum = tops[f * 16 + r16];
 #pragma unroll
       for (int w = 1; w < WK; ++w) sum += tops[w * MR + f * 16 + r16];
-      put_rows<MR>(side, pc, f, r16, wave * CT * 16 + 4 * g, wave == 0 && g == 0, tops[WK * MR + f * 16 + r16],
-                   sum, o);
+      put_rows<MR>(side, pc, f, r16, g, wave * CT * 16, wave == 0 && g == 0, tops[WK * MR + f * 16 + r16], sum, o);
       __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -764,7 +788,7 @@ __global__ __launch_bounds__(64 * WQ * WK, WQ * WK / 4) void latent_attention_ke
 // keys, the others on their way), P twice, and the small records.
 template <bool F8>
 struct Wide {
-  static constexpr int kRows = 64, kStep = F8 ? 64 : 32, kBufs = F8 ? 3 : 4, kAway = kBufs - 2;
+  static constexpr int kRows = kWideRows, kStep = F8 ? 64 : 32, kBufs = F8 ? 3 : 4, kAway = kBufs - 2;
   static constexpr int kData = kStep * Tile<F8>::kRowB, kBytes = kData + (F8 ? kStep * 4 : 0);
   static constexpr int kPRow = kStep * 2, kPBytes = kRows * kPRow;
   static constexpr int kP = kBufs * kBytes;             // P [2][query][keys] bf16
@@ -784,12 +808,11 @@ static_assert(Wide<true>::kLds <= 160 * 1024 && Wide<false>::kLds <= 160 * 1024,
 // to the output (64 queries x 128 columns each) and load the keys to come: the matrix
 // unit is fed by one while the other is at its softmax, at a barrier or at its loads,
 // and neither holds more than half of the registers (Q is 144, O 128 of 256).
-template <bool F8>
-__global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
+template <bool F8, typename Cache>
+__device__ __forceinline__ void attend_wide(const Args& a, Cache cache, int units, LatentPlace place, uint8_t* lds) {
   using L = Tile<F8>;
   using M = Wide<F8>;
   constexpr int MR = M::kRows, KT = M::kStep / 32;  // 16-key blocks of a wave's scores
-  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int r16 = lane & 15, g = lane >> 4;
   float* const tops = reinterpret_cast<float*>(lds + M::kTop);
@@ -798,11 +821,11 @@ __global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
   // P of a query: chunk c of 8 keys stands at c ^ swz_p(query)
   const int zp = M::kStep == 64 ? r16 >> 1 : r16 >> 2;
 
-  const LatentPlace place = latent_place(blockIdx.x, a.side_by_side);
   int cur;
-  if (!take_share<MR, 512>(a, place, side, reinterpret_cast<int*>(lds), &cur)) return;
+  if (!take_share<MR, 512>(a, units, place, side, reinterpret_cast<int*>(lds), &cur)) return;
   const Args& in = side->args;
-  const float scale_log2 = a.scale_log2;
+  float scale_log2 = a.scale_log2;
+  asm("" : "+v"(scale_log2));  // not in a scalar register
 
   if (wave < 4) {
     // ================ scores
@@ -995,10 +1018,10 @@ __global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
         const int at = __builtin_amdgcn_readlane(where, u - held), buffer = u % M::kBufs;
         const long long row = (at >= 0 ? (long long)at << 4 : 0) + (RG == 1 ? (w & 1) * 8 : 0);  // no page: some row, masked
         if (lane == 0) lds[M::kValid + buffer * 4 + w * RG / 2] = at >= 0 ? 1 : 0;
-        src = a.data + row * L::kRowB;
+        src = cache.data() + row * L::kRowB;
         dst = uniform(lds_address(lds) + buffer * M::kBytes + w * RG * 8 * L::kRowB);
         if constexpr (F8) {
-          src_scales = a.scales + row;
+          src_scales = cache.scales() + row;
           dst_scales = uniform(lds_address(lds) + buffer * M::kBytes + M::kData + w * RG * 32);
         }
       };
@@ -1047,22 +1070,26 @@ __global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
         const int flags = *reinterpret_cast<const int*>(lds + M::kFlags + (v & 1) * 4);
         const uint32_t valid = *reinterpret_cast<const uint32_t*>(lds + M::kValid + buffer * 4);
         const uint8_t* pbuf = lds + M::kP + (v & 1) * M::kPBytes + r16 * M::kPRow;
-        u32x4 p[4];
-        u32x4 words[2];
-        const auto get_p = [&](int h) __attribute__((always_inline)) {
-          if constexpr (F8) {
-            const uint8_t* from = lds + buffer * M::kBytes + M::kData + (h * 32 + 8 * g) * 4;
-            words[0] = ld_u32x4(from);
-            words[1] = ld_u32x4(from + 16);
-          }
+        constexpr int HS = M::kStep / 32;  // halves of 32 keys
+        u32x4 p[HS][4];
+        u32x4 words[HS][2];
+        const auto get_p = [&]() __attribute__((always_inline)) {
 #pragma unroll
-          for (int f = 0; f < 4; ++f) p[f] = ld_u32x4(pbuf + f * 16 * M::kPRow + (((4 * h + g) ^ zp) << 4));
+          for (int h = 0; h < HS; ++h) {
+            if constexpr (F8) {
+              const uint8_t* from = lds + buffer * M::kBytes + M::kData + (h * 32 + 8 * g) * 4;
+              words[h][0] = ld_u32x4(from);
+              words[h][1] = ld_u32x4(from + 16);
+            }
+#pragma unroll
+            for (int f = 0; f < 4; ++f) p[h][f] = ld_u32x4(pbuf + f * 16 * M::kPRow + (((4 * h + g) ^ zp) << 4));
+          }
         };
-        get_p(0);
+        get_p();
         load_all(u + M::kAway);  // at once: between the products they held the wave up for longer
         if (uniform(flags) != 0) {
           lds_barrier();
-          get_p(0);
+          get_p();
 #pragma unroll
           for (int f = 0; f < 4; ++f) {
             const float by = tops[2 * MR + f * 16 + r16];
@@ -1105,28 +1132,53 @@ __global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
         // and 5000 keys, 125.7 by widening, two products and rounding.  Exact for normal numbers; a
         // product below 2^-126 becomes some number below 2^-126.  Zeros stay zeros (P is zero
         // or normal): a key that a query does not see, or whose term vanished, may have any scale.
+        // Powers up to 2^0, latents up to 448, take one saturating subtraction.
         // The pair of ones is kept from the compiler, which would make compares and selects of
         // the minimum's product (8% more time).
         uint32_t ones = 0x00010001u;
         if constexpr (F8) asm("" : "+s"(ones));
-        const auto scale_p = [&](int h) __attribute__((always_inline)) {
-          if constexpr (F8) {
-            u16x2 add[4];
+        bool large = false;
+        if constexpr (F8) {
+          uint32_t any = 0;
+#pragma unroll
+          for (int h = 0; h < HS; ++h)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) any |= words[h][i >> 2][i & 3];
+          large = __any((any >> (8 * w)) & 128u);
+        }
+        u16x2 step_down[4];
+        const auto start_scale = [&](int h) __attribute__((always_inline)) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t pair = __builtin_amdgcn_perm(words[h][i >> 1][2 * (i & 1) + 1], words[h][i >> 1][2 * (i & 1)],
+                                                        0x0c040c00u + 0x00010001u * w);
+            step_down[i] = ((u16x2)(uint16_t)127 - __builtin_bit_cast(u16x2, pair)) * (uint16_t)128;
+          }
+        };
+        const auto scale = [&](int h, int f) __attribute__((always_inline)) {
+          if (!large) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const uint32_t w0 = words[i >> 1][2 * (i & 1)] >> (8 * w), w1 = words[i >> 1][2 * (i & 1) + 1] >> (8 * w);
-              add[i] = __builtin_bit_cast(u16x2, (w0 & 255u) | (w1 & 255u) << 16) * (uint16_t)128 - (uint16_t)(127 * 128);
+              const uint32_t pair = p[h][f][i];
+              p[h][f][i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, pair),
+                                                                                      step_down[i]));
             }
+          } else {
 #pragma unroll
-            for (int f = 0; f < 4; ++f)
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t pair = p[h][f][i];
+              const u16x2 from = __builtin_bit_cast(u16x2, pair);
+              const u16x2 sum = from - step_down[i] * __builtin_elementwise_min(from, __builtin_bit_cast(u16x2, ones));
+              p[h][f][i] = __builtin_bit_cast(uint32_t,
+                                              __builtin_elementwise_max(__builtin_bit_cast(s16x2, sum), s16x2{0, 0}));
+            }
+          }
+        };
+        const auto scale_p = [&](int h) __attribute__((always_inline)) {
+          if constexpr (F8) {
+            start_scale(h);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const uint32_t pair = p[f][i];
-                const u16x2 from = __builtin_bit_cast(u16x2, pair);
-                const u16x2 sum = add[i] * __builtin_elementwise_min(from, __builtin_bit_cast(u16x2, ones)) + from;
-                p[f][i] = __builtin_bit_cast(uint32_t,
-                                             __builtin_elementwise_max(__builtin_bit_cast(s16x2, sum), s16x2{0, 0}));
-              }
+            for (int f = 0; f < 4; ++f) scale(h, f);
           }
         };
         scale_p(0);
@@ -1136,12 +1188,11 @@ __global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
           if constexpr (i + kAhead < NF) ring[i % kAhead] = frag(i + kAhead);
           const bf16x8 xb = F8 ? e4m3x8_to_bf16x8(x[0], x[1]) : __builtin_bit_cast(bf16x8, x);
 #pragma unroll
-          for (int f = 0; f < 4; ++f) o[c][f] = mfma_bf16(xb, __builtin_bit_cast(bf16x8, p[f]), o[c][f]);
+          for (int f = 0; f < 4; ++f) o[c][f] = mfma_bf16(xb, __builtin_bit_cast(bf16x8, p[h][f]), o[c][f]);
           if constexpr (i % 2 == 1) {
             __builtin_amdgcn_sched_barrier(0);
           }
-          if constexpr (c == CT - 1 && h + 1 < M::kStep / 32) {
-            get_p(h + 1);
+          if constexpr (c == CT - 1 && h + 1 < HS) {
             scale_p(h + 1);
             __builtin_amdgcn_sched_barrier(0);
           }
@@ -1151,273 +1202,302 @@ __global__ __launch_bounds__(512, 2) void latent_attention_wide_kernel(Args a) {
 #pragma unroll
       for (int f = 0; f < 4; ++f) {
         const int q = f * 16 + r16;
-        put_rows<MR>(side, pc, f, r16, w * 128 + 4 * g, w == 0 && g == 0, fin[2 * MR + q], fin[q] + fin[MR + q], o);
+        put_rows<MR>(side, pc, f, r16, g, w * 128, w == 0 && g == 0, fin[2 * MR + q], fin[q] + fin[MR + q], o);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
 }
 
-// Joins the pieces of the query rows that were cut, in the order of the keys.
+// ---- the kernels
 
-// The record of a row; false where nothing is to be joined.
-__device__ __forceinline__ bool to_join(const Args& a, int mr, long long row, LatentRecord* where, int* r) {
-  const int4 rec = a.rows()[row];  // rows behind the last sequence have none: whatever stands there
-  *where = LatentRecord{rec.x, rec.y};
-  *r = rec.z;
-  return row >= (long long)max(a.cu_q[0], 0) * a.H && row < (long long)min(a.cu_q[a.B], a.T) * a.H &&
-         latent_record_joins(*where, a.side_by_side) && (unsigned)rec.z < (unsigned)mr;
+template <int MR>
+constexpr int tile_threads() { return MR == 16 ? 256 : 512; }
+template <int MR, bool F8>
+constexpr int tile_lds() { return MR == kWideRows ? Wide<F8>::kLds : Lds<MR, 4, F8>::kBytes; }
+
+template <int MR, bool F8, typename Cache>
+__device__ __forceinline__ void attend(const Args& a, Cache cache, int units, LatentPlace place, uint8_t* lds) {
+  if constexpr (MR == kWideRows) attend_wide<F8>(a, cache, units, place, lds);
+  else attend_narrow<MR / 16, 4, F8>(a, cache, units, place, lds);
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
-  return v;
-}
-__device__ __forceinline__ float wave_add(float v) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
-  return v;
+template <int MR, bool F8>
+__global__ __launch_bounds__(tile_threads<MR>(), tile_threads<MR>() / 256) void latent_attention_kernel(Args a) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  using C = std::conditional_t<MR == 32, CacheLate, Cache>;
+  attend<MR, F8>(a, C(a), kUnits / a.side_by_side, latent_place(blockIdx.x, a.side_by_side), lds);
 }
 
-// A piece's weight and part of the sum.  l may be NaN where the maximum is -inf (a NaN
-// that is a piece's only key), and the row is NaN then.
-__device__ __forceinline__ float piece_weight(float2 v, float base) { return __builtin_amdgcn_exp2f(v.x - base); }
-__device__ __forceinline__ float piece_sum(float2 v, float base) {
-  return v.y != 0.f ? v.y * piece_weight(v, base) : 0.f;
-}
-
-// Many rows, few pieces each: a wave per row, 8 columns per lane, the pieces' weights
-// 64 at a time in the lanes, four pieces' loads under way together.
-__global__ __launch_bounds__(256) void latent_join_kernel(Args a, int mr, int rows) {
-  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (row >= rows) return;
-  LatentRecord where;
-  int r;
-  if (!to_join(a, mr, row, &where, &r)) return;
-  const float2* ml = a.ml();
-  const float* part = a.part(mr) + lane * 4;
-  const auto at = [&](int j) { return (long long)latent_record_slot(where, a.side_by_side, j) * mr + r; };
-  // The first pieces' outputs come under their maxima, four pieces at a time: 71 registers
-  // leave room for seven waves per SIMD (chunks of 200 to 500 tokens: 2% less time for the
-  // whole call than with eight at a time, after the maxima).
-  f32x4 x[4][2];
-  const auto load = [&](int j) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float* from = part + at(min(j + i, where.pieces - 1)) * kLatent;  // past the last: again, unused
-      x[i][0] = *reinterpret_cast<const f32x4*>(from);
-      x[i][1] = *reinterpret_cast<const f32x4*>(from + 256);
-    }
-  };
-  load(0);
-  float top = -INFINITY;
-  float2 v = lane < where.pieces ? ml[at(lane)] : make_float2(-INFINITY, 0.f);
-  top = v.x;
-  for (int j = lane + 64; j < where.pieces; j += 64) top = fmaxf(top, ml[at(j)].x);
-  top = wave_max(top);
-  const float base = top == -INFINITY ? 0.f : top;
-  f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-  float sum = 0.f, w = 0.f;
-  for (int j = 0; j < where.pieces; j += 4) {
-    if (j % 64 == 0) {
-      if (j > 0) v = j + lane < where.pieces ? ml[at(j + lane)] : make_float2(-INFINITY, 0.f);
-      sum += piece_sum(v, base);
-      w = piece_weight(v, base);
-    }
-    if (j > 0) load(j);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float wi = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), j % 64 + i));
-      if (j + i < where.pieces) {
-        acc[0] += x[i][0] * wi;
-        acc[1] += x[i][1] * wi;
-      }
-    }
+// Two passes over the rows' keys in one launch: work-groups of their own for the shared
+// prefixes, in tiles of MRP rows, and for the sequences' own keys, in tiles of MRO.  Every
+// work-group deals the CUs to the two by the steps of each, one of the prefix's as long as
+// `weight` of the own, and finds the same numbers.  The arguments of both passes are read
+// through LDS: in scalar registers they would leave too few.
+template <int MRP, int MRO, bool F8>
+struct Shared {
+  static_assert(MRP >= MRO, "threads");
+  static constexpr int kThreads = tile_threads<MRP>();
+  static constexpr int kArgs =
+      ((tile_lds<MRP, F8>() > tile_lds<MRO, F8>() ? tile_lds<MRP, F8>() : tile_lds<MRO, F8>()) + 15) & ~15;
+  static constexpr int kLds = kArgs + 2 * sizeof(Args);
+  static_assert(kLds <= 160 * 1024, "LDS of a CU");
+};
+template <int MRP, int MRO, bool F8>
+__global__ __launch_bounds__(tile_threads<MRP>(), tile_threads<MRP>() / 256) void latent_shared_kernel(Args, Args, float) {
+  using S = Shared<MRP, MRO, F8>;
+  constexpr int NT = S::kThreads, NW = NT / 64, WORDS = (2 * sizeof(Args) + 4) / 4;
+  static_assert(sizeof(Args) % 8 == 0 && WORDS <= NT, "arguments");
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  int* const tot = reinterpret_cast<int*>(lds);
+  const Args* const both = reinterpret_cast<const Args*>(lds + S::kArgs);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const auto kernarg = (const __attribute__((address_space(4))) int*)__builtin_amdgcn_kernarg_segment_ptr();
+  if (threadIdx.x < WORDS - 1) reinterpret_cast<int*>(lds + S::kArgs)[threadIdx.x] = kernarg[threadIdx.x];
+  const float weight = __int_as_float(kernarg[WORDS - 1]);
+  __syncthreads();
+  int near = 0;  // the page tables' lines come under the loads of the lengths
+  if (threadIdx.x < 2) {
+    const Args& a = both[threadIdx.x];
+    near = a.pages.table[(long long)latent_near(blockIdx.x, kUnits, a.B) * a.pages.max_pages];
   }
-  sum = wave_add(sum);
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  int steps[2] = {0, 0};
+  for (int b = threadIdx.x; b < both[0].B; b += NT)
+    steps[0] = latent_add(steps[0], sequence<MRP>(both[0], b).work(kLatentExtra));
+  for (int b = threadIdx.x; b < both[1].B; b += NT)
+    steps[1] = latent_add(steps[1], sequence<MRO>(both[1], b).work(kLatentExtra));
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
-    *reinterpret_cast<u32x2*>(a.out + (long long)row * kLatent + h * 256 + lane * 4) =
-        u32x2{pack_bf16x2(acc[h][0] * inv, acc[h][1] * inv), pack_bf16x2(acc[h][2] * inv, acc[h][3] * inv)};
-  if (a.lse != nullptr && lane == 0)
-    a.lse[row] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
-}
-
-// Few rows, up to kUnits pieces each: a work-group per row and 128 columns, 32 lanes
-// across and the pieces dealt to 8 groups of lanes, 8 in flight each.  A wave per row /
-// this, whole call, us: 16 heads, e4m3, one sequence of 100001 69.4 / 28.2, 16 of 6000 28.7 /
-// 27.6, 32 of 6000 (512 rows) 40.1 / 40.3, 64 of 600 to 8000 (1024 rows) 50.4 / 53.1.
-__global__ __launch_bounds__(256) void latent_join_long_kernel(Args a, int mr) {
-  constexpr int ACROSS = 32, GROUPS = 256 / ACROSS;
-  __shared__ f32x4 red[256];
-  __shared__ float weight[kUnits], stat[8];
-  const int row = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  LatentRecord where;
-  int r;
-  if (!to_join(a, mr, row, &where, &r)) return;
-  const int across = threadIdx.x % ACROSS, group = threadIdx.x / ACROSS, col = (blockIdx.y * ACROSS + across) * 4;
-  const auto at = [&](int j) { return (long long)latent_record_slot(where, a.side_by_side, j) * mr + r; };
-  const float2 v = (int)threadIdx.x < where.pieces ? a.ml()[at(threadIdx.x)] : make_float2(-INFINITY, 0.f);
-  const float* part = a.part(mr) + col;
-  f32x4 x[8];
-  const auto load = [&](int j0) __attribute__((always_inline)) {
+  for (int i = 0; i < 2; ++i) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int j = j0 + group + GROUPS * i;
-      x[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (j < where.pieces) x[i] = *reinterpret_cast<const f32x4*>(part + at(j) * kLatent);
-    }
-  };
-  load(0);  // under the weights
-  float top = wave_max(v.x);
-  if (lane == 0) stat[wave] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(stat[0], stat[1]), fmaxf(stat[2], stat[3]));
-  const float base = top == -INFINITY ? 0.f : top;
-  float sum = wave_add(piece_sum(v, base));
-  weight[threadIdx.x] = piece_weight(v, base);
-  if (lane == 0) stat[4 + wave] = sum;
-  __syncthreads();
-  sum = (stat[4] + stat[5]) + (stat[6] + stat[7]);
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int j0 = 0;;) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) acc += x[i] * weight[j0 + group + GROUPS * i];
-    j0 += 8 * GROUPS;
-    if (j0 >= where.pieces) break;
-    load(j0);
+    for (int off = 32; off >= 1; off >>= 1) steps[i] = latent_add(steps[i], __shfl_xor(steps[i], off, 64));
+    if (lane == 0) tot[i * NW + wave] = steps[i];
   }
-  red[threadIdx.x] = acc;
   __syncthreads();
-  if (group != 0) return;
+  int all[2] = {0, 0};
 #pragma unroll
-  for (int i = 1; i < GROUPS; ++i) acc += red[i * ACROSS + across];
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  *reinterpret_cast<u32x2*>(a.out + (long long)row * kLatent + col) =
-      u32x2{pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv)};
-  if (a.lse != nullptr && col == 0)
-    a.lse[row] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+  for (int w = 0; w < NW; ++w) {
+    all[0] = latent_add(all[0], tot[w]);
+    all[1] = latent_add(all[1], tot[NW + w]);
+  }
+  __syncthreads();
+  const int groups = uniform(latent_split(all[0], all[1], weight, both[0].side_by_side, both[1].side_by_side));
+  asm volatile("" ::"v"(near));
+  const bool first = (int)blockIdx.x < groups;
+  const Args& a = both[first ? 0 : 1];
+  const int side = uniform(a.side_by_side), units = (first ? groups : kUnits - groups) / side;
+  LatentPlace place = latent_place(first ? blockIdx.x : blockIdx.x - groups, side);
+  asm("" : "+v"(place.unit), "+v"(place.lane));  // used between tiles only: not in scalar registers
+  if (MRO == MRP || first) {
+    attend<MRP, F8>(a, CacheLate(a), units, place, lds);
+  } else {
+    if (MRO < MRP && (int)threadIdx.x >= tile_threads<MRO>()) return;
+    attend<MRO, F8>(a, CacheLate(a), units, place, lds);
+  }
 }
 
-int launch_join(const Args& a, int mr, hipStream_t st) {
-  const unsigned rows = (unsigned)((long long)a.T * a.H);
-  if (rows <= kJoinRows)
-    hipLaunchKernelGGL(latent_join_long_kernel, dim3(rows, kLatent / 128), dim3(256), 0, st, a, mr);
-  else
-    hipLaunchKernelGGL(latent_join_kernel, dim3((rows + 3) / 4), dim3(256), 0, st, a, mr, (int)rows);
-  return (int)hipGetLastError();
+// ---- joins
+
+__device__ __forceinline__ bool has_tokens(const Args& a, long long row) {
+  return row >= (long long)max(a.cu_q[0], 0) * a.H && row < (long long)min(a.cu_q[a.B], a.T) * a.H;
 }
 
-// ---- two passes over the keys: shared prefixes, then a sequence's own
-
-// The pieces of one row in one pass.
+// The pieces of a row in one pass.  Rows behind the last sequence have no record, and
+// whatever stands in its place leads nowhere outside the workspace.
 struct Pieces {
-  const float2* ml;
-  const float* part;
-  long long first, rest, step;  // rows of `ml` and `part`: the first piece's; piece j > 0 at rest + j * step
-  int n;
-  __device__ __forceinline__ long long at(int j) const { return j == 0 ? first : rest + j * step; }
+  int first, rest, step;  // blocks of 16 rows: the first piece's; piece j > 0 at rest + j * step
+  int n, r16;
+  __device__ __forceinline__ int at(int j) const { return j == 0 ? first : rest + j * step; }
 };
 __device__ __forceinline__ Pieces pieces_of(const Args& a, int mr, long long row) {
-  Pieces p{a.whole_ml(), a.whole_part(), row, 0, 0, 0};
-  if (row < (long long)max(a.cu_q[0], 0) * a.H || row >= (long long)min(a.cu_q[a.B], a.T) * a.H) return p;  // no keys
+  Pieces p{0, 0, 0, 0, 0};
   const int4 rec = a.rows()[row];
-  const LatentRecord where{rec.x, rec.y};
-  p.n = 1;
-  if (latent_record_joins(where, a.side_by_side) && (unsigned)rec.z < (unsigned)mr) {
-    p.ml = a.ml();
-    p.part = a.part(mr);
+  if (!has_tokens(a, row) || (unsigned)rec.z >= (unsigned)mr) return p;
+  const int per = mr / 16, f = rec.z >> 4;
+  p.r16 = rec.z & 15;
+  const LatentRecord where{rec.x / per, rec.y};
+  if (latent_record_joins(where, a.side_by_side)) {
     p.n = where.pieces;
-    p.first = (long long)where.slot0 * mr + rec.z;
-    p.step = 2LL * a.side_by_side * mr;
-    p.rest = (long long)(where.slot0 & ~1) * mr + rec.z;
+    p.first = where.slot0 * per + f;
+    p.rest = (where.slot0 & ~1) * per + f;
+    p.step = 2 * a.side_by_side * per;
+  } else if (a.whole && rec.y == 1 && rec.x >= 2 * kUnits * per && rec.x < a.blocks(mr) - f) {
+    p.n = 1;
+    p.first = rec.x + f;
   }
   return p;
 }
 
-// Joins the pieces of both passes, the prefix's first: a wave per row, 8 columns per lane,
-// the pieces' weights 64 at a time in the lanes, four pieces' loads under way together.
-__global__ __launch_bounds__(256) void latent_shared_join_kernel(Args prefix, Args own, int prefix_mr, int own_mr) {
-  const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (row < (long long)max(own.cu_q[0], 0) * own.H || row >= (long long)min(own.cu_q[own.B], own.T) * own.H) return;
-  const Pieces p0 = pieces_of(prefix, prefix_mr, row), p1 = pieces_of(own, own_mr, row);
+__device__ __forceinline__ float quad_max(float v) {  // over the lanes of a row
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float quad_add(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+
+// Joins the pieces of 16 query rows in the order of the keys, those of the prefix (TWO)
+// first: lane g * 16 + i takes row i and columns 4g .. 4g + 3 of every 16, as the pieces
+// stand, and CB blocks of 16 columns.  PW waves take every PW-th four pieces each, eight
+// loads under way, with the weights of four pieces in the lanes, one per g, and meet in LDS.
+// TWO: every row; else those of tiles that were cut.
+template <bool TWO, int PW>
+__global__ __launch_bounds__(64 * (PW > 4 ? PW : 4)) void latent_join_kernel(Args prefix, Args own, int prefix_mr,
+                                                                          int own_mr, int rows) {
+  constexpr int CB = 2, AHEAD = 4, WAVES = PW > 4 ? PW : 4, TILES = WAVES / PW;  // units of 16 rows x CB blocks per work-group
+  __shared__ f32x4 red[PW > 1 ? WAVES : 1][CB][64];
+  __shared__ float2 red_ml[PW > 1 ? WAVES : 1][16];
+  const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6, pw = wave % PW;
+  const int unit = blockIdx.x * TILES + wave / PW, cb = unit % (32 / CB) * CB;
+  const long long row = (long long)(unit / (32 / CB)) * 16 + (lane & 15);
+  const bool in = row < rows;
+  Pieces p0{0, 0, 0, 0, 0}, p1 = p0;
+  if (in) {
+    p1 = pieces_of(own, own_mr, row);
+    if constexpr (TWO) p0 = pieces_of(prefix, prefix_mr, row);
+  }
   const int n = p0.n + p1.n;
+  const bool mine = TWO ? in && has_tokens(own, row) : n >= 2;
+  if (PW == 1 && !__any(mine)) return;
+  int most = mine ? n : 0;
+#pragma unroll
+  for (int off = 8; off >= 1; off >>= 1) most = max(most, __shfl_xor(most, off, 64));
   const auto stat = [&](int j) {
-    if (j >= n) return make_float2(-INFINITY, 0.f);
-    return j < p0.n ? p0.ml[p0.at(j)] : p1.ml[p1.at(j - p0.n)];
+    if (!mine || j >= n) return make_float2(-INFINITY, 0.f);
+    return TWO && j < p0.n ? prefix.ml()[(long long)p0.at(j) * 16 + p0.r16]
+                           : own.ml()[(long long)p1.at(j - p0.n) * 16 + p1.r16];
   };
-  f32x4 x[4][2];
+  const float* const part0 = TWO ? prefix.part(prefix_mr) + (cb * 64 + g * 16 + p0.r16) * 4 : nullptr;
+  const float* const part1 = own.part(own_mr) + (cb * 64 + g * 16 + p1.r16) * 4;
+  f32x4 x[AHEAD][CB];
   const auto load = [&](int j0) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int j = min(j0 + i, n - 1);  // past the last: again, unused
-      const float* from = (j < p0.n ? p0.part + p0.at(j) * kLatent : p1.part + p1.at(j - p0.n) * kLatent) + lane * 4;
-      x[i][0] = *reinterpret_cast<const f32x4*>(from);
-      x[i][1] = *reinterpret_cast<const f32x4*>(from + 256);
+    for (int i = 0; i < AHEAD; ++i) {
+      const int j = j0 + i;
+      const float* from = TWO && j < p0.n ? part0 + (long long)p0.at(j) * (32 * 256)
+                                          : part1 + (long long)p1.at(j - p0.n) * (32 * 256);
+#pragma unroll
+      for (int c = 0; c < CB; ++c) {
+        x[i][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (mine && j < n) x[i][c] = *reinterpret_cast<const f32x4*>(from + c * 256);
+      }
     }
   };
-  load(0);
-  float2 v = stat(lane);
+  load(pw * AHEAD);  // under the maxima
+  float2 v = stat(pw * AHEAD + g);
   float top = v.x;
-  for (int j = lane + 64; j < n; j += 64) top = fmaxf(top, stat(j).x);
-  top = wave_max(top);
+  for (int j = (pw + PW) * AHEAD; j < most; j += PW * AHEAD) top = fmaxf(top, stat(j + g).x);
+  top = quad_max(top);
   const float base = top == -INFINITY ? 0.f : top;
-  f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-  float sum = 0.f, w = 0.f;
-  for (int j = 0; j < n; j += 4) {
-    if (j % 64 == 0) {
-      if (j > 0) v = stat(j + lane);
-      sum += piece_sum(v, base);
-      w = piece_weight(v, base);
-    }
-    if (j > 0) load(j);
+  f32x4 acc[CB];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float wi = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), j % 64 + i));
-      if (j + i < n) {
-        acc[0] += x[i][0] * wi;
-        acc[1] += x[i][1] * wi;
+  for (int c = 0; c < CB; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // A piece's l may be NaN where its maximum is -inf (a NaN that is its only key), and the
+  // row is NaN then.
+  float sum = 0.f;
+  for (int j = pw * AHEAD; j < most; j += PW * AHEAD) {
+    if (j > pw * AHEAD) {
+      load(j);
+      v = stat(j + g);
+    }
+    const float w = __builtin_amdgcn_exp2f(v.x - base);
+    if (v.y != 0.f) sum += v.y * w;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const float wi = __shfl(w, (lane & 15) + 16 * i, 64);
+      if (mine && j + i < n) {
+#pragma unroll
+        for (int c = 0; c < CB; ++c) acc[c] += x[i][c] * wi;
       }
     }
   }
-  sum = wave_add(sum);
+  sum = quad_add(sum);
+  if constexpr (PW > 1) {
+#pragma unroll
+    for (int c = 0; c < CB; ++c) red[wave][c][lane] = acc[c];
+    if (g == 0) red_ml[wave][lane] = make_float2(top, sum);
+    __syncthreads();
+    if (pw != 0) return;
+#pragma unroll
+    for (int i = 1; i < PW; ++i) top = fmaxf(top, red_ml[wave + i][lane & 15].x);
+    const float all = top == -INFINITY ? 0.f : top, first = __builtin_amdgcn_exp2f(red_ml[wave][lane & 15].x - all);
+    sum = sum != 0.f ? sum * first : 0.f;
+#pragma unroll
+    for (int c = 0; c < CB; ++c) acc[c] *= first;
+#pragma unroll
+    for (int i = 1; i < PW; ++i) {
+      const float2 s = red_ml[wave + i][lane & 15];
+      const float w = __builtin_amdgcn_exp2f(s.x - all);
+      if (s.y != 0.f) sum += s.y * w;
+#pragma unroll
+      for (int c = 0; c < CB; ++c) acc[c] += red[wave + i][c][lane] * w;
+    }
+  }
+  if (!mine) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
-    *reinterpret_cast<u32x2*>(own.out + row * kLatent + h * 256 + lane * 4) =
-        u32x2{pack_bf16x2(acc[h][0] * inv, acc[h][1] * inv), pack_bf16x2(acc[h][2] * inv, acc[h][3] * inv)};
-  if (own.lse != nullptr && lane == 0)
+  for (int c = 0; c < CB; ++c)
+    *reinterpret_cast<u32x2*>(own.out + row * kLatent + (cb + c) * 16 + 4 * g) =
+        u32x2{pack_bf16x2(acc[c][0] * inv, acc[c][1] * inv), pack_bf16x2(acc[c][2] * inv, acc[c][3] * inv)};
+  if (own.lse != nullptr && cb == 0 && g == 0)
     own.lse[row] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
-template <int WQ, int WK, bool F8>
-int launch(const Args& a, hipStream_t st) {
-  constexpr int mr = 16 * WQ, lds = Lds<mr, WK, F8>::kBytes;
-  FERRET_HIP_CHECK((set_lds_limit_once<latent_attention_kernel<WQ, WK, F8>>(lds)));
-  hipLaunchKernelGGL((latent_attention_kernel<WQ, WK, F8>), dim3(kUnits), dim3(64 * WQ * WK), lds, st, a);
-  FERRET_HIP_CHECK(hipGetLastError());
-  return a.whole != nullptr ? FERRET_OK : launch_join(a, mr, st);
+template <bool TWO, int PW>
+int launch_join(const Args& prefix, const Args& own, int prefix_mr, int own_mr, hipStream_t st) {
+  constexpr int WAVES = PW > 4 ? PW : 4, TILES = WAVES / PW;
+  const long long rows = (long long)own.T * own.H, units = (rows + 15) / 16 * 16;
+  hipLaunchKernelGGL((latent_join_kernel<TWO, PW>), dim3((unsigned)((units + TILES - 1) / TILES)), dim3(64 * WAVES), 0, st,
+                     prefix, own, prefix_mr, own_mr, (int)rows);
+  return (int)hipGetLastError();
 }
 
-template <bool F8>
-int launch_wide(const Args& a, hipStream_t st) {
-  constexpr int lds = Wide<F8>::kLds;
-  FERRET_HIP_CHECK((set_lds_limit_once<latent_attention_wide_kernel<F8>>(lds)));
-  hipLaunchKernelGGL((latent_attention_wide_kernel<F8>), dim3(kUnits), dim3(512), lds, st, a);
+// Waves for the pieces of a row, by how many it has where all work-groups are at few rows.
+template <bool TWO>
+int pick_join(const Args& prefix, const Args& own, int prefix_mr, int own_mr, hipStream_t st) {
+  const long long pieces = (long long)kUnits * (own_mr + (TWO ? prefix_mr : 0)) / ((long long)own.T * own.H);
+  if (pieces >= 32) return launch_join<TWO, 16>(prefix, own, prefix_mr, own_mr, st);
+  if (pieces >= 10) return launch_join<TWO, 4>(prefix, own, prefix_mr, own_mr, st);
+  return launch_join<TWO, 1>(prefix, own, prefix_mr, own_mr, st);
+}
+
+template <int MR, bool F8>
+int launch(const Args& a, hipStream_t st) {
+  constexpr int lds = tile_lds<MR, F8>();
+  FERRET_HIP_CHECK((set_lds_limit_once<latent_attention_kernel<MR, F8>>(lds)));
+  hipLaunchKernelGGL((latent_attention_kernel<MR, F8>), dim3(kUnits), dim3(tile_threads<MR>()), lds, st, a);
   FERRET_HIP_CHECK(hipGetLastError());
-  return a.whole != nullptr ? FERRET_OK : launch_join(a, Wide<F8>::kRows, st);
+  return pick_join<false>(a, a, MR, MR, st);
 }
 
 template <bool F8>
 int launch_rows(int mr, const Args& a, hipStream_t st) {
   switch (mr) {
-    case 16: return launch<1, 4, F8>(a, st);
-    case 32: return launch<2, 4, F8>(a, st);
-    default: return launch_wide<F8>(a, st);
+    case 16: return launch<16, F8>(a, st);
+    case 32: return launch<32, F8>(a, st);
+    default: return launch<kWideRows, F8>(a, st);
   }
+}
+
+template <int MRP, int MRO, bool F8>
+int launch_shared(const Args& prefix, const Args& own, hipStream_t st) {
+  using S = Shared<MRP, MRO, F8>;
+  // What a step of the prefix's tiles takes of one of the own.
+  constexpr float weight = MRP == MRO ? 1.f : MRO == 32 ? 2.f : 3.f;
+  FERRET_HIP_CHECK((set_lds_limit_once<latent_shared_kernel<MRP, MRO, F8>>(S::kLds)));
+  hipLaunchKernelGGL((latent_shared_kernel<MRP, MRO, F8>), dim3(kUnits), dim3(S::kThreads), S::kLds, st, prefix, own,
+                     weight);
+  FERRET_HIP_CHECK(hipGetLastError());
+  return pick_join<true>(prefix, own, MRP, MRO, st);
+}
+
+template <bool F8>
+int launch_shared_rows(int prefix_mr, int own_mr, const Args& prefix, const Args& own, hipStream_t st) {
+  if (prefix_mr == 16) return launch_shared<16, 16, F8>(prefix, own, st);
+  if (prefix_mr == 32) return launch_shared<32, 32, F8>(prefix, own, st);
+  if (own_mr == 16) return launch_shared<kWideRows, 16, F8>(prefix, own, st);
+  if (own_mr == 32) return launch_shared<kWideRows, 32, F8>(prefix, own, st);
+  return launch_shared<kWideRows, kWideRows, F8>(prefix, own, st);
 }
 
 // Query rows per tile by the rows that a sequence has on average.  Us, e4m3, 64 sequences
@@ -1476,15 +1556,33 @@ Args pass_args(const void* q_latent, long long ql_token, long long ql_head, cons
   a.side_by_side = side_by_side(T, B, H);
   a.out = static_cast<uint16_t*>(out);
   a.lse = lse;
-  a.whole = nullptr;
+  a.whole = 0;
   a.ws = static_cast<uint8_t*>(ws);
   return a;
 }
 
-// Bytes of m, l and outputs of all rows.
-size_t whole_bytes(int T, int H) {
-  const size_t rows = (size_t)T * H;
-  return ((rows * sizeof(float2) + 255) & ~(size_t)255) + rows * kLatent * sizeof(float);
+// Bytes of the workspace of a pass in tiles of mr rows.
+size_t pass_bytes(int B, int T, int H, int mr, int whole) {
+  Args a{};
+  a.T = T;
+  a.H = H;
+  a.B = B;
+  a.whole = whole;
+  const size_t rows = ((size_t)T * H * sizeof(int4) + 255) & ~(size_t)255;
+  return rows + (size_t)a.blocks(mr) * 16 * (sizeof(float2) + kLatent * sizeof(float));
+}
+
+// Tiles of the two passes of shared prefixes: as one pass has them, the prefix's at least
+// the own's, and as small as those where that is little work: at most keys of
+// the table.
+struct SharedTiles {
+  int prefix, own;
+};
+SharedTiles shared_tiles(int G, int B, int T, int H, long long keys) {
+  const int own = tile_rows(T, B, H), prefix = tile_rows(T, G, H), most = prefix > own ? prefix : own;
+  if (prefix <= 32) return {most, most};
+  const long long steps = ((long long)T * H + own - 1) / own * ((keys + kKeys - 1) / kKeys);
+  return steps < 4 * kUnits ? SharedTiles{own, own} : SharedTiles{most, own};
 }
 
 }  // namespace
@@ -1496,8 +1594,7 @@ int ferret_check_pages(const int32_t* page_table, int B, int max_pages, int page
 
 extern "C" size_t ferret_latent_attention_workspace(int B, int T, int H) {
   if (B < 1 || T < 1 || H < 1 || (long long)T * H >= (1LL << 31)) return 0;
-  const size_t mr = tile_rows(T, B, H), rows = ((size_t)T * H * sizeof(int4) + 255) & ~(size_t)255;
-  return rows + 2 * kUnits * mr * (sizeof(float2) + kLatent * sizeof(float));
+  return pass_bytes(B, T, H, tile_rows(T, B, H), 0);
 }
 
 extern "C" int ferret_latent_attention(const void* q_latent, long long ql_token, long long ql_head,
@@ -1540,8 +1637,9 @@ extern "C" int ferret_latent_attention(const void* q_latent, long long ql_token,
 }
 
 extern "C" size_t ferret_latent_attention_shared_workspace(int G, int B, int T, int H) {
-  const size_t prefix = ferret_latent_attention_workspace(G, T, H), own = ferret_latent_attention_workspace(B, T, H);
-  return prefix == 0 || own == 0 ? 0 : ((prefix + 255) & ~(size_t)255) + ((own + 255) & ~(size_t)255) + 2 * whole_bytes(T, H);
+  if (G < 1 || B < 1 || T < 1 || H < 1 || (long long)T * H + 16LL * (G > B ? G : B) >= (1LL << 31)) return 0;
+  const SharedTiles mr = shared_tiles(G, B, T, H, 1LL << 31);  // the larger ones
+  return ((pass_bytes(G, T, H, mr.prefix, 1) + 255) & ~(size_t)255) + pass_bytes(B, T, H, mr.own, 1);
 }
 
 extern "C" int ferret_latent_attention_shared(const void* q_latent, long long ql_token, long long ql_head,
@@ -1564,11 +1662,12 @@ extern "C" int ferret_latent_attention_shared(const void* q_latent, long long ql
   FERRET_REQUIRE(((bits(q_latent) | bits(q_rotary) | bits(data) | bits(out)) & 15) == 0 &&
                      ((bits(scales) | bits(lse)) & 3) == 0 && ((ql_token | ql_head | qr_token | qr_head) & 7) == 0,
                  FERRET_ERR_ALIGN);
-  const int prefix_mr = tile_rows(T, G, H), own_mr = tile_rows(T, B, H);
-  rc = check_steps(G, max_prefix_pages, pages, page_size, T, H, prefix_mr);
-  if (rc == FERRET_OK) rc = check_steps(B, max_pages, pages, page_size, T, H, own_mr);
+  const SharedTiles mr = shared_tiles(G, B, T, H, (long long)max_prefix_pages * page_size);
+  rc = check_steps(G, max_prefix_pages, pages, page_size, T, H, mr.prefix);
+  if (rc == FERRET_OK) rc = check_steps(B, max_pages, pages, page_size, T, H, mr.own);
   if (rc != FERRET_OK) return rc;
   const size_t need = ferret_latent_attention_shared_workspace(G, B, T, H);
+  FERRET_REQUIRE(need != 0, FERRET_ERR_SHAPE);
   FERRET_REQUIRE(ws != nullptr && ws_bytes >= need && (bits(ws) & 15) == 0, FERRET_ERR_WORKSPACE);
   // In place is sound: `out` is written by the join alone.
   const bool over = in_place(out, q_latent, T, ql_token, H, ql_head, kLatent);
@@ -1580,23 +1679,17 @@ extern "C" int ferret_latent_attention_shared(const void* q_latent, long long ql
                          ints_range(cu_prefix, G + 1LL), ints_range(page_table, (uint64_t)B * max_pages),
                          ints_range(lens, B), ints_range(cu_q, B + 1LL)}),
                  FERRET_ERR_SHAPE);
-  uint8_t* at = static_cast<uint8_t*>(ws);
-  const auto take = [&](size_t bytes) { uint8_t* p = at; at += (bytes + 255) & ~(size_t)255; return p; };
+  const size_t prefix_bytes = (pass_bytes(G, T, H, mr.prefix, 1) + 255) & ~(size_t)255;
   Args prefix = pass_args(q_latent, ql_token, ql_head, q_rotary, qr_token, qr_head, data, scales,
                           Pages{prefix_table, max_prefix_pages, pages, page_size}, prefix_lens, cu_prefix, G, T, H,
-                          scale, 0, prefix_mr, nullptr, nullptr, take(ferret_latent_attention_workspace(G, T, H)));
+                          scale, 0, mr.prefix, nullptr, nullptr, ws);
   Args own = pass_args(q_latent, ql_token, ql_head, q_rotary, qr_token, qr_head, data, scales,
-                       Pages{page_table, max_pages, pages, page_size}, lens, cu_q, B, T, H, scale, causal, own_mr, out,
-                       lse, take(ferret_latent_attention_workspace(B, T, H)));
-  prefix.whole = take(whole_bytes(T, H));
-  own.whole = take(whole_bytes(T, H));
-  const hipStream_t st = (hipStream_t)stream;
-  for (const auto& [pass, mr] : {std::pair<const Args&, int>(prefix, prefix_mr), {own, own_mr}}) {
-    rc = scales != nullptr ? launch_rows<true>(mr, pass, st) : launch_rows<false>(mr, pass, st);
-    if (rc != FERRET_OK) return rc;
-  }
-  const long long rows = (long long)T * H;
-  hipLaunchKernelGGL(latent_shared_join_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, prefix, own,
-                     prefix_mr, own_mr);
-  return (int)hipGetLastError();
+                       Pages{page_table, max_pages, pages, page_size}, lens, cu_q, B, T, H, scale, causal, mr.own, out,
+                       lse, static_cast<uint8_t*>(ws) + prefix_bytes);
+  prefix.whole = own.whole = 1;
+  // Two side by side: the CUs are dealt to the passes in whole rounds of the XCDs.
+  prefix.side_by_side = plan_min(prefix.side_by_side, 2);
+  own.side_by_side = plan_min(own.side_by_side, 2);
+  return scales != nullptr ? launch_shared_rows<true>(mr.prefix, mr.own, prefix, own, (hipStream_t)stream)
+                           : launch_shared_rows<false>(mr.prefix, mr.own, prefix, own, (hipStream_t)stream);
 }

@@ -90,6 +90,19 @@ FERRET_HD LatentPlace latent_place(int block, int side) {
   return LatentPlace{block / (8 * side) * 8 + block % 8, block / 8 % side};
 }
 
+// Work-groups of kLatentUnits for the first of two lines of steps that one launch takes, each
+// dealt to units of its own, `side` work-groups to a unit: in proportion to the steps, one of the first
+// line's as long as `weight` of the second's; whole rounds of 8 units, so that a unit's
+// work-groups stay on one XCD; some for each line that has steps.
+FERRET_HD int latent_split(int first, int second, float weight, int first_side, int second_side) {
+  const int round = 8 * plan_max(first_side, second_side);
+  if (first == 0) return 0;
+  if (second == 0) return kLatentUnits;
+  const float a = weight * (float)first, share = a / (a + (float)second);
+  const int rounds = (int)(share * (float)(kLatentUnits / round) + 0.5f);
+  return round * plan_min(plan_max(rounds, 1), kLatentUnits / round - 1);
+}
+
 // A sequence that a unit's share may start in, were all alike: floor(unit * B / units),
 // without the product, which passes 32 bits from 2^23 sequences on.
 FERRET_HD int latent_near(int unit, int units, int B) { return unit * (B / units) + unit * (B % units) / units; }

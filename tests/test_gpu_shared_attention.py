@@ -150,6 +150,25 @@ def test_large_scores(ops):
         Shared([(400, [(300, 2), (20, 1)])], 16, 64, e4m3, 8, std=8.0).run(ops)
 
 
+@pytest.mark.parametrize("H,tokens", [(16, 1), (64, 1), (16, 9)])
+def test_latents_past_448(ops, H, tokens):
+    """Exponent bytes above 127 in some rows and blocks of 128 latents, in prefix and own keys."""
+    print(f"[case] shared large latents H={H} tokens={tokens}", flush=True)
+    s = Shared([(200, [(90, tokens), (40, tokens)])], H, 16, True, 20)
+    scales = s.batch.cache.scales.view(-1, 4)
+    rng = np.random.default_rng(21)
+    byte = scales.cpu().numpy()
+    for line, slots in enumerate(s.batch.slots):
+        pick = rng.random((len(slots), 4)) < 0.1
+        more = rng.integers(1, 7, (len(slots), 4)) * pick
+        byte[slots] += more.astype(np.uint8)
+        s.batch.lat[line] = s.batch.lat[line] * np.repeat(np.exp2(more), 128, axis=1)
+    assert (byte > 127).any()
+    scales.copy_(torch.from_numpy(byte))
+    s.ql = s.ql * 2.0 ** -9
+    s.run(ops)
+
+
 @pytest.mark.parametrize("e4m3", [False, True])
 def test_unseen_rows_do_not_reach(ops, e4m3):
     """NaN in every slot that no key has, pages' ends among them."""
