@@ -42,6 +42,7 @@
 #include "attention.hpp"
 #include "latent.hpp"
 
+#include <algorithm>
 #include <initializer_list>
 #include <type_traits>
 
@@ -1341,10 +1342,13 @@ __device__ __forceinline__ float quad_add(float v) {
 // stand, and CB blocks of 16 columns.  PW waves take every PW-th four pieces each, eight
 // loads under way, with the weights of four pieces in the lanes, one per g, and meet in LDS.
 // TWO: every row; else those of tiles that were cut.
+template <int PW>
+constexpr int join_blocks() { return PW >= 8 ? 1 : 2; }
 template <bool TWO, int PW>
 __global__ __launch_bounds__(64 * (PW > 4 ? PW : 4)) void latent_join_kernel(Args prefix, Args own, int prefix_mr,
                                                                           int own_mr, int rows) {
-  constexpr int CB = 2, AHEAD = 4, WAVES = PW > 4 ? PW : 4, TILES = WAVES / PW;  // units of 16 rows x CB blocks per work-group
+  constexpr int CB = join_blocks<PW>(), QUADS = 2 / CB, AHEAD = 4 * QUADS;
+  constexpr int WAVES = PW > 4 ? PW : 4, TILES = WAVES / PW;  // units of 16 rows x CB blocks per work-group
   __shared__ f32x4 red[PW > 1 ? WAVES : 1][CB][64];
   __shared__ float2 red_ml[PW > 1 ? WAVES : 1][16];
   const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6, pw = wave % PW;
@@ -1384,9 +1388,18 @@ __global__ __launch_bounds__(64 * (PW > 4 ? PW : 4)) void latent_join_kernel(Arg
     }
   };
   load(pw * AHEAD);  // under the maxima
-  float2 v = stat(pw * AHEAD + g);
-  float top = v.x;
-  for (int j = (pw + PW) * AHEAD; j < most; j += PW * AHEAD) top = fmaxf(top, stat(j + g).x);
+  float2 v[QUADS];
+  const auto stats = [&](int j0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < QUADS; ++q) v[q] = stat(j0 + 4 * q + g);
+  };
+  stats(pw * AHEAD);
+  float top = -INFINITY;
+#pragma unroll
+  for (int q = 0; q < QUADS; ++q) top = fmaxf(top, v[q].x);
+  for (int j = (pw + PW) * AHEAD; j < most; j += PW * AHEAD)
+#pragma unroll
+    for (int q = 0; q < QUADS; ++q) top = fmaxf(top, stat(j + 4 * q + g).x);
   top = quad_max(top);
   const float base = top == -INFINITY ? 0.f : top;
   f32x4 acc[CB];
@@ -1398,16 +1411,19 @@ __global__ __launch_bounds__(64 * (PW > 4 ? PW : 4)) void latent_join_kernel(Arg
   for (int j = pw * AHEAD; j < most; j += PW * AHEAD) {
     if (j > pw * AHEAD) {
       load(j);
-      v = stat(j + g);
+      stats(j);
     }
-    const float w = __builtin_amdgcn_exp2f(v.x - base);
-    if (v.y != 0.f) sum += v.y * w;
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      const float wi = __shfl(w, (lane & 15) + 16 * i, 64);
-      if (mine && j + i < n) {
+    for (int q = 0; q < QUADS; ++q) {
+      const float w = __builtin_amdgcn_exp2f(v[q].x - base);
+      if (v[q].y != 0.f) sum += v[q].y * w;
 #pragma unroll
-        for (int c = 0; c < CB; ++c) acc[c] += x[i][c] * wi;
+      for (int i = 0; i < 4; ++i) {
+        const float wi = __shfl(w, (lane & 15) + 16 * i, 64);
+        if (mine && j + 4 * q + i < n) {
+#pragma unroll
+          for (int c = 0; c < CB; ++c) acc[c] += x[4 * q + i][c] * wi;
+        }
       }
     }
   }
@@ -1446,17 +1462,26 @@ __global__ __launch_bounds__(64 * (PW > 4 ? PW : 4)) void latent_join_kernel(Arg
 template <bool TWO, int PW>
 int launch_join(const Args& prefix, const Args& own, int prefix_mr, int own_mr, hipStream_t st) {
   constexpr int WAVES = PW > 4 ? PW : 4, TILES = WAVES / PW;
-  const long long rows = (long long)own.T * own.H, units = (rows + 15) / 16 * 16;
+  const long long rows = (long long)own.T * own.H, units = (rows + 15) / 16 * (32 / join_blocks<PW>());
   hipLaunchKernelGGL((latent_join_kernel<TWO, PW>), dim3((unsigned)((units + TILES - 1) / TILES)), dim3(64 * WAVES), 0, st,
                      prefix, own, prefix_mr, own_mr, (int)rows);
   return (int)hipGetLastError();
 }
 
-// Waves for the pieces of a row, by how many it has where all work-groups are at few rows.
+// Waves for the pieces of a row, by how many it has at most: all work-groups at the rows
+// there are, a step each at least.  Us, whole call, with 1 / 4 / 8 / 16 waves: 16 heads, e4m3,
+// one sequence of 100001 (256 pieces) - / - / 29.7 / 28.0; 128 heads, four of 9831 (32) - / 34.2 /
+// 34.1 / 38.9; 64 sequences behind 8192 keys (16 + 4) 50.7 / 49.2 / - / 58.5; 128 heads, 32
+// behind 6001 (8) 86 / 91 / - / -.
+long long most_pieces(const Args& a, int mr) {
+  const long long dealt = (long long)kUnits * mr / ((long long)a.T * a.H);
+  return std::min<long long>(dealt, (long long)a.pages.max_pages * a.pages.page_size / kKeys + 1);
+}
 template <bool TWO>
 int pick_join(const Args& prefix, const Args& own, int prefix_mr, int own_mr, hipStream_t st) {
-  const long long pieces = (long long)kUnits * (own_mr + (TWO ? prefix_mr : 0)) / ((long long)own.T * own.H);
-  if (pieces >= 32) return launch_join<TWO, 16>(prefix, own, prefix_mr, own_mr, st);
+  const long long pieces = most_pieces(own, own_mr) + (TWO ? most_pieces(prefix, prefix_mr) : 0);
+  if (pieces >= 200) return launch_join<TWO, 16>(prefix, own, prefix_mr, own_mr, st);
+  if (pieces >= 24) return launch_join<TWO, 8>(prefix, own, prefix_mr, own_mr, st);
   if (pieces >= 10) return launch_join<TWO, 4>(prefix, own, prefix_mr, own_mr, st);
   return launch_join<TWO, 1>(prefix, own, prefix_mr, own_mr, st);
 }
