@@ -245,23 +245,27 @@ int ferret_int8_run(const ferret::i8::Plan& plan, ferret::i8::Args p, hipStream_
 
 using namespace ferret;
 
-static bool int8_shape(int M, int N, int K) {
-  return M >= 1 && N >= 8 && N % 8 == 0 && K >= 16 && K <= 65536 && K % 16 == 0 && (long long)M * N < (1LL << 40);
+// False where the shape is refused.
+static bool int8_plan(int M, int N, int K, i8::Plan* plan) {
+  if (M < 1 || M >= 1 << 22 || N < 8 || N >= 1 << 22 || N % 8 != 0 || K < 16 || K > 65536 || K % 16 != 0) return false;
+  *plan = i8::plan(M, N, K);
+  // a launch holds less than 2^32 threads, 512 at most to a work-group
+  return i8::cdiv(N, i8::kTiles[plan->tile].rows) * plan->tok_tiles * plan->splits < 1 << 23;
 }
 
 extern "C" size_t ferret_int8_gemm_workspace(int M, int N, int K) {
-  if (!int8_shape(M, N, K)) return 0;
-  return i8::workspace(i8::plan(M, N, K), M, N);
+  i8::Plan plan;
+  return int8_plan(M, N, K, &plan) ? i8::workspace(plan, M, N) : 0;
 }
 
 extern "C" int ferret_int8_gemm(const void* a, const float* sa, const void* b, const float* sb, const void* residual,
                                 void* y, int M, int N, int K, void* ws, size_t ws_bytes, void* stream) {
   FERRET_REQUIRE(a && sa && b && sb && y, FERRET_ERR_NULL);
-  FERRET_REQUIRE(int8_shape(M, N, K), FERRET_ERR_SHAPE);
+  i8::Plan plan;
+  FERRET_REQUIRE(int8_plan(M, N, K, &plan), FERRET_ERR_SHAPE);
   const auto bits = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
   FERRET_REQUIRE(((bits(a) | bits(b) | bits(sb) | bits(residual) | bits(y)) & 15) == 0 && (bits(sa) & 3) == 0,
                  FERRET_ERR_ALIGN);
-  const i8::Plan plan = i8::plan(M, N, K);
   const size_t need = i8::workspace(plan, M, N);
   FERRET_REQUIRE(need == 0 || (ws != nullptr && ws_bytes >= need && (bits(ws) & 15) == 0), FERRET_ERR_WORKSPACE);
   const uint64_t m = M, n = N, k = K;

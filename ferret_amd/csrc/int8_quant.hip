@@ -103,7 +103,7 @@ using namespace ferret;
 extern "C" int ferret_quant_act_int8(const void* x, long long x_stride, int M, int K, void* q, float* scale,
                                      void* stream) {
   FERRET_REQUIRE(x != nullptr && q != nullptr && scale != nullptr, FERRET_ERR_NULL);
-  FERRET_REQUIRE(M >= 1 && K >= 16 && K <= 32768 && K % 16 == 0, FERRET_ERR_SHAPE);
+  FERRET_REQUIRE(M >= 1 && M < (1 << 22) && K >= 16 && K <= 32768 && K % 16 == 0, FERRET_ERR_SHAPE);  // 2^32 threads
   FERRET_REQUIRE(M == 1 || (x_stride >= K && x_stride < (1LL << 40)), FERRET_ERR_SHAPE);
   const auto bits = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
   FERRET_REQUIRE((bits(x) & 15) == 0 && (bits(q) & 15) == 0 && (bits(scale) & 3) == 0 && (M == 1 || x_stride % 8 == 0),

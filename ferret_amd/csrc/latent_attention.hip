@@ -1662,7 +1662,7 @@ extern "C" int ferret_latent_attention(const void* q_latent, long long ql_token,
 }
 
 extern "C" size_t ferret_latent_attention_shared_workspace(int G, int B, int T, int H) {
-  if (G < 1 || B < 1 || T < 1 || H < 1 || (long long)T * H + 16LL * (G > B ? G : B) >= (1LL << 31)) return 0;
+  if (G < 1 || B < 1 || T < 1 || H < 1 || (long long)T * H >= (1LL << 26) || (G > B ? G : B) >= 1 << 26) return 0;
   const SharedTiles mr = shared_tiles(G, B, T, H, 1LL << 31);  // the larger ones
   return ((pass_bytes(G, T, H, mr.prefix, 1) + 255) & ~(size_t)255) + pass_bytes(B, T, H, mr.own, 1);
 }
@@ -1679,7 +1679,7 @@ extern "C" int ferret_latent_attention_shared(const void* q_latent, long long ql
   int rc = ferret_check_pages(prefix_table, G, max_prefix_pages, pages, page_size);
   if (rc == FERRET_OK) rc = ferret_check_pages(page_table, B, max_pages, pages, page_size);
   if (rc != FERRET_OK) return rc;
-  FERRET_REQUIRE(T >= 1 && H >= 1 && H <= 1024 && (long long)T * H < (1LL << 31), FERRET_ERR_SHAPE);
+  FERRET_REQUIRE(T >= 1 && H >= 1 && H <= 1024 && (long long)T * H < (1LL << 26), FERRET_ERR_SHAPE);  // 2^32 threads
   FERRET_REQUIRE(scale > 0.f && scale < 1e30f, FERRET_ERR_SHAPE);
   for (const long long stride : {ql_token, ql_head, qr_token, qr_head})
     FERRET_REQUIRE(stride >= 0 && stride < (1LL << 31), FERRET_ERR_SHAPE);

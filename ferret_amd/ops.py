@@ -420,7 +420,7 @@ def quant_act_int8(x: torch.Tensor, q: torch.Tensor | None = None, scale: torch.
 
     The activations of int8_gemm.  x may be a row slice of a wider tensor (not expanded rows); a row
     with an Inf or NaN gets zeros and the scale NaN, so that its products are NaN.  K % 16 == 0,
-    K <= 32768; outputs overlap neither each other nor x.
+    K <= 32768, M < 2^22; outputs overlap neither each other nor x.
     """
     r = _lib.native().quant_act_int8(x, q, scale)
     if r is not None:
@@ -453,7 +453,7 @@ def int8_gemm(a: torch.Tensor, sa: torch.Tensor, b: torch.Tensor, sb: torch.Tens
 
     The whole sum is exact, then fp32 and one rounding to bf16: a token's result has the same
     bits whatever else is in the call.  Tokens from quant_act_int8, weights quantised the same way once at load.
-    N % 8 == 0, K % 16 == 0, K <= 65536.  `workspace` of int8_gemm_workspace_bytes is taken from
+    N % 8 == 0, K % 16 == 0, K <= 65536, M and N < 2^22.  `workspace` of int8_gemm_workspace_bytes is taken from
     torch's caching allocator unless one is passed; calls that overlap in time (streams, graphs) need
     one each.  `out` may be the residual itself and overlaps nothing else.
     """
@@ -827,7 +827,7 @@ def latent_attention_shared(q_latent: torch.Tensor, q_rotary: torch.Tensor, cach
     it see no prefix, and a prefix may be empty.  A prefix is read and multiplied once for all its
     tokens.  Index tensors stay on the device (a captured call replays with other lengths);
     `workspace` of latent_attention_shared_workspace_bytes, `out`, tokens that see no key and rows behind the
-    last sequence as in latent_attention.
+    last sequence as in latent_attention.  T * H < 2^26.
     """
     _latent_cache(cache)
     r = _lib.native().latent_attention_shared(q_latent, q_rotary, cache.data, cache.scales, prefix_table, prefix_lens,

@@ -274,8 +274,8 @@ int ferret_moe_combine(const void* o, const float* w, int T, int topk, int N, vo
  * x [M,K] with rows x_stride elements apart (a multiple of 8, K or more), q int8 [M,K]
  * packed, scale f32 [M].  A row with an Inf or NaN gets zeros and the scale NaN.  Outputs
  * overlap nothing.  The reference has no 8-bit integer path; this and the product below
- * are the library's own contract.  Requirements: M >= 1, K % 16 == 0, 16 <= K <= 32768;
- * x and q on 16-byte bounds (FERRET_ERR_ALIGN).
+ * are the library's own contract.  Requirements: 1 <= M < 2^22, K % 16 == 0, 16 <= K <=
+ * 32768; x and q on 16-byte bounds (FERRET_ERR_ALIGN).
  */
 int ferret_quant_act_int8(const void* x, long long x_stride, int M, int K, void* q, float* scale, void* stream);
 
@@ -287,8 +287,8 @@ int ferret_quant_act_int8(const void* x, long long x_stride, int M, int K, void*
  * to fp32.  So the same bits come out whatever the other tokens of the call, and for
  * every workspace.  ws: ferret_int8_gemm_workspace(M, N, K) bytes on a 16-byte bound (0:
  * none, may be NULL); calls that overlap in time need one each.  y may be residual itself and
- * overlaps nothing else.  Requirements: M >= 1, N >= 8, N % 8 == 0, 16 <= K <= 65536, K %
- * 16 == 0, M * N < 2^40; pointers but sa on 16-byte bounds (FERRET_ERR_ALIGN).
+ * overlaps nothing else.  Requirements: 1 <= M < 2^22, 8 <= N < 2^22, N % 8 == 0, 16 <= K <= 65536,
+ * K % 16 == 0, no more than 2^23 tiles; pointers but sa on 16-byte bounds (FERRET_ERR_ALIGN).
  */
 size_t ferret_int8_gemm_workspace(int M, int N, int K);
 int ferret_int8_gemm(const void* a, const float* sa, const void* b, const float* sb, const void* residual, void* y,
@@ -399,7 +399,7 @@ int ferret_latent_attention(const void* q_latent, long long ql_token, long long 
  * its sequences, which stand side by side); tokens outside [cu_prefix[0], cu_prefix[G]) see
  * no prefix.  Both tables are of the one cache.  Everything else, the softmax's statement, out in
  * place, lse, tokens without keys, Inf and NaN, and the range of the sums, as
- * ferret_latent_attention; requirements for both tables.
+ * ferret_latent_attention; its requirements for both tables, and T * H < 2^26.
  * ws: ferret_latent_attention_shared_workspace(G, B, T, H) bytes, on a 16-byte bound.
  */
 size_t ferret_latent_attention_shared_workspace(int G, int B, int T, int H);

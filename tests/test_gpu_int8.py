@@ -235,3 +235,25 @@ def test_native_and_python_paths_agree(hip, monkeypatch):
     there = [*ops.quant_act_int8(x), ops.int8_gemm(*case)]
     for u, v in zip(here, there):
         assert u.dtype == v.dtype and torch.equal(u.view(torch.uint8), v.view(torch.uint8))
+
+
+def test_offsets_past_32_bits(hip):
+    """Tokens and weights of more than 2^32 bytes: the last rows as they are alone."""
+    print("[case] int8 far rows", flush=True)
+    K, far = 32768, 140000
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.zeros((far, K), dtype=torch.bfloat16, device="cuda")
+    x[-70:] = torch.randn((70, K), generator=g, device="cuda").to(torch.bfloat16)
+    q, s = ops.quant_act_int8(x)
+    few = x[-70:].clone()
+    del x
+    tq, ts = ops.quant_act_int8(few)
+    check_quant(few.float().cpu().numpy(), tq, ts)
+    assert torch.equal(q[-70:], tq) and torch.equal(s[-70:], ts) and not q[:-70].any()
+    w, ws = ops.quant_act_int8(torch.randn((72, K), generator=g, device="cuda").to(torch.bfloat16))
+    want = I.product(*(t.cpu().numpy() for t in (tq, ts, w, ws)))
+    assert np.array_equal(bits(ops.int8_gemm(q, s, w, ws)[-70:]), want)
+    for M in (1, 70):       # q as weights
+        y = ops.int8_gemm(w[:M].contiguous(), ws[:M].contiguous(), q, s)
+        assert np.array_equal(bits(y)[:, -70:], I.product(*(t.cpu().numpy() for t in (w[:M], ws[:M], tq, ts))))
+        assert not y[:, :-70].any()

@@ -314,3 +314,41 @@ def test_another_stream_and_captured_replays(ops):
         torch.cuda.synchronize()
         batch[i].check(*out)
         assert torch.equal(out[0], eager[i][0]) and torch.equal(out[1], eager[i][1]), i
+
+
+def test_rows_past_32_bits_of_the_cache(ops):
+    """The last pages of a cache of 9 GB: the bits of the small one."""
+    print("[case] shared far pages", flush=True)
+    for e4m3, H in ((True, 16), (False, 16), (True, 64), (False, 64)):
+        s = Shared([(300, [(30, 1), (65, 4)])], H, 16, e4m3, 22)
+        want, want_lse = s.call(ops)
+        small = s.batch.cache
+        pages = 9 * 2 ** 30 // (small.data.stride(0) * small.data.element_size())
+        far, gap = ops.LatentCache.empty(pages, 16, small.data.dtype if not e4m3 else torch.float8_e4m3fn), pages - s.batch.pages
+        far.data[gap:] = small.data
+        if e4m3:
+            far.scales[gap:] = small.scales
+        kw = s.index()
+        for name in ("prefix_table", "page_table"):
+            kw[name] = torch.where(kw[name] >= 0, kw[name] + gap, kw[name])
+        out, lse = ops.latent_attention_shared(bf16_tensor(s.ql), bf16_tensor(s.qr), far, **kw, scale=SCALE, return_lse=True)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse), (e4m3, H)
+        del far
+
+
+def test_two_calls_at_once(ops):
+    """Two streams, each with calls of its own in flight."""
+    print("[case] shared on two streams", flush=True)
+    both = [Shared([(3000, [(500, 1), (70, 2)])], 16, 64, True, 23), Shared([(900, [(20, 1)] * 9)], 64, 16, False, 24)]
+    want = [s.call(ops) for s in both]
+    args = [(bf16_tensor(s.ql), bf16_tensor(s.qr), s.batch.cache, s.index()) for s in both]
+    streams = [torch.cuda.Stream() for _ in both]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, (ql, qr, cache, kw) in enumerate(args):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(ops.latent_attention_shared(ql, qr, cache, **kw, scale=SCALE, return_lse=True))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        assert all(torch.equal(o, want[i][0]) and torch.equal(l, want[i][1]) for o, l in got[i]), i

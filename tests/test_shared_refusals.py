@@ -72,6 +72,20 @@ def test_shared(L):
         (26, X + 1024, -2), (25, O + 64, -2)])
 
 
+def test_sizes_past_a_launch(L):
+    """Rows, tiles and query rows whose launch would pass 2^32 threads."""
+    far = 1 << 45  # no range ends in another
+    assert L.ferret_quant_act_int8(P, 64, 1 << 22, 64, far, 2 * far, None) == -2
+    for m, n in ((1 << 22, 64), (64, 1 << 22), ((1 << 22) - 8, (1 << 22) - 8)):
+        assert L.ferret_int8_gemm_workspace(m, n, 64) == 0
+        assert L.ferret_int8_gemm(P, far, 2 * far, 3 * far, None, 4 * far, m, n, 64, None, 0, None) == -2
+    T, ws = 1 << 20, L.ferret_latent_attention_shared_workspace
+    assert ws(1, 1, T, 64) == 0 and ws(1, 1, T - 1, 64) > 0 and ws(1, 1 << 26, 1, 1) == 0
+    assert L.ferret_latent_attention_shared(
+        P, 64 * 512, 512, far, 64 * 64, 64, 2 * far, None, 100, 64, 3 * far, 3 * far + 512, 3 * far + 1024, 1, 8,
+        3 * far + 1536, 3 * far + 2048, 3 * far + 2560, 1, 8, T, 64, 0.07, 1, 4 * far, None, 5 * far, far, None) == -2
+
+
 def test_python_names_what_is_wrong():
     from ferret_amd import ops
     x = torch.zeros((2, 128), dtype=torch.bfloat16)
