@@ -14,26 +14,41 @@
 // work-group finds its piece by itself from lens and cu_q: no host read, so the
 // call can be captured into a graph and replayed with other lengths.
 //
-// Up to 32 rows per tile (latent_attention_kernel), a step: the 64 cached rows come into
+// Up to 32 rows per tile (attend_narrow), a step: the 64 cached rows come into
 // LDS by asynchronous loads, once for key and value.  S^T = K Q^T is dealt to the waves
 // by queries (WQ) and keys (WK), with the keys as MFMA rows, so that a lane holds the
 // scores of one query; its softmax terms go through LDS as bf16, and for O^T = V^T P^T
 // every wave takes all queries and a share of the 512 columns.  So no product is done
 // twice and a row is read from LDS WQ times as key and once as value; the output tile
 // stays in registers.  V^T is read with the transposing LDS loads (ds_read_b64_tr):
-// 16 columns by key.  64 rows (latent_attention_wide_kernel): scores and output are
-// done by waves of their own, side by side.
+// 16 columns by key.  64 rows (attend_wide): scores and output are done by waves of their
+// own, side by side.
 // e4m3 rows stay e4m3 in LDS.  Keys are widened and scaled in one instruction (exact);
 // values are widened unscaled, and each probability is multiplied by its key's power
 // of two instead, before (16 and 32 rows: one copy of P per block of 128 columns) or
 // after (64 rows) it is rounded to bf16: exact, so nothing is lost by it.
 //
+// Shared prefixes, where a sequence's rows fill a tile of 64 or the prefix is short
+// (latent_prefixed_kernel): the prefix's keys stand before the sequence's own on one line, which
+// starts a step anew where they begin.  One pass as without a prefix; the tokens of a prefix
+// share its rows in the caches, and there is nothing more to share in the products.
+// Where the rows of a sequence fill no tile and the prefix is long (latent_shared_kernel): the
+// softmax of a row over a prefix and its own keys is the join of two softmaxes, so the prefix is a
+// sequence like any other whose rows are all of its tokens' heads, in full tiles: 64 sequences of 16
+// heads take a quarter of the steps.  One launch takes both lines, dealt to work-groups of their
+// own; every tile, whole or cut, leaves partials, and one join takes a row's pieces of both.
+//
 // What bounds it.  16 heads, one token: the cache's bytes; 64 sequences of 600 to 8000
 // keys, e4m3, 49 us, 3.6 TB/s with launch and joins, of which the kernel takes 45.  64
-// rows: no one unit.  32 sequences of 8192, 128 heads, bf16, 100 us: the matrix units
+// rows: no one unit.  32 sequences of 8192, 128 heads, bf16, 98 us: the matrix units
 // are busy for 40% of the cycles, LDS for 27%, the vector units for 20%, and memory
-// delivers 3.0 TB/s; the clock falls to 2.0 GHz under it.  e4m3, 92 us: the vector
-// units take 39%, widening the keys twice and the values once, beside 40% of products.
+// delivers 3.0 TB/s; the clock falls to 2.0 GHz under it.  e4m3: the vector units take 39%,
+// widening the keys twice and the values once, beside 40% of products.  Chunks of 60 to 300 tokens
+// behind a prefix of 5000 keys, 16 heads, e4m3, 168 us: without half of the output's products 22
+// less, without the widening 9, the exponentials 5, the loads 5, or the powers of two on P 10: a step is
+// the chain of all of them.  64 sequences of 100 to 1200 behind 8192 shared keys, 16 heads, e4m3, 49 us:
+// 10 until the first product (lengths, deal, page table and first rows are loads one after another),
+// eight steps of 2, 33 MB of partials out, and a join of 8 that reads 40 MB.
 //
 // Numerics: S, m, l and O are fp32; P is rounded to bf16 for the MFMA (half a step,
 // 2^-8 relative, random over the keys), l sums the unrounded P.  The running
@@ -61,6 +76,9 @@ struct Args {
   const uint32_t* scales;
   Pages pages;
   const int32_t *lens, *cu_q;
+  // Prefixed kernels: the pages of each prefix, of `pages`'s size, its keys and its tokens.
+  const int32_t *prefix_table, *prefix_lens, *cu_prefix;
+  int prefixes, max_prefix_pages;
   int B, T, H;
   float scale_log2;  // scale * log2(e)
   int causal;
@@ -86,10 +104,32 @@ struct Args {
   __host__ __device__ float* part(int mr) const { return reinterpret_cast<float*>(ml() + (size_t)blocks(mr) * 16); }
 };
 
-template <int MR>
-__device__ __forceinline__ LatentSeq sequence(const Args& a, int b) {
-  return latent_seq(a.cu_q[b], a.cu_q[b + 1], a.lens[b], a.T, a.H, MR, a.side_by_side,
-                    a.pages.max_pages * a.pages.page_size);
+// The prefix of a sequence: its line of the table and its keys.  The sequence's own keys
+// follow on the next whole step.
+struct Prefix {
+  int line, keys;
+  __device__ __forceinline__ int base() const { return latent_base(keys); }
+};
+__device__ __forceinline__ Prefix prefix_of(const Args& a, int q0) {
+  int at = 0, end = a.prefixes;  // the last prefix of at .. end - 1 that starts at q0 or before
+  while (end - at > 1) {
+    const int half = (at + end) / 2;
+    if (a.cu_prefix[half] <= q0) at = half;
+    else end = half;
+  }
+  const bool in = a.cu_prefix[0] <= q0 && q0 < a.cu_prefix[a.prefixes];
+  return Prefix{at, in ? min(max(a.prefix_lens[at], 0), a.max_prefix_pages * a.pages.page_size) : 0};
+}
+
+template <int MR, bool PRE>
+__device__ __forceinline__ LatentSeq sequence(const Args& a, int b, Prefix* prefix) {
+  LatentSeq s = latent_seq(a.cu_q[b], a.cu_q[b + 1], a.lens[b], a.T, a.H, MR, a.side_by_side,
+                           a.pages.max_pages * a.pages.page_size);
+  if constexpr (PRE) {
+    *prefix = prefix_of(a, s.q0);
+    latent_behind(&s, prefix->keys);
+  }
+  return s;
 }
 
 template <bool F8>
@@ -111,10 +151,19 @@ struct Side {
   int chunk, extra;      // the deal
   int seq_at, b;         // the sequence at hand and its place on the line
   LatentSeq seq;
+  Prefix prefix;         // of a prefixed kernel's sequence
   int first_row;         // the tile's first row among all [T * H]
   int block;             // of the partial result, -1 for a whole tile that goes to `out`
   int end;               // of this work-group's share of the line
 };
+
+// HIDDEN: its address in a vector register, or the compiler keeps those of all its fields in scalar ones.
+template <bool HIDDEN>
+__device__ __forceinline__ Side* side_at(uint8_t* lds) {
+  FERRET_LDS Side* at = (FERRET_LDS Side*)lds;
+  if constexpr (HIDDEN) asm("" : "+v"(at));
+  return (Side*)at;
+}
 
 // By fields: a struct's copy would stand in scratch memory.
 __device__ __forceinline__ void put_seq(LatentSeq* to, const LatentSeq& s) {
@@ -203,17 +252,19 @@ __device__ __forceinline__ int swz(int r) { return (((r >> 1) ^ r) & 4) | (r & 2
 
 // The start of a work-group's share of the line: false where it has none.  The page
 // table's first lines come under the loads of the lengths.  tot: 24 words of LDS.
-template <int MR, int NT>
+template <int MR, int NT, bool PRE>
 __device__ __forceinline__ bool take_share(const Args& a, int units, LatentPlace place, Side* side, int* tot, int* cur) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int near =
       a.pages.table[(long long)latent_near(place.unit, units, a.B) * a.pages.max_pages];
+  const int near_prefix = PRE ? a.prefix_table[(threadIdx.x & 31) % a.max_prefix_pages] : 0;
   const int per = (a.B + NT - 1) / NT;
   const int b0 = threadIdx.x * per;
   LatentSeq s{};
+  Prefix prefix{0, 0};
   int mine = 0, my_groups = 0;
   for (int i = 0; i < per && b0 + i < a.B; ++i) {
-    s = sequence<MR>(a, b0 + i);
+    s = sequence<MR, PRE>(a, b0 + i, &prefix);
     mine = latent_add(mine, s.work(0));
     my_groups = latent_add(my_groups, s.groups);
   }
@@ -232,7 +283,7 @@ __device__ __forceinline__ bool take_share(const Args& a, int units, LatentPlace
     tot[NW + wave] = incl_groups;
   }
   __syncthreads();
-  asm volatile("" ::"v"(near));
+  asm volatile("" ::"v"(near), "v"(near_prefix));
   int before = 0, all = 0, groups_before = 0, groups = 0;
 #pragma unroll
   for (int w = 0; w < NW; ++w) {
@@ -263,17 +314,21 @@ __device__ __forceinline__ bool take_share(const Args& a, int units, LatentPlace
     int at = excl, i = 0;
     if (per > 1)
       for (;; ++i) {
-        s = sequence<MR>(a, b0 + i);
+        s = sequence<MR, PRE>(a, b0 + i, &prefix);
         if (start < at + s.work(extra) || i + 1 == per) break;
         at += s.work(extra);
       }
     side->b = b0 + i;
     put_seq(&side->seq, s);
+    if constexpr (PRE) {
+      side->prefix.line = prefix.line;
+      side->prefix.keys = prefix.keys;
+    }
     side->seq_at = at;
     side->chunk = chunk;
     side->extra = extra;
     side->end = min(start + chunk, total);
-    put_args(&side->args, a);
+    if constexpr (!PRE) put_args(&side->args, a);  // else `a` stands there
   }
   *cur = uniform(start);
   __syncthreads();
@@ -286,20 +341,26 @@ struct Piece {
   bool one;               // the sequence has one new token
   int row0, row_last;     // query rows of the sequence
   int see_all, see_any;   // keys that the first and the last token of the tile see
+  // Prefixed kernels, in vector registers: the prefix, its keys, and the first of the sequence's own.
+  int line, prefix, base;
+  int gap;  // the prefix's keys where keys that nobody sees follow in its last step, else below 0
+  __device__ __forceinline__ bool ends_in(int t, int keys) const { return (unsigned)(gap - t * keys) < (unsigned)keys; }
 };
 
 // The piece at `cur`, its place noted in LDS and its rows' record in the workspace;
 // false where there are no keys (the extra steps) or no rows (fewer tiles than
 // work-groups side by side).
-template <int MR>
+template <int MR, bool PRE>
 __device__ __forceinline__ bool next_piece(LatentPlace place, Side* side, int cur, Piece* p) {
   const Args& in = side->args;
   const int extra = side->extra;
   int b = uniform(side->b), seq_at = uniform(side->seq_at);
   LatentSeq s = get_seq(&side->seq);
+  Prefix prefix{0, 0};
+  if constexpr (PRE) prefix = Prefix{side->prefix.line, side->prefix.keys};
   while (cur >= seq_at + s.work(extra) && b + 1 < in.B) {  // the next sequence with rows
     seq_at += s.work(extra);
-    s = sequence<MR>(in, ++b);
+    s = sequence<MR, PRE>(in, ++b, &prefix);
   }
   p->b = b = uniform(b);
   p->len = uniform(s.len);
@@ -312,35 +373,58 @@ __device__ __forceinline__ bool next_piece(LatentPlace place, Side* side, int cu
   p->row_last = uniform(min(p->row0 + MR, s.rows) - 1);
   if (p->row_last < p->row0 || p->s0 >= steps) return false;
   p->past = p->len - n + 1;
+  p->line = prefix.line;
+  p->prefix = prefix.keys;
+  p->base = prefix.base();
+  p->gap = PRE ? uniform(p->prefix < p->base ? p->prefix : -1) : -1;
+  // Used at the piece's ends and where a step has keys to clear: not in scalar registers where they are short.
+  if constexpr (PRE) asm("" : "+v"(p->line), "+v"(p->prefix), "+v"(p->base));
   const bool causal = in.causal && n > 1;  // one token sees all
-  p->see_all = causal ? uniform(max(p->past + p->row0 / in.H, 0)) : p->len;
-  p->see_any = causal ? uniform(max(p->past + p->row_last / in.H, 0)) : p->len;
+  p->see_all = uniform(causal ? max(p->past + p->row0 / in.H, p->base) : p->len);
+  p->see_any = uniform(causal ? max(p->past + p->row_last / in.H, p->base) : p->len);
   p->one = n == 1;
   const int chunk = side->chunk, first_row = p->q0 * in.H + p->row0;
+  const int rows_last = p->row_last - p->row0;
   // A whole tile's place: sequences start on a block of their own.
   const int whole = 2 * kUnits * (MR / 16) + (p->q0 * in.H >> 4) + b + (p->row0 >> 4);
   __syncthreads();  // the piece before is done with its record and buffers
   if (threadIdx.x == 0) {
     side->b = b;
     put_seq(&side->seq, s);
+    if constexpr (PRE) {
+      side->prefix.line = prefix.line;
+      side->prefix.keys = prefix.keys;
+    }
     side->seq_at = seq_at;
     side->first_row = first_row;
     side->block = p->s0 == 0 && p->s1 >= steps
                       ? (in.whole ? whole : -1)
                       : latent_slot(place.unit, place.lane, in.side_by_side, cur, chunk) * (MR / 16);
   }
-  if (p->s0 == 0 && (int)threadIdx.x <= p->row_last - p->row0) {
+  if (p->s0 == 0 && (int)threadIdx.x <= rows_last) {
     const LatentRecord r = latent_record(place.unit, place.lane, in.side_by_side, cur, steps, chunk);
     in.rows()[first_row + threadIdx.x] = make_int4(r.pieces == 1 ? whole : r.slot0 * (MR / 16), r.pieces, threadIdx.x, 0);
   }
+  if constexpr (PRE || MR == 32) asm("" : "+v"(p->row0), "+v"(p->row_last), "+v"(p->q0), "+v"(p->b));
   return true;
 }
 
 // Where 16-row block `block` (of the sequence) of the wave's lanes stands in the cache, in
 // units of 16 rows, -1 where it has no page.
-__device__ __forceinline__ int find_block(const Pages& pages, const int32_t* table, int block) {
-  const int pos = block * 16, page = pos / pages.page_size;
-  const int id = pos >= 0 && page < pages.max_pages ? table[page] : -1;
+template <bool PRE>
+__device__ __forceinline__ int find_block(const Args& in, const Piece& p, const int32_t* table, int block) {
+  const Pages& pages = in.pages;
+  int pos = block * 16, max_pages = pages.max_pages;
+  bool there = pos >= 0;
+  if constexpr (PRE) {
+    const bool prefix = pos < p.base;
+    there = there && (!prefix || pos < p.prefix);
+    max_pages = prefix ? in.max_prefix_pages : max_pages;
+    table = (prefix ? in.prefix_table : pages.table) + (long long)(prefix ? p.line : p.b) * max_pages;
+    pos -= prefix ? 0 : p.base;
+  }
+  const int page = pos / pages.page_size;
+  const int id = there && page < max_pages ? table[page] : -1;
   const long long row = page_row(id, pages.pages, pages.page_size, pos - page * pages.page_size);
   return row < 0 ? -1 : (int)(row >> 4);
 }
@@ -355,7 +439,7 @@ __device__ __forceinline__ int get_queries(const Args& in, const Piece& p, int r
   for (int k = 0; k < 16; ++k) qf[k] = ld_u32x4(ql + (F8 ? 64 * (k >> 1) + 16 * g + 8 * (k & 1) : 32 * k + 8 * g));
 #pragma unroll
   for (int k = 0; k < 2; ++k) qf[16 + k] = ld_u32x4(qr + 32 * k + 8 * g);
-  return r <= p.row_last ? max(in.causal ? p.past + tok : p.len, 0) : 0;
+  return r <= p.row_last ? max(in.causal ? p.past + tok : p.len, p.base) : 0;
 }
 
 // Inf and NaN among 16 bytes of values become zeros.
@@ -383,18 +467,18 @@ __device__ __forceinline__ u32x4 only_finite(u32x4 v) {
 // a key of bf16 latents with an Inf may score -inf and have no weight, and 0 * Inf makes
 // that column NaN in the steps that all queries see: so it does here.
 template <bool F8, int STEP, int CT, int WQ>
-__device__ __forceinline__ void clear_unseen(const Args& in, const Piece& p, uint8_t* buf, int first, uint32_t ok,
-                                             int chunk, f32x4 (&o)[CT][WQ]) {
+__device__ __forceinline__ void clear_unseen(const Args& in, const Piece& p, int see_all, int see_any, uint8_t* buf,
+                                             int first, uint32_t ok, int chunk, f32x4 (&o)[CT][WQ]) {
   constexpr int VC = F8 ? CT : 2 * CT, ROW = F8 ? kRowE4m3 : kRowBf16;
   const int lane = threadIdx.x & 63, r16 = lane & 15, g = lane >> 4;
   const auto place = [&](int r, int c) { return buf + r * ROW + (((chunk + c) ^ swz(r)) << 4); };
   // Every row seen by all or by none: a loop of its own where scalar registers are left for it
   // (128 heads, bf16, 32 sequences of 900 to 6000: 58.5 us, 59.3 without).
-  if (WQ == 4 && p.see_all >= p.see_any) {
+  if (WQ == 4 && see_all >= see_any) {
 #pragma unroll 1
     for (int i0 = 0; i0 < STEP * VC; i0 += 64) {
       const int r = (i0 + lane) / VC;
-      if (first + r >= p.see_any || !((ok >> (8 * (r >> 4))) & 1))
+      if (first + r >= see_any || !((ok >> (8 * (r >> 4))) & 1))
         *reinterpret_cast<u32x4*>(place(r, lane % VC)) = u32x4{0u, 0u, 0u, 0u};
     }
     return;
@@ -402,11 +486,11 @@ __device__ __forceinline__ void clear_unseen(const Args& in, const Piece& p, uin
 #pragma unroll 1
   for (int i0 = 0; i0 < STEP * VC; i0 += 64) {
     const int r = (i0 + lane) / VC, key = first + r;
-    const bool none = key >= p.see_any || !((ok >> (8 * (r >> 4))) & 1), some = !none && key >= p.see_all;
+    const bool none = key >= see_any || !((ok >> (8 * (r >> 4))) & 1), some = !none && key >= see_all;
     u32x4* const at = reinterpret_cast<u32x4*>(place(r, lane % VC));
     u32x4 x = {0u, 0u, 0u, 0u}, fine = x;
     if (some) fine = only_finite<F8>(x = *at);
-    if (!F8 && p.see_all < p.see_any) {
+    if (!F8 && see_all < see_any) {
       const bool bad = x[0] != fine[0] || x[1] != fine[1] || x[2] != fine[2] || x[3] != fine[3];
       for (unsigned long long rest = __ballot(bad); rest != 0;) {
         const int first_bad = __ffsll((long long)rest) - 1, row = (i0 + first_bad) / VC;
@@ -467,7 +551,7 @@ __device__ __forceinline__ void put_rows(const Side* side, const Piece& p, int f
 
 // WQ x WK waves: 16 queries x 64 / WK keys each for the scores, all queries x
 // 512 / (WQ WK) columns for the output.
-template <int WQ, int WK, bool F8, typename Cache>
+template <int WQ, int WK, bool F8, bool PRE, typename Cache>
 __device__ __forceinline__ void attend_narrow(const Args& a, Cache cache, int units, LatentPlace place, uint8_t* lds) {
   using L = Tile<F8>;
   constexpr int MR = 16 * WQ, NW = WQ * WK, NT = 64 * NW;
@@ -479,10 +563,10 @@ __device__ __forceinline__ void attend_narrow(const Args& a, Cache cache, int un
   const int r16 = lane & 15, g = lane >> 4;
   const int wq = wave / WK, wk = wave % WK;
   float* const tops = reinterpret_cast<float*>(lds + M::kTop);
-  Side* const side = reinterpret_cast<Side*>(lds + M::kSide);
+  Side* const side = side_at<PRE>(lds + M::kSide);
 
   int cur;
-  if (!take_share<MR, NT>(a, units, place, side, reinterpret_cast<int*>(lds), &cur)) return;
+  if (!take_share<MR, NT, PRE>(a, units, place, side, reinterpret_cast<int*>(lds), &cur)) return;
   const Args& in = side->args;
   float scale_log2 = a.scale_log2;
   asm("" : "+v"(scale_log2));  // not in a scalar register
@@ -497,7 +581,7 @@ __device__ __forceinline__ void attend_narrow(const Args& a, Cache cache, int un
 
   while (cur < uniform(side->end)) {
     Piece pc;
-    const bool there = next_piece<MR>(place, side, cur, &pc);
+    const bool there = next_piece<MR, PRE>(place, side, cur, &pc);
     const int s0 = pc.s0, see_all = pc.see_all, see_any = pc.see_any;
     cur += pc.s1 - s0;
     if (!there) continue;
@@ -512,10 +596,10 @@ __device__ __forceinline__ void attend_narrow(const Args& a, Cache cache, int un
 
     // The page table, 64 steps at a time: lane i holds where the 16 rows stand that the
     // wave loads from (RG groups of 8 of them) in step held + i.
-    const int32_t* table = in.pages.table + (long long)pc.b * in.pages.max_pages;
+    const int32_t* table = PRE ? nullptr : in.pages.table + (long long)pc.b * in.pages.max_pages;
     int held = s0, where;
     const auto look_up = [&]() __attribute__((always_inline)) {
-      where = find_block(in.pages, table, min(held + lane, last - 1) * (kKeys / 16) + wave * RG / 2);
+      where = find_block<PRE>(in, pc, table, min(held + lane, last - 1) * (kKeys / 16) + wave * RG / 2);
     };
     look_up();
 
@@ -627,8 +711,10 @@ __device__ __forceinline__ void attend_narrow(const Args& a, Cache cache, int un
 
       // ---- masks: only where the step passes what some row sees, or misses a page
       const uint32_t ok = uniform(*reinterpret_cast<const uint32_t*>(lds + M::kValid + (t % L::kBufs) * 4));
-      if ((t + 1) * kKeys > see_all || ok != 0x01010101u) {
-        const int left = sees - (t * kKeys + wk * KT * 16 + 4 * g);
+      const bool gap = PRE && pc.ends_in(t, kKeys);
+      if ((t + 1) * kKeys > see_all || ok != 0x01010101u || gap) {
+        const int all = gap ? pc.gap : see_all, any = gap ? pc.gap : see_any;
+        const int left = (gap ? min(sees, pc.gap) : sees) - (t * kKeys + wk * KT * 16 + 4 * g);
 #pragma unroll
         for (int k = 0; k < KT; ++k) {
           const int upto = (ok >> (8 * (wk * KT + k))) & 1 ? left - k * 16 : 0;
@@ -636,11 +722,11 @@ __device__ __forceinline__ void attend_narrow(const Args& a, Cache cache, int un
           for (int i = 0; i < 4; ++i) sc[k][i] = i < upto ? sc[k][i] : -INFINITY;
         }
         lds_barrier();  // the keys have been read
-        clear_unseen<F8, kKeys>(in, pc, buf, t * kKeys, ok, wave * CT * (F8 ? 1 : 2), o);
+        clear_unseen<F8, kKeys>(in, pc, all, any, buf, t * kKeys, ok, wave * CT * (F8 ? 1 : 2), o);
         if constexpr (F8) {
           if (threadIdx.x < kKeys) {
             const int r = threadIdx.x;
-            if (t * kKeys + r >= see_any || !((ok >> (8 * (r >> 4))) & 1))
+            if (t * kKeys + r >= any || !((ok >> (8 * (r >> 4))) & 1))
               reinterpret_cast<uint32_t*>(buf + L::kData)[r] = 0x7f7f7f7fu;
           }
           lds_barrier();  // the scale words are read next
@@ -809,7 +895,7 @@ static_assert(Wide<true>::kLds <= 160 * 1024 && Wide<false>::kLds <= 160 * 1024,
 // to the output (64 queries x 128 columns each) and load the keys to come: the matrix
 // unit is fed by one while the other is at its softmax, at a barrier or at its loads,
 // and neither holds more than half of the registers (Q is 144, O 128 of 256).
-template <bool F8, typename Cache>
+template <bool F8, bool PRE, typename Cache>
 __device__ __forceinline__ void attend_wide(const Args& a, Cache cache, int units, LatentPlace place, uint8_t* lds) {
   using L = Tile<F8>;
   using M = Wide<F8>;
@@ -818,12 +904,12 @@ __device__ __forceinline__ void attend_wide(const Args& a, Cache cache, int unit
   const int r16 = lane & 15, g = lane >> 4;
   float* const tops = reinterpret_cast<float*>(lds + M::kTop);
   float* const fin = reinterpret_cast<float*>(lds + M::kFin);
-  Side* const side = reinterpret_cast<Side*>(lds + M::kSide);
+  Side* const side = side_at<PRE>(lds + M::kSide);
   // P of a query: chunk c of 8 keys stands at c ^ swz_p(query)
   const int zp = M::kStep == 64 ? r16 >> 1 : r16 >> 2;
 
   int cur;
-  if (!take_share<MR, 512>(a, units, place, side, reinterpret_cast<int*>(lds), &cur)) return;
+  if (!take_share<MR, 512, PRE>(a, units, place, side, reinterpret_cast<int*>(lds), &cur)) return;
   const Args& in = side->args;
   float scale_log2 = a.scale_log2;
   asm("" : "+v"(scale_log2));  // not in a scalar register
@@ -833,7 +919,7 @@ __device__ __forceinline__ void attend_wide(const Args& a, Cache cache, int unit
     const int wq = wave >> 1, wk = wave & 1;
     while (cur < uniform(side->end)) {
       Piece pc;
-      const bool there = next_piece<MR>(place, side, cur, &pc);
+      const bool there = next_piece<MR, PRE>(place, side, cur, &pc);
       cur += pc.s1 - pc.s0;
       if (!there) continue;
       const int u0 = pc.s0 * (64 / M::kStep);
@@ -946,12 +1032,14 @@ __device__ __forceinline__ void attend_wide(const Args& a, Cache cache, int unit
 
         // ---- masks: only where the step passes what some row sees, or misses a page
         const uint32_t have = (uint32_t)uniform(valid) >> (8 * wk * KT);
-        if ((u + 1) * M::kStep > pc.see_all || (have & (KT == 2 ? 0x0101u : 1u)) != (KT == 2 ? 0x0101u : 1u)) {
+        const bool gap = PRE && pc.ends_in(u, M::kStep);
+        if ((u + 1) * M::kStep > pc.see_all || gap || (have & (KT == 2 ? 0x0101u : 1u)) != (KT == 2 ? 0x0101u : 1u)) {
 #pragma unroll
           for (int f = 0; f < 2; ++f)
 #pragma unroll
             for (int k = 0; k < KT; ++k) {
-              const int upto = (have >> (8 * k)) & 1 ? sees[f] - (u * M::kStep + (wk * KT + k) * 16 + 4 * g) : 0;
+              const int seen = gap ? min(sees[f], pc.gap) : sees[f];
+              const int upto = (have >> (8 * k)) & 1 ? seen - (u * M::kStep + (wk * KT + k) * 16 + 4 * g) : 0;
 #pragma unroll
               for (int i = 0; i < 4; ++i) sc[k][f][i] = i < upto ? sc[k][f][i] : -INFINITY;
             }
@@ -995,17 +1083,17 @@ __device__ __forceinline__ void attend_wide(const Args& a, Cache cache, int unit
     }
     while (cur < uniform(side->end)) {
       Piece pc;
-      const bool there = next_piece<MR>(place, side, cur, &pc);
+      const bool there = next_piece<MR, PRE>(place, side, cur, &pc);
       cur += pc.s1 - pc.s0;
       if (!there) continue;
       const int u0 = pc.s0 * (64 / M::kStep);
       const int end = min(pc.s1 * (64 / M::kStep), (pc.see_any + M::kStep - 1) / M::kStep);
 
       // Where the wave's 16-row block stands in steps held .. held + 63, a lane each.
-      const int32_t* table = in.pages.table + (long long)pc.b * in.pages.max_pages;
+      const int32_t* table = PRE ? nullptr : in.pages.table + (long long)pc.b * in.pages.max_pages;
       int held = u0, where;
       const auto look_up = [&]() __attribute__((always_inline)) {
-        where = find_block(in.pages, table, min(held + lane, end - 1) * (M::kStep / 16) + w * RG / 2);
+        where = find_block<PRE>(in, pc, table, min(held + lane, end - 1) * (M::kStep / 16) + w * RG / 2);
       };
       look_up();
       const uint8_t* src;
@@ -1102,9 +1190,10 @@ __device__ __forceinline__ void attend_wide(const Args& a, Cache cache, int unit
         uint8_t* buf = lds + buffer * M::kBytes;
         constexpr uint32_t kAll = M::kStep == 64 ? 0x01010101u : 0x0101u;
         const uint32_t ok = (uint32_t)uniform(valid) & kAll;
-        const bool edge = (v + 1) * M::kStep > pc.see_all || ok != kAll;
+        const bool gap = PRE && pc.ends_in(v, M::kStep);
+        const bool edge = (v + 1) * M::kStep > pc.see_all || ok != kAll || gap;
         if (edge) {
-          clear_unseen<F8, M::kStep>(in, pc, buf, v * M::kStep, ok, w * (F8 ? 8 : 16), o);
+          clear_unseen<F8, M::kStep>(in, pc, gap ? pc.gap : pc.see_all, gap ? pc.gap : pc.see_any, buf, v * M::kStep, ok, w * (F8 ? 8 : 16), o);
           asm volatile("" ::: "memory");
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -1129,8 +1218,8 @@ __device__ __forceinline__ void attend_wide(const Args& a, Cache cache, int unit
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) ring[i] = frag(i);
         // e4m3: a probability takes its key's power of two for the wave's columns, by adding
-        // to the exponents of two at a time: 121.5 us for chunks of 200 and 500 tokens on 3500
-        // and 5000 keys, 125.7 by widening, two products and rounding.  Exact for normal numbers; a
+        // to the exponents of two at a time: 118 us for chunks of 200 and 500 tokens on 3500
+        // and 5000 keys, 122 by widening, two products and rounding.  Exact for normal numbers; a
         // product below 2^-126 becomes some number below 2^-126.  Zeros stay zeros (P is zero
         // or normal): a key that a query does not see, or whose term vanished, may have any scale.
         // Powers up to 2^0, latents up to 448, take one saturating subtraction.
@@ -1215,48 +1304,75 @@ __device__ __forceinline__ void attend_wide(const Args& a, Cache cache, int unit
 template <int MR>
 constexpr int tile_threads() { return MR == 16 ? 256 : 512; }
 template <int MR, bool F8>
+constexpr int tile_side() { return MR == kWideRows ? Wide<F8>::kSide : Lds<MR, 4, F8>::kSide; }
+template <int MR, bool F8>
 constexpr int tile_lds() { return MR == kWideRows ? Wide<F8>::kLds : Lds<MR, 4, F8>::kBytes; }
 
-template <int MR, bool F8, typename Cache>
+template <int MR, bool F8, bool PRE, typename Cache>
 __device__ __forceinline__ void attend(const Args& a, Cache cache, int units, LatentPlace place, uint8_t* lds) {
-  if constexpr (MR == kWideRows) attend_wide<F8>(a, cache, units, place, lds);
-  else attend_narrow<MR / 16, 4, F8>(a, cache, units, place, lds);
+  if constexpr (MR == kWideRows) attend_wide<F8, PRE>(a, cache, units, place, lds);
+  else attend_narrow<MR / 16, 4, F8, PRE>(a, cache, units, place, lds);
 }
 
+// N words of the kernel's arguments into LDS.
+template <int N>
+__device__ __forceinline__ void args_to_lds(void* to) {
+  const auto from = (const __attribute__((address_space(4))) int*)__builtin_amdgcn_kernarg_segment_ptr();
+  if (threadIdx.x < N) static_cast<int*>(to)[threadIdx.x] = from[threadIdx.x];
+  __syncthreads();
+}
+
+// One pass over the rows' keys.
 template <int MR, bool F8>
 __global__ __launch_bounds__(tile_threads<MR>(), tile_threads<MR>() / 256) void latent_attention_kernel(Args a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   using C = std::conditional_t<MR == 32, CacheLate, Cache>;
-  attend<MR, F8>(a, C(a), kUnits / a.side_by_side, latent_place(blockIdx.x, a.side_by_side), lds);
+  LatentPlace place = latent_place(blockIdx.x, a.side_by_side);
+  if constexpr (MR == 32) asm("" : "+v"(place.unit), "+v"(place.lane));
+  attend<MR, F8, false>(a, C(a), kUnits / a.side_by_side, place, lds);
+}
+
+// One pass, the keys of a sequence's prefix before its own.  The arguments are read through
+// LDS: in scalar registers they would leave too few.
+template <int MR, bool F8>
+__global__ __launch_bounds__(tile_threads<MR>(), tile_threads<MR>() / 256) void latent_prefixed_kernel(Args args) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  Side* const side = reinterpret_cast<Side*>(lds + tile_side<MR, F8>());
+  args_to_lds<sizeof(Args) / 4>(&side->args);
+  const Args& a = side->args;
+  const int lanes = uniform(a.side_by_side);
+  LatentPlace place = latent_place(blockIdx.x, lanes);
+  asm("" : "+v"(place.unit), "+v"(place.lane));
+  using C = std::conditional_t<MR == 32, CacheLate, Cache>;
+  attend<MR, F8, true>(a, C(args), kUnits / lanes, place, lds);
 }
 
 // Two passes over the rows' keys in one launch: work-groups of their own for the shared
-// prefixes, in tiles of MRP rows, and for the sequences' own keys, in tiles of MRO.  Every
+// prefixes, in tiles of 64 rows, and for the sequences' own keys, in tiles of MRO.  Every
 // work-group deals the CUs to the two by the steps of each, one of the prefix's as long as
 // `weight` of the own, and finds the same numbers.  The arguments of both passes are read
 // through LDS: in scalar registers they would leave too few.
-template <int MRP, int MRO, bool F8>
+template <int MRO, bool F8>
 struct Shared {
-  static_assert(MRP >= MRO, "threads");
-  static constexpr int kThreads = tile_threads<MRP>();
-  static constexpr int kArgs =
-      ((tile_lds<MRP, F8>() > tile_lds<MRO, F8>() ? tile_lds<MRP, F8>() : tile_lds<MRO, F8>()) + 15) & ~15;
-  static constexpr int kLds = kArgs + 2 * sizeof(Args);
+  static_assert(MRO < kWideRows, "tiles");
+  static constexpr int kThreads = tile_threads<kWideRows>();
+  static constexpr int kOwn = tile_lds<MRO, F8>(), kPrefix = tile_lds<kWideRows, F8>();
+  static constexpr int kArgs = ((kOwn > kPrefix ? kOwn : kPrefix) + 15) & ~15;
+  static constexpr int kLds = kArgs + 2 * sizeof(Args) + 8;  // and the weight
   static_assert(kLds <= 160 * 1024, "LDS of a CU");
 };
-template <int MRP, int MRO, bool F8>
-__global__ __launch_bounds__(tile_threads<MRP>(), tile_threads<MRP>() / 256) void latent_shared_kernel(Args, Args, float) {
-  using S = Shared<MRP, MRO, F8>;
+template <int MRO, bool F8>
+__global__ __launch_bounds__(tile_threads<kWideRows>(), tile_threads<kWideRows>() / 256) void latent_shared_kernel(Args, Args,
+                                                                                                                float) {
+  using S = Shared<MRO, F8>;
   constexpr int NT = S::kThreads, NW = NT / 64, WORDS = (2 * sizeof(Args) + 4) / 4;
   static_assert(sizeof(Args) % 8 == 0 && WORDS <= NT, "arguments");
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   int* const tot = reinterpret_cast<int*>(lds);
   const Args* const both = reinterpret_cast<const Args*>(lds + S::kArgs);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const auto kernarg = (const __attribute__((address_space(4))) int*)__builtin_amdgcn_kernarg_segment_ptr();
-  if (threadIdx.x < WORDS - 1) reinterpret_cast<int*>(lds + S::kArgs)[threadIdx.x] = kernarg[threadIdx.x];
-  const float weight = __int_as_float(kernarg[WORDS - 1]);
-  __syncthreads();
+  args_to_lds<WORDS>(lds + S::kArgs);
+  const float weight = __int_as_float(uniform(reinterpret_cast<const int*>(lds + S::kArgs)[WORDS - 1]));
   int near = 0;  // the page tables' lines come under the loads of the lengths
   if (threadIdx.x < 2) {
     const Args& a = both[threadIdx.x];
@@ -1264,9 +1380,9 @@ __global__ __launch_bounds__(tile_threads<MRP>(), tile_threads<MRP>() / 256) voi
   }
   int steps[2] = {0, 0};
   for (int b = threadIdx.x; b < both[0].B; b += NT)
-    steps[0] = latent_add(steps[0], sequence<MRP>(both[0], b).work(kLatentExtra));
+    steps[0] = latent_add(steps[0], sequence<kWideRows, false>(both[0], b, nullptr).work(kLatentExtra));
   for (int b = threadIdx.x; b < both[1].B; b += NT)
-    steps[1] = latent_add(steps[1], sequence<MRO>(both[1], b).work(kLatentExtra));
+    steps[1] = latent_add(steps[1], sequence<MRO, false>(both[1], b, nullptr).work(kLatentExtra));
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
 #pragma unroll
@@ -1288,11 +1404,11 @@ __global__ __launch_bounds__(tile_threads<MRP>(), tile_threads<MRP>() / 256) voi
   const int side = uniform(a.side_by_side), units = (first ? groups : kUnits - groups) / side;
   LatentPlace place = latent_place(first ? blockIdx.x : blockIdx.x - groups, side);
   asm("" : "+v"(place.unit), "+v"(place.lane));  // used between tiles only: not in scalar registers
-  if (MRO == MRP || first) {
-    attend<MRP, F8>(a, CacheLate(a), units, place, lds);
+  if (first) {
+    attend<kWideRows, F8, false>(a, CacheLate(a), units, place, lds);
   } else {
-    if (MRO < MRP && (int)threadIdx.x >= tile_threads<MRO>()) return;
-    attend<MRO, F8>(a, CacheLate(a), units, place, lds);
+    if ((int)threadIdx.x >= tile_threads<MRO>()) return;
+    attend<MRO, F8, false>(a, CacheLate(a), units, place, lds);
   }
 }
 
@@ -1471,11 +1587,11 @@ int launch_join(const Args& prefix, const Args& own, int prefix_mr, int own_mr, 
 // Waves for the pieces of a row, by how many it has at most: all work-groups at the rows
 // there are, a step each at least.  Us, whole call, with 1 / 4 / 8 / 16 waves: 16 heads, e4m3,
 // one sequence of 100001 (256 pieces) - / - / 29.7 / 28.0; 128 heads, four of 9831 (32) - / 34.2 /
-// 34.1 / 38.9; 64 sequences behind 8192 keys (16 + 4) 50.7 / 49.2 / - / 58.5; 128 heads, 32
-// behind 6001 (8) 86 / 91 / - / -.
+// 34.1 / 38.9; 64 sequences behind 8192 keys (16 + 4) 50.7 / 49.2 / - / 58.5.
 long long most_pieces(const Args& a, int mr) {
   const long long dealt = (long long)kUnits * mr / ((long long)a.T * a.H);
-  return std::min<long long>(dealt, (long long)a.pages.max_pages * a.pages.page_size / kKeys + 1);
+  const long long table = (long long)a.pages.max_pages + (a.prefix_table != nullptr ? a.max_prefix_pages : 0);
+  return std::min<long long>(dealt, table * a.pages.page_size / kKeys + 1);
 }
 template <bool TWO>
 int pick_join(const Args& prefix, const Args& own, int prefix_mr, int own_mr, hipStream_t st) {
@@ -1486,11 +1602,11 @@ int pick_join(const Args& prefix, const Args& own, int prefix_mr, int own_mr, hi
   return launch_join<TWO, 1>(prefix, own, prefix_mr, own_mr, st);
 }
 
-template <int MR, bool F8>
+template <int MR, bool F8, void (*kernel)(Args)>
 int launch(const Args& a, hipStream_t st) {
   constexpr int lds = tile_lds<MR, F8>();
-  FERRET_HIP_CHECK((set_lds_limit_once<latent_attention_kernel<MR, F8>>(lds)));
-  hipLaunchKernelGGL((latent_attention_kernel<MR, F8>), dim3(kUnits), dim3(tile_threads<MR>()), lds, st, a);
+  FERRET_HIP_CHECK((set_lds_limit_once<kernel>(lds)));
+  hipLaunchKernelGGL(kernel, dim3(kUnits), dim3(tile_threads<MR>()), lds, st, a);
   FERRET_HIP_CHECK(hipGetLastError());
   return pick_join<false>(a, a, MR, MR, st);
 }
@@ -1498,31 +1614,34 @@ int launch(const Args& a, hipStream_t st) {
 template <bool F8>
 int launch_rows(int mr, const Args& a, hipStream_t st) {
   switch (mr) {
-    case 16: return launch<16, F8>(a, st);
-    case 32: return launch<32, F8>(a, st);
-    default: return launch<kWideRows, F8>(a, st);
+    case 16: return launch<16, F8, latent_attention_kernel<16, F8>>(a, st);
+    case 32: return launch<32, F8, latent_attention_kernel<32, F8>>(a, st);
+    default: return launch<kWideRows, F8, latent_attention_kernel<kWideRows, F8>>(a, st);
   }
 }
 
-template <int MRP, int MRO, bool F8>
+template <bool F8>
+int launch_prefixed(int mr, const Args& a, hipStream_t st) {
+  switch (mr) {
+    case 16: return launch<16, F8, latent_prefixed_kernel<16, F8>>(a, st);
+    case 32: return launch<32, F8, latent_prefixed_kernel<32, F8>>(a, st);
+    default: return launch<kWideRows, F8, latent_prefixed_kernel<kWideRows, F8>>(a, st);
+  }
+}
+
+template <int MRO, bool F8>
 int launch_shared(const Args& prefix, const Args& own, hipStream_t st) {
-  using S = Shared<MRP, MRO, F8>;
-  // What a step of the prefix's tiles takes of one of the own.
-  constexpr float weight = MRP == MRO ? 1.f : MRO == 32 ? 2.f : 3.f;
-  FERRET_HIP_CHECK((set_lds_limit_once<latent_shared_kernel<MRP, MRO, F8>>(S::kLds)));
-  hipLaunchKernelGGL((latent_shared_kernel<MRP, MRO, F8>), dim3(kUnits), dim3(S::kThreads), S::kLds, st, prefix, own,
-                     weight);
+  using S = Shared<MRO, F8>;
+  constexpr float weight = MRO == 32 ? 2.f : 3.f;  // what a step of the prefix's tiles takes of one of the own
+  FERRET_HIP_CHECK((set_lds_limit_once<latent_shared_kernel<MRO, F8>>(S::kLds)));
+  hipLaunchKernelGGL((latent_shared_kernel<MRO, F8>), dim3(kUnits), dim3(S::kThreads), S::kLds, st, prefix, own, weight);
   FERRET_HIP_CHECK(hipGetLastError());
-  return pick_join<true>(prefix, own, MRP, MRO, st);
+  return pick_join<true>(prefix, own, kWideRows, MRO, st);
 }
 
 template <bool F8>
-int launch_shared_rows(int prefix_mr, int own_mr, const Args& prefix, const Args& own, hipStream_t st) {
-  if (prefix_mr == 16) return launch_shared<16, 16, F8>(prefix, own, st);
-  if (prefix_mr == 32) return launch_shared<32, 32, F8>(prefix, own, st);
-  if (own_mr == 16) return launch_shared<kWideRows, 16, F8>(prefix, own, st);
-  if (own_mr == 32) return launch_shared<kWideRows, 32, F8>(prefix, own, st);
-  return launch_shared<kWideRows, kWideRows, F8>(prefix, own, st);
+int launch_shared_rows(int own_mr, const Args& prefix, const Args& own, hipStream_t st) {
+  return own_mr == 16 ? launch_shared<16, F8>(prefix, own, st) : launch_shared<32, F8>(prefix, own, st);
 }
 
 // Query rows per tile by the rows that a sequence has on average.  Us, e4m3, 64 sequences
@@ -1545,10 +1664,10 @@ int side_by_side(int T, int B, int H) {
 
 // Steps of a whole batch are counted in 32 bits, rounded up to whole shares; a step's
 // end stays below 2^31.
-int check_steps(int B, int max_pages, int pages, int page_size, int T, int H, int mr) {
-  FERRET_REQUIRE((long long)max_pages * page_size <= (1LL << 31) - 2 * kKeys, FERRET_ERR_SHAPE);
+int check_steps(int B, long long keys, int pages, int page_size, int T, int H, int mr) {
+  FERRET_REQUIRE(keys <= (1LL << 31) - 2 * kKeys, FERRET_ERR_SHAPE);
   FERRET_REQUIRE((long long)pages * page_size < (1LL << 35), FERRET_ERR_SHAPE);
-  const long long tiles = (long long)T * H / mr + B, most = ((long long)max_pages * page_size + kKeys - 1) / kKeys + kLatentExtra;
+  const long long tiles = (long long)T * H / mr + B, most = (keys + kKeys - 1) / kKeys + kLatentExtra;
   FERRET_REQUIRE(tiles * most < (1LL << 31) - kUnits, FERRET_ERR_SHAPE);
   return FERRET_OK;
 }
@@ -1570,6 +1689,8 @@ Args pass_args(const void* q_latent, long long ql_token, long long ql_head, cons
   a.pages = pages;
   a.lens = lens;
   a.cu_q = cu_q;
+  a.prefix_table = a.prefix_lens = a.cu_prefix = nullptr;
+  a.prefixes = a.max_prefix_pages = 0;
   a.B = B;
   a.T = T;
   a.H = H;
@@ -1597,17 +1718,18 @@ size_t pass_bytes(int B, int T, int H, int mr, int whole) {
   return rows + (size_t)a.blocks(mr) * 16 * (sizeof(float2) + kLatent * sizeof(float));
 }
 
-// Tiles of the two passes of shared prefixes: as one pass has them, the prefix's at least
-// the own's, and as small as those where that is little work: at most keys of
-// the table.
-struct SharedTiles {
-  int prefix, own;
-};
-SharedTiles shared_tiles(int G, int B, int T, int H, long long keys) {
-  const int own = tile_rows(T, B, H), prefix = tile_rows(T, G, H), most = prefix > own ? prefix : own;
-  if (prefix <= 32) return {most, most};
+// Whether prefixes of `keys` keys at most get a pass of their own: where a sequence fills no
+// tile of 64 rows but a prefix's tokens do, and the steps that the sequences would else take over
+// their prefixes are more than ten per CU, so that the quarter or half of them that is left
+// makes up for the partials of every row.  Us, two passes / one: 16 heads, 64 sequences behind 8192
+// keys, e4m3 49 / 69 (8192 steps), 8 prompts of 600 to 3500 with 8 samples each, bf16 33.8 / 37.6
+// (3500), 64 behind 2000 34.1 / 33.7 (2000), 16 behind 8192 34.2 / 30.1 (2000); 32 heads, 64 behind
+// 8192 73 / 88, behind 2000 44.8 / 42.9; 64 heads, 64 behind 2000 59 / 49; 128 heads, 32 behind
+// 6001, bf16 84 / 78.
+bool prefix_pass(int G, int B, int T, int H, long long keys) {
+  const int own = tile_rows(T, B, H);
   const long long steps = ((long long)T * H + own - 1) / own * ((keys + kKeys - 1) / kKeys);
-  return steps < 4 * kUnits ? SharedTiles{own, own} : SharedTiles{most, own};
+  return own < kWideRows && tile_rows(T, G, H) == kWideRows && steps >= 10 * kUnits;
 }
 
 }  // namespace
@@ -1640,7 +1762,7 @@ extern "C" int ferret_latent_attention(const void* q_latent, long long ql_token,
                      ((bits(scales) | bits(lse)) & 3) == 0 && ((ql_token | ql_head | qr_token | qr_head) & 7) == 0,
                  FERRET_ERR_ALIGN);
   const int mr = tile_rows(T, B, H);
-  const int steps = check_steps(B, max_pages, pages, page_size, T, H, mr);
+  const int steps = check_steps(B, (long long)max_pages * page_size, pages, page_size, T, H, mr);
   if (steps != FERRET_OK) return steps;
   const size_t need = ferret_latent_attention_workspace(B, T, H);
   FERRET_REQUIRE(ws != nullptr && ws_bytes >= need && (bits(ws) & 15) == 0, FERRET_ERR_WORKSPACE);
@@ -1663,8 +1785,10 @@ extern "C" int ferret_latent_attention(const void* q_latent, long long ql_token,
 
 extern "C" size_t ferret_latent_attention_shared_workspace(int G, int B, int T, int H) {
   if (G < 1 || B < 1 || T < 1 || H < 1 || (long long)T * H >= (1LL << 26) || (G > B ? G : B) >= 1 << 26) return 0;
-  const SharedTiles mr = shared_tiles(G, B, T, H, 1LL << 31);  // the larger ones
-  return ((pass_bytes(G, T, H, mr.prefix, 1) + 255) & ~(size_t)255) + pass_bytes(B, T, H, mr.own, 1);
+  const int own = tile_rows(T, B, H);
+  if (!prefix_pass(G, B, T, H, 1LL << 31)) return pass_bytes(B, T, H, own, 0);
+  // A call with shorter tables takes one pass, and less.
+  return ((pass_bytes(G, T, H, kWideRows, 1) + 255) & ~(size_t)255) + pass_bytes(B, T, H, own, 1);
 }
 
 extern "C" int ferret_latent_attention_shared(const void* q_latent, long long ql_token, long long ql_head,
@@ -1687,14 +1811,18 @@ extern "C" int ferret_latent_attention_shared(const void* q_latent, long long ql
   FERRET_REQUIRE(((bits(q_latent) | bits(q_rotary) | bits(data) | bits(out)) & 15) == 0 &&
                      ((bits(scales) | bits(lse)) & 3) == 0 && ((ql_token | ql_head | qr_token | qr_head) & 7) == 0,
                  FERRET_ERR_ALIGN);
-  const SharedTiles mr = shared_tiles(G, B, T, H, (long long)max_prefix_pages * page_size);
-  rc = check_steps(G, max_prefix_pages, pages, page_size, T, H, mr.prefix);
-  if (rc == FERRET_OK) rc = check_steps(B, max_pages, pages, page_size, T, H, mr.own);
+  const int own_mr = tile_rows(T, B, H);
+  const bool two = prefix_pass(G, B, T, H, (long long)max_prefix_pages * page_size);
+  FERRET_REQUIRE(((long long)max_pages + max_prefix_pages) * page_size <= (1LL << 31) - 4 * kKeys, FERRET_ERR_SHAPE);
+  rc = two ? check_steps(G, (long long)max_prefix_pages * page_size, pages, page_size, T, H, kWideRows) : FERRET_OK;
+  if (rc == FERRET_OK)
+    rc = check_steps(B, ((long long)max_pages + (two ? 0 : max_prefix_pages)) * page_size + (two ? 0 : kKeys), pages, page_size,
+                     T, H, own_mr);
   if (rc != FERRET_OK) return rc;
   const size_t need = ferret_latent_attention_shared_workspace(G, B, T, H);
   FERRET_REQUIRE(need != 0, FERRET_ERR_SHAPE);
   FERRET_REQUIRE(ws != nullptr && ws_bytes >= need && (bits(ws) & 15) == 0, FERRET_ERR_WORKSPACE);
-  // In place is sound: `out` is written by the join alone.
+  // In place is sound: in one pass as there, and in two `out` is written by the join alone.
   const bool over = in_place(out, q_latent, T, ql_token, H, ql_head, kLatent);
   FERRET_REQUIRE(!clash({Range{out, (uint64_t)T * H * kLatent * 2}, Range{lse, (uint64_t)T * H * 4}, Range{ws, need}},
                         {bf16_range(over ? nullptr : q_latent, T, ql_token, H, ql_head, kLatent),
@@ -1704,17 +1832,25 @@ extern "C" int ferret_latent_attention_shared(const void* q_latent, long long ql
                          ints_range(cu_prefix, G + 1LL), ints_range(page_table, (uint64_t)B * max_pages),
                          ints_range(lens, B), ints_range(cu_q, B + 1LL)}),
                  FERRET_ERR_SHAPE);
-  const size_t prefix_bytes = (pass_bytes(G, T, H, mr.prefix, 1) + 255) & ~(size_t)255;
+  const size_t prefix_bytes = two ? (pass_bytes(G, T, H, kWideRows, 1) + 255) & ~(size_t)255 : 0;
+  Args own = pass_args(q_latent, ql_token, ql_head, q_rotary, qr_token, qr_head, data, scales,
+                       Pages{page_table, max_pages, pages, page_size}, lens, cu_q, B, T, H, scale, causal, own_mr, out, lse,
+                       static_cast<uint8_t*>(ws) + prefix_bytes);
+  if (!two) {
+    own.prefix_table = prefix_table;
+    own.prefix_lens = prefix_lens;
+    own.cu_prefix = cu_prefix;
+    own.prefixes = G;
+    own.max_prefix_pages = max_prefix_pages;
+    return scales != nullptr ? launch_prefixed<true>(own_mr, own, (hipStream_t)stream)
+                             : launch_prefixed<false>(own_mr, own, (hipStream_t)stream);
+  }
   Args prefix = pass_args(q_latent, ql_token, ql_head, q_rotary, qr_token, qr_head, data, scales,
                           Pages{prefix_table, max_prefix_pages, pages, page_size}, prefix_lens, cu_prefix, G, T, H,
-                          scale, 0, mr.prefix, nullptr, nullptr, ws);
-  Args own = pass_args(q_latent, ql_token, ql_head, q_rotary, qr_token, qr_head, data, scales,
-                       Pages{page_table, max_pages, pages, page_size}, lens, cu_q, B, T, H, scale, causal, mr.own, out,
-                       lse, static_cast<uint8_t*>(ws) + prefix_bytes);
+                          scale, 0, kWideRows, nullptr, nullptr, ws);
   prefix.whole = own.whole = 1;
   // Two side by side: the CUs are dealt to the passes in whole rounds of the XCDs.
   prefix.side_by_side = plan_min(prefix.side_by_side, 2);
-  own.side_by_side = plan_min(own.side_by_side, 2);
-  return scales != nullptr ? launch_shared_rows<true>(mr.prefix, mr.own, prefix, own, (hipStream_t)stream)
-                           : launch_shared_rows<false>(mr.prefix, mr.own, prefix, own, (hipStream_t)stream);
+  return scales != nullptr ? launch_shared_rows<true>(own_mr, prefix, own, (hipStream_t)stream)
+                           : launch_shared_rows<false>(own_mr, prefix, own, (hipStream_t)stream);
 }

@@ -48,6 +48,14 @@ FERRET_HD LatentSeq latent_seq(int start, int end, int len, int T, int H, int mr
   return s;
 }
 
+// A sequence whose own keys stand behind those of a prefix: on the next whole step, so that no
+// step has keys of both.
+FERRET_HD int latent_base(int prefix) { return (prefix + kLatentKeys - 1) / kLatentKeys * kLatentKeys; }
+FERRET_HD void latent_behind(LatentSeq* s, int prefix) {
+  s->len += latent_base(prefix);
+  s->steps = plan_max((s->len + kLatentKeys - 1) / kLatentKeys, 1);
+}
+
 // The line of all (sequence, group, step) is dealt in equal shares to `units` =
 // kLatentUnits / side units of `side` work-groups.  Each group is followed by `extra`
 // steps without keys, so that a unit that goes on to a second tile (its queries, and the

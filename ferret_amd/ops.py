@@ -824,8 +824,8 @@ def latent_attention_shared(q_latent: torch.Tensor, q_rotary: torch.Tensor, cach
     [G, max_prefix_pages] names, and then the keys of its own sequence as in latent_attention: page_table
     [B, max_pages], lens and cu_q count the sequences' own keys and new tokens alone.  cu_prefix int32
     [G+1] gives the packed new tokens of each prefix, whose sequences stand side by side; tokens outside
-    it see no prefix, and a prefix may be empty.  A prefix is read and multiplied once for all its
-    tokens.  Index tensors stay on the device (a captured call replays with other lengths);
+    it see no prefix, and a prefix may be empty.  A prefix is kept
+    once; where its tokens fill tiles that their sequences do not, it is multiplied once for all of them too.  Index tensors stay on the device (a captured call replays with other lengths);
     `workspace` of latent_attention_shared_workspace_bytes, `out`, tokens that see no key and rows behind the
     last sequence as in latent_attention.  T * H < 2^26.
     """

@@ -396,10 +396,11 @@ int ferret_latent_attention(const void* q_latent, long long ql_token, long long 
  * tokens included).
  * prefix_table int32 [G, max_prefix_pages], prefix_lens int32 [G] (0 for none) and
  * cu_prefix int32 [G + 1], ascending: the packed new tokens that see prefix g (all tokens of
- * its sequences, which stand side by side); tokens outside [cu_prefix[0], cu_prefix[G]) see
- * no prefix.  Both tables are of the one cache.  Everything else, the softmax's statement, out in
+ * its sequences, which stand side by side: none belongs to two); tokens outside [cu_prefix[0],
+ * cu_prefix[G]) see no prefix.  Both tables are of the one cache.  Everything else, the softmax's statement, out in
  * place, lse, tokens without keys, Inf and NaN, and the range of the sums, as
- * ferret_latent_attention; its requirements for both tables, and T * H < 2^26.
+ * ferret_latent_attention; its requirements for both tables, together (max_pages +
+ * max_prefix_pages) * page_size <= 2^31 - 256, and T * H < 2^26.
  * ws: ferret_latent_attention_shared_workspace(G, B, T, H) bytes, on a 16-byte bound.
  */
 size_t ferret_latent_attention_shared_workspace(int G, int B, int T, int H);

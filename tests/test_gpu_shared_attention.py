@@ -69,10 +69,29 @@ class Shared:
             g += p is not None
         return worst
 
+    def wide(self):
+        """The index with a prefix table wide enough that prefixes get a pass of their own, or None where the rows
+        do not: entries past the lengths are no pages."""
+        T, B = sum(self.new), len(self.own)
+        rows = T * self.H // B
+        if rows > 32 or T * self.H // self.G <= 32:
+            return None
+        tiles = -(-T * self.H // (16 if rows <= 16 else 32))
+        kw = self.index()
+        columns = -(-2560 * 64 // (tiles * self.page)) + 1
+        table = torch.full((self.G, max(columns, kw["prefix_table"].shape[1])), -1, dtype=torch.int32, device="cuda")
+        table[:, :kw["prefix_table"].shape[1]] = kw["prefix_table"]
+        return dict(kw, prefix_table=table)
+
     def run(self, ops, causal=True):
         out, lse = self.call(ops, causal=causal)
         torch.cuda.synchronize()
         print(f"    worst {self.check(out, lse, causal):.3f} of the bound", flush=True)
+        wide = self.wide()
+        if wide is not None:
+            two = self.call(ops, causal=causal, **wide)
+            torch.cuda.synchronize()
+            print(f"    worst {self.check(*two, causal):.3f} of the bound, prefixes in a pass of their own", flush=True)
         return out, lse
 
 
@@ -352,3 +371,83 @@ def test_two_calls_at_once(ops):
     torch.cuda.synchronize()
     for i in (0, 1):
         assert all(torch.equal(o, want[i][0]) and torch.equal(l, want[i][1]) for o, l in got[i]), i
+
+
+def test_a_captured_prefix_pass(ops):
+    """Prefixes in a pass of their own: replays with other lengths, missing pages and a NaN that stays with its prefix."""
+    print("[case] shared captured, prefixes apart", flush=True)
+    for e4m3 in (True, False):
+        batch = [Shared([(p, [(a, 1)] * 3 + [(b, 1)]), (q, [(c, 1)] * 5)], 16, 16, e4m3, 25)
+                 for p, q, a, b, c in ((300, 640, 30, 65, 9), (17, 0, 1, 200, 64), (5000, 1300, 64, 0, 33))]
+        columns = max(s.wide()["prefix_table"].shape[1] for s in batch)
+        own = max(s.batch.table.shape[1] for s in batch)
+        pages = max(s.batch.pages for s in batch)
+
+        def state(s):
+            kw = s.index()
+            for name, most in (("prefix_table", columns), ("page_table", own)):
+                wide = torch.full((kw[name].shape[0], most), -1, dtype=torch.int32, device="cuda")
+                wide[:, :kw[name].shape[1]] = kw[name][:, :most]
+                kw[name] = wide
+            cache = ops.LatentCache.empty(pages, 16, torch.float8_e4m3fn if e4m3 else torch.bfloat16)
+            cache.data.zero_()
+            cache.data[:s.batch.pages] = s.batch.cache.data
+            if e4m3:
+                cache.scales.fill_(127)
+                cache.scales[:s.batch.pages] = s.batch.cache.scales
+            return dict(kw, ql=bf16_tensor(s.ql), qr=bf16_tensor(s.qr), data=cache.data,
+                        **({"scales": cache.scales} if e4m3 else {}))
+        states = [state(s) for s in batch]
+        now = {k: v.clone() for k, v in states[0].items()}
+
+        def call(now):
+            kw = {k: v for k, v in now.items() if k not in ("ql", "qr", "data", "scales")}
+            return ops.latent_attention_shared(now["ql"], now["qr"], ops.LatentCache(now["data"], now.get("scales")), **kw,
+                                               scale=SCALE, return_lse=True)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            call(now)
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = call(now)
+        for i in (1, 2, 0, 2):
+            for k, v in states[i].items():
+                now[k].copy_(v)
+            g.replay()
+            want = call(states[i])
+            torch.cuda.synchronize()
+            batch[i].check(*out)
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1]), i
+        bad = dict(states[0], data=states[0]["data"].clone())
+        want = call(states[0])
+        page = int(bad["prefix_table"][1, 3])
+        if e4m3:
+            bad["data"][page, 5, 70] = 0x7f
+        else:
+            bad["data"][page, 5, 70] = float("nan")
+        got = call(bad)
+        assert torch.isnan(got[0][4:]).all() and torch.equal(got[0][:4], want[0][:4])
+        gone = dict(states[0], prefix_table=states[0]["prefix_table"].clone())
+        gone["prefix_table"][0, 2] = -1
+        got = call(gone)
+        s = batch[0]
+        keep = np.ones(300, dtype=bool)
+        keep[32:48] = False
+        s.batch.lat[0], s.batch.rot[0] = s.batch.lat[0][keep], s.batch.rot[0][keep]
+        s.groups = [(284, s.groups[0][1]), s.groups[1]]
+        s.check(*got)
+
+
+def test_workspace_of_both_ways(ops):
+    """One workspace size whatever the tables; nothing is written past it."""
+    print("[case] shared workspaces", flush=True)
+    s = Shared([(900, [(20, 1)] * 7)], 16, 16, True, 26)
+    need = ops.latent_attention_shared_workspace_bytes(1, 7, 7, 16)
+    for kw in (s.index(), s.wide()):
+        ws = torch.full((need + 256,), 0xa5, dtype=torch.uint8, device="cuda")
+        out = ops.latent_attention_shared(bf16_tensor(s.ql), bf16_tensor(s.qr), s.batch.cache, **kw, scale=SCALE,
+                                          workspace=ws)
+        again = s.call(ops, **kw)
+        assert torch.equal(out, again[0]) and (ws[need:] == 0xa5).all()
