@@ -9,7 +9,14 @@
 //
 // One pass: a row stays in the registers of the WPR waves that own it, its largest
 // value as a 15-bit pattern (unsigned maxima order Inf and NaN above all numbers).
-// HBM-bound: 2 bytes read and 1 written per element.
+// HBM-bound: 2 bytes read and 1 written per element.  8192 rows of 7168 take 29.0 us, 6.1
+// TB/s; 32 rows of 4096 2.8 us in the kernel, the launch.
+//
+// As many waves per row as leave a lane two chunks: more loads of a lane wait longer for
+// the first, fewer leave little to do between the two passes.  Us, 32 / 1000 / 8192 rows: K 4096,
+// 8 x 1 2.9 / 4.5 / 22.7, 4 x 2 3.0 / 4.1 / 20.3, 2 x 4 3.5 / 4.1 / 19.2; K 7168, 16 x 1 3.1 / 7.3 / 38.6, 8 x 2
+// 3.0 / 6.0 / 29.7, 4 x 4 3.5 / 6.6 / 32.5; K 2048, 4 x 1 2.8 / 3.5 / 13.3, 2 x 2 3.0 / 3.3 / 11.9, 1 x 4
+// 3.2 / 3.9 / 12.7.
 #include "common.hpp"
 #include "ranges.hpp"
 
@@ -116,10 +123,9 @@ extern "C" int ferret_quant_act_int8(const void* x, long long x_stride, int M, i
   const int chunks = K / 8;
   if (chunks <= 64) return launch<1, 1>(a, st);
   if (chunks <= 128) return launch<1, 2>(a, st);
-  if (chunks <= 192) return launch<1, 3>(a, st);
   if (chunks <= 256) return launch<2, 2>(a, st);
-  if (chunks <= 512) return launch<8, 1>(a, st);
+  if (chunks <= 512) return launch<4, 2>(a, st);
   if (chunks <= 1024) return launch<8, 2>(a, st);
-  if (chunks <= 2048) return launch<8, 4>(a, st);
+  if (chunks <= 2048) return launch<16, 2>(a, st);
   return launch<16, 4>(a, st);
 }
