@@ -56,6 +56,17 @@ FERRET_HD void latent_behind(LatentSeq* s, int prefix) {
   s->steps = plan_max((s->len + kLatentKeys - 1) / kLatentKeys, 1);
 }
 
+// The prefix whose tokens, starts[g] .. starts[g + 1] - 1, hold q0; -1 where none does.
+FERRET_HD int latent_prefix(const int* starts, int prefixes, int q0) {
+  int at = 0, end = prefixes;  // the last of at .. end - 1 that starts at q0 or before
+  while (end - at > 1) {
+    const int half = at + (end - at) / 2;
+    if (starts[half] <= q0) at = half;
+    else end = half;
+  }
+  return starts[0] <= q0 && q0 < starts[prefixes] ? at : -1;
+}
+
 // The line of all (sequence, group, step) is dealt in equal shares to `units` =
 // kLatentUnits / side units of `side` work-groups.  Each group is followed by `extra`
 // steps without keys, so that a unit that goes on to a second tile (its queries, and the

@@ -91,3 +91,52 @@ def test_two_lines_in_one_launch(tmp_path):
     subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", f"-I{ROOT}/ferret_amd/csrc", str(src), "-o", str(exe)], check=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True)
     assert r.returncode == 0, r.stdout
+
+
+SEARCH = r"""
+#include <cstdio>
+#include <cstdlib>
+#include <vector>
+#include "latent_plan.hpp"
+using namespace ferret;
+int main() {
+  std::srand(12);
+  for (int i = 0; i < 20000; ++i) {
+    const int G = 1 + std::rand() % 12;
+    std::vector<int> starts(G + 1);
+    starts[0] = std::rand() % 5;
+    for (int g = 0; g < G; ++g) starts[g + 1] = starts[g] + (std::rand() % 3 == 0 ? 0 : std::rand() % 9);
+    for (int q = 0; q <= starts[G] + 2; ++q) {
+      int want = -1;
+      for (int g = 0; g < G; ++g)
+        if (starts[g] <= q && q < starts[g + 1]) want = g;
+      if (latent_prefix(starts.data(), G, q) != want) return std::printf("token %d\n", q), 1;
+    }
+    for (int& x : starts) x = std::rand() - std::rand();  // whatever stands there, a line of the table
+    for (int q = 0; q < 50; ++q) {
+      const int g = latent_prefix(starts.data(), G, std::rand() % 1000);
+      if (g < -1 || g >= G) return std::printf("line %d\n", g), 1;
+    }
+  }
+  // own keys behind a prefix's: on the next whole step, nothing lost
+  for (int prefix = 0; prefix < 400; ++prefix)
+    for (int len = 0; len < 200; ++len) {
+      LatentSeq s = latent_seq(0, 1, len, 1, 16, 16, 1, 1 << 20);
+      latent_behind(&s, prefix);
+      const int base = latent_base(prefix);
+      if (base < prefix || base >= prefix + kLatentKeys || base % kLatentKeys || s.len != base + len) return std::printf("base\n"), 1;
+      if (s.steps < 1 || s.steps * kLatentKeys < s.len || (s.steps > 1 && (s.steps - 1) * kLatentKeys >= s.len)) return std::printf("steps\n"), 1;
+    }
+  return 0;
+}
+"""
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="g++ not installed")
+def test_the_prefix_of_a_sequence(tmp_path):
+    src, exe = tmp_path / "search.cpp", tmp_path / "search"
+    src.write_text(SEARCH)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", f"-I{ROOT}/ferret_amd/csrc", str(src), "-o", str(exe)],
+                   check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout
