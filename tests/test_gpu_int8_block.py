@@ -214,3 +214,39 @@ def test_a_step_captured_and_replayed(ops):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want)), k
         assert torch.equal(one.cache.data, two.cache.data) and torch.equal(one.cache.scales, two.cache.scales), k
+
+
+def test_two_graphs_on_one_workspace(ops):
+    """Graphs of other products and batches, captured on the same workspaces and replayed in turn."""
+    print("[case] int8 block shared workspaces", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(8)
+    shapes = [(3, 64, 32768), (100, 512, 16384)]
+    need = max(ops.int8_gemm_workspace_bytes(*s) for s in shapes)
+    assert min(ops.int8_gemm_workspace_bytes(*s) for s in shapes) > 0
+    layer = Layer(ops)
+    runs = [Run(ops, layer, e4m3) for e4m3 in (True, False)]
+    states = [run.step(new) for run, new in zip(runs, STEPS[:2])]
+    attention = ops.latent_attention_shared_workspace_bytes(2, 5, 9, H)
+    ws, ws2 = (torch.empty(n, dtype=torch.uint8, device="cuda") for n in (need, attention))
+    calls, want = [], []
+    for (M, N, K), run, (_, ql, qr, _, _), new in zip(shapes, runs, states, STEPS):
+        a, b = (ops.quant_act_int8(torch.randn((n, K), generator=g, device="cuda").to(torch.bfloat16)) for n in (M, N))
+        index = (run.table, run.lens, i32([0, sum(new[:SAMPLES[0]]), sum(new)]), run.own, i32(run.have), i32(starts(new)))
+
+        def call(a=a, b=b, ql=ql, qr=qr, cache=run.cache, index=index):
+            return (ops.int8_gemm(*a, *b, workspace=ws),
+                    ops.latent_attention_shared(ql, qr, cache, *index, SCALE, workspace=ws2))
+        want.append(tuple(t.clone() for t in call()))
+        calls.append(call)
+    graphs = [torch.cuda.CUDAGraph() for _ in calls]
+    out = []
+    for graph, call in zip(graphs, calls):
+        with torch.cuda.graph(graph):
+            out.append(call())
+    for i in (0, 1, 1, 0, 1, 0):
+        for t in out[i]:
+            t.fill_(7)
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(out[i], want[i])), i
+        calls[1 - i]()
