@@ -1715,18 +1715,19 @@ size_t pass_bytes(int B, int T, int H, int mr, int whole) {
   return rows + (size_t)a.blocks(mr) * 16 * (sizeof(float2) + kLatent * sizeof(float));
 }
 
-// Whether prefixes of `keys` keys at most get a pass of their own: where a sequence fills no
-// tile of 64 rows but a prefix's tokens do, and the steps that the sequences would else take over
-// their prefixes are more than ten per CU, so that the quarter or half of them that is left
-// makes up for the partials of every row.  Us, two passes / one: 16 heads, 64 sequences behind 8192
-// keys, e4m3 49 / 69 (8192 steps), 8 prompts of 600 to 3500 with 8 samples each, bf16 33.8 / 37.6
-// (3500), 64 behind 2000 34.1 / 33.7 (2000), 16 behind 8192 34.2 / 30.1 (2000); 32 heads, 64 behind
-// 8192 73 / 88, behind 2000 44.8 / 42.9; 64 heads, 64 behind 2000 59 / 49; 128 heads, 32 behind
-// 6001, bf16 84 / 78.
+// Whether prefixes of `keys` keys at most get a pass of their own: where the steps that it saves
+// pay for the partials of every row.  A step takes 1 for a tile of 16 rows, 1.7 of 32, 3 of 64; a
+// sequence is one tile where it fills none of 64, a prefix's tokens are tiles of 64.  Saved steps
+// and us, two passes / one: 16 heads, 64 sequences behind 8192 keys, e4m3, 2048: 49 / 69; 8 prompts of
+// 2600 with 8 samples each 656: 35.4 / 36.9, 16 prompts with 4 each 656: 37.2 / 37.0; 64 behind 2000
+// 512: 34.1 / 33.7; 16 behind 8192 512: 34.2 / 30.1; 21 prompts of 6000 with 3 each, bf16, none: 76 / 71; 32
+// heads, 64 behind 8192 1638: 70 / 88, 32 behind 12000 1203: 66.5 / 69.2, behind 6000 602: 50.6 / 45.5.
 bool prefix_pass(int G, int B, int T, int H, long long keys) {
   const int own = tile_rows(T, B, H);
-  const long long steps = ((long long)T * H + own - 1) / own * ((keys + kKeys - 1) / kKeys);
-  return own < kWideRows && tile_rows(T, G, H) == kWideRows && steps >= 10 * kUnits;
+  if (own == kWideRows) return false;
+  const long long tiles = plan_min(B, T), rows = ((long long)T * H + G - 1) / G;
+  const long long saved = tiles * (own == 16 ? 10 : 17) - G * ((rows + kWideRows - 1) / kWideRows) * 30;  // tenths, per step
+  return saved > 0 && saved * ((keys + kKeys - 1) / kKeys) >= 25LL * kUnits;
 }
 
 }  // namespace

@@ -74,11 +74,12 @@ class Shared:
         do not: entries past the lengths are no pages."""
         T, B = sum(self.new), len(self.own)
         rows = T * self.H // B
-        if rows > 32 or T * self.H // self.G <= 32:
+        saved = min(B, T) * (10 if rows <= 16 else 17) - self.G * -(-(-(-T * self.H // self.G)) // 64) * 30
+        if rows > 32 or saved <= 0:
             return None
-        tiles = -(-T * self.H // (16 if rows <= 16 else 32))
         kw = self.index()
-        columns = -(-2560 * 64 // (tiles * self.page)) + 1
+        steps = -(-6400 // saved)
+        columns = -(-steps * 64 // self.page) + 1
         table = torch.full((self.G, max(columns, kw["prefix_table"].shape[1])), -1, dtype=torch.int32, device="cuda")
         table[:, :kw["prefix_table"].shape[1]] = kw["prefix_table"]
         return dict(kw, prefix_table=table)
@@ -377,7 +378,7 @@ def test_a_captured_prefix_pass(ops):
     """Prefixes in a pass of their own: replays with other lengths, missing pages and a NaN that stays with its prefix."""
     print("[case] shared captured, prefixes apart", flush=True)
     for e4m3 in (True, False):
-        batch = [Shared([(p, [(a, 1)] * 3 + [(b, 1)]), (q, [(c, 1)] * 5)], 16, 16, e4m3, 25)
+        batch = [Shared([(p, [(a, 1)] * 3 + [(b, 1)]), (q, [(c, 1)] * 4)], 16, 16, e4m3, 25)
                  for p, q, a, b, c in ((300, 640, 30, 65, 9), (17, 0, 1, 200, 64), (5000, 1300, 64, 0, 33))]
         columns = max(s.wide()["prefix_table"].shape[1] for s in batch)
         own = max(s.batch.table.shape[1] for s in batch)
@@ -451,3 +452,24 @@ def test_workspace_of_both_ways(ops):
                                           workspace=ws)
         again = s.call(ops, **kw)
         assert torch.equal(out, again[0]) and (ws[need:] == 0xa5).all()
+
+
+@pytest.mark.parametrize("H,members", [(16, 4), (16, 8), (1, 9), (5, 40), (32, 2), (24, 5), (17, 30)])
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_prefixes_in_a_pass_of_their_own(ops, H, members, e4m3):
+    """Full and ragged tiles of a prefix, cut in pieces and whole, beside short, long and missing own keys."""
+    print(f"[case] shared prefix pass H={H} members={members} e4m3={e4m3}", flush=True)
+    own = [(0, 1), (3000, 1), (65, 1), (1, 1), (64, 1), (200, 1)]
+    s = Shared([(1700, [own[i % 6] for i in range(members)]), (0, [(40, 1)] * members), (63, [own[i % 4] for i in range(members)])],
+               H, 16, e4m3, 27)
+    assert s.wide() is not None
+    s.run(ops)
+
+
+def test_other_tokens_beside_a_prefix_pass(ops):
+    """Sequences before and behind the prefixes, of several tokens, some not causal."""
+    print("[case] shared prefix pass with others", flush=True)
+    s = Shared([(None, [(90, 2), (7, 1)]), (500, [(30, 1), (2, 2), (64, 1), (9, 1)] * 3), (None, [(65, 1), (130, 1)])], 8, 16, True, 28)
+    assert s.wide() is not None
+    s.run(ops)
+    s.run(ops, causal=False)
