@@ -1188,7 +1188,8 @@ __device__ __forceinline__ void attend_wide(const Args& a, Cache cache, int unit
         const bool gap = PRE && pc.ends_in(v, M::kStep);
         const bool edge = (v + 1) * M::kStep > pc.see_all || ok != kAll || gap;
         if (edge) {
-          clear_unseen<F8, M::kStep>(in, pc, gap ? pc.gap : pc.see_all, gap ? pc.gap : pc.see_any, buf, v * M::kStep, ok, w * (F8 ? 8 : 16), o);
+          clear_unseen<F8, M::kStep>(in, pc, gap ? pc.gap : pc.see_all, gap ? pc.gap : pc.see_any, buf, v * M::kStep, ok,
+                                     w * (F8 ? 8 : 16), o);
           asm volatile("" ::: "memory");
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -1357,8 +1358,8 @@ struct Shared {
   static_assert(kLds <= 160 * 1024, "LDS of a CU");
 };
 template <int MRO, bool F8>
-__global__ __launch_bounds__(tile_threads<kWideRows>(), tile_threads<kWideRows>() / 256) void latent_shared_kernel(Args, Args,
-                                                                                                                float) {
+__global__ __launch_bounds__(tile_threads<kWideRows>(), tile_threads<kWideRows>() / 256)
+void latent_shared_kernel(Args, Args, float) {
   using S = Shared<MRO, F8>;
   constexpr int NT = S::kThreads, NW = NT / 64, WORDS = (2 * sizeof(Args) + 4) / 4;
   static_assert(sizeof(Args) % 8 == 0 && WORDS <= NT, "arguments");
@@ -1810,12 +1811,12 @@ extern "C" int ferret_latent_attention_shared(const void* q_latent, long long ql
                      ((bits(scales) | bits(lse)) & 3) == 0 && ((ql_token | ql_head | qr_token | qr_head) & 7) == 0,
                  FERRET_ERR_ALIGN);
   const int own_mr = tile_rows(T, B, H);
-  const bool two = prefix_pass(G, B, T, H, (long long)max_prefix_pages * page_size);
-  FERRET_REQUIRE(((long long)max_pages + max_prefix_pages) * page_size <= (1LL << 31) - 4 * kKeys, FERRET_ERR_SHAPE);
-  rc = two ? check_steps(G, (long long)max_prefix_pages * page_size, pages, page_size, T, H, kWideRows) : FERRET_OK;
+  const long long prefix_keys = (long long)max_prefix_pages * page_size, own_keys = (long long)max_pages * page_size;
+  const bool two = prefix_pass(G, B, T, H, prefix_keys);
+  FERRET_REQUIRE(prefix_keys + own_keys <= (1LL << 31) - 4 * kKeys, FERRET_ERR_SHAPE);
+  rc = two ? check_steps(G, prefix_keys, pages, page_size, T, H, kWideRows) : FERRET_OK;
   if (rc == FERRET_OK)
-    rc = check_steps(B, ((long long)max_pages + (two ? 0 : max_prefix_pages)) * page_size + (two ? 0 : kKeys), pages, page_size,
-                     T, H, own_mr);
+    rc = check_steps(B, own_keys + (two ? 0 : prefix_keys + kKeys), pages, page_size, T, H, own_mr);
   if (rc != FERRET_OK) return rc;
   const size_t need = ferret_latent_attention_shared_workspace(G, B, T, H);
   FERRET_REQUIRE(need != 0, FERRET_ERR_SHAPE);
