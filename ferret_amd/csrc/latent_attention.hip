@@ -1736,10 +1736,13 @@ bool prefix_pass(int G, int B, int T, int H, long long keys) {
 
 using namespace ferret;
 
+// Query rows of a call: the join of 16 rows takes 1024 threads, and a launch holds less than 2^32.
+static bool latent_rows_fit(int T, int H) { return (long long)T * H <= (1LL << 26) - 16; }
+
 int ferret_check_pages(const int32_t* page_table, int B, int max_pages, int pages, int page_size);
 
 extern "C" size_t ferret_latent_attention_workspace(int B, int T, int H) {
-  if (B < 1 || T < 1 || H < 1 || (long long)T * H >= (1LL << 31)) return 0;
+  if (B < 1 || T < 1 || H < 1 || !latent_rows_fit(T, H)) return 0;
   return pass_bytes(B, T, H, tile_rows(T, B, H), 0);
 }
 
@@ -1752,7 +1755,7 @@ extern "C" int ferret_latent_attention(const void* q_latent, long long ql_token,
   FERRET_REQUIRE(q_latent && q_rotary && data && lens && cu_q && out, FERRET_ERR_NULL);
   const int rc = ferret_check_pages(page_table, B, max_pages, pages, page_size);
   if (rc != FERRET_OK) return rc;
-  FERRET_REQUIRE(T >= 1 && H >= 1 && H <= 1024 && (long long)T * H < (1LL << 31), FERRET_ERR_SHAPE);
+  FERRET_REQUIRE(T >= 1 && H >= 1 && H <= 1024 && latent_rows_fit(T, H), FERRET_ERR_SHAPE);
   FERRET_REQUIRE(scale > 0.f && scale < 1e30f, FERRET_ERR_SHAPE);
   for (const long long stride : {ql_token, ql_head, qr_token, qr_head})
     FERRET_REQUIRE(stride >= 0 && stride < (1LL << 31), FERRET_ERR_SHAPE);
@@ -1783,7 +1786,7 @@ extern "C" int ferret_latent_attention(const void* q_latent, long long ql_token,
 }
 
 extern "C" size_t ferret_latent_attention_shared_workspace(int G, int B, int T, int H) {
-  if (G < 1 || B < 1 || T < 1 || H < 1 || (long long)T * H >= (1LL << 26) || (G > B ? G : B) >= 1 << 26) return 0;
+  if (G < 1 || B < 1 || T < 1 || H < 1 || !latent_rows_fit(T, H) || (G > B ? G : B) >= 1 << 26) return 0;
   const int own = tile_rows(T, B, H);
   if (!prefix_pass(G, B, T, H, 1LL << 31)) return pass_bytes(B, T, H, own, 0);
   // A call with shorter tables takes one pass, and less.
@@ -1802,7 +1805,7 @@ extern "C" int ferret_latent_attention_shared(const void* q_latent, long long ql
   int rc = ferret_check_pages(prefix_table, G, max_prefix_pages, pages, page_size);
   if (rc == FERRET_OK) rc = ferret_check_pages(page_table, B, max_pages, pages, page_size);
   if (rc != FERRET_OK) return rc;
-  FERRET_REQUIRE(T >= 1 && H >= 1 && H <= 1024 && (long long)T * H < (1LL << 26), FERRET_ERR_SHAPE);  // 2^32 threads
+  FERRET_REQUIRE(T >= 1 && H >= 1 && H <= 1024 && latent_rows_fit(T, H), FERRET_ERR_SHAPE);
   FERRET_REQUIRE(scale > 0.f && scale < 1e30f, FERRET_ERR_SHAPE);
   for (const long long stride : {ql_token, ql_head, qr_token, qr_head})
     FERRET_REQUIRE(stride >= 0 && stride < (1LL << 31), FERRET_ERR_SHAPE);

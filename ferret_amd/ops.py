@@ -777,7 +777,7 @@ def latent_attention(q_latent: torch.Tensor, q_rotary: torch.Tensor, cache: Late
     with other lengths.  `workspace` of latent_attention_workspace_bytes is
     taken from torch's caching allocator unless one is passed; calls that
     overlap in time (streams, graphs) need one each.  `out` may be q_latent
-    itself where that is packed, and overlaps nothing else.
+    itself where that is packed, and overlaps nothing else.  T * H <= 2^26 - 16.
     """
     _latent_cache(cache)
     r = _lib.native().latent_attention(q_latent, q_rotary, cache.data, cache.scales, page_table, lens, cu_q,
@@ -827,7 +827,7 @@ def latent_attention_shared(q_latent: torch.Tensor, q_rotary: torch.Tensor, cach
     it see no prefix, and a prefix may be empty.  A prefix is kept
     once; where its tokens fill tiles that their sequences do not, it is multiplied once for all of them too.  Index tensors stay on the device (a captured call replays with other lengths);
     `workspace` of latent_attention_shared_workspace_bytes, `out`, tokens that see no key and rows behind the
-    last sequence as in latent_attention.  T * H < 2^26.
+    last sequence as in latent_attention.  T * H <= 2^26 - 16.
     """
     _latent_cache(cache)
     r = _lib.native().latent_attention_shared(q_latent, q_rotary, cache.data, cache.scales, prefix_table, prefix_lens,

@@ -379,8 +379,8 @@ int ferret_latent_cache_read(const void* data, const void* scales, int pages, in
  * rounded to bf16; the same call gives the same bits.  Sums are fp32 and hold terms of
  * up to 256 times the latents: finite where 256 * keys * max|latent| stays below 2^128.
  * out may stand exactly on packed q_latent.
- * Requirements: T >= 1, 1 <= H <= 1024, 0 < scale < 1e30, max_pages * page_size
- * <= 2^31 - 128.
+ * Requirements: T >= 1, 1 <= H <= 1024, T * H <= 2^26 - 16, 0 < scale < 1e30, max_pages *
+ * page_size <= 2^31 - 128.
  */
 size_t ferret_latent_attention_workspace(int B, int T, int H);
 int ferret_latent_attention(const void* q_latent, long long ql_token, long long ql_head, const void* q_rotary,
@@ -400,7 +400,7 @@ int ferret_latent_attention(const void* q_latent, long long ql_token, long long 
  * cu_prefix[G]) see no prefix.  Both tables are of the one cache.  Everything else, the softmax's statement, out in
  * place, lse, tokens without keys, Inf and NaN, and the range of the sums, as
  * ferret_latent_attention; its requirements for both tables, together (max_pages +
- * max_prefix_pages) * page_size <= 2^31 - 256, and T * H < 2^26.
+ * max_prefix_pages) * page_size <= 2^31 - 256.
  * ws: ferret_latent_attention_shared_workspace(G, B, T, H) bytes, on a 16-byte bound.
  */
 size_t ferret_latent_attention_shared_workspace(int G, int B, int T, int H);
