@@ -68,6 +68,7 @@ constexpr int kKeys = kLatentKeys, kUnits = kLatentUnits;
 constexpr int kWideRows = 64;   // query rows of the largest tile
 constexpr int kAhead = 4;      // LDS fragments read ahead
 constexpr int kFence = 4;      // fragments between scheduling fences
+constexpr int kManyGroups = 256;  // work-groups of a join for rows of many pieces
 
 struct Args {
   const uint16_t *ql, *qr;
@@ -86,15 +87,18 @@ struct Args {
   int side_by_side;  // row tiles of a sequence taken at the same time
   uint16_t* out;  // [T, H, 512]
   float* lse;     // [T, H] or null
-  // The workspace: rows [T * H] (int4), then ml [blocks][16] (m and l), then the partial
+  // The workspace, behind many [kUnits]: rows [T * H] (int4), then ml [blocks][16] (m and l), then the partial
   // outputs [blocks][32][64][4], `blocks` of 16 query rows: 2 * kUnits slots of a tile each,
   // then, where there is a second pass over the rows' keys (shared prefixes), the whole
   // tiles, which go to `out` else.  A block's outputs stand as the matrix units leave them, lane g * 16 +
   // r holding columns 4g .. 4g + 3 of 16 of row r, so that a store or load of a wave is 1 KB
   // in one piece: rows of 2 KB, 64 bytes at a time, took 4 us a tile.  A row's record is {first
-  // block of the tile in its first slot or as a whole, pieces, row in tile, -}.
+  // block of the tile in its first slot or as a whole, pieces, row in tile, -}.  many: by
+  // work-group the first row of the tile that it begins and that has more than kLatentMany pieces,
+  // -1 where it begins none (only the last one of its share goes on in others).
   uint8_t* ws;
   int whole;  // whether whole tiles go to the workspace
+  __host__ __device__ int* many() const { return reinterpret_cast<int*>(ws) - kUnits; }
   __host__ __device__ int4* rows() const { return reinterpret_cast<int4*>(ws); }
   __host__ __device__ int blocks(int mr) const { return 2 * kUnits * (mr / 16) + (whole ? whole_blocks() : 0); }
   __host__ __device__ int whole_blocks() const { return T * H / 16 + B + kWideRows / 16; }
@@ -303,7 +307,10 @@ __device__ __forceinline__ bool take_share(const Args& a, int units, LatentPlace
   const LatentDeal deal = latent_deal(all, groups, whole, units, a.min_steps);
   const int total = deal.total, chunk = deal.chunk, extra = deal.extra;
   const int start = uniform((int)min((long long)place.unit * chunk, (long long)total));
-  if (start >= total) return false;
+  if (start >= total) {
+    if (threadIdx.x == 0) a.many()[place.unit * a.side_by_side + place.lane] = -1;
+    return false;
+  }
   const int excl = before + incl - mine + extra * (groups_before + incl_groups - my_groups);
   if (excl <= start && start < excl + mine + extra * my_groups) {
     int at = excl, i = 0;
@@ -324,6 +331,18 @@ __device__ __forceinline__ bool take_share(const Args& a, int units, LatentPlace
     side->extra = extra;
     side->end = min(start + chunk, total);
     if constexpr (!PRE) put_args(&side->args, a);  // else `a` stands there
+  }
+  const int last = min(start + chunk, total) - 1;
+  if (excl <= last && last < excl + mine + extra * my_groups) {  // one thread
+    int at = excl;
+    if (per > 1)
+      for (int i = 0;; ++i) {
+        s = sequence<MR, PRE>(a, b0 + i, &prefix);
+        if (last < at + s.work(extra) || i + 1 == per) break;
+        at += s.work(extra);
+      }
+    a.many()[place.unit * a.side_by_side + place.lane] =
+        latent_many(s, at, extra, last + 1, chunk, a.side_by_side, place.lane, MR, a.H);
   }
   *cur = uniform(start);
   __syncthreads();
@@ -1393,7 +1412,13 @@ void latent_shared_kernel(Args, Args, float) {
     all[1] = latent_add(all[1], tot[NW + w]);
   }
   __syncthreads();
-  const int groups = uniform(latent_split(all[0], all[1], weight, both[0].side_by_side, both[1].side_by_side));
+  const int split = latent_split(all[0], all[1], weight, both[0].side_by_side, both[1].side_by_side);
+  if (threadIdx.x == 0) {  // the rest of the other pass's list, which its own work-groups do not reach
+    const int block = blockIdx.x;
+    const bool prefix = block < split;
+    both[prefix ? 1 : 0].many()[prefix ? kUnits - split + block : block] = -1;
+  }
+  const int groups = uniform(split);
   asm volatile("" ::"v"(near));
   const bool first = (int)blockIdx.x < groups;
   const Args& a = both[first ? 0 : 1];
@@ -1410,30 +1435,47 @@ void latent_shared_kernel(Args, Args, float) {
 
 // ---- joins
 
-__device__ __forceinline__ bool has_tokens(const Args& a, long long row) {
-  return row >= (long long)max(a.cu_q[0], 0) * a.H && row < (long long)min(a.cu_q[a.B], a.T) * a.H;
+// What a join takes of a pass.
+struct Parts {
+  const int* many;
+  const int4* rows;
+  const float2* ml;
+  const float* part;
+  const int32_t* cu_q;
+  int B, T, H;
+  int per;      // blocks of 16 rows of a tile
+  int side;     // side by side
+  int blocks;   // blocks, whole tiles among them: 0 where those went to `out`
+  // Whether a row belongs to a token of the pass.
+  __device__ __forceinline__ bool has(long long row) const {
+    return row >= (long long)max(cu_q[0], 0) * H && row < (long long)min(cu_q[B], T) * H;
+  }
+};
+Parts parts_of(const Args& a, int mr) {
+  return Parts{a.many(), a.rows(), a.ml(), a.part(mr), a.cu_q, a.B, a.T, a.H, mr / 16, a.side_by_side,
+               a.whole ? a.blocks(mr) : 0};
 }
 
 // The pieces of a row in one pass.  Rows behind the last sequence have no record, and
 // whatever stands in its place leads nowhere outside the workspace.
 struct Pieces {
   int first, rest, step;  // blocks of 16 rows: the first piece's; piece j > 0 at rest + j * step
-  int n, r16;
+  int n, row;             // pieces; the row's place in its tile
   __device__ __forceinline__ int at(int j) const { return j == 0 ? first : rest + j * step; }
 };
-__device__ __forceinline__ Pieces pieces_of(const Args& a, int mr, long long row) {
+__device__ __forceinline__ Pieces pieces_of(const Parts& a, long long row) {
   Pieces p{0, 0, 0, 0, 0};
-  const int4 rec = a.rows()[row];
-  if (!has_tokens(a, row) || (unsigned)rec.z >= (unsigned)mr) return p;
-  const int per = mr / 16, f = rec.z >> 4;
-  p.r16 = rec.z & 15;
-  const LatentRecord where{rec.x / per, rec.y};
-  if (latent_record_joins(where, a.side_by_side)) {
+  const int4 rec = a.rows[row];
+  if (!a.has(row) || (unsigned)rec.z >= (unsigned)(a.per * 16)) return p;
+  const int f = rec.z >> 4;
+  p.row = rec.z;
+  const LatentRecord where{rec.x / a.per, rec.y};
+  if (latent_record_joins(where, a.side)) {
     p.n = where.pieces;
-    p.first = where.slot0 * per + f;
-    p.rest = (where.slot0 & ~1) * per + f;
-    p.step = 2 * a.side_by_side * per;
-  } else if (a.whole && rec.y == 1 && rec.x >= 2 * kUnits * per && rec.x < a.blocks(mr) - f) {
+    p.first = where.slot0 * a.per + f;
+    p.rest = (where.slot0 & ~1) * a.per + f;
+    p.step = 2 * a.side * a.per;
+  } else if (rec.y == 1 && rec.x >= 2 * kUnits * a.per && rec.x < a.blocks - f) {
     p.n = 1;
     p.first = rec.x + f;
   }
@@ -1450,41 +1492,27 @@ __device__ __forceinline__ float quad_add(float v) {
 }
 
 // Joins the pieces of 16 query rows in the order of the keys, those of the prefix (TWO)
-// first: lane g * 16 + i takes row i and columns 4g .. 4g + 3 of every 16, as the pieces
-// stand, and CB blocks of 16 columns.  PW waves take every PW-th four pieces each, eight
-// loads under way, with the weights of four pieces in the lanes, one per g, and meet in LDS.
-// TWO: every row; else those of tiles that were cut.
-template <int PW>
-constexpr int join_blocks() { return PW >= 8 ? 1 : 2; }
-template <bool TWO, int PW>
-__global__ __launch_bounds__(64 * (PW > 4 ? PW : 4)) void latent_join_kernel(Args prefix, Args own, int prefix_mr,
-                                                                          int own_mr, int rows) {
-  constexpr int CB = join_blocks<PW>(), QUADS = 2 / CB, AHEAD = 4 * QUADS;
-  constexpr int WAVES = PW > 4 ? PW : 4, TILES = WAVES / PW;  // units of 16 rows x CB blocks per work-group
-  __shared__ f32x4 red[PW > 1 ? WAVES : 1][CB][64];
-  __shared__ float2 red_ml[PW > 1 ? WAVES : 1][16];
-  const int lane = threadIdx.x & 63, g = lane >> 4, wave = threadIdx.x >> 6, pw = wave % PW;
-  const int unit = blockIdx.x * TILES + wave / PW, cb = unit % (32 / CB) * CB;
-  const long long row = (long long)(unit / (32 / CB)) * 16 + (lane & 15);
-  const bool in = row < rows;
-  Pieces p0{0, 0, 0, 0, 0}, p1 = p0;
-  if (in) {
-    p1 = pieces_of(own, own_mr, row);
-    if constexpr (TWO) p0 = pieces_of(prefix, prefix_mr, row);
-  }
+// first: lane g * 16 + i takes row i (`row` and its pieces, where `mine`) and columns 4g .. 4g + 3 of
+// every 16, as the pieces stand, and CB blocks of 16 columns from block cb on.  PW waves, pw of them
+// each, take every PW-th four pieces or eight, eight loads under way, with the weights of four
+// pieces in the lanes, one per g, and meet in LDS at `red`, a wave's share each.
+template <bool TWO, int PW, int CB>
+__device__ __forceinline__ void join_rows(const Parts& prefix, const Parts& own, uint16_t* out, float* lse, long long row,
+                                          bool mine, const Pieces& p0, const Pieces& p1, int cb, int pw,
+                                          f32x4 (*red)[CB][64], float2 (*red_ml)[16]) {
+  constexpr int QUADS = 2 / CB, AHEAD = 4 * QUADS;
+  const int lane = threadIdx.x & 63, g = lane >> 4;
   const int n = p0.n + p1.n;
-  const bool mine = TWO ? in && has_tokens(own, row) : n >= 2;
-  if (PW == 1 && !__any(mine)) return;
   int most = mine ? n : 0;
 #pragma unroll
   for (int off = 8; off >= 1; off >>= 1) most = max(most, __shfl_xor(most, off, 64));
   const auto stat = [&](int j) {
     if (!mine || j >= n) return make_float2(-INFINITY, 0.f);
-    return TWO && j < p0.n ? prefix.ml()[(long long)p0.at(j) * 16 + p0.r16]
-                           : own.ml()[(long long)p1.at(j - p0.n) * 16 + p1.r16];
+    return TWO && j < p0.n ? prefix.ml[(long long)p0.at(j) * 16 + (p0.row & 15)]
+                           : own.ml[(long long)p1.at(j - p0.n) * 16 + (p1.row & 15)];
   };
-  const float* const part0 = TWO ? prefix.part(prefix_mr) + (cb * 64 + g * 16 + p0.r16) * 4 : nullptr;
-  const float* const part1 = own.part(own_mr) + (cb * 64 + g * 16 + p1.r16) * 4;
+  const float* const part0 = TWO ? prefix.part + (cb * 64 + g * 16 + (p0.row & 15)) * 4 : nullptr;
+  const float* const part1 = own.part + (cb * 64 + g * 16 + (p1.row & 15)) * 4;
   f32x4 x[AHEAD][CB];
   const auto load = [&](int j0) __attribute__((always_inline)) {
 #pragma unroll
@@ -1542,60 +1570,153 @@ __global__ __launch_bounds__(64 * (PW > 4 ? PW : 4)) void latent_join_kernel(Arg
   sum = quad_add(sum);
   if constexpr (PW > 1) {
 #pragma unroll
-    for (int c = 0; c < CB; ++c) red[wave][c][lane] = acc[c];
-    if (g == 0) red_ml[wave][lane] = make_float2(top, sum);
+    for (int c = 0; c < CB; ++c) red[pw][c][lane] = acc[c];
+    if (g == 0) red_ml[pw][lane] = make_float2(top, sum);
     __syncthreads();
     if (pw != 0) return;
 #pragma unroll
-    for (int i = 1; i < PW; ++i) top = fmaxf(top, red_ml[wave + i][lane & 15].x);
-    const float all = top == -INFINITY ? 0.f : top, first = __builtin_amdgcn_exp2f(red_ml[wave][lane & 15].x - all);
+    for (int i = 1; i < PW; ++i) top = fmaxf(top, red_ml[i][lane & 15].x);
+    const float all = top == -INFINITY ? 0.f : top, first = __builtin_amdgcn_exp2f(red_ml[0][lane & 15].x - all);
     sum = sum != 0.f ? sum * first : 0.f;
 #pragma unroll
     for (int c = 0; c < CB; ++c) acc[c] *= first;
 #pragma unroll
     for (int i = 1; i < PW; ++i) {
-      const float2 s = red_ml[wave + i][lane & 15];
+      const float2 s = red_ml[i][lane & 15];
       const float w = __builtin_amdgcn_exp2f(s.x - all);
       if (s.y != 0.f) sum += s.y * w;
 #pragma unroll
-      for (int c = 0; c < CB; ++c) acc[c] += red[wave + i][c][lane] * w;
+      for (int c = 0; c < CB; ++c) acc[c] += red[i][c][lane] * w;
     }
   }
   if (!mine) return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
   for (int c = 0; c < CB; ++c)
-    *reinterpret_cast<u32x2*>(own.out + row * kLatent + (cb + c) * 16 + 4 * g) =
+    *reinterpret_cast<u32x2*>(out + row * kLatent + (cb + c) * 16 + 4 * g) =
         u32x2{pack_bf16x2(acc[c][0] * inv, acc[c][1] * inv), pack_bf16x2(acc[c][2] * inv, acc[c][3] * inv)};
-  if (own.lse != nullptr && cb == 0 && g == 0)
-    own.lse[row] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+  if (lse != nullptr && cb == 0 && g == 0)
+    lse[row] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
-template <bool TWO, int PW>
+// The first row of tile k of those that have more than kLatentMany pieces, -1 where there are
+// fewer, and their number.
+struct Many {
+  int first, n;
+};
+__device__ __forceinline__ Many many_tile(const int* many, int k) {
+  static_assert(kUnits == 256, "four work-groups per lane");
+  const int lane = threadIdx.x & 63;
+  const int4 at = reinterpret_cast<const int4*>(many)[lane];
+  const int first[4] = {at.x, at.y, at.z, at.w};
+  Many tile{-1, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const unsigned long long all = __ballot(first[i] >= 0);
+    const bool here = first[i] >= 0 && tile.n + __popcll(all & ((1ull << lane) - 1)) == k;
+    const unsigned long long found = __ballot(here);
+    if (found != 0) tile.first = __shfl(first[i], __ffsll((long long)found) - 1, 64);
+    tile.n += __popcll(all);
+  }
+  return tile;
+}
+
+// Units of 16 query rows and CB blocks of 16 columns, PW waves to each.  TWO: every row; else
+// those of tiles that were cut.  MANY: before the units come kManyGroups work-groups for
+// the rows of more than kLatentMany pieces, which the units leave out: what a row has follows
+// from the lengths, which the host does not read.  Us, whole call, e4m3, 16 heads, the units
+// alone / with these: one of 100001 keys beside 15 of 100 39.2 / 30.4, beside 31 85.1 / 30.5, beside
+// 63 79.2 / 31.7; four of 30000 beside 28 of 500 41.4 / 29.8; 32 of 600 to 8000 33.3 / 33.0; of 6000
+// 36.5 / 37.1.  In work-groups of four waves: 34 for the first three, 32.4 and 36.5 for the last two.
+template <int PW>
+constexpr int join_blocks() { return PW >= 8 ? 1 : 2; }
+template <int PW, bool MANY>
+constexpr int join_waves() { return PW > 4 ? PW : MANY ? kLatentManyWaves : 4; }
+template <bool TWO, int PW, bool MANY>
+__global__ __launch_bounds__((64 * join_waves<PW, MANY>()))
+void latent_join_kernel(Parts prefix, Parts own, uint16_t* out, float* lse, int rows) {
+  constexpr int CB = join_blocks<PW>(), WAVES = join_waves<PW, MANY>(), TILES = WAVES / PW;
+  __shared__ f32x4 red[PW > 1 || MANY ? WAVES * CB : 1][64];
+  __shared__ float2 red_ml[WAVES][16];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  int block = blockIdx.x;
+  if constexpr (MANY) {
+    if (block < kManyGroups) {
+#pragma unroll
+      for (int pass = 0; pass < (TWO ? 2 : 1); ++pass) {
+        const int* const list = pass == 0 ? own.many : prefix.many;
+        const int per = pass == 0 ? own.per : prefix.per;
+        for (;; block += kManyGroups) {
+          const Many tile = many_tile(list, block / (32 * per));
+          if (tile.first < 0) {
+            block -= tile.n * 32 * per;
+            break;
+          }
+          const int at = block / 32 % per * 16 + (lane & 15);
+          const long long row = (long long)tile.first + at;
+          Pieces p0{0, 0, 0, 0, 0}, p1 = p0;
+          if (row < rows) {
+            p1 = pieces_of(own, row);
+            if constexpr (TWO) p0 = pieces_of(prefix, row);
+          }
+          const bool mine = pass == 0 ? p1.row == at && p1.n > kLatentMany
+                                      : p0.row == at && p0.n > kLatentMany && p1.n <= kLatentMany;
+          // the wave's number from a vector register: with two passes scalar ones are short
+          join_rows<TWO, WAVES, 1>(prefix, own, out, lse, row, mine, p0, p1, block % 32, threadIdx.x >> 6,
+                                   reinterpret_cast<f32x4(*)[1][64]>(red), red_ml);
+          __syncthreads();  // `red` has been read
+        }
+      }
+      return;
+    }
+    block -= kManyGroups;
+  }
+  const int unit = block * TILES + wave / PW;
+  const long long row = (long long)(unit / (32 / CB)) * 16 + (lane & 15);
+  Pieces p0{0, 0, 0, 0, 0}, p1 = p0;
+  if (row < rows) {
+    p1 = pieces_of(own, row);
+    if constexpr (TWO) p0 = pieces_of(prefix, row);
+  }
+  bool mine = TWO ? row < rows && own.has(row) : p1.n >= 2;
+  if (MANY && (p0.n > kLatentMany || p1.n > kLatentMany)) mine = false;
+  if (PW == 1 && !__any(mine)) return;
+  join_rows<TWO, PW, CB>(prefix, own, out, lse, row, mine, p0, p1, unit % (32 / CB) * CB, wave % PW,
+                         reinterpret_cast<f32x4(*)[CB][64]>(red + wave / PW * PW * CB), red_ml + wave / PW * PW);
+}
+
+template <bool TWO, int PW, bool MANY>
 int launch_join(const Args& prefix, const Args& own, int prefix_mr, int own_mr, hipStream_t st) {
-  constexpr int WAVES = PW > 4 ? PW : 4, TILES = WAVES / PW;
+  constexpr int TILES = join_waves<PW, MANY>() / PW;
   const long long rows = (long long)own.T * own.H, units = (rows + 15) / 16 * (32 / join_blocks<PW>());
-  hipLaunchKernelGGL((latent_join_kernel<TWO, PW>), dim3((unsigned)((units + TILES - 1) / TILES)), dim3(64 * WAVES), 0, st,
-                     prefix, own, prefix_mr, own_mr, (int)rows);
+  hipLaunchKernelGGL((latent_join_kernel<TWO, PW, MANY>),
+                     dim3((unsigned)((units + TILES - 1) / TILES + (MANY ? kManyGroups : 0))),
+                     dim3(64 * join_waves<PW, MANY>()), 0, st, parts_of(prefix, prefix_mr), parts_of(own, own_mr), own.out,
+                     own.lse, (int)rows);
   return (int)hipGetLastError();
 }
 
-// Waves for the pieces of a row, by how many it has at most: all work-groups at the rows
-// there are, a step each at least.  Us, whole call, with 1 / 4 / 8 / 16 waves: 16 heads, e4m3,
-// one sequence of 100001 (256 pieces) - / - / 29.7 / 28.0; 128 heads, four of 9831 (32) - / 34.2 /
-// 34.1 / 38.9; 64 sequences behind 8192 keys (16 + 4) 50.7 / 49.2 / - / 58.5.
-long long most_pieces(const Args& a, int mr) {
+// The pieces of a row, a step each at least: on average, and at most.
+struct Counts {
+  long long mean, most;
+};
+Counts pieces(const Args& a, int mr) {
   const long long dealt = (long long)kUnits * mr / ((long long)a.T * a.H);
   const long long table = (long long)a.pages.max_pages + (a.prefix_table != nullptr ? a.max_prefix_pages : 0);
-  return std::min<long long>(dealt, table * a.pages.page_size / kKeys + 1);
+  const long long steps = table * a.pages.page_size / kKeys + 1;
+  return Counts{std::min(dealt, steps), std::min<long long>(kUnits / a.side_by_side, steps)};
 }
 template <bool TWO>
 int pick_join(const Args& prefix, const Args& own, int prefix_mr, int own_mr, hipStream_t st) {
-  const long long pieces = most_pieces(own, own_mr) + (TWO ? most_pieces(prefix, prefix_mr) : 0);
-  if (pieces >= 200) return launch_join<TWO, 16>(prefix, own, prefix_mr, own_mr, st);
-  if (pieces >= 24) return launch_join<TWO, 8>(prefix, own, prefix_mr, own_mr, st);
-  if (pieces >= 10) return launch_join<TWO, 4>(prefix, own, prefix_mr, own_mr, st);
-  return launch_join<TWO, 1>(prefix, own, prefix_mr, own_mr, st);
+  const Counts o = pieces(own, own_mr), p = TWO ? pieces(prefix, prefix_mr) : Counts{0, 0};
+  const LatentJoin join = latent_join(o.mean + p.mean, std::max(o.most, p.most), (long long)own.T * own.H);
+  if (join.waves == 16) return launch_join<TWO, 16, false>(prefix, own, prefix_mr, own_mr, st);
+  if (join.waves == 8) return launch_join<TWO, 8, false>(prefix, own, prefix_mr, own_mr, st);
+  if (join.waves == 4)
+    return join.many ? launch_join<TWO, 4, true>(prefix, own, prefix_mr, own_mr, st)
+                     : launch_join<TWO, 4, false>(prefix, own, prefix_mr, own_mr, st);
+  return join.many ? launch_join<TWO, 1, true>(prefix, own, prefix_mr, own_mr, st)
+                   : launch_join<TWO, 1, false>(prefix, own, prefix_mr, own_mr, st);
 }
 
 template <int MR, bool F8, void (*kernel)(Args)>
@@ -1701,7 +1822,7 @@ Args pass_args(const void* q_latent, long long ql_token, long long ql_head, cons
   a.out = static_cast<uint16_t*>(out);
   a.lse = lse;
   a.whole = 0;
-  a.ws = static_cast<uint8_t*>(ws);
+  a.ws = static_cast<uint8_t*>(ws) + kUnits * sizeof(int);
   return a;
 }
 
@@ -1713,7 +1834,7 @@ size_t pass_bytes(int B, int T, int H, int mr, int whole) {
   a.B = B;
   a.whole = whole;
   const size_t rows = ((size_t)T * H * sizeof(int4) + 255) & ~(size_t)255;
-  return rows + (size_t)a.blocks(mr) * 16 * (sizeof(float2) + kLatent * sizeof(float));
+  return kUnits * sizeof(int) + rows + (size_t)a.blocks(mr) * 16 * (sizeof(float2) + kLatent * sizeof(float));
 }
 
 // Whether prefixes of `keys` keys at most get a pass of their own: where the steps that it saves
