@@ -94,10 +94,11 @@ struct Args {
   // r holding columns 4g .. 4g + 3 of 16 of row r, so that a store or load of a wave is 1 KB
   // in one piece: rows of 2 KB, 64 bytes at a time, took 4 us a tile.  A row's record is {first
   // block of the tile in its first slot or as a whole, pieces, row in tile, -}.  many: by
-  // work-group the first row of the tile that it begins and that has more than kLatentMany pieces,
+  // work-group the first row of the tile that it begins and that has more than `few` pieces,
   // -1 where it begins none (only the last one of its share goes on in others).
   uint8_t* ws;
   int whole;  // whether whole tiles go to the workspace
+  int few;    // pieces of a tile past which it is noted in many()
   __host__ __device__ int* many() const { return reinterpret_cast<int*>(ws) - kUnits; }
   __host__ __device__ int4* rows() const { return reinterpret_cast<int4*>(ws); }
   __host__ __device__ int blocks(int mr) const { return 2 * kUnits * (mr / 16) + (whole ? whole_blocks() : 0); }
@@ -342,7 +343,7 @@ __device__ __forceinline__ bool take_share(const Args& a, int units, LatentPlace
         at += s.work(extra);
       }
     a.many()[place.unit * a.side_by_side + place.lane] =
-        latent_many(s, at, extra, last + 1, chunk, a.side_by_side, place.lane, MR, a.H);
+        latent_many(s, at, extra, last + 1, chunk, a.side_by_side, place.lane, MR, a.H, a.few);
   }
   *cur = uniform(start);
   __syncthreads();
@@ -1494,13 +1495,13 @@ __device__ __forceinline__ float quad_add(float v) {
 // Joins the pieces of 16 query rows in the order of the keys, those of the prefix (TWO)
 // first: lane g * 16 + i takes row i (`row` and its pieces, where `mine`) and columns 4g .. 4g + 3 of
 // every 16, as the pieces stand, and CB blocks of 16 columns from block cb on.  PW waves, pw of them
-// each, take every PW-th four pieces or eight, eight loads under way, with the weights of four
-// pieces in the lanes, one per g, and meet in LDS at `red`, a wave's share each.
-template <bool TWO, int PW, int CB>
+// each, take every PW-th QUADS times four pieces, whose loads are under way together, with the weights
+// of four pieces in the lanes, one per g, and meet in LDS at `red`, a wave's share each.
+template <bool TWO, int PW, int CB, int QUADS = 2 / CB>
 __device__ __forceinline__ void join_rows(const Parts& prefix, const Parts& own, uint16_t* out, float* lse, long long row,
                                           bool mine, const Pieces& p0, const Pieces& p1, int cb, int pw,
                                           f32x4 (*red)[CB][64], float2 (*red_ml)[16]) {
-  constexpr int QUADS = 2 / CB, AHEAD = 4 * QUADS;
+  constexpr int AHEAD = 4 * QUADS;
   const int lane = threadIdx.x & 63, g = lane >> 4;
   const int n = p0.n + p1.n;
   int most = mine ? n : 0;
@@ -1599,8 +1600,7 @@ __device__ __forceinline__ void join_rows(const Parts& prefix, const Parts& own,
     lse[row] = sum == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
-// The first row of tile k of those that have more than kLatentMany pieces, -1 where there are
-// fewer, and their number.
+// The first row of tile k of those that are noted, -1 where there are fewer, and their number.
 struct Many {
   int first, n;
 };
@@ -1623,18 +1623,18 @@ __device__ __forceinline__ Many many_tile(const int* many, int k) {
 
 // Units of 16 query rows and CB blocks of 16 columns, PW waves to each.  TWO: every row; else
 // those of tiles that were cut.  MANY: before the units come kManyGroups work-groups for
-// the rows of more than kLatentMany pieces, which the units leave out: what a row has follows
+// the rows of more than `few` pieces, which the units leave out: what a row has follows
 // from the lengths, which the host does not read.  Us, whole call, e4m3, 16 heads, the units
-// alone / with these: one of 100001 keys beside 15 of 100 39.2 / 30.4, beside 31 85.1 / 30.5, beside
-// 63 79.2 / 31.7; four of 30000 beside 28 of 500 41.4 / 29.8; 32 of 600 to 8000 33.3 / 33.0; of 6000
-// 36.5 / 37.1.  In work-groups of four waves: 34 for the first three, 32.4 and 36.5 for the last two.
+// alone / with these: one of 100001 keys beside 15 of 100 38.9 / 30.0, beside 31 85.1 / 30.3, beside
+// 63 79.1 / 31.6; four of 30000 beside 28 of 500 41.4 / 29.4; 32 of 600 to 8000 33.3 / 32.9; of 6000
+// 36.4 / 36.7.  In work-groups of four waves: 34 for the first three, 32.4 and 36.5 for the last two.
 template <int PW>
 constexpr int join_blocks() { return PW >= 8 ? 1 : 2; }
 template <int PW, bool MANY>
 constexpr int join_waves() { return PW > 4 ? PW : MANY ? kLatentManyWaves : 4; }
 template <bool TWO, int PW, bool MANY>
 __global__ __launch_bounds__((64 * join_waves<PW, MANY>()))
-void latent_join_kernel(Parts prefix, Parts own, uint16_t* out, float* lse, int rows) {
+void latent_join_kernel(Parts prefix, Parts own, uint16_t* out, float* lse, int rows, int few) {
   constexpr int CB = join_blocks<PW>(), WAVES = join_waves<PW, MANY>(), TILES = WAVES / PW;
   __shared__ f32x4 red[PW > 1 || MANY ? WAVES * CB : 1][64];
   __shared__ float2 red_ml[WAVES][16];
@@ -1659,11 +1659,12 @@ void latent_join_kernel(Parts prefix, Parts own, uint16_t* out, float* lse, int 
             p1 = pieces_of(own, row);
             if constexpr (TWO) p0 = pieces_of(prefix, row);
           }
-          const bool mine = pass == 0 ? p1.row == at && p1.n > kLatentMany
-                                      : p0.row == at && p0.n > kLatentMany && p1.n <= kLatentMany;
-          // the wave's number from a vector register: with two passes scalar ones are short
-          join_rows<TWO, WAVES, 1>(prefix, own, out, lse, row, mine, p0, p1, block % 32, threadIdx.x >> 6,
-                                   reinterpret_cast<f32x4(*)[1][64]>(red), red_ml);
+          const bool mine = pass == 0 ? p1.row == at && p1.n > few
+                                      : p0.row == at && p0.n > few && p1.n <= few;
+          // The wave's number from a vector register: with two passes scalar ones are short.  So are vector ones:
+          // eight pieces each leave the units three waves per SIMD where they had five, 54 us for 49.
+          join_rows<TWO, WAVES, 1, TWO ? 1 : 2>(prefix, own, out, lse, row, mine, p0, p1, block % 32,
+                                                threadIdx.x >> 6, reinterpret_cast<f32x4(*)[1][64]>(red), red_ml);
           __syncthreads();  // `red` has been read
         }
       }
@@ -1679,7 +1680,7 @@ void latent_join_kernel(Parts prefix, Parts own, uint16_t* out, float* lse, int 
     if constexpr (TWO) p0 = pieces_of(prefix, row);
   }
   bool mine = TWO ? row < rows && own.has(row) : p1.n >= 2;
-  if (MANY && (p0.n > kLatentMany || p1.n > kLatentMany)) mine = false;
+  if (MANY && (p0.n > few || p1.n > few)) mine = false;
   if (PW == 1 && !__any(mine)) return;
   join_rows<TWO, PW, CB>(prefix, own, out, lse, row, mine, p0, p1, unit % (32 / CB) * CB, wave % PW,
                          reinterpret_cast<f32x4(*)[CB][64]>(red + wave / PW * PW * CB), red_ml + wave / PW * PW);
@@ -1692,8 +1693,22 @@ int launch_join(const Args& prefix, const Args& own, int prefix_mr, int own_mr, 
   hipLaunchKernelGGL((latent_join_kernel<TWO, PW, MANY>),
                      dim3((unsigned)((units + TILES - 1) / TILES + (MANY ? kManyGroups : 0))),
                      dim3(64 * join_waves<PW, MANY>()), 0, st, parts_of(prefix, prefix_mr), parts_of(own, own_mr), own.out,
-                     own.lse, (int)rows);
+                     own.lse, (int)rows, own.few);
   return (int)hipGetLastError();
+}
+template <bool TWO>
+int pick_join(const LatentJoin& join, const Args& prefix, const Args& own, int prefix_mr, int own_mr, hipStream_t st) {
+  const bool many = join.few != INT_MAX;
+  switch (join.waves) {
+    case 16: return launch_join<TWO, 16, false>(prefix, own, prefix_mr, own_mr, st);
+    case 8: return launch_join<TWO, 8, false>(prefix, own, prefix_mr, own_mr, st);
+    case 4:
+      return many ? launch_join<TWO, 4, true>(prefix, own, prefix_mr, own_mr, st)
+                  : launch_join<TWO, 4, false>(prefix, own, prefix_mr, own_mr, st);
+    default:
+      return many ? launch_join<TWO, 1, true>(prefix, own, prefix_mr, own_mr, st)
+                  : launch_join<TWO, 1, false>(prefix, own, prefix_mr, own_mr, st);
+  }
 }
 
 // The pieces of a row, a step each at least: on average, and at most.
@@ -1706,26 +1721,17 @@ Counts pieces(const Args& a, int mr) {
   const long long steps = table * a.pages.page_size / kKeys + 1;
   return Counts{std::min(dealt, steps), std::min<long long>(kUnits / a.side_by_side, steps)};
 }
-template <bool TWO>
-int pick_join(const Args& prefix, const Args& own, int prefix_mr, int own_mr, hipStream_t st) {
-  const Counts o = pieces(own, own_mr), p = TWO ? pieces(prefix, prefix_mr) : Counts{0, 0};
-  const LatentJoin join = latent_join(o.mean + p.mean, std::max(o.most, p.most), (long long)own.T * own.H);
-  if (join.waves == 16) return launch_join<TWO, 16, false>(prefix, own, prefix_mr, own_mr, st);
-  if (join.waves == 8) return launch_join<TWO, 8, false>(prefix, own, prefix_mr, own_mr, st);
-  if (join.waves == 4)
-    return join.many ? launch_join<TWO, 4, true>(prefix, own, prefix_mr, own_mr, st)
-                     : launch_join<TWO, 4, false>(prefix, own, prefix_mr, own_mr, st);
-  return join.many ? launch_join<TWO, 1, true>(prefix, own, prefix_mr, own_mr, st)
-                   : launch_join<TWO, 1, false>(prefix, own, prefix_mr, own_mr, st);
-}
 
 template <int MR, bool F8, void (*kernel)(Args)>
-int launch(const Args& a, hipStream_t st) {
+int launch(Args a, hipStream_t st) {
+  const Counts n = pieces(a, MR);
+  const LatentJoin join = latent_join(n.mean, n.most, (long long)a.T * a.H);
+  a.few = join.few;
   constexpr int lds = tile_lds<MR, F8>();
   FERRET_HIP_CHECK((set_lds_limit_once<kernel>(lds)));
   hipLaunchKernelGGL(kernel, dim3(kUnits), dim3(tile_threads<MR>()), lds, st, a);
   FERRET_HIP_CHECK(hipGetLastError());
-  return pick_join<false>(a, a, MR, MR, st);
+  return pick_join<false>(join, a, a, MR, MR, st);
 }
 
 template <bool F8>
@@ -1747,15 +1753,18 @@ int launch_prefixed(int mr, const Args& a, hipStream_t st) {
 }
 
 template <int MRO, bool F8>
-int launch_shared(const Args& prefix, const Args& own, hipStream_t st) {
+int launch_shared(Args prefix, Args own, hipStream_t st) {
   using S = Shared<MRO, F8>;
+  const Counts p = pieces(prefix, kWideRows), o = pieces(own, MRO);
+  const LatentJoin join = latent_join(p.mean + o.mean, std::max(p.most, o.most), (long long)own.T * own.H);
+  prefix.few = own.few = join.few;
   // What a step of the prefix's tiles takes of one of the own.  Us, 64 sequences behind 8192 keys, e4m3:
   // 16 heads 50.8 with 2, 49.0 with 3, 52.7 with 4; 32 heads 72.7 with 1.5, 69.4 with 2, 82.5 with 3.
   constexpr float weight = MRO == 32 ? 2.f : 3.f;
   FERRET_HIP_CHECK((set_lds_limit_once<latent_shared_kernel<MRO, F8>>(S::kLds)));
   hipLaunchKernelGGL((latent_shared_kernel<MRO, F8>), dim3(kUnits), dim3(S::kThreads), S::kLds, st, prefix, own, weight);
   FERRET_HIP_CHECK(hipGetLastError());
-  return pick_join<true>(prefix, own, kWideRows, MRO, st);
+  return pick_join<true>(join, prefix, own, kWideRows, MRO, st);
 }
 
 template <bool F8>
@@ -1822,6 +1831,7 @@ Args pass_args(const void* q_latent, long long ql_token, long long ql_head, cons
   a.out = static_cast<uint16_t*>(out);
   a.lse = lse;
   a.whole = 0;
+  a.few = INT_MAX;
   a.ws = static_cast<uint8_t*>(ws) + kUnits * sizeof(int);
   return a;
 }

@@ -19,7 +19,6 @@ namespace ferret {
 constexpr int kLatentKeys = 64;    // keys per step
 constexpr int kLatentUnits = 256;  // work-groups the work is dealt to: one per CU
 constexpr int kLatentExtra = 5;    // steps that going from one tile to the next costs
-constexpr int kLatentMany = 12;    // pieces of a tile past which its rows are joined by work-groups of their own
 
 FERRET_HD int plan_min(int a, int b) { return a < b ? a : b; }
 FERRET_HD int plan_max(int a, int b) { return a > b ? a : b; }
@@ -144,15 +143,16 @@ FERRET_HD LatentRecord latent_record(int unit, int lane, int side, int cur, int 
 FERRET_HD int latent_record_slot(const LatentRecord& r, int side, int piece) {
   return piece == 0 ? r.slot0 : (r.slot0 & ~1) + 2 * side * piece;
 }
-// The first row, among all, of the tile of more than kLatentMany pieces that a work-group begins, -1
+// The first row, among all, of the tile of more than `few` pieces that a work-group begins, -1
 // where it begins none: the tile is the last of its share, which ends at `end` of the line, in
 // sequence `s`, at `seq_at`, and takes all of the next shares but the last of its own.
 FERRET_HD int latent_many(const LatentSeq& s, int seq_at, int extra, int end, int chunk, int side, int lane, int mr,
-                          int H) {
-  if (s.steps <= (kLatentMany - 1) * chunk) return -1;
+                          int H, int few) {
+  const long long whole = (long long)(few - 1) * chunk;
+  if (s.steps <= whole) return -1;
   const int group = (end - 1 - seq_at) / (s.steps + extra), at = seq_at + group * (s.steps + extra);
   const int row0 = (group * side + lane) * mr;
-  const bool many = group < s.groups && at >= end - chunk && s.steps > end - at + (kLatentMany - 1) * chunk;
+  const bool many = group < s.groups && at >= end - chunk && s.steps > end - at + whole;
   return many && row0 < s.rows ? s.q0 * H + row0 : -1;
 }
 // More than one piece, all of them inside the workspace (a row that no sequence
@@ -163,22 +163,22 @@ FERRET_HD bool latent_record_joins(const LatentRecord& r, int side) {
 }
 
 // How the pieces of `rows` rows are joined: by `waves` waves to 16 rows, which take
-// latent_join_ahead() pieces at a time together, and with `many` the rows of more than kLatentMany pieces
-// by work-groups of kLatentManyWaves waves.  mean: a row's pieces on average, all work-groups at the rows
+// latent_join_ahead() pieces at a time together, but rows of more than `few` pieces by work-groups of
+// kLatentManyWaves waves.  mean: a row's pieces on average, all work-groups at the rows
 // there are; most: where one sequence has nearly all of the keys.  Us, whole call, with 1 / 4 / 8 /
 // 16 waves: 16 heads, e4m3, one sequence of 100001 (256 pieces) - / - / 29.7 / 28.0; 128 heads, four of 9831 (32)
-// - / 34.2 / 34.1 / 38.9; 64 sequences behind 8192 keys (16 + 4) 50.7 / 49.2 / - / 58.5.  Without `many` where
-// a row cannot have that many more: chunks of 200 to 500 tokens (32 pieces at most), 64 rows to a tile, 168.9 against 175.4.
+// - / 34.2 / 34.1 / 38.9; 64 sequences behind 8192 keys (16 + 4) 50.7 / 49.2 / - / 58.5.  These with 12 for
+// few: 54.  Rows that can have 32 pieces at most (chunks of 200 to 500 tokens): 168.9, with few 12 175.4.
 constexpr int kLatentManyWaves = 8;
 constexpr long long kLatentManyRows = 1 << 20;  // with more, the others' joins take longer than any one row's
 struct LatentJoin {
-  int waves;
-  bool many;
+  int waves, few;  // few: INT_MAX where every row is joined alike
 };
 inline LatentJoin latent_join(long long mean, long long most, long long rows) {
-  if (mean >= 200) return LatentJoin{16, false};
-  if (mean >= 24) return LatentJoin{8, false};
-  return LatentJoin{mean >= 10 ? 4 : 1, most >= 4 * kLatentMany && rows <= kLatentManyRows};
+  if (mean >= 200) return LatentJoin{16, INT_MAX};
+  if (mean >= 24) return LatentJoin{8, INT_MAX};
+  const bool alike = most < 48 || rows > kLatentManyRows;
+  return mean >= 10 ? LatentJoin{4, alike ? INT_MAX : 48} : LatentJoin{1, alike ? INT_MAX : 12};
 }
 inline int latent_join_ahead(int waves) { return waves * (waves >= 8 ? 8 : 4); }
 

@@ -20,7 +20,7 @@ using namespace ferret;
 
 static int worst = 0;
 
-// The tiles of more than kLatentMany pieces are those that the work-groups note, each by the one that begins it.
+// The tiles of more than `few` pieces are those that the work-groups note, each by the one that begins it.
 static int walk(const std::vector<int>& n, const std::vector<int>& lens, int H, int mr, int side, int most, int min_steps) {
   std::vector<LatentSeq> seqs;
   int T = 0, q0 = 0, all = 0, groups = 0;
@@ -33,6 +33,11 @@ static int walk(const std::vector<int>& n, const std::vector<int>& lens, int H, 
   bool whole = true;
   for (const auto& s : seqs) whole = whole && latent_fits(s, latent_chunk(all, units, min_steps));
   const LatentDeal d = latent_deal(all, groups, whole, units, min_steps);
+  const long long rows = (long long)T * H, steps = most / kLatentKeys + 1;
+  long long mean = (long long)kLatentUnits * mr / rows, top = kLatentUnits / side;
+  if (steps < mean) mean = steps;
+  if (steps < top) top = steps;
+  const LatentJoin j = latent_join(mean, top, rows);
   std::set<int> want, got;
   int at = 0, longest = 0;
   for (const auto& s : seqs)
@@ -40,7 +45,7 @@ static int walk(const std::vector<int>& n, const std::vector<int>& lens, int H, 
       const int unit = at / d.chunk, pieces = latent_record(unit, 0, side, at, s.steps, d.chunk).pieces;
       if (pieces > longest) longest = pieces;
       for (int lane = 0; lane < side; ++lane)
-        if ((g * side + lane) * mr < s.rows && pieces > kLatentMany) want.insert(s.q0 * H + (g * side + lane) * mr);
+        if ((g * side + lane) * mr < s.rows && pieces > j.few) want.insert(s.q0 * H + (g * side + lane) * mr);
     }
   for (int block = 0; block < kLatentUnits; ++block) {
     const LatentPlace p = latent_place(block, side);
@@ -48,20 +53,15 @@ static int walk(const std::vector<int>& n, const std::vector<int>& lens, int H, 
     if (start >= d.total) continue;
     int b = 0, seq_at = 0;
     while (seq_at + seqs[b].work(d.extra) <= end - 1) seq_at += seqs[b++].work(d.extra);
-    const int row = latent_many(seqs[b], seq_at, d.extra, end, d.chunk, side, p.lane, mr, H);
+    const int row = latent_many(seqs[b], seq_at, d.extra, end, d.chunk, side, p.lane, mr, H, j.few);
     if (row >= 0 && !got.insert(row).second) return 1;
   }
   if (want != got) return 2;
   // what one wave or group of waves takes one after another
-  const long long rows = (long long)T * H, steps = most / kLatentKeys + 1;
-  long long mean = (long long)kLatentUnits * mr / rows, top = kLatentUnits / side;
-  if (steps < mean) mean = steps;
-  if (steps < top) top = steps;
   if (longest > top) return 3;
-  const LatentJoin j = latent_join(mean, top, rows);
-  const int left = j.many && longest > kLatentMany ? kLatentMany : longest;
+  const int left = longest > j.few ? j.few : longest;
   const int by_units = (left + latent_join_ahead(j.waves) - 1) / latent_join_ahead(j.waves);
-  const int by_many = j.many ? (longest + latent_join_ahead(kLatentManyWaves) - 1) / latent_join_ahead(kLatentManyWaves) : 0;
+  const int by_many = longest > j.few ? (longest + latent_join_ahead(kLatentManyWaves) - 1) / latent_join_ahead(kLatentManyWaves) : 0;
   for (int r : {by_units, by_many})
     if (r > worst) worst = r;
   return 0;
