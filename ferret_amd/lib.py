@@ -85,6 +85,16 @@ class FerretError(RuntimeError):
         self.code = code
 
 
+class _Int(ctypes.c_int):
+    """An int argument: ctypes takes the low 32 bits of any number, and a call would run on other sizes."""
+
+    @classmethod
+    def from_param(cls, v):
+        if isinstance(v, int) and not -(1 << 31) <= v < 1 << 31:
+            raise ValueError(f"{v} does not fit the 32 bits of an int")
+        return ctypes.c_int.from_param(v)
+
+
 _LIB = None
 _NATIVE = None
 NATIVE_PATH = os.path.join(os.path.dirname(LIB_PATH), "_native.so")
@@ -129,7 +139,7 @@ def load():
     for name, (res, args) in SIGNATURES.items():
         fn = getattr(lib, name)
         fn.restype = res
-        fn.argtypes = args
+        fn.argtypes = [_Int if t is _c_int else t for t in args]
     _LIB = lib
     return lib
 

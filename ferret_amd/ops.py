@@ -29,9 +29,17 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def _counted(t: torch.Tensor, name: str) -> None:
+    """Dimensions that the C ABI counts in 32 bits."""
+    if any(n >= 1 << 31 for n in t.shape):
+        raise ValueError(f"{name}'s dimensions must be below 2^31, got shape {tuple(t.shape)}")
+
+
 def _dev(t: torch.Tensor, name: str, dtype=None, ndim=None) -> int:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
+    if ndim is not None:
+        _counted(t, name)
     if t.device.type != "cuda":
         raise ValueError(f"{name} must be a GPU tensor (got {t.device}); ferret_amd has no CPU path")
     if dtype is not None and t.dtype not in (dtype if isinstance(dtype, tuple) else (dtype,)):
@@ -535,6 +543,7 @@ def _rows(t: torch.Tensor, name: str, shape: tuple, dtype=torch.bfloat16) -> tup
     dimensions in elements, all on the kernels' bounds of 16 bytes."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
+    _counted(t, name)
     if t.device.type != "cuda":
         raise ValueError(f"{name} must be a GPU tensor (got {t.device}); ferret_amd has no CPU path")
     if t.dtype != dtype:
