@@ -1772,15 +1772,6 @@ int launch_shared_rows(int own_mr, const Args& prefix, const Args& own, hipStrea
   return own_mr == 16 ? launch_shared<16, F8>(prefix, own, st) : launch_shared<32, F8>(prefix, own, st);
 }
 
-// Query rows per tile by the rows that a sequence has on average.  Us, e4m3, 64 sequences
-// of 3000: 32 heads 46.9 in tiles of 32, 56.7 of 16, 48.7 of 64; 16 heads of 600 to 8000
-// 50.4 of 16, 54.6 of 32; 32 of 3000, 64 heads 39.8 of 64, 45.3 of 32; 128 heads, bf16,
-// 32 of 900 to 6000 58.8 of 64 against 80.6 of 32.
-int tile_rows(int T, int B, int H) {
-  const long long rows = (long long)T * H / B;
-  return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-}
-
 // Row tiles side by side by the tiles that a sequence has on average: work-groups of one
 // XCD that walk the same keys at the same time.  128 heads (two tiles), bf16, 32 sequences of
 // 900 to 6000: 58.8 us two at a time, 66.0 one after another, 79.9 four; 500 new tokens of
@@ -1847,21 +1838,6 @@ size_t pass_bytes(int B, int T, int H, int mr, int whole) {
   return kUnits * sizeof(int) + rows + (size_t)a.blocks(mr) * 16 * (sizeof(float2) + kLatent * sizeof(float));
 }
 
-// Whether prefixes of `keys` keys at most get a pass of their own: where the steps that it saves
-// pay for the partials of every row.  A step takes 1 for a tile of 16 rows, 1.7 of 32, 3 of 64; a
-// sequence is one tile where it fills none of 64, a prefix's tokens are tiles of 64.  Saved steps
-// and us, two passes / one: 16 heads, 64 sequences behind 8192 keys, e4m3, 2048: 49 / 69; 8 prompts of
-// 2600 with 8 samples each 656: 35.4 / 36.9, 16 prompts with 4 each 656: 37.2 / 37.0; 64 behind 2000
-// 512: 34.1 / 33.7; 16 behind 8192 512: 34.2 / 30.1; 21 prompts of 6000 with 3 each, bf16, none: 76 / 71; 32
-// heads, 64 behind 8192 1638: 70 / 88, 32 behind 12000 1203: 66.5 / 69.2, behind 6000 602: 50.6 / 45.5.
-bool prefix_pass(int G, int B, int T, int H, long long keys) {
-  const int own = tile_rows(T, B, H);
-  if (own == kWideRows) return false;
-  const long long tiles = plan_min(B, T), rows = ((long long)T * H + G - 1) / G;
-  const long long saved = tiles * (own == 16 ? 10 : 17) - G * ((rows + kWideRows - 1) / kWideRows) * 30;  // tenths, per step
-  return saved > 0 && saved * ((keys + kKeys - 1) / kKeys) >= 25LL * kUnits;
-}
-
 }  // namespace
 }  // namespace ferret
 
@@ -1874,7 +1850,7 @@ int ferret_check_pages(const int32_t* page_table, int B, int max_pages, int page
 
 extern "C" size_t ferret_latent_attention_workspace(int B, int T, int H) {
   if (B < 1 || T < 1 || H < 1 || !latent_rows_fit(T, H)) return 0;
-  return pass_bytes(B, T, H, tile_rows(T, B, H), 0);
+  return pass_bytes(B, T, H, latent_tile_rows(T, B, H), 0);
 }
 
 extern "C" int ferret_latent_attention(const void* q_latent, long long ql_token, long long ql_head,
@@ -1894,7 +1870,7 @@ extern "C" int ferret_latent_attention(const void* q_latent, long long ql_token,
   FERRET_REQUIRE(((bits(q_latent) | bits(q_rotary) | bits(data) | bits(out)) & 15) == 0 &&
                      ((bits(scales) | bits(lse)) & 3) == 0 && ((ql_token | ql_head | qr_token | qr_head) & 7) == 0,
                  FERRET_ERR_ALIGN);
-  const int mr = tile_rows(T, B, H);
+  const int mr = latent_tile_rows(T, B, H);
   const int steps = check_steps(B, (long long)max_pages * page_size, pages, page_size, T, H, mr);
   if (steps != FERRET_OK) return steps;
   const size_t need = ferret_latent_attention_workspace(B, T, H);
@@ -1918,8 +1894,8 @@ extern "C" int ferret_latent_attention(const void* q_latent, long long ql_token,
 
 extern "C" size_t ferret_latent_attention_shared_workspace(int G, int B, int T, int H) {
   if (G < 1 || B < 1 || T < 1 || H < 1 || !latent_rows_fit(T, H) || (G > B ? G : B) >= 1 << 26) return 0;
-  const int own = tile_rows(T, B, H);
-  if (!prefix_pass(G, B, T, H, 1LL << 31)) return pass_bytes(B, T, H, own, 0);
+  const int own = latent_tile_rows(T, B, H);
+  if (!latent_prefix_pass(G, B, T, H, 1LL << 31)) return pass_bytes(B, T, H, own, 0);
   // A call with shorter tables takes one pass, and less.
   return ((pass_bytes(G, T, H, kWideRows, 1) + 255) & ~(size_t)255) + pass_bytes(B, T, H, own, 1);
 }
@@ -1944,9 +1920,9 @@ extern "C" int ferret_latent_attention_shared(const void* q_latent, long long ql
   FERRET_REQUIRE(((bits(q_latent) | bits(q_rotary) | bits(data) | bits(out)) & 15) == 0 &&
                      ((bits(scales) | bits(lse)) & 3) == 0 && ((ql_token | ql_head | qr_token | qr_head) & 7) == 0,
                  FERRET_ERR_ALIGN);
-  const int own_mr = tile_rows(T, B, H);
+  const int own_mr = latent_tile_rows(T, B, H);
   const long long prefix_keys = (long long)max_prefix_pages * page_size, own_keys = (long long)max_pages * page_size;
-  const bool two = prefix_pass(G, B, T, H, prefix_keys);
+  const bool two = latent_prefix_pass(G, B, T, H, prefix_keys);
   FERRET_REQUIRE(prefix_keys + own_keys <= (1LL << 31) - 4 * kKeys, FERRET_ERR_SHAPE);
   rc = two ? check_steps(G, prefix_keys, pages, page_size, T, H, kWideRows) : FERRET_OK;
   if (rc == FERRET_OK)

@@ -182,4 +182,35 @@ inline LatentJoin latent_join(long long mean, long long most, long long rows) {
 }
 inline int latent_join_ahead(int waves) { return waves * (waves >= 8 ? 8 : 4); }
 
+// Query rows per tile by the rows that a sequence has on average.  Us, e4m3, 64 sequences
+// of 3000: 32 heads 46.9 in tiles of 32, 56.7 of 16, 48.7 of 64; 16 heads of 600 to 8000
+// 50.4 of 16, 54.6 of 32; 32 of 3000, 64 heads 39.8 of 64, 45.3 of 32; 128 heads, bf16,
+// 32 of 900 to 6000 58.8 of 64 against 80.6 of 32.
+inline int latent_tile_rows(int T, int B, int H) {
+  const long long rows = (long long)T * H / B;
+  return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+}
+
+// Whether prefixes of `keys` keys at most get a pass of their own: where the steps that it saves
+// pay for the partials of every row: for 2.5 steps per CU at the least, and for a step per 2560 rows and
+// CU where those are more.  A step takes 1 for a tile of 16 rows, 1.7 of 32, 3 of 64; a
+// sequence is one tile where it fills none of 64, a prefix's tokens are tiles of 64.  Saved steps
+// and us, two passes / one: 16 heads, 64 sequences behind 8192 keys, e4m3, 2048: 49 / 69; 8 prompts of
+// 2600 with 8 samples each 656: 35.4 / 36.9, 16 prompts with 4 each 656: 37.2 / 37.0; 64 behind 2000
+// 512: 34.1 / 33.7; 16 behind 8192 512: 34.2 / 30.1; 21 prompts of 6000 with 3 each, bf16, none: 76 / 71; 32
+// heads, 64 behind 8192 1638: 70 / 88, 32 behind 12000 1203: 66.5 / 69.2, behind 6000 602: 50.6 / 45.5.
+// Many rows: 400 of 16 heads behind 1024 1600: 66 / 74; 512 of 32 heads, bf16, behind 512 819: 105 / 86, behind
+// 1024 1638: 117 / 109, behind 2048 3277: 148 / 160.  Over 420 batches of 4 to 32 heads, 16 to 512 sequences and
+// 1 to 64 prefixes of 400 to 9000 keys the choice takes 1% longer than the better way on average, 7% in 95 of 100;
+// at most 40%: 21 prompts of 9000 with 3 sequences of 4 heads each, where the tiles of 64 are a fifth full and one
+// pass is chosen.
+inline bool latent_prefix_pass(int G, int B, int T, int H, long long keys) {
+  const int own = latent_tile_rows(T, B, H);
+  if (own == 64) return false;
+  const long long tiles = plan_min(B, T), all = (long long)T * H, rows = (all + G - 1) / G;
+  const long long saved = tiles * (own == 16 ? 10 : 17) - G * ((rows + 63) / 64) * 30;  // tenths, per step
+  const long long least = 25LL * kLatentUnits;
+  return saved > 0 && saved * ((keys + kLatentKeys - 1) / kLatentKeys) >= (all > least ? all : least);
+}
+
 }  // namespace ferret
