@@ -50,17 +50,14 @@ struct Cfg {
   static constexpr int kLds = kRing > kEpi ? kRing : kEpi;
   static constexpr int kQuads = kRows / 4;                     // groups of four outputs of a token
   static_assert(kThreads <= 1024 && RT % WR == 0 && TT % WT == 0 && (KS / 64) % WK == 0, "waves");
-  static_assert(kStage % 1024 == 0 && kLds <= 160 * 1024, "LDS budget");
+  static_assert(KS >= 256 && kStage % 1024 == 0 && kLds <= 160 * 1024, "LDS budget");  // 16 chunks to a row: swz
   static_assert(NS >= 2 && (NS - 2) * kLd < 63, "vmcnt range");
 };
 
 // Slot of 16-byte chunk c of stage row `row`: the lanes of a fragment that LDS serves
 // together (rows 0 - 3 and 12 - 15 of one chunk with 4 - 11 of the next) fall on distinct
 // banks.
-template <int KS>
-__device__ __forceinline__ int swz(int row, int c) {
-  return KS >= 256 ? c ^ row : c ^ ((((row >> 1) ^ row) & 4) | (row & 2) | ((row >> 2) & 1));
-}
+__device__ __forceinline__ int swz(int row, int c) { return c ^ row; }
 
 // Wait until at most min(n, N) stages of L loads are in flight.
 template <int L, int N>
@@ -100,7 +97,7 @@ __global__ __launch_bounds__(64 * WR * WT * WK) void int8_tiled_kernel(Args p) {
     const int j = min(wave * C::kLd + i, C::kInstr - 1);
     constexpr int LR = 64 / C::kIRows;         // lanes of a row
     const int lr = C::kIRows * j + lane / LR;  // stage row
-    chunk[i] = swz<KS>(lr & 15, lane % LR);
+    chunk[i] = swz(lr & 15, lane % LR);
     const size_t row = j < C::kWInstr ? min(row0 + lr, p.N - 1) : min(tok0 + lr - C::kRows, p.M - 1);
     src[i] = (j < C::kWInstr ? p.b : p.a) + row * p.K;
   }
@@ -139,7 +136,7 @@ __global__ __launch_bounds__(64 * WR * WT * WK) void int8_tiled_kernel(Args p) {
     const int left = chunks - step_at(step) * (KS / 16);  // chunks of the stage below K
 #pragma unroll
     for (int k = 0; k < C::kKB; ++k) {
-      const int ch = 4 * (wk * C::kKB + k) + g, c = swz<KS>(r, ch) << 4;
+      const int ch = 4 * (wk * C::kKB + k) + g, c = swz(r, ch) << 4;
       u32x4 wf[C::kRB], xf[C::kTB];
 #pragma unroll
       for (int x = 0; x < C::kRB; ++x)

@@ -58,8 +58,8 @@ struct Sq {
 // - 15 and 20 - 27 of 32, or the others) fall on distinct banks.
 template <int KS>
 __device__ __forceinline__ int sq_swz(int row, int c) {
-  const int x = row >> 2;
-  return KS == 256 ? c ^ (row & 15) : KS == 128 ? c ^ ((row >> 1) & 7) : c ^ ((((x ^ (x >> 1)) & 1) << 1) | ((x >> 1) & 1));
+  static_assert(KS == 128 || KS == 256, "bytes of a stage row");
+  return KS == 256 ? c ^ (row & 15) : c ^ ((row >> 1) & 7);
 }
 
 template <int BN, int BM, int KS, int NW, int NT, int WR, int WT>
