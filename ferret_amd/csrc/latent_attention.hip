@@ -1473,9 +1473,9 @@ __device__ __forceinline__ Pieces pieces_of(const Parts& a, long long row) {
   const LatentRecord where{rec.x / a.per, rec.y};
   if (latent_record_joins(where, a.side)) {
     p.n = where.pieces;
-    p.first = where.slot0 * a.per + f;
-    p.rest = (where.slot0 & ~1) * a.per + f;
     p.step = 2 * a.side * a.per;
+    p.first = latent_record_slot(where, a.side, 0) * a.per + f;
+    p.rest = latent_record_slot(where, a.side, 1) * a.per + f - p.step;
   } else if (rec.y == 1 && rec.x >= 2 * kUnits * a.per && rec.x < a.blocks - f) {
     p.n = 1;
     p.first = rec.x + f;
