@@ -21,3 +21,12 @@ def hip():
         pytest.skip("no GPU visible")
     from ferret_amd import lib
     return lib.load()
+
+
+@pytest.fixture(autouse=True)
+def _native_call_path():
+    """A test that puts something else in the place of lib.native leaves the next one the library's own."""
+    from ferret_amd import lib
+    native = lib.native
+    yield
+    lib.native = native
