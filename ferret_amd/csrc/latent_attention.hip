@@ -1662,7 +1662,7 @@ void latent_join_kernel(Parts prefix, Parts own, uint16_t* out, float* lse, int 
           const bool mine = pass == 0 ? p1.row == at && p1.n > few
                                       : p0.row == at && p0.n > few && p1.n <= few;
           // The wave's number from a vector register: with two passes scalar ones are short.  So are vector ones:
-          // eight pieces each leave the units three waves per SIMD where they had five, 54 us for 49.
+          // with eight pieces each the units have three waves per SIMD instead of five.
           join_rows<TWO, WAVES, 1, TWO ? 1 : 2>(prefix, own, out, lse, row, mine, p0, p1, block % 32,
                                                 threadIdx.x >> 6, reinterpret_cast<f32x4(*)[1][64]>(red), red_ml);
           __syncthreads();  // `red` has been read
@@ -1703,8 +1703,9 @@ int pick_join(const LatentJoin& join, const Args& prefix, const Args& own, int p
     case 16: return launch_join<TWO, 16, false>(prefix, own, prefix_mr, own_mr, st);
     case 8: return launch_join<TWO, 8, false>(prefix, own, prefix_mr, own_mr, st);
     case 4:
-      return many ? launch_join<TWO, 4, true>(prefix, own, prefix_mr, own_mr, st)
-                  : launch_join<TWO, 4, false>(prefix, own, prefix_mr, own_mr, st);
+      if constexpr (!TWO)
+        if (many) return launch_join<TWO, 4, true>(prefix, own, prefix_mr, own_mr, st);
+      return launch_join<TWO, 4, false>(prefix, own, prefix_mr, own_mr, st);
     default:
       return many ? launch_join<TWO, 1, true>(prefix, own, prefix_mr, own_mr, st)
                   : launch_join<TWO, 1, false>(prefix, own, prefix_mr, own_mr, st);
@@ -1725,7 +1726,7 @@ Counts pieces(const Args& a, int mr) {
 template <int MR, bool F8, void (*kernel)(Args)>
 int launch(Args a, hipStream_t st) {
   const Counts n = pieces(a, MR);
-  const LatentJoin join = latent_join(n.mean, n.most, (long long)a.T * a.H);
+  const LatentJoin join = latent_join(n.mean, n.most, (long long)a.T * a.H, false);
   a.few = join.few;
   constexpr int lds = tile_lds<MR, F8>();
   FERRET_HIP_CHECK((set_lds_limit_once<kernel>(lds)));
@@ -1756,7 +1757,7 @@ template <int MRO, bool F8>
 int launch_shared(Args prefix, Args own, hipStream_t st) {
   using S = Shared<MRO, F8>;
   const Counts p = pieces(prefix, kWideRows), o = pieces(own, MRO);
-  const LatentJoin join = latent_join(p.mean + o.mean, std::max(p.most, o.most), (long long)own.T * own.H);
+  const LatentJoin join = latent_join(p.mean + o.mean, std::max(p.most, o.most), (long long)own.T * own.H, true);
   prefix.few = own.few = join.few;
   // What a step of the prefix's tiles takes of one of the own.  Us, 64 sequences behind 8192 keys, e4m3:
   // 16 heads 50.8 with 2, 49.0 with 3, 52.7 with 4; 32 heads 72.7 with 1.5, 69.4 with 2, 82.5 with 3.

@@ -209,3 +209,29 @@ def test_nan_stays_with_its_tokens(ops, e4m3):
     got = plant(2 + 6, 29)      # the last key of sequence 6
     others = [i for i in range(8) if i != 6]
     assert torch.isnan(got[6]).all() and torch.equal(got[others], want[others])
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_no_tokens_behind_the_prefixes(ops, e4m3):
+    """All of the work-groups go to the sequences where no token sees a prefix, all to the prefixes where the sequences'
+    keys are none, and where there are no tokens nothing is written."""
+    print(f"[case] two passes, none of one line e4m3={e4m3}", flush=True)
+    s = Shared([(300, [(30, 1), (65, 1), (0, 1), (64, 1)]), (75, [(7, 1)] * 4)], 16, 16, e4m3, 31)
+    kw = s.wide()
+    for none in ([0, 0, 0], [4, 4, 4], [8, 8, 8]):
+        out, lse = two_passes(ops, s, kw={**kw, "cu_prefix": i32(none)})
+        want = ops.latent_attention(bf16_tensor(s.ql), bf16_tensor(s.qr), s.batch.cache, kw["page_table"], kw["lens"],
+                                    kw["cu_q"], SCALE, return_lse=True)
+        alone = Shared([(None, s.own)], 16, 16, e4m3, 31)
+        alone.batch, alone.ql, alone.qr, alone.G = s.batch, s.ql, s.qr, 2
+        alone.check(out, lse)
+        alone.check(*want)
+    out, lse = two_passes(ops, s, kw={**kw, "lens": i32([0] * 8)})
+    s.groups = [(300, [(0, 1)] * 4), (75, [(0, 1)] * 4)]
+    for line in range(2, 10):
+        s.batch.lat[line], s.batch.rot[line] = s.batch.lat[line][:0], s.batch.rot[line][:0]
+    s.check(out, lse)
+    out = torch.full((8, 16, 512), 7.0, dtype=torch.bfloat16, device="cuda")
+    two = {**kw, "cu_q": i32([0] * 9), "cu_prefix": i32([0] * 3)}
+    ops.latent_attention_shared(bf16_tensor(s.ql), bf16_tensor(s.qr), s.batch.cache, **two, scale=SCALE, out=out)
+    assert (out == 7).all()

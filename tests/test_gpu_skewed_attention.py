@@ -4,7 +4,8 @@ import numpy as np
 import pytest
 import torch
 
-from tests.attention_helpers import SCALE, Batch, bf16_tensor, bf16_values, check_absorbed, i32, starts
+from oracle import attention as A
+from tests.attention_helpers import SCALE, Batch, assert_near, bf16_tensor, bf16_values, check_absorbed, i32, starts
 from tests.test_gpu_shared_attention import Shared
 
 pytestmark = pytest.mark.gpu
@@ -117,3 +118,40 @@ def test_shared_prefixes(ops, name, H, e4m3):
     s = Shared(GROUPS[name], H, 64, e4m3, H)
     assert s.wide() is not None
     s.run(ops)
+
+
+@pytest.mark.parametrize("H,members", [(16, 70), (32, 45)])
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_many_sequences_behind_two_prefixes(ops, H, members, e4m3):
+    """Few pieces on average in both passes, many of one prefix and of one sequence: rows with many of either, of both
+    and of none.  Some sequences against the formula, all against latent_attention over joined tables."""
+    print(f"[case] skewed shared, many sequences H={H} members={members} e4m3={e4m3}", flush=True)
+    page, long = 64, members // 3
+    groups = [(8960, [(20 + i % 50, 1) for i in range(members)]), (64, [(1 + i % 70, 1) for i in range(members)])]
+    groups[0][1][long] = (20000, 1)
+    groups[1][1][5] = (30000, 1)
+    s = Shared(groups, H, page, e4m3, H)
+    assert s.wide() is not None
+    out, lse = s.call(ops, **s.wide())
+    kw = s.index()
+    table = torch.full((2 * members, 140 + kw["page_table"].shape[1]), -1, dtype=torch.int32, device="cuda")
+    for g, pages in ((0, 140), (1, 1)):
+        lines = slice(g * members, (g + 1) * members)
+        table[lines, :pages] = kw["prefix_table"][g, :pages]
+        table[lines, pages:pages + kw["page_table"].shape[1]] = kw["page_table"][lines]
+    lens = kw["lens"] + torch.tensor([8960] * members + [64] * members, dtype=torch.int32, device="cuda")
+    ref = ops.latent_attention(bf16_tensor(s.ql), bf16_tensor(s.qr), s.batch.cache, table, lens, kw["cu_q"], SCALE)
+    torch.cuda.synchronize()
+    assert (out.float() - ref.float()).abs().max() < 2 ** -6 * ref.float().abs().max()
+    out, lse = out.float().cpu().numpy(), lse.cpu().numpy()
+    for b in (0, long, members - 1, members, members + 5, 2 * members - 1):
+        g = b // members
+        lat = np.concatenate([s.batch.lat[g], s.batch.lat[2 + b]])
+        k = np.concatenate([lat, np.concatenate([s.batch.rot[g], s.batch.rot[2 + b]])], 1)
+        see = np.ones((1, len(k)), dtype=bool)
+        for h in range(0, H, 5):
+            q = np.concatenate([s.ql[b:b + 1, h], s.qr[b:b + 1, h]], 1)
+            o, ref_l, spread, reach = A.attend(q, k, lat, SCALE, see)
+            eo, el = A.bounds(o, ref_l, spread, reach, 576, len(k))
+            assert_near(out[b:b + 1, h], o, eo, f"seq {b} head {h}")
+            assert_near(lse[b:b + 1, h], ref_l, el, f"lse seq {b} head {h}")

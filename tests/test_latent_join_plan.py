@@ -37,7 +37,7 @@ static int walk(const std::vector<int>& n, const std::vector<int>& lens, int H, 
   long long mean = (long long)kLatentUnits * mr / rows, top = kLatentUnits / side;
   if (steps < mean) mean = steps;
   if (steps < top) top = steps;
-  const LatentJoin j = latent_join(mean, top, rows);
+  const LatentJoin j = latent_join(mean, top, rows, false);
   std::set<int> want, got;
   int at = 0, longest = 0;
   for (const auto& s : seqs)
