@@ -14,8 +14,8 @@
 // last one of their row, with the tokens' as zeros.  v_mfma_i32_16x16x64_i8: weight rows
 // are the A side, tokens the B side, so a lane holds four outputs in a row of one token.
 // Tiles of 16 rows and 512 bytes let 4096 rows fill the CUs in one launch: 4096 x 12288 at
-// 16 tokens 12.0 us, 13.5 in tiles of 64 rows and splits of K (two launches); 4096 x 4096 at 1
-// 6.1 against 8.4.  24576 x 4096 at 1 token, 96 rows, 17.5 us, 5.8 TB/s.
+// 16 tokens 11.3 to 11.7 us, 12.6 in tiles of 32 rows and 13.0 of 64, with splits of K (two launches);
+// 4096 x 4096 at 1 6.2, 7.5 and 8.7.  24576 x 4096 at 1 token, 96 rows, 17.0 to 17.6 us, 5.7 TB/s or more.
 //
 // Every work-group starts at another K step (row tile index modulo its steps) and wraps
 // around: in lockstep, all of them read the same columns of rows a power of two

@@ -42,8 +42,8 @@
 // keys, e4m3, 49 us, 3.6 TB/s with launch and joins, of which the kernel takes 45.  64
 // rows: no one unit.  32 sequences of 8192, 128 heads, bf16, 98 us: the matrix units
 // are busy for 40% of the cycles, LDS for 27%, the vector units for 20%, and memory
-// delivers 3.0 TB/s; the clock falls to 2.0 GHz under it.  e4m3: the vector units take 39%,
-// widening the keys twice and the values once, beside 40% of products.  Chunks of 60 to 300 tokens
+// delivers 3.0 TB/s; the clock falls to 2.0 GHz under it.  e4m3: the vector units take 35%,
+// widening the keys twice and the values once, beside 41% of products.  Chunks of 60 to 300 tokens
 // behind a prefix of 5000 keys, 16 heads, e4m3, 168 us: without half of the output's products 22
 // less, without the widening 9, the exponentials 5, the loads 5, or the powers of two on P 10: a step is
 // the chain of all of them.  64 sequences of 100 to 1200 behind 8192 shared keys, 16 heads, e4m3, 49 us:

@@ -391,17 +391,19 @@ int ferret_latent_attention(const void* q_latent, long long ql_token, long long 
 
 /*
  * ferret_latent_attention for a batch whose sequences share prefixes: a token sees all
- * prefix_lens[g] keys of its prefix g, which are read once for all of its tokens, then
- * keys of its own sequence as there (lens, causal and page_table count those alone, new
- * tokens included).
+ * prefix_lens[g] keys of its prefix g, which is kept once, then keys of its own sequence as
+ * there (lens, causal and page_table count those alone, new tokens included).  Where T * H / B
+ * is 32 or less, prefix_table is wide and the tokens of a prefix are many, the prefix's keys are
+ * multiplied once for all of its tokens; else every sequence goes through them again.
  * prefix_table int32 [G, max_prefix_pages], prefix_lens int32 [G] (0 for none) and
  * cu_prefix int32 [G + 1], ascending: the packed new tokens that see prefix g (all tokens of
- * its sequences, which stand side by side: none belongs to two); tokens outside [cu_prefix[0],
+ * its sequences, which stand side by side: none belongs to two, and no sequence is cut); tokens outside [cu_prefix[0],
  * cu_prefix[G]) see no prefix.  Both tables are of the one cache.  Everything else, the softmax's statement, out in
  * place, lse, tokens without keys, Inf and NaN, and the range of the sums, as
  * ferret_latent_attention; its requirements for both tables, together (max_pages +
  * max_prefix_pages) * page_size <= 2^31 - 256.
- * ws: ferret_latent_attention_shared_workspace(G, B, T, H) bytes, on a 16-byte bound.
+ * ws: ferret_latent_attention_shared_workspace(G, B, T, H) bytes, on a 16-byte bound,
+ * whatever the widths of the tables.
  */
 size_t ferret_latent_attention_shared_workspace(int G, int B, int T, int H);
 int ferret_latent_attention_shared(const void* q_latent, long long ql_token, long long ql_head, const void* q_rotary,
