@@ -166,8 +166,9 @@ FERRET_HD bool latent_record_joins(const LatentRecord& r, int side) {
 // latent_join_ahead() pieces at a time together, but rows of more than `few` pieces by work-groups of
 // kLatentManyWaves waves.  mean: a row's pieces on average, all work-groups at the rows
 // there are; most: where one sequence has nearly all of the keys.  Us, whole call, with 1 / 4 / 8 /
-// 16 waves: 16 heads, e4m3, one sequence of 100001 (256 pieces) - / - / 29.7 / 28.0; 128 heads, four of 9831 (32)
-// - / 34.2 / 34.1 / 38.9; 64 sequences behind 8192 keys (16 + 4) 50.7 / 49.2 / - / 58.5.  Every row alike / as
+// 16 waves: 16 heads, e4m3, one sequence of 100001 (256 pieces) - / - / 29.7 / 28.0; bf16, two of 2863 and 10431 (128)
+// - / - / 20.5 / 19.6; 128 heads, four of 9831 (512 rows, 32 pieces) - / 34.2 / 34.1 / 38.9; chunks of 27 and 54 tokens,
+// 8 heads (648 rows, 25) - / 27.3 / 31.0 / -; 64 sequences behind 8192 keys (16 + 4) 50.7 / 49.2 / - / 58.5.  Every row alike / as
 // here: rows that can have 32 pieces at most (chunks of 200 to 500 tokens) 168.9, with few 12 175.4; two passes, of
 // which a row has pieces of both, 128 sequences behind 4096 55.3, with few 48 57.8; 256 behind 4096 (5 pieces on
 // average) 73.6 / 74.5, with one of 120000 own keys 97.7 / 86.9.
@@ -177,8 +178,8 @@ struct LatentJoin {
   int waves, few;  // few: INT_MAX where every row is joined alike
 };
 inline LatentJoin latent_join(long long mean, long long most, long long rows, bool two_passes) {
-  if (mean >= 200) return LatentJoin{16, INT_MAX};
-  if (mean >= 24) return LatentJoin{8, INT_MAX};
+  if (mean >= 48 && rows <= 128) return LatentJoin{16, INT_MAX};
+  if (mean >= 24 && rows <= 512) return LatentJoin{8, INT_MAX};
   const bool alike = most < 48 || rows > kLatentManyRows;
   return mean >= 10 ? LatentJoin{4, alike || two_passes ? INT_MAX : 48} : LatentJoin{1, alike ? INT_MAX : 12};
 }

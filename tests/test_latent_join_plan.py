@@ -101,3 +101,16 @@ def test_no_row_is_joined_piece_after_piece(tmp_path):
     subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", f"-I{ROOT}/ferret_amd/csrc", str(src), "-o", str(exe)], check=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True)
     assert r.returncode == 0, r.stdout
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="g++ not installed")
+def test_waves_of_few_and_of_many_rows(tmp_path):
+    """Eight and sixteen waves to 16 rows only where the rows leave room for them: 648 rows of 25 pieces took 31.0 us with
+    eight and 27.3 with four, 32 rows of 128 20.5 with eight and 19.6 with sixteen."""
+    src, exe = tmp_path / "waves.cpp", tmp_path / "waves"
+    src.write_text('#include <cstdio>\n#include "latent_plan.hpp"\nint main() { const long long at[][2] = {{25, 648}, {128, 32}, {64, '
+                   '64}, {48, 128}, {48, 129}, {32, 512}, {24, 513}, {16, 256}, {8, 512}, {1, 16000}};\nfor (const auto& a : at) '
+                   'std::printf("%d ", ferret::latent_join(a[0], 256, a[1], false).waves); }\n')
+    subprocess.run(["g++", "-std=c++17", f"-I{ROOT}/ferret_amd/csrc", str(src), "-o", str(exe)], check=True)
+    out = subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout
+    assert [int(x) for x in out.split()] == [4, 16, 16, 16, 8, 8, 4, 4, 1, 1]
